@@ -396,6 +396,81 @@ int kvbp_residual_add(kvbp_stream_t stream, int32_t rows, int32_t hidden, void* 
 int kvbp_demote_int8(kvbp_stream_t stream, void* kcache, void* vcache, int32_t layers, int32_t B, int32_t Hkv,
                      int32_t S, const int32_t* slots, int32_t stride, const int32_t* counts, int32_t* dev_err);
 
+/* ---- Low-bit serving: a paged KV cache in 4 bits, and 8-bit integer projections ----------
+ * (No counterpart in the reference, whose cache and weights stay bf16.)
+ *
+ * Paged 4-bit cache.  A pool holds n_pages pages of page_size slots (a multiple of 16) of
+ * Hkv heads: [n_pages][Hkv][page_size / 16] blocks of KVBP_KV4_BLOCK bytes, 16-byte
+ * aligned.  page_table [B][max_pages] int32 names each sequence's pages: its logical slot s
+ * lives in page page_table[b][s / page_size]; a page belongs to one sequence, or is shared by
+ * several that only read it.  A row of 128 values is four groups of 32 with an f16 scale each:
+ *   scale = f16(min(max|x| / 7, 65504)), value = (code - 8) * scale,
+ *   code = 8 + clip(rint(x / scale), -7, 7)
+ * so values beyond 7 * 65504 saturate, and a NaN makes its group NaN.  Bytes of a block (16
+ * slots of one head): K codes of slot s at 64 s (dim 32 j + 8 t + n is nibble n of the 32-bit
+ * word 4 t + j); V codes from 1024 (slot s = 4 t + 2 h + e: dim 32 i + 4 g + n is nibble n of
+ * the 16-bit word at 512 h + 64 g + 16 t + 4 i + 2 e); K scales at 2048 + 8 s + 2 j; V scales
+ * at 2176 + 32 t + 16 h + 4 i + 2 e.
+ * A slot outside [0, max_pages * page_size), a sequence outside [0, B) or a page outside
+ * [0, n_pages) is skipped and sets KVBP_DEV_INDEX.  head_dim is 128. */
+#define KVBP_KV4_BLOCK 2304
+
+/* Append: kvbp_qkv_rope_scatter's work into the 4-bit pages.  qkv [rows][ldq] bf16 holds Hq
+ * query, Hkv key and Hkv value heads; bias [(Hq + 2 Hkv) * 128], q_norm_w / k_norm_w [128]
+ * (RMSNorm with eps) and inv_freq [64] (rotation of (d, d + 64) by positions[r] *
+ * inv_freq[d]; without it positions is not read) may be NULL.  All arithmetic is fp32, the
+ * angle is reduced in double; q is rounded once to bf16 (q_out [rows][Hq][128]; Hq may be 0
+ * with q_out NULL), k and v once to their codes.  Row r belongs to sequence seq[r], or
+ * r / rows_per_seq when seq is NULL, and goes to logical slot slots[r] (< 0: not stored).
+ * The slots of one call must differ: of two rows for one slot either one's bytes may stay.
+ * ldq a multiple of 4; qkv and q_out 8-byte aligned. */
+int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, const int32_t* seq, int32_t B,
+                    int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t max_pages,
+                    const void* qkv, int32_t ldq, const void* bias, const void* q_norm_w, const void* k_norm_w,
+                    float eps, const float* inv_freq, const int32_t* positions, const int32_t* slots,
+                    const int32_t* page_table, void* q_out, void* pool, int32_t* dev_err);
+
+/* Read-back of listed slots as bf16((code - 8) * scale): row r, head h to k_out / v_out +
+ * r * row_stride + h * head_stride (elements; multiples of 4, outputs 8-byte aligned), e.g.
+ * [rows][Hkv][128] or the prefill attention's [Hkv][rows][128].  Rows of a skipped or
+ * negative slot are zeros. */
+int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, const int32_t* seq, int32_t B,
+                    int32_t Hkv, int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t max_pages,
+                    const int32_t* slots, const int32_t* page_table, const void* pool, void* k_out, void* v_out,
+                    int64_t row_stride, int64_t head_stride, int32_t* dev_err);
+
+/* Attention of one token per sequence over the 4-bit pages, with the per-slot eviction
+ * score: out[b] = softmax(scale * q . k) v over the live slots of sequence b -- logical
+ * slots s < lens[b] (0 allowed) with slot_pos[b][s] >= 0 (slot_pos [B][S], or NULL: all).
+ * q, out [B][Hq][128] bf16, 16-byte aligned; Hq / Hkv <= 8.  step_score [B][S] float (may be
+ * NULL, non-negative on entry) is max-accumulated with each live slot's largest probability
+ * over the heads, as kvbp_decode_attn_score does.  lens above max_pages * page_size (or S,
+ * when slot_pos or step_score is given) is cut there and sets KVBP_DEV_INDEX.  A sequence
+ * without a live slot gives zeros (and KVBP_DEV_NO_VALID_SLOT when lens[b] > 0).  Softmax
+ * statistics and sums are fp32; values in free slots and past lens never reach the result.
+ * workspace: kvbp_kv4_attn_workspace bytes, 16-byte aligned, free to reuse by the next call
+ * on the same stream (calls that may overlap need one each); nothing is kept in it. */
+int64_t kvbp_kv4_attn_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t max_slots, int32_t with_score);
+int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t page_size,
+                  int32_t n_pages, int32_t max_pages, const void* q, const void* pool, const int32_t* page_table,
+                  const int32_t* lens, const int32_t* slot_pos, int32_t S, float scale, void* out, float* step_score,
+                  void* workspace, int64_t workspace_bytes, int32_t* dev_err);
+
+/* Per-token 8-bit quantisation: scale[r] = max|x[r]| / 127, q[r][k] = rint(127 x / max|x|)
+ * (zeros and scale 0 for a zero row; a row with a NaN or infinity gets codes 0 and a scale
+ * that is not finite).  x [rows][ldx] bf16, q [rows][ldq] int8 (16-byte aligned rows: ldq a
+ * multiple of 16); columns of q past K are left as they were. */
+int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t K, const void* x, int64_t ldx, void* q,
+                         int64_t ldq, float* scale);
+
+/* Product in 8-bit integers: out[m][n] = (sum_k xq[m][k] * w[n][k]) * x_scale[m] * w_scale[n]
+ * (+ bias[n], bf16, may be NULL), exact 32-bit integer sums, K <= 131071; out bf16 [M][ldo],
+ * or float when fp32_out (partial sums to be reduced).  xq [M][ldq] and w [N][ldw] int8 with
+ * 16-byte aligned rows; M, N and K are free, columns past K are not read into the sums. */
+int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w, int64_t ldw,
+                   const float* w_scale, const void* xq, int64_t ldq, const float* x_scale, const void* bias,
+                   void* out, int64_t ldo, int32_t* dev_err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -132,6 +132,18 @@ SIGNATURES = {
     "kvbp_demote_int8": (C.c_int, [P, P, P, I32, I32, I32, I32, P, I32, P, P]),
     "kvbp_prefill_gemm": (C.c_int, [P, I32, I32, I32, I32, P, P, I32, P, I32, P]),
     "kvbp_unpack_weight": (C.c_int, [P, I32, I32, P, P]),
+    "kvbp_kv4_append": (
+        C.c_int,
+        [P, I32, I32, P, I32, I32, I32, I32, I32, I32, I32, P, I32, P, P, P, F32, P, P, P, P, P, P, P],
+    ),
+    "kvbp_kv4_gather": (C.c_int, [P, I32, I32, P, I32, I32, I32, I32, I32, I32, P, P, P, P, P, I64, I64, P]),
+    "kvbp_kv4_attn_workspace": (I64, [I32, I32, I32, I32, I32]),
+    "kvbp_kv4_attn": (
+        C.c_int,
+        [P, I32, I32, I32, I32, I32, I32, I32, P, P, P, P, P, I32, F32, P, P, P, I64, P],
+    ),
+    "kvbp_int8_quant_rows": (C.c_int, [P, I32, I32, P, I64, P, I64, P]),
+    "kvbp_int8_gemm": (C.c_int, [P, I32, I32, I32, I32, P, I64, P, P, I64, P, P, P, I64, P]),
 }
 EXTRA_SIGNATURES = {
     "kvbp_decode_attn_score_cs": (C.c_int, [P, I32, I32, I32, I32, I32, P, P, P, P, P, P, P, P, I32]),

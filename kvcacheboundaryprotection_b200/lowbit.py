@@ -1,0 +1,302 @@
+"""Low-bit serving operators: a paged KV cache held in 4 bits, and projections in 8-bit
+integers.  ``include/kvbp.h`` states the formats and the arithmetic.
+
+* ``kv4_pool`` makes a pool of pages; ``kv4_append`` finishes the q/k/v rows (bias, q/k
+  RMSNorm, RoPE) and stores K and V in 4 bits; ``kv4_attend`` is one token's attention over
+  the pages with the per-slot eviction score; ``kv4_gather`` reads slots back as bf16.
+* ``int8_quantize_rows`` rounds rows to 8 bits with a scale each (a token's activations, or a
+  weight's output channels); ``int8_linear`` is the projection of bf16 rows by such a weight.
+
+Every call enqueues on the current stream of its tensors' device, allocates what it returns
+(and its workspace) from torch's caching allocator, and can be captured in a CUDA graph.
+Arguments that do not fit raise ``ValueError``; problems found on the device (a slot or page
+out of range) set bits of ``dev_err``, an int32 tensor of one element, when one is given.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import capi
+from .capi import check, lib
+
+BLOCK = 2304  # bytes of 16 slots of one kv head (KVBP_KV4_BLOCK)
+HEAD_DIM = 128
+_I32_MAX = 2**31 - 1
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, shape: tuple) -> None:
+    """``t`` is a dense tensor of this type, device and shape (None: any size)."""
+    if t.dtype is not dtype or t.device != dev:
+        raise ValueError(f"{name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
+    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _on(dev: torch.device) -> int:
+    """The current stream of ``dev``, which is made the current device for the call."""
+    if dev.type != "cuda":
+        raise ValueError("the low-bit operators run on CUDA devices only")
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+class _Device:
+    """Makes a tensor's device current for a launch (a no-op where it is already)."""
+
+    def __init__(self, dev: torch.device):
+        self.idx = dev.index
+        self.prev = -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.idx:
+            self.prev = cur
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *a):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+
+
+def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) -> torch.Tensor:
+    """A pool of ``n_pages`` zeroed pages: uint8 [n_pages, n_kv_heads, page_size / 16, 2304]."""
+    if page_size <= 0 or page_size % 16:
+        raise ValueError(f"page_size {page_size} is not a multiple of 16")
+    if n_pages <= 0 or n_kv_heads <= 0:
+        raise ValueError("n_pages and n_kv_heads must be > 0")
+    return torch.zeros(n_pages, n_kv_heads, page_size // 16, BLOCK, dtype=torch.uint8,
+                       device=torch.device("cuda") if device is None else device)
+
+
+def _pool(pool: torch.Tensor, table: torch.Tensor) -> tuple:
+    """(pages, kv heads, page size, sequences, pages per sequence) after the checks."""
+    dev = pool.device
+    if dev.type != "cuda":
+        raise ValueError("the low-bit operators run on CUDA devices only")
+    _need(pool, "pool", torch.uint8, dev, (None, None, None, BLOCK))
+    _need(table, "page_table", torch.int32, dev, (None, None))
+    return pool.shape[0], pool.shape[1], pool.shape[2] * 16, table.shape[0], table.shape[1]
+
+
+def _rows(rows: int, B: int, seq: Optional[torch.Tensor], dev: torch.device) -> int:
+    """Rows per sequence when no ``seq`` names each row's sequence."""
+    if seq is not None:
+        _need(seq, "seq", torch.int32, dev, (rows,))
+        return 1
+    if B == 0 or rows % B:
+        raise ValueError(f"{rows} rows do not divide over {B} sequences: pass seq")
+    return max(1, rows // B)
+
+
+def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, qkv: torch.Tensor, slots: torch.Tensor, *, n_heads: int,
+               seq: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+               inv_freq: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               q_out: Optional[torch.Tensor] = None, dev_err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Finish rows of the q/k/v projection and store their K and V in the 4-bit pages.
+
+    ``qkv`` [rows, (n_heads + 2 kv_heads) * 128] bf16 (rows may be strided); row r goes to
+    logical slot ``slots[r]`` (negative: not stored) of sequence ``seq[r]`` (default: the
+    rows divide evenly over the page table's sequences).  With ``inv_freq`` [64] float32,
+    q and k are rotated by ``positions[r]``.  Returns q [rows, n_heads, 128] bf16."""
+    n_pages, hkv, page, B, width = _pool(pool, page_table)
+    dev = pool.device
+    if qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.dim() != 2:
+        raise ValueError("qkv must be a bfloat16 matrix on the pool's device")
+    rows, nh = qkv.shape[0], n_heads + 2 * hkv
+    if n_heads < 0 or qkv.shape[1] != nh * HEAD_DIM:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns, {n_heads} + 2 * {hkv} heads need {nh * HEAD_DIM}")
+    if rows and (qkv.stride(1) != 1 or (rows > 1 and qkv.stride(0) < qkv.shape[1])):
+        raise ValueError("qkv's columns must be contiguous and its rows must not overlap")
+    _need(slots, "slots", torch.int32, dev, (rows,))
+    per = _rows(rows, B, seq, dev)
+    if (inv_freq is None) != (positions is None):
+        raise ValueError("positions and inv_freq go together")
+    if inv_freq is not None:
+        _need(inv_freq, "inv_freq", torch.float32, dev, (HEAD_DIM // 2,))
+        _need(positions, "positions", torch.int32, dev, (rows,))
+    if bias is not None:
+        _need(bias, "bias", torch.bfloat16, dev, (nh * HEAD_DIM,))
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _need(t, name, torch.bfloat16, dev, (HEAD_DIM,))
+    if q_out is None:
+        q_out = torch.empty(rows, n_heads, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    else:
+        _need(q_out, "q_out", torch.bfloat16, dev, (rows, n_heads, HEAD_DIM))
+    if dev_err is not None:
+        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+    if rows == 0:
+        return q_out
+    if n_pages == 0 or width == 0 or hkv == 0 or page == 0:
+        raise ValueError("the pool and the page table must not be empty")
+    with _Device(dev):
+        check(
+            lib().kvbp_kv4_append(
+                _on(dev), rows, per, _ptr(seq), B, n_heads, hkv, HEAD_DIM, page, n_pages, width, _ptr(qkv),
+                qkv.stride(0) if rows > 1 else qkv.shape[1], _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), _ptr(positions), _ptr(slots),
+                _ptr(page_table), _ptr(q_out) if n_heads else None, _ptr(pool), _ptr(dev_err),
+            ),
+            "kv4_append",
+        )
+    return q_out
+
+
+def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, *,
+               seq: Optional[torch.Tensor] = None, heads_first: bool = False,
+               dev_err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V of the listed slots as the bf16 values their codes stand for: two tensors
+    [rows, kv_heads, 128], or [kv_heads, rows, 128] (the prefill attention's layout) with
+    ``heads_first``.  Rows of negative or out-of-range slots are zeros."""
+    n_pages, hkv, page, B, width = _pool(pool, page_table)
+    dev, rows = pool.device, slots.shape[0] if slots.dim() == 1 else -1
+    _need(slots, "slots", torch.int32, dev, (rows,) if rows >= 0 else (None,))
+    per = _rows(rows, B, seq, dev)
+    if dev_err is not None:
+        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+    shape = (hkv, rows, HEAD_DIM) if heads_first else (rows, hkv, HEAD_DIM)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    if rows == 0:
+        return k, v
+    if n_pages == 0 or width == 0 or hkv == 0 or page == 0:
+        raise ValueError("the pool and the page table must not be empty")
+    row_stride, head_stride = (HEAD_DIM, rows * HEAD_DIM) if heads_first else (hkv * HEAD_DIM, HEAD_DIM)
+    with _Device(dev):
+        check(
+            lib().kvbp_kv4_gather(
+                _on(dev), rows, per, _ptr(seq), B, hkv, HEAD_DIM, page, n_pages, width, _ptr(slots), _ptr(page_table),
+                _ptr(pool), _ptr(k), _ptr(v), row_stride, head_stride, _ptr(dev_err),
+            ),
+            "kv4_gather",
+        )
+    return k, v
+
+
+def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, q: torch.Tensor, *,
+               slot_pos: Optional[torch.Tensor] = None, step_score: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               dev_err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token's attention per sequence: q [B, heads, 128] bf16 over the live slots
+    s < lens[b] with slot_pos[b, s] >= 0 (all of them without ``slot_pos`` [B, S]).
+    ``step_score`` [B, S] float32 is max-accumulated with every live slot's largest
+    probability over the heads.  ``scale`` defaults to 1 / sqrt(128).  Returns out
+    [B, heads, 128] bf16; a sequence without a live slot gives zeros."""
+    n_pages, hkv, page, B, width = _pool(pool, page_table)
+    dev = pool.device
+    _need(lens, "lens", torch.int32, dev, (B,))
+    _need(q, "q", torch.bfloat16, dev, (B, None, HEAD_DIM))
+    hq = q.shape[1]
+    if hkv == 0 or hq == 0 or hq % hkv or hq // hkv > 8:
+        raise ValueError(f"{hq} query heads over {hkv} kv heads: whole groups of at most 8 are supported")
+    S = 0
+    for t, name, dt in ((slot_pos, "slot_pos", torch.int32), (step_score, "step_score", torch.float32)):
+        if t is not None:
+            _need(t, name, dt, dev, (B, S or None))
+            S = t.shape[1]
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, "out", torch.bfloat16, dev, (B, hq, HEAD_DIM))
+    if dev_err is not None:
+        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+    if B == 0:
+        return out
+    if n_pages == 0 or width == 0 or page == 0 or ((slot_pos is not None or step_score is not None) and S == 0):
+        raise ValueError("the pool, the page table, slot_pos and step_score must not be empty")
+    L = lib()
+    limit = min(width * page, S) if S else width * page
+    ws_bytes = L.kvbp_kv4_attn_workspace(B, hq, hkv, limit, step_score is not None)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _Device(dev):
+        check(
+            L.kvbp_kv4_attn(
+                _on(dev), B, hq, hkv, HEAD_DIM, page, n_pages, width, _ptr(q), _ptr(pool), _ptr(page_table), _ptr(lens),
+                _ptr(slot_pos), S, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, _ptr(out), _ptr(step_score),
+                _ptr(ws), ws_bytes, _ptr(dev_err),
+            ),
+            "kv4_attn",
+        )
+    return out
+
+
+def _matrix(x: torch.Tensor, name: str, dtype: torch.dtype) -> None:
+    if x.dim() != 2 or x.dtype is not dtype or x.device.type != "cuda":
+        raise ValueError(f"{name} must be a {dtype} matrix on a CUDA device")
+    if x.shape[0] and x.shape[1] and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+        raise ValueError(f"{name}'s columns must be contiguous and its rows must not overlap")
+
+
+def int8_quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of a bf16 matrix in 8 bits: codes int8 [rows, K] (a view of storage whose rows
+    start on 16-byte boundaries, as ``int8_linear`` wants its weight) and scales float32
+    [rows]; x is about codes * scale."""
+    _matrix(x, "x", torch.bfloat16)
+    rows, K = x.shape
+    dev = x.device
+    pitch = (K + 15) // 16 * 16
+    q = torch.zeros(rows, pitch, dtype=torch.int8, device=dev) if pitch != K else torch.empty(
+        rows, K, dtype=torch.int8, device=dev)
+    s = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows and K:
+        with _Device(dev):
+            check(lib().kvbp_int8_quant_rows(_on(dev), rows, K, _ptr(x), x.stride(0) if rows > 1 else K, _ptr(q), pitch,
+                                             _ptr(s)), "int8_quant_rows")
+    else:
+        s.zero_()
+    return q[:, :K], s
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
+                dev_err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [M, K] bf16 times w [N, K] int8 (rows on 16-byte boundaries, scales w_scale [N]) plus
+    bias [N] bf16: each row of x is rounded to 8 bits with its own scale, the sums are exact
+    32-bit integers, and y = sum * x_scale * w_scale + bias is rounded once to ``out_dtype``
+    (bfloat16 or float32)."""
+    _matrix(x, "x", torch.bfloat16)
+    _matrix(w, "w", torch.int8)
+    M, K = x.shape
+    N, dev = w.shape[0], x.device
+    if w.device != dev or w.shape[1] != K:
+        raise ValueError(f"w must be [N, {K}] on {dev}, got {tuple(w.shape)} on {w.device}")
+    if K == 0 or N == 0:
+        raise ValueError("int8_linear needs at least one input and one output feature")
+    ldw = w.stride(0) if N > 1 else (K + 15) // 16 * 16
+    if ldw % 16 or w.data_ptr() % 16:
+        raise ValueError("w's rows must start on 16-byte boundaries (int8_quantize_rows makes such weights)")
+    _need(w_scale, "w_scale", torch.float32, dev, (N,))
+    if bias is not None:
+        _need(bias, "bias", torch.bfloat16, dev, (N,))
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be bfloat16 or float32")
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    else:
+        _need(out, "out", out_dtype, dev, (M, N))
+    if dev_err is not None:
+        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+    if M == 0:
+        return out
+    L = lib()
+    pitch = (K + 15) // 16 * 16
+    # codes and scales of x in one allocation (the scales behind the codes)
+    ws = torch.empty(M * pitch + 4 * M, dtype=torch.uint8, device=dev)
+    xq = ws.data_ptr()
+    xs = xq + M * pitch
+    with _Device(dev):
+        st = _on(dev)
+        check(L.kvbp_int8_quant_rows(st, M, K, x.data_ptr(), x.stride(0) if M > 1 else K, xq, pitch, xs),
+              "int8_quant_rows")
+        check(L.kvbp_int8_gemm(st, int(out_dtype is torch.float32), M, N, K, w.data_ptr(), ldw, w_scale.data_ptr(), xq,
+                               pitch, xs, _ptr(bias), out.data_ptr(), N, _ptr(dev_err)), "int8_gemm")
+    return out
