@@ -228,118 +228,657 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
   *reinterpret_cast<uint2*>(v_out + at + 64) = o[1][1];
 }
 
-// Attention of one token per sequence.  One CTA of 8 warps per (kv head, sequence); a warp
-// takes slots w, w + 8, ... with an online softmax per query head, lane l holding dims
-// 4 l .. 4 l + 3; the warps' (max, sum, O) are merged in shared memory.  With a score, a
-// second walk over K forms each slot's probabilities from the final (max, sum).
-template <int G>
-__global__ void __launch_bounds__(256) attend_kernel(const __nv_bfloat16* __restrict__ q, Pool pool,
-                                                     const int* __restrict__ lens, const int* __restrict__ slot_pos,
-                                                     int S, int limit, float scale, int Hq,
-                                                     __nv_bfloat16* __restrict__ out, float* __restrict__ step_score,
-                                                     int* err) {
+// ---- attention of one token per sequence ------------------------------------------------
+// softmax(scale q . k) v for the <= 8 query heads of a kv head, slots on the M side of
+// mma.sync m16n8k16 (f16 operands, fp32 sums) and heads on N.
+//
+// What bounds it: HBM, 144 bytes per slot and kv head -- 46 codes per clock and SM at the
+// copy bandwidth, so unpacking has to cost about one instruction per code:
+//  * (word & 0x000f000f) | 0x64006400 is the f16 pair 1024 + n, (word & 0x00f000f0) |
+//    0x64006400 the pair 1024 + 16 n; one packed add or multiply-add makes either the exact
+//    code n - 8: 9 instructions per 8 codes.  (Feeding the MMA the biased pairs, or the bare
+//    bits as f16 subnormals, and taking the bias off the sums saves 4 of the 9 but not the
+//    precision: the MMA aligns products by their operands' exponent fields, 10 bits above the
+//    code's own, and its sums came out 2^-16 off.)
+//  * scales never touch the codes: K's multiply the four group sums in fp32, V's multiply the
+//    softmax weights (P' = P * scale, f16, rounded at 2^-11: half a bf16 output step is 2^-9).
+// P is 2^(x - ref) with ref = max(x) - e, e chosen from the tile's largest V scale so that
+// P * scale <= 2^14: f16 keeps 11 bits of P' over its whole range whatever V's magnitude.
+// q is brought to [2^14, 2^15) by a power of two for the same reason (exact: q is bf16).
+// A masked slot's logit is -inf and its V scale zero, so nothing it holds (NaN scales of
+// never-written memory included) reaches a sum; codes are finite whatever their bits.
+//
+// Work split: the 16-slot blocks of all sequences and heads in one line, cut into equal
+// ranges, one per CTA (two CTAs of 8 warps per SM), whatever the lengths.  A range crosses
+// heads; within a head's part ("segment") the warps take turns at 32-slot stages, each warp
+// with its own two-stage ring of bulk copies that runs on across segments, so no barrier
+// stands in the stream.  At the end of a segment the warps' (ref, sum, O) meet in shared
+// memory; a whole head is written out, a part of one goes to the workspace (at most two per
+// CTA) for the combine kernel.  Logits for the eviction score go to the workspace too: the
+// probabilities need the final (ref, sum).
+constexpr int kWarps = 8;
+constexpr int kStages = 2;       // per warp
+constexpr int kStageBlocks = 2;  // 16-slot blocks per stage
+constexpr int kMaxSeqs = 512;    // sequences per launch (their lengths live in shared memory)
+constexpr int kMaxCtas = 320;
+constexpr int kMinBlocks = 16;   // blocks per CTA at least
+constexpr int kHeadPitch = 132;  // floats between heads of a partial O (conflict-free float4 stores)
+constexpr int kPart = 8 * 128 + 16;  // floats of one partial: O[8][128], ref[8], sum[8]
+
+// Workspace: int header[2 + kMaxSeqs + 1] {blocks per CTA, -, first block of each sequence},
+// partials [kMaxCtas][2][kPart], and with a score the whole heads' (ref, sum) [B][Hkv][8][2]
+// and the logits [B][Hkv][S16][gs] in units of ln 2.
+constexpr size_t kHeaderBytes = ((2 + kMaxSeqs + 1) * 4 + 15) / 16 * 16;
+constexpr size_t kPartBytes = static_cast<size_t>(kMaxCtas) * 2 * kPart * 4;
+
+struct AttnArgs {
+  const __nv_bfloat16* q;
+  Pool pool;
+  const int* lens;
+  const int* slot_pos;
+  __nv_bfloat16* out;
+  float* step_score;
+  int* header;
+  float* part;
+  float* stats;   // null without a score
+  float* logits;  // null without a score
+  int* err;
+  float scale;
+  int Hq, S, limit;
+  int s16, gs;  // logit rows per head, floats per row
+};
+
+struct Smem {
+  uint8_t ring[kWarps][kStages][kStageBlocks * kBlock];
+  float part[kWarps][8][kHeadPitch];
+  float ref[kWarps][8], sum[kWarps][8];
+  uint64_t full[kWarps][kStages];
+  uint32_t mask[kWarps][kStages];
+  int first[kMaxSeqs + 1];  // first block of each sequence's first head
+  int len[kMaxSeqs];
+  int wsum[kWarps];
+};
+static_assert(sizeof(Smem) <= 115712 - 16, "two CTAs per SM");
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The codes n - 8 of nibbles 0 and 4 / 1 and 5 of a word, as f16 pairs for the MMA.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  const uint32_t c = 0xe408e408u;  // -1032
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t code_pair_hi(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  const uint32_t m = 0x2c002c00u, c = 0xd480d480u;  // 1 / 16, -72
+  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(m), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// A range's part of one (sequence, kv head): blocks [sb0, sb0 + n) of the head's nsb.
+struct Segment {
+  int b, h, sb0, n, nsb;
+  __device__ __forceinline__ void at(const Smem& sm, int Hkv, int pos, int end) {  // b: any sequence at or before pos
+    while (sm.first[b + 1] <= pos) ++b;
+    nsb = (sm.len[b] + 15) >> 4;
+    const int o = pos - sm.first[b];
+    h = o / nsb;
+    sb0 = o - h * nsb;
+    n = min(nsb - sb0, end - pos);
+  }
+  // blocks per stage: short segments are spread over all warps
+  __device__ __forceinline__ int per() const { return n <= kWarps ? 1 : kStageBlocks; }
+};
+
+// The lengths' prefix sums into shared memory; returns the number of blocks of all heads.
+__device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
+  const int B = a.pool.B, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kEach = kMaxSeqs / (kWarps * 32);
+  int v[kEach], t = 0;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int b = tid * kEach + u;
+    int n = b < B ? a.lens[b] : 0;
+    if (n < 0 || n > a.limit) {
+      if (report) set_err(a.err, kErrIndex);
+      n = n < 0 ? 0 : a.limit;
+    }
+    if (b < B) sm.len[b] = n;
+    v[u] = t;
+    t += ((n + 15) >> 4) * a.pool.Hkv;
+  }
+  int inc = t;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) sm.wsum[warp] = inc;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sm.wsum[w];
+    total += sm.wsum[w];
+  }
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int b = tid * kEach + u;
+    if (b < B) sm.first[b] = before + inc - t + v[u];
+  }
+  if (tid == 0) sm.first[B] = total;
+  __syncthreads();
+  return total;
+}
+
+__global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int Hkv = a.pool.Hkv, group = a.Hq / Hkv;
+  if (lane == 0)
+    for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[warp][s], 1);
+  fence_barrier_init();
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float sm[8][G], sl[8][G], so[8][G][128];
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = Hq / pool.Hkv;
-  int n = lens[b];
-  if (n < 0 || n > limit) {
-    if (threadIdx.x == 0 && h == 0) set_err(err, kErrIndex);
-    n = n < 0 ? 0 : limit;
+  const int total = plan(a, sm, blockIdx.x == 0);
+  int R = (total + gridDim.x - 1) / gridDim.x;
+  if (R < kMinBlocks) R = kMinBlocks;
+  if (blockIdx.x == 0) {
+    if (tid == 0) a.header[0] = R;
+    for (int b = tid; b <= a.pool.B; b += kWarps * 32) a.header[2 + b] = sm.first[b];
   }
-  float qf[G][4], m[G], l[G], o[G][4];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const uint2 w = g < group ? *reinterpret_cast<const uint2*>(q + (static_cast<size_t>(b) * Hq + h * group + g) * 128 + 4 * lane)
-                              : make_uint2(0, 0);
-    qf[g][0] = bf16lo(w.x), qf[g][1] = bf16hi(w.x), qf[g][2] = bf16lo(w.y), qf[g][3] = bf16hi(w.y);
-    m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) o[g][k] = 0.f;
+  const int start = static_cast<int>(min(static_cast<long long>(blockIdx.x) * R, static_cast<long long>(total)));
+  const int end = min(total - start, R) + start;
+  if (start >= end) return;
+
+  // -- the stage to be issued next: found one stage ahead, so that its page and mask loads
+  //    are not waited for
+  Segment is;
+  {
+    int lo = 0, hi = a.pool.B - 1;  // the last sequence that starts at or before ``start``
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sm.first[mid] <= start) lo = mid;
+      else hi = mid - 1;
+    }
+    is.b = lo;
   }
-  const float to2 = scale * 1.4426950408889634f;  // logits in units of ln 2
-  auto block = [&](int s) -> const uint8_t* {  // the slot's block, null when it is masked
-    if (slot_pos && slot_pos[static_cast<size_t>(b) * S + s] < 0) return nullptr;
-    const uint8_t* p = pool.block_of(b, s, err, lane == 0 && h == 0);
-    return p ? p + h * pool.hstride() : nullptr;
-  };
-  auto logits = [&](const uint8_t* blk, int in, float (&s)[G]) {
-    const uint32_t c = *reinterpret_cast<const uint16_t*>(blk + k_code_offset(in, lane));
-    const float ks = __half2float(*reinterpret_cast<const __half*>(blk + k_scale_offset(in, lane >> 3)));
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float d = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) d += qf[g][k] * static_cast<float>(static_cast<int>((c >> (4 * k)) & 15u) - 8);
-      d *= ks;
-#pragma unroll
-      for (int off = 16; off; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
-      s[g] = d * to2;
+  is.at(sm, Hkv, start, end);
+  Segment cs = is;
+  int ipos = start, iturn = 0;
+  bool have = false, live = false;
+  int cnt = 0, sb = 0, ih = 0, page = -1, inner = 0;
+  auto fetch = [&]() {
+    for (;;) {
+      const int per = is.per(), k = (warp + kWarps * iturn) * per;
+      if (k < is.n) {
+        ++iturn;
+        cnt = min(per, is.n - k);
+        sb = is.sb0 + k;
+        ih = is.h;
+        page = -1;
+        const int slot = sb * 16 + lane;
+        live = lane < cnt * 16 && slot < sm.len[is.b];
+        if (live && a.slot_pos) live = a.slot_pos[static_cast<size_t>(is.b) * a.S + slot] >= 0;
+        if (lane < cnt) {
+          const int s = (sb + lane) * 16, pi = s / a.pool.page;
+          inner = (s - pi * a.pool.page) >> 4;
+          page = a.pool.table[static_cast<size_t>(is.b) * a.pool.max_pages + pi];
+        }
+        have = true;
+        return;
+      }
+      ipos += is.n;
+      if (ipos >= end) {
+        have = false;
+        return;
+      }
+      is.at(sm, Hkv, ipos, end);
+      iturn = 0;
     }
   };
-  bool any = false;
-  for (int s = warp; s < n; s += 8) {
-    const uint8_t* blk = block(s);
-    if (!blk) continue;
-    any = true;
-    float x[G];
-    logits(blk, s & 15, x);
-    const uint32_t c = *reinterpret_cast<const uint16_t*>(blk + v_code_offset(s & 15, lane));
-    const float vs = __half2float(*reinterpret_cast<const __half*>(blk + v_scale_offset(s & 15, lane >> 3)));
+  auto issue = [&](int st) {
+    if (!have) return;
+    const bool ok = lane < cnt && page >= 0 && page < a.pool.n_pages;
+    if (lane < cnt && !ok) set_err(a.err, kErrIndex);
+    const uint32_t okm = __ballot_sync(0xffffffffu, ok);
+    const uint32_t mask = __ballot_sync(0xffffffffu, live && ((okm >> (lane >> 4)) & 1u));
+    if (lane == 0) {
+      sm.mask[warp][st] = mask;
+      mbar_expect_tx(&sm.full[warp][st], __popc(okm) * kBlock);
+    }
+    __syncwarp();
+    if (ok)
+      bulk_load(sm.ring[warp][st] + lane * kBlock,
+                a.pool.base + ((static_cast<size_t>(page) * Hkv + ih) * (a.pool.page >> 4) + inner) * kBlock, kBlock,
+                &sm.full[warp][st]);
+  };
+  fetch();
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float mn = fmaxf(m[g], x[g]), f = exp2f(m[g] - mn), p = exp2f(x[g] - mn);
-      m[g] = mn;
-      l[g] = l[g] * f + p;
+  for (int s = 0; s < kStages; ++s) {
+    issue(s);
+    if (have) fetch();
+  }
+
+  int st = 0, phase = 0;  // the stage consumed next
+  bool dead = false;      // a copy never arrived: stop streaming, keep the barriers
+  const int sg = 4 * (g >> 1) + (g & 1);  // slot (of 16) of MMA row g; row g + 8 is slot sg + 2
+  for (int pos = start; pos < end;) {
+    // q of this head as the MMA's B operand [group j][step u][2], heads on the columns
+    uint32_t qf[4][2][2];
+    float xs[2];
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(cs.b) * a.Hq + cs.h * group + g) * 128);
+      uint4 w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        o[g][k] = o[g][k] * f + p * (static_cast<float>(static_cast<int>((c >> (4 * k)) & 15u) - 8) * vs);
+      for (int j = 0; j < 4; ++j) w[j] = g < group ? src[4 * j + t] : make_uint4(0, 0, 0, 0);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max((ws[k] >> 16) & 0x7fffu, ws[k] & 0x7fffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^up brings the head's largest |q| to [2^14, 2^15)
+      const int up = min(14 + 127 - static_cast<int>(top >> 7), 126);
+      const float f = __int_as_float((up + 127) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float d[8] = {bf16lo(w[j].x) * f, bf16hi(w[j].x) * f, bf16lo(w[j].y) * f, bf16hi(w[j].y) * f,
+                            bf16lo(w[j].z) * f, bf16hi(w[j].z) * f, bf16lo(w[j].w) * f, bf16hi(w[j].w) * f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[j][u][e] = half2_bits(__floats2half2_rn(d[2 * u + e], d[2 * u + e + 4]));
+      }
+      // a thread's C columns are heads 2 t and 2 t + 1: logits in units of ln 2 per unit of
+      // their sums, scale log2(e) / 2^up, in two factors (2^-up alone can overflow)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int upe = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
+        xs[e] = a.scale * 1.4426950408889634f * __int_as_float((127 - (upe >> 1)) << 23) *
+                __int_as_float((127 - (upe - (upe >> 1))) << 23);
+      }
+    }
+    float o[8][4], l[2] = {0.f, 0.f}, ref[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+
+    const int per = cs.per();
+    for (int k = warp * per; k < cs.n; k += kWarps * per) {
+      const int nb = min(per, cs.n - k);
+      if (!dead && !__all_sync(0xffffffffu, mbar_wait_bounded(&sm.full[warp][st], phase))) {
+        dead = true;  // let the other stages' copies land before the CTA can exit
+        if (lane == 0) set_err(a.err, kErrWaitTimeout);
+        for (int s = 1; s < kStages; ++s)
+          mbar_wait_bounded(&sm.full[warp][(st + s) % kStages], phase ^ (st + s >= kStages), 1u << 16);
+        __syncwarp();
+      }
+      const uint32_t mask = dead ? 0u : sm.mask[warp][st];
+      const uint8_t* base = sm.ring[warp][st];
+      float x[kStageBlocks][4];
+      uint32_t sv_top = 0;
+      float* lg = a.logits ? a.logits + (static_cast<size_t>(cs.b * Hkv + cs.h) * a.s16 + (cs.sb0 + k) * 16) * a.gs : nullptr;
+#pragma unroll
+      for (int bl = 0; bl < kStageBlocks; ++bl) {
+        if (bl < nb) {
+          const uint8_t* blk = base + bl * kBlock;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(blk + 64 * sg + 16 * t);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(blk + 64 * (sg + 2) + 16 * t);
+          const uint2 s0 = *reinterpret_cast<const uint2*>(blk + kKScale + 8 * sg);
+          const uint2 s1 = *reinterpret_cast<const uint2*>(blk + kKScale + 8 * (sg + 2));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          const float2 f0[2] = {__half22float2(bits_half2(s0.x)), __half22float2(bits_half2(s0.y))};
+          const float2 f1[2] = {__half22float2(bits_half2(s1.x)), __half22float2(bits_half2(s1.y))};
+          float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t u0 = w0[j] >> 8, u1 = w1[j] >> 8;
+            mma_f16(c, code_pair(w0[j]), code_pair(w1[j]), code_pair_hi(w0[j]), code_pair_hi(w1[j]), qf[j][0][0],
+                    qf[j][0][1]);
+            mma_f16(c, code_pair(u0), code_pair(u1), code_pair_hi(u0), code_pair_hi(u1), qf[j][1][0], qf[j][1][1]);
+            const float a0 = j & 1 ? f0[j >> 1].y : f0[j >> 1].x, a1 = j & 1 ? f1[j >> 1].y : f1[j >> 1].x;
+            y[0] += a0 * c[0];
+            y[1] += a0 * c[1];
+            y[2] += a1 * c[2];
+            y[3] += a1 * c[3];
+          }
+          const bool v0 = (mask >> (16 * bl + sg)) & 1u, v1 = (mask >> (16 * bl + sg + 2)) & 1u;
+          x[bl][0] = v0 ? y[0] * xs[0] : -INFINITY;
+          x[bl][1] = v0 ? y[1] * xs[1] : -INFINITY;
+          x[bl][2] = v1 ? y[2] * xs[0] : -INFINITY;
+          x[bl][3] = v1 ? y[3] * xs[1] : -INFINITY;
+          if (lg && 2 * t < a.gs) {
+            *reinterpret_cast<float2*>(lg + (16 * bl + sg) * a.gs + 2 * t) = make_float2(x[bl][0], x[bl][1]);
+            *reinterpret_cast<float2*>(lg + (16 * bl + sg + 2) * a.gs + 2 * t) = make_float2(x[bl][2], x[bl][3]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[bl][e] = -INFINITY;
+        }
+      }
+      // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3): zero where masked
+      uint32_t keep[kStageBlocks][2];
+#pragma unroll
+      for (int bl = 0; bl < kStageBlocks; ++bl)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
+          keep[bl][h] = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+        }
+      auto v_scales = [&](int bl, int h) {
+        uint4 v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
+        v.x &= keep[bl][h], v.y &= keep[bl][h], v.z &= keep[bl][h], v.w &= keep[bl][h];
+        return v;
+      };
+#pragma unroll
+      for (int bl = 0; bl < kStageBlocks; ++bl)
+        if (bl < nb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 v = v_scales(bl, h);  // non-negative halves: their bits order like their values
+            sv_top = __vmaxu2(sv_top, __vmaxu2(__vmaxu2(v.x, v.y), __vmaxu2(v.z, v.w)));
+          }
+      sv_top = max(sv_top & 0xffffu, sv_top >> 16);
+      sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 1));
+      sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 2));
+      const int e = min(15, 28 - static_cast<int>((sv_top >> 10) & 31u));  // P * scale < 2^14
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float m = fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        const float r = fmaxf(ref[c], m - static_cast<float>(e));
+        f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
+        ref[c] = r;
+        l[c] *= f[c];
+      }
+      if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
+      }
+      const float r0 = ref[0] == -INFINITY ? 0.f : ref[0], r1 = ref[1] == -INFINITY ? 0.f : ref[1];
+#pragma unroll
+      for (int bl = 0; bl < kStageBlocks; ++bl) {
+        if (bl >= nb) continue;
+        const uint8_t* blk = base + bl * kBlock;
+        const float p0 = ex2(x[bl][0] - r0), p1 = ex2(x[bl][1] - r1), p2 = ex2(x[bl][2] - r0), p3 = ex2(x[bl][3] - r1);
+        l[0] += p0 + p2;
+        l[1] += p1 + p3;
+        const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
+        const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
+        const uint4 s0 = v_scales(bl, 0), s1 = v_scales(bl, 1);
+        const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t);
+        const uint4 v1 = *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t);
+        const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb4[4] = {s1.x, s1.y, s1.z, s1.w};
+        const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t c0 = half2_bits(__hmul2(b0, bits_half2(sa[i]))), c1 = half2_bits(__hmul2(b1, bits_half2(sb4[i])));
+          const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
+          mma_f16(o[2 * i], code_pair(w0[i]), code_pair_hi(w0[i]), code_pair(w1[i]), code_pair_hi(w1[i]), c0, c1);
+          mma_f16(o[2 * i + 1], code_pair(u0), code_pair_hi(u0), code_pair(u1), code_pair_hi(u1), c0, c1);
+        }
+      }
+      __syncwarp();
+      if (!dead) {
+        issue(st);
+        if (have) fetch();
+      }
+      if (++st == kStages) st = 0, phase ^= 1;
+    }
+
+    // -- the warps' parts of this segment meet
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
+      if (g == 0) sm.ref[warp][2 * t + c] = ref[c], sm.sum[warp][2 * t + c] = l[c];
+    }
+    if (warp * per < cs.n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (2 * t + c < group) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(&sm.part[warp][2 * t + c][32 * i + 4 * g]) =
+                make_float4(o[2 * i][c], o[2 * i][c + 2], o[2 * i + 1][c], o[2 * i + 1][c + 2]);
+        }
+    }
+    __syncthreads();
+    const bool whole = cs.n == cs.nsb;
+    if (warp < group) {  // one query head per warp, four dims per lane
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.ref[w][warp]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float rw = sm.ref[w][warp];
+        const float lw = sm.sum[w][warp];
+        if (rw > -INFINITY || lw != 0.f) {  // also a NaN sum
+          const float fw = rw == M ? 1.0f : ex2(rw - M);
+          const float4 v = *reinterpret_cast<const float4*>(&sm.part[w][warp][4 * lane]);
+          L += lw * fw;
+          acc.x += v.x * fw, acc.y += v.y * fw, acc.z += v.z * fw, acc.w += v.w * fw;
+        }
+      }
+      if (whole) {
+        const bool none = L == 0.f;
+        const float r = none ? 0.f : 1.0f / L;
+        __nv_bfloat16* dst = a.out + (static_cast<size_t>(cs.b) * a.Hq + cs.h * group + warp) * 128 + 4 * lane;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
+        if (lane == 0) {
+          if (none) set_err(a.err, kErrNoValidSlot);
+          if (a.stats) {
+            float* s = a.stats + (static_cast<size_t>(cs.b * Hkv + cs.h) * 8 + warp) * 2;
+            s[0] = M;
+            s[1] = L;
+          }
+        }
+      } else {
+        float* p = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (pos == start ? 0 : 1)) * kPart;
+        *reinterpret_cast<float4*>(p + warp * 128 + 4 * lane) = acc;
+        if (lane == 0) p[1024 + warp] = M, p[1032 + warp] = L;
+      }
+    }
+    pos += cs.n;
+    if (pos < end) {
+      cs.at(sm, Hkv, pos, end);
+      __syncthreads();  // the parts have been read: the next segment may write its own
     }
   }
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    if (lane == 0) sm[warp][g] = m[g], sl[warp][g] = l[g];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) so[warp][g][4 * lane + k] = o[g][k];
-  }
-  const int found = __syncthreads_or(any);
-  if (!found && n > 0 && threadIdx.x == 0) set_err(err, kErrNoValidSlot);
-  float M[G], R[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    M[g] = -INFINITY;
-    for (int w = 0; w < 8; ++w) M[g] = fmaxf(M[g], sm[w][g]);
-    float L = 0.f;
-    for (int w = 0; w < 8; ++w) L += sm[w][g] > -INFINITY ? sl[w][g] * exp2f(sm[w][g] - M[g]) : sl[w][g];
-    R[g] = found ? 1.0f / L : 0.f;
-  }
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    if (g >= group || threadIdx.x >= 128) continue;
-    float v = 0.f;
-    if (found)
-      for (int w = 0; w < 8; ++w) {
-        const float f = sm[w][g] > -INFINITY ? exp2f(sm[w][g] - M[g]) : 0.f;
-        v += f > 0.f || f != f ? so[w][g][threadIdx.x] * f : 0.f;
+}
+
+// Finishes what the streaming kernel left: CTAs x < Hkv join the parts of head (x, sequence)
+// (or write zeros for an empty sequence); the others form the eviction score of 256 slots of
+// a sequence from the logits and the final (ref, sum) of its heads.  Latency-bound: one launch.
+__global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ float2 fin[];  // (ref, 1 / sum) of every query head of the sequence
+  const int Hkv = a.pool.Hkv, group = a.Hq / Hkv, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int R = a.header[0], first = a.header[2 + b], nsb = (a.header[2 + b + 1] - first) / Hkv;
+  // parts of head h: CTAs c0 .. c1, in the first slot of each but the one it starts inside
+  auto part_of = [&](int c, int s0) { return a.part + (static_cast<size_t>(c) * 2 + (c * static_cast<long long>(R) >= s0 ? 0 : 1)) * kPart; };
+  if (static_cast<int>(blockIdx.x) < Hkv) {
+    const int h = blockIdx.x;
+    if (warp >= group) return;
+    __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + h * group + warp) * 128 + 4 * lane;
+    if (nsb == 0) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
+      return;
+    }
+    const int s0 = first + h * nsb, c0 = s0 / R, c1 = (s0 + nsb - 1) / R;
+    if (c0 == c1) return;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, part_of(c, s0)[1024 + warp]);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float* p = part_of(c, s0);
+      const float rw = p[1024 + warp], lw = p[1032 + warp];
+      const float4 v = *reinterpret_cast<const float4*>(p + warp * 128 + 4 * lane);
+      if (rw > -INFINITY || lw != 0.f) {
+        const float fw = rw == M ? 1.0f : ex2(rw - M);
+        L += lw * fw;
+        acc.x += v.x * fw, acc.y += v.y * fw, acc.z += v.z * fw, acc.w += v.w * fw;
       }
-    out[(static_cast<size_t>(b) * Hq + h * group + g) * 128 + threadIdx.x] = __float2bfloat16_rn(v * R[g]);
+    }
+    const bool none = L == 0.f;
+    const float r = none ? 0.f : 1.0f / L;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
+    if (none && lane == 0) set_err(a.err, kErrNoValidSlot);
+    return;
   }
-  if (!step_score || !found) return;
-  for (int s = warp; s < n; s += 8) {
-    const uint8_t* blk = block(s);
-    if (!blk) continue;
-    float x[G], p = 0.f;
-    logits(blk, s & 15, x);
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-      if (g < group) {
-        const float e = exp2f(x[g] - M[g]) * R[g];
-        if (e != e && lane == 0) set_err(err, kErrNanScore);
-        p = fmaxf(p, e);
+  if (nsb == 0) return;
+  const int s = (blockIdx.x - Hkv) * 256 + threadIdx.x;
+  if ((blockIdx.x - Hkv) * 256 >= nsb * 16) return;
+  for (int q = warp; q < a.Hq; q += 8) {  // one query head per warp, the parts over the lanes
+    const int h = q / group, w = q - h * group;
+    const int s0 = first + h * nsb, c0 = s0 / R, c1 = (s0 + nsb - 1) / R;
+    float M, L;
+    if (c0 == c1) {
+      const float* st = a.stats + (static_cast<size_t>(b * Hkv + h) * 8 + w) * 2;
+      M = st[0], L = st[1];
+    } else {
+      M = -INFINITY, L = 0.f;
+      for (int c = c0 + lane; c <= c1; c += 32) {
+        const float* p = part_of(c, s0);
+        const float rw = p[1024 + w], lw = p[1032 + w], m = fmaxf(M, rw);
+        if (m > -INFINITY) L = L * (M == m ? 1.0f : ex2(M - m)) + lw * (rw == m ? 1.0f : ex2(rw - m));
+        else L += lw;
+        M = m;
       }
-    if (lane == 0) atomicMax(reinterpret_cast<int*>(step_score + static_cast<size_t>(b) * S + s), __float_as_int(p));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        const float rw = __shfl_xor_sync(0xffffffffu, M, o), lw = __shfl_xor_sync(0xffffffffu, L, o), m = fmaxf(M, rw);
+        if (m > -INFINITY) L = L * (M == m ? 1.0f : ex2(M - m)) + lw * (rw == m ? 1.0f : ex2(rw - m));
+        else L += lw;
+        M = m;
+      }
+    }
+    if (lane == 0) fin[q] = make_float2(M > -INFINITY ? M : 0.f, L == 0.f ? 0.f : 1.0f / L);
   }
+  __syncthreads();
+  if (s >= nsb * 16 || s >= a.S) return;
+  float top = 0.f;
+  bool nan = false;
+  for (int h = 0; h < Hkv; ++h) {
+    const float* x = a.logits + (static_cast<size_t>(b * Hkv + h) * a.s16 + s) * a.gs;
+    for (int w = 0; w < group; ++w) {
+      const float2 f = fin[h * group + w];
+      const float p = ex2(x[w] - f.x) * f.y;
+      nan |= p != p;
+      top = fmaxf(top, p);
+    }
+  }
+  if (nan) set_err(a.err, kErrNanScore);
+  float* dst = a.step_score + static_cast<size_t>(b) * a.S + s;
+  if (top > *dst) *dst = top;
+}
+
+static int floats_per_row(int group) { return group <= 2 ? 2 : group <= 4 ? 4 : 8; }
+
+// Sequences per launch: their lengths fit shared memory and the line of blocks 32 bits.
+static int seqs_per_launch(int B, int Hkv, int limit) {
+  const long long line = static_cast<long long>(Hkv) * ((limit + 15) / 16);
+  long long n = kMaxSeqs;
+  if (line * n > 0x7fff0000ll) n = 0x7fff0000ll / line;
+  return static_cast<int>(n < B ? n : B);
+}
+
+static long long workspace_bytes(int B, int Hq, int Hkv, int limit, bool score) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || limit < 0) return 0;
+  long long n = kHeaderBytes + kPartBytes;
+  if (score) {
+    const long long pairs = static_cast<long long>(seqs_per_launch(B, Hkv, limit)) * Hkv;
+    n += pairs * 64 + pairs * ((limit + 15ll) / 16 * 16) * floats_per_row((Hq + Hkv - 1) / Hkv) * 4;
+  }
+  return n;
+}
+
+static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const void* q, const int* lens,
+                  const int* slot_pos, int S, float scale, void* out, float* step_score, void* ws, long long ws_bytes,
+                  int* err) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return fail(kStatusCuda, "kv4_attn: no CUDA device");
+  cudaError_t e = cudaFuncSetAttribute(attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
+  if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn: %s", cudaGetErrorString(e));
+  const int Hkv = pool.Hkv, group = Hq / Hkv;
+  long long limit = static_cast<long long>(pool.max_pages) * pool.page;
+  if ((slot_pos || step_score) && S < limit) limit = S;
+  const int each = seqs_per_launch(B, Hkv, static_cast<int>(limit));
+  if (each <= 0) return fail(kStatusUnsupported, "kv4_attn: too many heads and slots");
+  if (ws_bytes < workspace_bytes(B, Hq, Hkv, static_cast<int>(limit), step_score != nullptr))
+    return fail(kStatusArg, "kv4_attn: workspace of %lld bytes is too small", ws_bytes);
+  const int nsb = static_cast<int>((limit + 15) / 16);
+  for (int b0 = 0; b0 < B; b0 += each) {
+    AttnArgs a;
+    a.q = static_cast<const __nv_bfloat16*>(q) + static_cast<size_t>(b0) * Hq * 128;
+    a.pool = pool;
+    a.pool.B = B - b0 < each ? B - b0 : each;
+    a.pool.table = pool.table + static_cast<size_t>(b0) * pool.max_pages;
+    a.lens = lens + b0;
+    a.slot_pos = slot_pos ? slot_pos + static_cast<size_t>(b0) * S : nullptr;
+    a.out = static_cast<__nv_bfloat16*>(out) + static_cast<size_t>(b0) * Hq * 128;
+    a.step_score = step_score ? step_score + static_cast<size_t>(b0) * S : nullptr;
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    a.header = reinterpret_cast<int*>(w);
+    a.part = reinterpret_cast<float*>(w + kHeaderBytes);
+    a.stats = step_score ? reinterpret_cast<float*>(w + kHeaderBytes + kPartBytes) : nullptr;
+    a.logits = step_score ? a.stats + static_cast<size_t>(each) * Hkv * 16 : nullptr;
+    a.err = err;
+    a.scale = scale;
+    a.Hq = Hq;
+    a.S = S;
+    a.limit = static_cast<int>(limit);
+    a.s16 = nsb * 16;
+    a.gs = floats_per_row(group);
+    const long long line = static_cast<long long>(a.pool.B) * Hkv * nsb;
+    long long grid = (line + kMinBlocks - 1) / kMinBlocks;
+    const int most = 2 * sms < kMaxCtas ? 2 * sms : kMaxCtas;
+    grid = grid < 1 ? 1 : grid > most ? most : grid;
+    e = launch_pdl(attend_kernel, dim3(static_cast<unsigned>(grid)), dim3(kWarps * 32), sizeof(Smem), stream, dim3(0), a);
+    if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
+    const int chunks = step_score ? (nsb * 16 + 255) / 256 : 0;
+    e = launch_pdl(combine_kernel, dim3(Hkv + chunks, a.pool.B), dim3(256), step_score ? Hq * sizeof(float2) : 0, stream,
+                   dim3(0), a);
+    if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
+  }
+  return kStatusOk;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -415,8 +954,7 @@ extern "C" int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_
 }
 
 extern "C" int64_t kvbp_kv4_attn_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t max_slots, int32_t with_score) {
-  (void)B, (void)Hq, (void)Hkv, (void)max_slots, (void)with_score;
-  return 16;
+  return kv4::workspace_bytes(B, Hq, Hkv, max_slots, with_score != 0);
 }
 
 extern "C" int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_t Hkv, int32_t head_dim,
@@ -427,19 +965,13 @@ extern "C" int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_
   kv4::Pool p;
   if (int st = kv4::make_pool("kv4_attn", B, Hkv, head_dim, page_size, n_pages, max_pages, pool, page_table, &p))
     return st;
-  if (!q || !lens || !out) return fail(kvbp::kStatusArg, "kv4_attn: null pointer");
+  if (!q || !lens || !out || !workspace) return fail(kvbp::kStatusArg, "kv4_attn: null pointer");
   if (Hq <= 0 || Hq % Hkv) return fail(kvbp::kStatusArg, "kv4_attn: Hq must be a multiple of Hkv");
   if (Hq / Hkv > 8) return fail(kvbp::kStatusUnsupported, "kv4_attn: query group %d > 8", Hq / Hkv);
+  if (Hq > 4096) return fail(kvbp::kStatusUnsupported, "kv4_attn: %d query heads > 4096", Hq);
   if (S < 0 || ((slot_pos || step_score) && S == 0)) return fail(kvbp::kStatusArg, "kv4_attn: bad slot stride");
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
-    return fail(kvbp::kStatusArg, "kv4_attn: q and out must be 16-byte aligned");
-  if (B > 65535 || Hkv > 65535) return fail(kvbp::kStatusArg, "kv4_attn: bad size");
-  int limit = max_pages * page_size;
-  if ((slot_pos || step_score) && S < limit) limit = S;
-  const cudaError_t e = kvbp::launch_pdl(
-      kv4::attend_kernel<8>, dim3(Hkv, B), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0),
-      static_cast<const __nv_bfloat16*>(q), p, lens, slot_pos, S, limit, scale, Hq, static_cast<__nv_bfloat16*>(out),
-      step_score, dev_err);
-  if (e != cudaSuccess) return fail(kvbp::kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
-  return kvbp::kStatusOk;
+  if (!kv4::aligned16(q) || !kv4::aligned16(out) || !kv4::aligned16(workspace))
+    return fail(kvbp::kStatusArg, "kv4_attn: q, out and the workspace must be 16-byte aligned");
+  return kv4::attend(reinterpret_cast<cudaStream_t>(stream), B, Hq, p, q, lens, slot_pos, S, scale, out, step_score,
+                     workspace, workspace_bytes, dev_err);
 }

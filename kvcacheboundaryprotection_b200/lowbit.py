@@ -80,8 +80,6 @@ def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) ->
 def _pool(pool: torch.Tensor, table: torch.Tensor) -> tuple:
     """(pages, kv heads, page size, sequences, pages per sequence) after the checks."""
     dev = pool.device
-    if dev.type != "cuda":
-        raise ValueError("the low-bit operators run on CUDA devices only")
     _need(pool, "pool", torch.uint8, dev, (None, None, None, BLOCK))
     _need(table, "page_table", torch.int32, dev, (None, None))
     return pool.shape[0], pool.shape[1], pool.shape[2] * 16, table.shape[0], table.shape[1]
@@ -230,8 +228,8 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
 
 
 def _matrix(x: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    if x.dim() != 2 or x.dtype is not dtype or x.device.type != "cuda":
-        raise ValueError(f"{name} must be a {dtype} matrix on a CUDA device")
+    if x.dim() != 2 or x.dtype is not dtype:
+        raise ValueError(f"{name} must be a {dtype} matrix")
     if x.shape[0] and x.shape[1] and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         raise ValueError(f"{name}'s columns must be contiguous and its rows must not overlap")
 
