@@ -144,6 +144,8 @@ SIGNATURES = {
     ),
     "kvbp_int8_quant_rows": (C.c_int, [P, I32, I32, P, I64, P, I64, P]),
     "kvbp_int8_gemm": (C.c_int, [P, I32, I32, I32, I32, P, I64, P, P, I64, P, P, P, I64, P]),
+    "kvbp_int8_linear_workspace": (I64, [I32, I32]),
+    "kvbp_int8_linear": (C.c_int, [P, I32, I32, I32, I32, P, I64, P, P, I64, P, P, I64, P, I64, P]),
 }
 EXTRA_SIGNATURES = {
     "kvbp_decode_attn_score_cs": (C.c_int, [P, I32, I32, I32, I32, I32, P, P, P, P, P, P, P, P, I32]),

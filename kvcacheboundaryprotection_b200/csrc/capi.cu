@@ -4,6 +4,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "../../include/kvbp.h"
 #include "kvbp_internal.h"
 
@@ -17,6 +19,26 @@ int fail(int status, const char* fmt, ...) {
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
   return status;
+}
+
+int prepare_device(const void* kernel, int smem) {
+  struct Entry {
+    const void* kernel;
+    int dev, sms;
+  };
+  static std::mutex lock;
+  static Entry seen[256];
+  static int n = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::lock_guard<std::mutex> hold(lock);
+  for (int i = 0; i < n; ++i)
+    if (seen[i].kernel == kernel && seen[i].dev == dev) return seen[i].sms;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  if (n < 256) seen[n++] = Entry{kernel, dev, sms};
+  return sms;
 }
 
 }  // namespace kvbp

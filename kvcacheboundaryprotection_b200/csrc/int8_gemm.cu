@@ -17,8 +17,10 @@ constexpr int kVec = 8;
 __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int K,
                                                          int vec, int8_t* __restrict__ q, long long ldq,
                                                          float* __restrict__ scale) {
-  pdl_launch_dependents();
   pdl_wait();
+  // only now: what runs before this kernel is complete when a dependent starts, so
+  // kvbp_int8_linear's product may fetch weights before it waits for the codes
+  pdl_launch_dependents();
   __shared__ uint32_t red[8];
   const size_t r = blockIdx.x;
   const int tid = threadIdx.x;
@@ -67,19 +69,41 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
   for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(code(__bfloat162float(row[i])));
 }
 
+// ---- the product on the 5th-generation tensor cores (tcgen05.mma kind::i8) -------------
+// The weight block is the M = 128 operand and the tokens the N = NT one, both K-major int8
+// tiles of 128 bytes of K fetched by 2-D TMA with the 128-byte swizzle (rows and columns
+// past the matrices arrive as zeros: sizes are free); the accumulator is int32 in TMEM, lane =
+// output channel, column = token, so a warp's stores of one token's 32 channels are contiguous.
+// Integer sums are exact, so K may be split and joined in any order with the same bits.
 struct Args {
-  const int8_t* w;
-  long long ldw;
   const float* sw;
-  const int8_t* xq;
-  long long ldq;
   const float* sx;
   const __nv_bfloat16* bias;
   void* out;
   long long ldo;
   int M, N, K, f32;
+  int early;  // the weight is known to be complete before the kernel before this one ends
+  int* err;
 };
 
+constexpr int kBK = 128;               // bytes (= codes) of K per stage: one swizzle atom
+constexpr int kTileW = 128 * kBK;      // weight tile
+constexpr int kThreads = 6 * 32;       // producer, MMA, four epilogue warps
+
+__host__ __device__ constexpr uint32_t idesc_i8(int N) {  // D s32, A and B s8, both K-major, M = 128
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ int ld_dsmem_s32(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void store(const Args& a, int m, int n, int acc, float sx, float sw, float bias) {
   const float y = static_cast<float>(acc) * sx * sw + bias;
   const size_t at = static_cast<size_t>(m) * a.ldo + n;
@@ -88,40 +112,360 @@ __device__ __forceinline__ void store(const Args& a, int m, int n, int acc, floa
   else
     static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
 }
+// Barrier among ``nthreads`` threads; true on all of them when ``v`` is on any.
+__device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
+// this thread's 16 or 32 accumulator columns from TMEM
+template <int C>
+__device__ __forceinline__ void ld_acc(uint32_t taddr, int (&v)[C]) {
+  float f[C];
+  if constexpr (C == 32) tc_ld32(taddr, f);
+  else tc_ld16(taddr, f);
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = __float_as_int(f[i]);
+}
 
-// 64 x 64 output tile per CTA, 64-byte K steps in shared memory, dp4a.
-__global__ void __launch_bounds__(256) gemm_kernel(const Args a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ int sx[64][17], sw[64][17];
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tid = threadIdx.x;
-  const int tm = tid / 16, tn = tid % 16;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    for (int i = tid; i < 64 * 16; i += 256) {
-      const int r = i / 16, k = k0 + (i % 16) * 4;
-      uint32_t vx = 0, vw = 0;
-      for (int e = 0; e < 4; ++e) {
-        if (k + e < a.K && m0 + r < a.M) vx |= static_cast<uint32_t>(static_cast<uint8_t>(a.xq[static_cast<size_t>(m0 + r) * a.ldq + k + e])) << (8 * e);
-        if (k + e < a.K && n0 + r < a.N) vw |= static_cast<uint32_t>(static_cast<uint8_t>(a.w[static_cast<size_t>(n0 + r) * a.ldw + k + e])) << (8 * e);
-      }
-      sx[r][i % 16] = static_cast<int>(vx);
-      sw[r][i % 16] = static_cast<int>(vw);
+// One output tile (128 channels x NT tokens) per cluster; the cluster's CTAs share the tile's
+// K range (gridDim.x = cluster size) and join their int32 partial tiles over distributed shared
+// memory.  Bound by the weight stream when tokens are few: stages are sized for two CTAs per SM.
+template <int NT>
+struct Ring {
+  static constexpr int kStage = kTileW + NT * kBK;
+  static constexpr int kStages = (NT <= 32 ? 5 : NT == 64 ? 4 : 3);
+  static constexpr int kBytes = kStages * kStage + 1024 + 256;
+  static_assert(kStages * kStage >= NT * 128 * 4, "the partial tile reuses the ring");
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, 2)
+    split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a) {
+  using R = Ring<NT>;
+  constexpr int kCols = NT < 32 ? 32 : NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + R::kStages * R::kStage);
+  uint64_t* empty = full + R::kStages;
+  uint64_t* done = empty + R::kStages;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+  int* bad = reinterpret_cast<int*>(tslot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = gridDim.x, rank = blockIdx.x;
+  const int n0 = blockIdx.y * 128, m0 = blockIdx.z * NT;
+  const int steps = (a.K + kBK - 1) / kBK;
+  const int k0 = static_cast<int>(static_cast<long long>(rank) * steps / S);
+  const int nk = static_cast<int>(static_cast<long long>(rank + 1) * steps / S) - k0;
+
+  if (tid == 0) {
+    for (int s = 0; s < R::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    __syncthreads();
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sx[tm + 16 * i][k], sw[tn + 16 * j][k], acc[i][j]);
-    __syncthreads();
+    mbar_init(done, 1);
+    *bad = 0;
+    fence_barrier_init();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-      if (m < a.M && n < a.N)
-        store(a, m, n, acc[i][j], a.sx[m], a.sw[n], a.bias ? __bfloat162float(a.bias[n]) : 0.f);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *tslot;
+  auto healthy = [&]() { return !*reinterpret_cast<volatile int*>(bad); };
+  auto wait_or_fail = [&](uint64_t* bar, uint32_t ph) {
+    if (mbar_wait_bounded(bar, ph)) return true;
+    set_err(a.err, kErrWaitTimeout);
+    atomicExch(bad, 1);
+    return false;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&wmap);
+      prefetch_tmap(&xmap);
+      if (!a.early) pdl_wait();
+      auto load_w = [&](int u) {
+        const int st = u % R::kStages;
+        mbar_expect_tx(&full[st], R::kStage);
+        tma_load_2d(base + st * R::kStage, &wmap, &full[st], (k0 + u) * kBK, n0);
+      };
+      auto load_x = [&](int u) {
+        const int st = u % R::kStages;
+        tma_load_2d(base + st * R::kStage + kTileW, &xmap, &full[st], (k0 + u) * kBK, m0);
+      };
+      const int first = nk < R::kStages ? nk : R::kStages;
+      for (int u = 0; u < first; ++u) load_w(u);
+      if (a.early) pdl_wait();  // the tokens' codes come from the kernel before this one
+      for (int u = 0; u < first; ++u) load_x(u);
+      int issued = first;
+      for (int u = first; u < nk && healthy(); ++u, ++issued) {
+        if (!wait_or_fail(&empty[u % R::kStages], static_cast<uint32_t>(u / R::kStages - 1) & 1)) break;
+        load_w(u);
+        load_x(u);
+      }
+      pdl_launch_dependents();
+      if (!healthy())  // let the copies in flight land before the CTA can exit
+        for (int u = issued > R::kStages ? issued - R::kStages : 0; u < issued; ++u)
+          mbar_wait_bounded(&full[u % R::kStages], static_cast<uint32_t>(u / R::kStages) & 1, 1u << 16);
     }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int u = 0; u < nk && healthy(); ++u) {
+        const int st = u % R::kStages;
+        if (!wait_or_fail(&full[st], static_cast<uint32_t>(u / R::kStages) & 1)) break;
+        tc_after();
+        const uint32_t sw = smem_u32(base + st * R::kStage), sx = sw + kTileW;
+#pragma unroll
+        for (int ks = 0; ks < kBK / 32; ++ks)
+          mma_i8(tmem, tc_sdesc(sw + ks * 32), tc_sdesc(sx + ks * 32), idesc_i8(NT), (u > 0 || ks > 0) ? 1u : 0u);
+        tc_commit(&empty[st]);
+      }
+      tc_commit(done);
+    }
+    __syncwarp();
+  }
+  const bool ok = wait_or_fail(done, 0) && healthy();
+  tc_after();
+  pdl_wait();  // before the scales are read and anything is written
+  const bool all_ok = !__syncthreads_or(!ok);
+  const int cols = min(NT, a.M - m0);  // live tokens of the tile
+  int* part = reinterpret_cast<int*>(base);  // [token][128 channels], over the drained ring
+  if (warp >= 2 && all_ok) {
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const int ch = q * 32 + lane, n = n0 + ch;
+    const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    constexpr int C = NT < 32 ? 16 : 32;
+    const float sw = n < a.N ? a.sw[n] : 0.f;
+    const float bias = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < NT && c < cols; c += C) {
+      int v[C];
+      ld_acc<C>(acc + c, v);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (c + i >= cols) break;
+        if (S > 1) part[(c + i) * 128 + ch] = v[i];
+        else if (n < a.N) store(a, m0 + c + i, n, v[i], a.sx[m0 + c + i], sw, bias);
+      }
+    }
+  }
+  if (S > 1) {
+    cluster_sync_all();
+    // this CTA's share of the tile's live elements
+    const int E = cols * 128, e1 = static_cast<int>(static_cast<long long>(rank + 1) * E / S);
+    if (all_ok)
+      for (int e = static_cast<int>(static_cast<long long>(rank) * E / S) + tid; e < e1; e += kThreads) {
+        const uint32_t at = smem_u32(part + e);
+        int sum = 0;
+#pragma unroll 8
+        for (int r = 0; r < S; ++r) sum += ld_dsmem_s32(mapa_u32(at, r));
+        const int m = m0 + (e >> 7), n = n0 + (e & 127);
+        if (n < a.N) store(a, m, n, sum, a.sx[m], a.sw[n], a.bias ? __bfloat162float(a.bias[n]) : 0.f);
+      }
+    cluster_sync_all();  // no CTA leaves while a peer may still read its part
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+}
+
+// Many tokens: persistent, one CTA per SM over 128 x 256 tiles in a grouped raster, a ring of
+// four 48 KiB stages that runs on across tiles, and two accumulators in TMEM so that the MMAs
+// of one tile run while the epilogue warps drain the other.
+constexpr int kPN = 256;
+constexpr int kPStages = 4;
+constexpr int kPStage = kTileW + kPN * kBK;
+constexpr int kPBytes = kPStages * kPStage + 1024 + 256 + 2 * kPN * 4;
+constexpr int kBand = 16;  // channel tiles per raster band
+
+__global__ void __launch_bounds__(kThreads, 1)
+    persist_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sxs = reinterpret_cast<float*>(base + kPStages * kPStage);  // [2][kPN] token scales of a tile
+  uint64_t* full = reinterpret_cast<uint64_t*>(sxs + 2 * kPN);
+  uint64_t* empty = full + kPStages;
+  uint64_t* accfull = empty + kPStages;
+  uint64_t* accempty = accfull + 2;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(accempty + 2);
+  int* bad = reinterpret_cast<int*>(tslot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tn = (a.N + 127) / 128, tm = (a.M + kPN - 1) / kPN;
+  const long long tiles = static_cast<long long>(tn) * tm;
+  const int steps = (a.K + kBK - 1) / kBK;
+  // tile t: bands of kBand channel tiles, tokens the slow index within a band
+  auto tile_of = [&](long long t, int& n0, int& m0) {
+    const long long per = static_cast<long long>(kBand) * tm;
+    const int band = static_cast<int>(t / per);
+    const int in = static_cast<int>(t - band * per), width = min(kBand, tn - band * kBand);
+    n0 = (band * kBand + in % width) * 128;
+    m0 = in / width * kPN;
+  };
+  if (tid == 0) {
+    for (int s = 0; s < kPStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&accempty[b], 4);
+    }
+    *bad = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(2 * kPN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *tslot;
+  auto healthy = [&]() { return !*reinterpret_cast<volatile int*>(bad); };
+  auto wait_or_fail = [&](uint64_t* bar, uint32_t ph) {
+    if (mbar_wait_bounded(bar, ph)) return true;
+    set_err(a.err, kErrWaitTimeout);
+    atomicExch(bad, 1);
+    return false;
+  };
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&wmap);
+      prefetch_tmap(&xmap);
+      long long g = 0;
+      for (long long t = blockIdx.x; t < tiles && healthy(); t += gridDim.x) {
+        int n0, m0;
+        tile_of(t, n0, m0);
+        for (int u = 0; u < steps; ++u, ++g) {
+          const int st = static_cast<int>(g % kPStages);
+          if (g >= kPStages && !wait_or_fail(&empty[st], static_cast<uint32_t>(g / kPStages - 1) & 1)) break;
+          if (!healthy()) break;
+          mbar_expect_tx(&full[st], kPStage);
+          tma_load_2d(base + st * kPStage, &wmap, &full[st], u * kBK, n0);
+          tma_load_2d(base + st * kPStage + kTileW, &xmap, &full[st], u * kBK, m0);
+        }
+      }
+      pdl_launch_dependents();
+      if (!healthy())
+        for (long long u = g > kPStages ? g - kPStages : 0; u < g; ++u)
+          mbar_wait_bounded(&full[u % kPStages], static_cast<uint32_t>(u / kPStages) & 1, 1u << 16);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      long long g = 0;
+      int i = 0;
+      for (long long t = blockIdx.x; t < tiles && healthy(); t += gridDim.x, ++i) {
+        const int buf = i & 1;
+        if (i >= 2 && !wait_or_fail(&accempty[buf], static_cast<uint32_t>((i >> 1) - 1) & 1)) break;
+        tc_after();
+        const uint32_t acc = tmem + static_cast<uint32_t>(buf * kPN);
+        bool ok = true;
+        for (int u = 0; u < steps; ++u, ++g) {
+          const int st = static_cast<int>(g % kPStages);
+          if (!wait_or_fail(&full[st], static_cast<uint32_t>(g / kPStages) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_after();
+          const uint32_t sw = smem_u32(base + st * kPStage), sx = sw + kTileW;
+#pragma unroll
+          for (int ks = 0; ks < kBK / 32; ++ks)
+            mma_i8(acc, tc_sdesc(sw + ks * 32), tc_sdesc(sx + ks * 32), idesc_i8(kPN), (u > 0 || ks > 0) ? 1u : 0u);
+          tc_commit(&empty[st]);
+        }
+        if (!ok) break;
+        tc_commit(&accfull[buf]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, et = tid - 64;  // 128 epilogue threads
+    int i = 0;
+    for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+      const int buf = i & 1;
+      int n0, m0;
+      tile_of(t, n0, m0);
+      const int n = n0 + q * 32 + lane, cols = min(kPN, a.M - m0);
+      for (int c = et; c < kPN; c += 128) sxs[buf * kPN + c] = c < cols ? a.sx[m0 + c] : 0.f;
+      const float sw = n < a.N ? a.sw[n] : 0.f;
+      const float bias = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+      const bool ok = wait_or_fail(&accfull[buf], static_cast<uint32_t>(i >> 1) & 1);
+      tc_after();
+      // the tile's scales are in place, and all four warps leave together after a failed wait
+      if (named_bar_or(1, 128, !ok || !healthy())) break;
+      const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * kPN);
+      const size_t row = static_cast<size_t>(m0) * a.ldo + n;
+#pragma unroll 1
+      for (int c = 0; c < cols; c += 32) {
+        int v[32];
+        ld_acc<32>(acc + c, v);
+        if (n < a.N) {
+          if (a.f32) {
+            float* dst = static_cast<float*>(a.out) + row + static_cast<size_t>(c) * a.ldo;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c + k < cols) dst[k * a.ldo] = static_cast<float>(v[k]) * sxs[buf * kPN + c + k] * sw + bias;
+          } else {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + row + static_cast<size_t>(c) * a.ldo;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c + k < cols)
+                dst[k * a.ldo] = __float2bfloat16_rn(static_cast<float>(v[k]) * sxs[buf * kPN + c + k] * sw + bias);
+          }
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&accempty[buf]);
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kPN));
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// An int8 matrix [rows][ld] as tiles of ``box`` rows x 128 columns, 128-byte swizzled.
+static CUresult tile_map(CUtensorMap* map, const void* p, int rows, int K, long long ld, int box) {
+  static EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  }();
+  if (!fn) return CUDA_ERROR_NOT_FOUND;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t boxes[2] = {kBK, static_cast<cuuint32_t>(box)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+template <int NT>
+static cudaError_t launch_split(cudaStream_t st, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, int S) {
+  if (prepare_device(reinterpret_cast<const void*>(split_kernel<NT>), Ring<NT>::kBytes) <= 0) return cudaErrorNoDevice;
+  const dim3 grid(S, (a.N + 127) / 128, (a.M + NT - 1) / NT);
+  return launch_pdl(split_kernel<NT>, grid, dim3(kThreads), Ring<NT>::kBytes, st, S > 1 ? dim3(S, 1, 1) : dim3(0), wm, xm, a);
 }
 
 static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
@@ -138,14 +482,52 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
   return kStatusOk;
 }
 
-static int gemm(cudaStream_t st, const Args& a) {
-  if (!a.w || !a.sw || !a.xq || !a.sx || !a.out) return fail(kStatusArg, "int8_gemm: null pointer");
-  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.ldw < a.K || a.ldq < a.K || a.ldo < a.N) return fail(kStatusArg, "int8_gemm: bad size");
-  // the sum of K products of up to 127 * 127 (128 * 128 for raw codes) stays in 32 bits
+// CTAs that share a tile's K range: enough to give every SM two CTAs, each at least four
+// stages of K, within a portable cluster.
+static int splits(long long tiles, int steps, int sms) {
+  long long s = 2ll * sms / tiles;
+  if (s > steps / 4) s = steps / 4;
+  return s < 1 ? 1 : s > 8 ? 8 : static_cast<int>(s);
+}
+
+static int check(const Args& a, const void* w, long long ldw, const void* xq, long long ldq) {
+  if (!w || !a.sw || !xq || !a.sx || !a.out) return fail(kStatusArg, "int8_gemm: null pointer");
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || ldw < a.K || ldq < a.K || a.ldo < a.N) return fail(kStatusArg, "int8_gemm: bad size");
+  // the sum of K products of up to 127 * 128 stays in 32 bits
   if (a.K > 131071) return fail(kStatusUnsupported, "int8_gemm: K %d > 131071 could overflow the 32-bit sums", a.K);
-  if (misaligned(a.w, 16) || misaligned(a.xq, 16) || a.ldw % 16 || a.ldq % 16)
+  if (misaligned(w, 16) || misaligned(xq, 16) || ldw % 16 || ldq % 16)
     return fail(kStatusArg, "int8_gemm: w and xq rows must be 16-byte aligned");
-  const cudaError_t e = launch_pdl(gemm_kernel, dim3((a.N + 63) / 64, (a.M + 63) / 64), dim3(256), 0, st, dim3(0), a);
+  if (misaligned(a.out, a.f32 ? 4 : 2)) return fail(kStatusArg, "int8_gemm: misaligned output");
+  if ((a.N + 127) / 128 > 65535) return fail(kStatusUnsupported, "int8_gemm: N %d is too large", a.N);
+  return kStatusOk;
+}
+
+static int gemm(cudaStream_t st, const Args& a, const void* w, long long ldw, const void* xq, long long ldq) {
+  if (int bad = check(a, w, ldw, xq, ldq)) return bad;
+  const int sms = prepare_device(reinterpret_cast<const void*>(persist_kernel), kPBytes);
+  if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
+  const long long tn = (a.N + 127) / 128;
+  const int steps = (a.K + kBK - 1) / kBK;
+  const bool many = tn * ((a.M + kPN - 1) / kPN) >= sms;
+  const int NT = many ? kPN : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  const long long tm = (a.M + NT - 1) / NT;
+  if (!many && tm > 65535) return fail(kStatusUnsupported, "int8_gemm: too many tiles");
+  CUtensorMap wm, xm;
+  CUresult r = tile_map(&wm, w, a.N, a.K, ldw, 128);
+  if (r == CUDA_SUCCESS) r = tile_map(&xm, xq, a.M, a.K, ldq, NT);
+  if (r != CUDA_SUCCESS) return fail(kStatusCuda, "int8_gemm: tensor map failed (%d)", static_cast<int>(r));
+  const int S = splits(tn * tm, steps, sms);
+  cudaError_t e;
+  if (many)
+    e = launch_pdl(persist_kernel, dim3(static_cast<unsigned>(tn * tm < sms ? tn * tm : sms)), dim3(kThreads), kPBytes, st, dim3(0), wm, xm, a);
+  else if (NT == 16)
+    e = launch_split<16>(st, wm, xm, a, S);
+  else if (NT == 32)
+    e = launch_split<32>(st, wm, xm, a, S);
+  else if (NT == 64)
+    e = launch_split<64>(st, wm, xm, a, S);
+  else
+    e = launch_split<128>(st, wm, xm, a, S);
   if (e != cudaSuccess) return fail(kStatusCuda, "int8_gemm launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
@@ -163,8 +545,25 @@ extern "C" int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t 
 extern "C" int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
                               int64_t ldw, const float* w_scale, const void* xq, int64_t ldq, const float* x_scale,
                               const void* bias, void* out, int64_t ldo, int32_t* dev_err) {
-  (void)dev_err;
-  kvbp::i8::Args a{static_cast<const int8_t*>(w), ldw, w_scale, static_cast<const int8_t*>(xq), ldq, x_scale,
-                   static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0};
-  return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a);
+  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, dev_err};
+  return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, xq, ldq);
+}
+
+extern "C" int64_t kvbp_int8_linear_workspace(int32_t M, int32_t K) {
+  return M <= 0 || K <= 0 ? 0 : static_cast<int64_t>(M) * ((K + 15) / 16 * 16) + 4ll * M;
+}
+
+extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
+                                int64_t ldw, const float* w_scale, const void* x, int64_t ldx, const void* bias,
+                                void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, int32_t* dev_err) {
+  if (!workspace) return kvbp::fail(kvbp::kStatusArg, "int8_linear: null pointer");
+  if (workspace_bytes < kvbp_int8_linear_workspace(M, K))
+    return kvbp::fail(kvbp::kStatusArg, "int8_linear: workspace of %lld bytes is too small", static_cast<long long>(workspace_bytes));
+  const int64_t ldq = (static_cast<int64_t>(K) + 15) / 16 * 16;
+  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + ldq * M);
+  // the product's arguments first: a refused call leaves the workspace alone
+  const kvbp::i8::Args a{w_scale, scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 1, dev_err};
+  if (int st = kvbp::i8::check(a, w, ldw, workspace, ldq)) return st;
+  if (int st = kvbp_int8_quant_rows(stream, M, K, x, ldx, workspace, ldq, scale)) return st;
+  return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, workspace, ldq);
 }

@@ -242,8 +242,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
 //    code's own, and its sums came out 2^-16 off.)
 //  * scales never touch the codes: K's multiply the four group sums in fp32, V's multiply the
 //    softmax weights (P' = P * scale, f16, rounded at 2^-11: half a bf16 output step is 2^-9).
-// P is 2^(x - ref) with ref = max(x) - e, e chosen from the tile's largest V scale so that
-// P * scale <= 2^14: f16 keeps 11 bits of P' over its whole range whatever V's magnitude.
+// P is 2^(x - ref) with ref = max(x) - e, e chosen from the exponents of the tile's V scales so
+// that P * scale < 2^14: P' keeps f16's 11 bits far below the largest weight whatever V's
+// magnitude (to 2^-29 of it for scales below 1).
 // q is brought to [2^14, 2^15) by a power of two for the same reason (exact: q is bf16).
 // A masked slot's logit is -inf and its V scale zero, so nothing it holds (NaN scales of
 // never-written memory included) reaches a sum; codes are finite whatever their bits.
@@ -412,8 +413,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
   const int end = min(total - start, R) + start;
   if (start >= end) return;
 
-  // -- the stage to be issued next: found one stage ahead, so that its page and mask loads
-  //    are not waited for
+  // -- the stage to be issued next is found one stage ahead, so that its page and mask loads
+  //    are not waited for; lane i < cnt follows the stage's block i (page index pi, block
+  //    ``inner`` of the page), which moves by whole turns of the warps within a segment
+  const int ppb = a.pool.page >> 4;  // blocks per page
+  const size_t page_bytes = static_cast<size_t>(Hkv) * ppb * kBlock;
+  constexpr int kTurn = kWarps * kStageBlocks;
+  const int turn_pages = kTurn / ppb, turn_inner = kTurn - turn_pages * ppb;
   Segment is;
   {
     int lo = 0, hi = a.pool.B - 1;  // the last sequence that starts at or before ``start``
@@ -426,43 +432,54 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
   }
   is.at(sm, Hkv, start, end);
   Segment cs = is;
-  int ipos = start, iturn = 0;
+  int ipos = start, left = 0;  // left: blocks of the segment from this warp's next stage on
   bool have = false, live = false;
-  int cnt = 0, sb = 0, ih = 0, page = -1, inner = 0;
+  int slot = 0, pi = 0, inner = 0, cnt = 0, page = -1, in_page = 0, is_len = 0;
+  const uint8_t* ihead = nullptr;
+  const uint8_t* iaddr = nullptr;
+  const int* itable = nullptr;
+  const int* islots = nullptr;
+  auto enter = [&]() {  // this warp's first stage of segment ``is``
+    const int per = is.per(), k = warp * per;
+    left = is.n - k;
+    slot = (is.sb0 + k) * 16 + lane;
+    const int blk = is.sb0 + k + (lane < kStageBlocks ? lane : 0);
+    pi = blk / ppb;
+    inner = blk - pi * ppb;
+    is_len = sm.len[is.b];
+    ihead = a.pool.base + static_cast<size_t>(is.h) * ppb * kBlock;
+    itable = a.pool.table + static_cast<size_t>(is.b) * a.pool.max_pages;
+    islots = a.slot_pos ? a.slot_pos + static_cast<size_t>(is.b) * a.S : nullptr;
+  };
   auto fetch = [&]() {
-    for (;;) {
-      const int per = is.per(), k = (warp + kWarps * iturn) * per;
-      if (k < is.n) {
-        ++iturn;
-        cnt = min(per, is.n - k);
-        sb = is.sb0 + k;
-        ih = is.h;
-        page = -1;
-        const int slot = sb * 16 + lane;
-        live = lane < cnt * 16 && slot < sm.len[is.b];
-        if (live && a.slot_pos) live = a.slot_pos[static_cast<size_t>(is.b) * a.S + slot] >= 0;
-        if (lane < cnt) {
-          const int s = (sb + lane) * 16, pi = s / a.pool.page;
-          inner = (s - pi * a.pool.page) >> 4;
-          page = a.pool.table[static_cast<size_t>(is.b) * a.pool.max_pages + pi];
-        }
-        have = true;
-        return;
-      }
+    while (left <= 0) {
       ipos += is.n;
       if (ipos >= end) {
         have = false;
         return;
       }
       is.at(sm, Hkv, ipos, end);
-      iturn = 0;
+      enter();
     }
+    const int per = is.per();
+    cnt = min(per, left);
+    live = lane < cnt * 16 && slot < is_len;
+    if (live && islots) live = islots[slot] >= 0;
+    page = lane < cnt ? itable[pi] : -1;
+    in_page = inner;
+    iaddr = ihead;
+    have = true;
+    left -= kWarps * per;  // a segment of one-block stages has one turn only
+    slot += kTurn * 16;
+    pi += turn_pages;
+    inner += turn_inner;
+    if (inner >= ppb) inner -= ppb, ++pi;
   };
   auto issue = [&](int st) {
     if (!have) return;
-    const bool ok = lane < cnt && page >= 0 && page < a.pool.n_pages;
-    if (lane < cnt && !ok) set_err(a.err, kErrIndex);
+    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.n_pages);
     const uint32_t okm = __ballot_sync(0xffffffffu, ok);
+    if (okm != (1u << cnt) - 1u && lane < cnt && !ok) set_err(a.err, kErrIndex);
     const uint32_t mask = __ballot_sync(0xffffffffu, live && ((okm >> (lane >> 4)) & 1u));
     if (lane == 0) {
       sm.mask[warp][st] = mask;
@@ -470,10 +487,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
     }
     __syncwarp();
     if (ok)
-      bulk_load(sm.ring[warp][st] + lane * kBlock,
-                a.pool.base + ((static_cast<size_t>(page) * Hkv + ih) * (a.pool.page >> 4) + inner) * kBlock, kBlock,
+      bulk_load(sm.ring[warp][st] + lane * kBlock, iaddr + page * page_bytes + in_page * kBlock, kBlock,
                 &sm.full[warp][st]);
   };
+  enter();
   fetch();
 #pragma unroll
   for (int s = 0; s < kStages; ++s) {
@@ -531,6 +548,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
       for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
 
     const int per = cs.per();
+    float* lg = a.logits && 2 * t < a.gs
+                    ? a.logits + (static_cast<size_t>(cs.b * Hkv + cs.h) * a.s16 + cs.sb0 * 16 + sg) * a.gs + 2 * t
+                    : nullptr;
     for (int k = warp * per; k < cs.n; k += kWarps * per) {
       const int nb = min(per, cs.n - k);
       if (!dead && !__all_sync(0xffffffffu, mbar_wait_bounded(&sm.full[warp][st], phase))) {
@@ -543,8 +563,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
       const uint32_t mask = dead ? 0u : sm.mask[warp][st];
       const uint8_t* base = sm.ring[warp][st];
       float x[kStageBlocks][4];
-      uint32_t sv_top = 0;
-      float* lg = a.logits ? a.logits + (static_cast<size_t>(cs.b * Hkv + cs.h) * a.s16 + (cs.sb0 + k) * 16) * a.gs : nullptr;
+      const bool all = mask == 0xffffffffu;  // every slot of a whole stage is live
 #pragma unroll
       for (int bl = 0; bl < kStageBlocks; ++bl) {
         if (bl < nb) {
@@ -570,46 +589,46 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
             y[2] += a1 * c[2];
             y[3] += a1 * c[3];
           }
-          const bool v0 = (mask >> (16 * bl + sg)) & 1u, v1 = (mask >> (16 * bl + sg + 2)) & 1u;
-          x[bl][0] = v0 ? y[0] * xs[0] : -INFINITY;
-          x[bl][1] = v0 ? y[1] * xs[1] : -INFINITY;
-          x[bl][2] = v1 ? y[2] * xs[0] : -INFINITY;
-          x[bl][3] = v1 ? y[3] * xs[1] : -INFINITY;
-          if (lg && 2 * t < a.gs) {
-            *reinterpret_cast<float2*>(lg + (16 * bl + sg) * a.gs + 2 * t) = make_float2(x[bl][0], x[bl][1]);
-            *reinterpret_cast<float2*>(lg + (16 * bl + sg + 2) * a.gs + 2 * t) = make_float2(x[bl][2], x[bl][3]);
+          x[bl][0] = y[0] * xs[0];
+          x[bl][1] = y[1] * xs[1];
+          x[bl][2] = y[2] * xs[0];
+          x[bl][3] = y[3] * xs[1];
+          if (!all) {
+            const uint32_t m = mask >> (16 * bl + sg);
+            if (!(m & 1u)) x[bl][0] = x[bl][1] = -INFINITY;
+            if (!(m & 4u)) x[bl][2] = x[bl][3] = -INFINITY;
+          }
+          if (lg) {
+            float* to = lg + (k + bl) * 16 * a.gs;
+            *reinterpret_cast<float2*>(to) = make_float2(x[bl][0], x[bl][1]);
+            *reinterpret_cast<float2*>(to + 2 * a.gs) = make_float2(x[bl][2], x[bl][3]);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[bl][e] = -INFINITY;
         }
       }
-      // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3): zero where masked
-      uint32_t keep[kStageBlocks][2];
+      // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3), zero where
+      // masked (the memory may hold anything).  Their exponent fields or-ed together are at
+      // least the largest: e only has to be small enough, and it stays above -4.
+      uint4 sv[kStageBlocks][2];
+      uint32_t bits = 0;
 #pragma unroll
       for (int bl = 0; bl < kStageBlocks; ++bl)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
-          keep[bl][h] = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-        }
-      auto v_scales = [&](int bl, int h) {
-        uint4 v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
-        v.x &= keep[bl][h], v.y &= keep[bl][h], v.z &= keep[bl][h], v.w &= keep[bl][h];
-        return v;
-      };
-#pragma unroll
-      for (int bl = 0; bl < kStageBlocks; ++bl)
-        if (bl < nb)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 v = v_scales(bl, h);  // non-negative halves: their bits order like their values
-            sv_top = __vmaxu2(sv_top, __vmaxu2(__vmaxu2(v.x, v.y), __vmaxu2(v.z, v.w)));
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (bl < nb) v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
+          if (!all) {
+            const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
+            const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+            v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
           }
-      sv_top = max(sv_top & 0xffffu, sv_top >> 16);
-      sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 1));
-      sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 2));
-      const int e = min(15, 28 - static_cast<int>((sv_top >> 10) & 31u));  // P * scale < 2^14
+          sv[bl][h] = v;
+          bits |= v.x | v.y | v.z | v.w;
+        }
+      bits = __reduce_or_sync(0xffffffffu, bits);
+      const int e = min(15, 28 - static_cast<int>(((bits | bits >> 16) >> 10) & 31u));  // P * scale < 2^14
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -636,7 +655,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
         l[1] += p1 + p3;
         const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
         const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
-        const uint4 s0 = v_scales(bl, 0), s1 = v_scales(bl, 1);
+        const uint4 s0 = sv[bl][0], s1 = sv[bl][1];
         const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t);
         const uint4 v1 = *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t);
         const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb4[4] = {s1.x, s1.y, s1.z, s1.w};
@@ -722,18 +741,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
 
 // Finishes what the streaming kernel left: CTAs x < Hkv join the parts of head (x, sequence)
 // (or write zeros for an empty sequence); the others form the eviction score of 256 slots of
-// a sequence from the logits and the final (ref, sum) of its heads.  Latency-bound: one launch.
+// a sequence from the logits and the final (ref, sum) of its heads.  One launch for both:
+// they are short and latency-bound, so loads are issued as early and as many as possible.
 __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ float2 fin[];  // (ref, 1 / sum) of every query head of the sequence
   const int Hkv = a.pool.Hkv, group = a.Hq / Hkv, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int R = a.header[0], first = a.header[2 + b], nsb = (a.header[2 + b + 1] - first) / Hkv;
-  // parts of head h: CTAs c0 .. c1, in the first slot of each but the one it starts inside
-  auto part_of = [&](int c, int s0) { return a.part + (static_cast<size_t>(c) * 2 + (c * static_cast<long long>(R) >= s0 ? 0 : 1)) * kPart; };
+  // the part of head (b, h), first block s0, that CTA c left: in the CTA's first place where
+  // the CTA's range starts inside the head
+  auto part_of = [&](int c, int s0) {
+    return a.part + (static_cast<size_t>(c) * 2 + (c * static_cast<long long>(R) >= s0 ? 0 : 1)) * kPart;
+  };
+  auto join = [](float& M, float& L, float m, float l) {  // (M, L) += (m, l)
+    const float top = fmaxf(M, m);
+    L = L * (M == top ? 1.0f : ex2(M - top)) + l * (m == top ? 1.0f : ex2(m - top));
+    M = top;
+  };
   if (static_cast<int>(blockIdx.x) < Hkv) {
     const int h = blockIdx.x;
-    if (warp >= group) return;
+    if (warp >= group) return;  // one query head per warp, four dims per lane
     __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + h * group + warp) * 128 + 4 * lane;
     if (nsb == 0) {
       *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
@@ -743,16 +771,35 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
     if (c0 == c1) return;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, part_of(c, s0)[1024 + warp]);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float* p = part_of(c, s0);
-      const float rw = p[1024 + warp], lw = p[1032 + warp];
-      const float4 v = *reinterpret_cast<const float4*>(p + warp * 128 + 4 * lane);
-      if (rw > -INFINITY || lw != 0.f) {
-        const float fw = rw == M ? 1.0f : ex2(rw - M);
-        L += lw * fw;
-        acc.x += v.x * fw, acc.y += v.y * fw, acc.z += v.z * fw, acc.w += v.w * fw;
+    for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts at a time: lane i the (ref, sum) of part i
+      const int nc = min(32, c1 - cb + 1);
+      float rw = -INFINITY, lw = 0.f;
+      if (lane < nc) {
+        const float* p = part_of(cb + lane, s0);
+        rw = p[1024 + warp], lw = p[1032 + warp];
+      }
+      float top = fmaxf(M, rw);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float f = M == top ? 1.0f : ex2(M - top);
+      M = top;
+      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+      const float fw = rw == top ? 1.0f : ex2(rw - top);
+      float add = lw * fw;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+      L = L * f + add;
+      for (int i = 0; i < nc; i += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          v[u] = i + u < nc ? *reinterpret_cast<const float4*>(part_of(cb + i + u, s0) + warp * 128 + 4 * lane)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float g = __shfl_sync(0xffffffffu, fw, (i + u) & 31);
+          if (i + u < nc) acc.x += v[u].x * g, acc.y += v[u].y * g, acc.z += v[u].z * g, acc.w += v[u].w * g;
+        }
       }
     }
     const bool none = L == 0.f;
@@ -761,51 +808,67 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
     if (none && lane == 0) set_err(a.err, kErrNoValidSlot);
     return;
   }
-  if (nsb == 0) return;
   const int s = (blockIdx.x - Hkv) * 256 + threadIdx.x;
-  if ((blockIdx.x - Hkv) * 256 >= nsb * 16) return;
-  for (int q = warp; q < a.Hq; q += 8) {  // one query head per warp, the parts over the lanes
+  if (static_cast<int>(blockIdx.x - Hkv) * 256 >= nsb * 16) return;
+  const bool mine = s < nsb * 16 && s < a.S;
+  // eight threads per query head, the parts over them
+  const int sub = threadIdx.x & 7;
+  for (int q0 = 0; q0 < a.Hq; q0 += 32) {
+    const int q = min(q0 + (static_cast<int>(threadIdx.x) >> 3), a.Hq - 1);
     const int h = q / group, w = q - h * group;
     const int s0 = first + h * nsb, c0 = s0 / R, c1 = (s0 + nsb - 1) / R;
-    float M, L;
+    float M = -INFINITY, L = 0.f;
     if (c0 == c1) {
-      const float* st = a.stats + (static_cast<size_t>(b * Hkv + h) * 8 + w) * 2;
-      M = st[0], L = st[1];
+      const float2 v = *reinterpret_cast<const float2*>(a.stats + (static_cast<size_t>(b * Hkv + h) * 8 + w) * 2);
+      if (sub == 0) M = v.x, L = v.y;
     } else {
-      M = -INFINITY, L = 0.f;
-      for (int c = c0 + lane; c <= c1; c += 32) {
+      for (int c = c0 + sub; c <= c1; c += 8) {
         const float* p = part_of(c, s0);
-        const float rw = p[1024 + w], lw = p[1032 + w], m = fmaxf(M, rw);
-        if (m > -INFINITY) L = L * (M == m ? 1.0f : ex2(M - m)) + lw * (rw == m ? 1.0f : ex2(rw - m));
-        else L += lw;
-        M = m;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        const float rw = __shfl_xor_sync(0xffffffffu, M, o), lw = __shfl_xor_sync(0xffffffffu, L, o), m = fmaxf(M, rw);
-        if (m > -INFINITY) L = L * (M == m ? 1.0f : ex2(M - m)) + lw * (rw == m ? 1.0f : ex2(rw - m));
-        else L += lw;
-        M = m;
+        join(M, L, p[1024 + w], p[1032 + w]);
       }
     }
-    if (lane == 0) fin[q] = make_float2(M > -INFINITY ? M : 0.f, L == 0.f ? 0.f : 1.0f / L);
+#pragma unroll
+    for (int o = 4; o; o >>= 1)
+      join(M, L, __shfl_xor_sync(0xffffffffu, M, o), __shfl_xor_sync(0xffffffffu, L, o));
+    if (sub == 0) fin[q] = make_float2(M > -INFINITY ? M : 0.f, L == 0.f ? 0.f : 1.0f / L);
   }
+  float* dst = a.step_score + static_cast<size_t>(b) * a.S + s;
+  float top = mine ? *dst : 0.f;
+  const float before = top;
   __syncthreads();
-  if (s >= nsb * 16 || s >= a.S) return;
-  float top = 0.f;
+  if (!mine) return;
   bool nan = false;
-  for (int h = 0; h < Hkv; ++h) {
-    const float* x = a.logits + (static_cast<size_t>(b * Hkv + h) * a.s16 + s) * a.gs;
-    for (int w = 0; w < group; ++w) {
-      const float2 f = fin[h * group + w];
-      const float p = ex2(x[w] - f.x) * f.y;
-      nan |= p != p;
-      top = fmaxf(top, p);
+  auto fold = [&](float x, int q) {
+    const float2 f = fin[q];
+    const float p = ex2(x - f.x) * f.y;
+    nan |= p != p;
+    top = fmaxf(top, p);
+  };
+  const float* x = a.logits + (static_cast<size_t>(b * Hkv) * a.s16 + s) * a.gs;
+  const size_t head = static_cast<size_t>(a.s16) * a.gs;
+#pragma unroll 4
+  for (int h = 0; h < Hkv; ++h, x += head) {
+    if (a.gs == 2) {
+      const float2 v = *reinterpret_cast<const float2*>(x);
+      fold(v.x, h * group);
+      if (group > 1) fold(v.y, h * group + 1);
+    } else {
+      const float4 v = *reinterpret_cast<const float4*>(x);
+      fold(v.x, h * group);
+      fold(v.y, h * group + 1);
+      fold(v.z, h * group + 2);
+      if (group > 3) fold(v.w, h * group + 3);
+      if (a.gs == 8) {
+        const float4 u = *reinterpret_cast<const float4*>(x + 4);
+        fold(u.x, h * group + 4);
+        if (group > 5) fold(u.y, h * group + 5);
+        if (group > 6) fold(u.z, h * group + 6);
+        if (group > 7) fold(u.w, h * group + 7);
+      }
     }
   }
   if (nan) set_err(a.err, kErrNanScore);
-  float* dst = a.step_score + static_cast<size_t>(b) * a.S + s;
-  if (top > *dst) *dst = top;
+  if (top > before) *dst = top;
 }
 
 static int floats_per_row(int group) { return group <= 2 ? 2 : group <= 4 ? 4 : 8; }
@@ -831,12 +894,9 @@ static long long workspace_bytes(int B, int Hq, int Hkv, int limit, bool score) 
 static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const void* q, const int* lens,
                   const int* slot_pos, int S, float scale, void* out, float* step_score, void* ws, long long ws_bytes,
                   int* err) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return fail(kStatusCuda, "kv4_attn: no CUDA device");
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
-  if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn: %s", cudaGetErrorString(e));
+  const int sms = prepare_device(reinterpret_cast<const void*>(attend_kernel), sizeof(Smem));
+  if (sms <= 0) return fail(kStatusCuda, "kv4_attn: no usable CUDA device");
+  cudaError_t e;
   const int Hkv = pool.Hkv, group = Hq / Hkv;
   long long limit = static_cast<long long>(pool.max_pages) * pool.page;
   if ((slot_pos || step_score) && S < limit) limit = S;

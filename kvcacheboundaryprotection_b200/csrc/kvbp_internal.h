@@ -48,6 +48,10 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// SMs of the current device (0: none usable), after letting ``kernel`` use ``smem`` bytes of
+// dynamic shared memory there.  Asked once per kernel and device.
+int prepare_device(const void* kernel, int smem);
+
 // Optional parts of the decode attention launch (all null: attention + per-slot score).
 struct AttnExtra {
   const uint8_t* head_keep = nullptr;  // per-KV-head retention [B][Hkv][S]

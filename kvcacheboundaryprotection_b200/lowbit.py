@@ -25,7 +25,7 @@ from .capi import check, lib
 
 BLOCK = 2304  # bytes of 16 slots of one kv head (KVBP_KV4_BLOCK)
 HEAD_DIM = 128
-_I32_MAX = 2**31 - 1
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -33,38 +33,27 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, shape: tuple) -> None:
-    """``t`` is a dense tensor of this type, device and shape (None: any size)."""
+    """``t`` is a dense tensor of this type, device and shape."""
+    if t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous():
+        return
     if t.dtype is not dtype or t.device != dev:
         raise ValueError(f"{name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
-    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _on(dev: torch.device) -> int:
-    """The current stream of ``dev``, which is made the current device for the call."""
+def _launch(fn, what: str, dev: torch.device, *args) -> None:
+    """``fn(stream, *args)`` on the current stream of ``dev``, with ``dev`` as the current
+    device."""
     if dev.type != "cuda":
         raise ValueError("the low-bit operators run on CUDA devices only")
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-class _Device:
-    """Makes a tensor's device current for a launch (a no-op where it is already)."""
-
-    def __init__(self, dev: torch.device):
-        self.idx = dev.index
-        self.prev = -1
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.idx:
-            self.prev = cur
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *a):
-        if self.prev >= 0:
-            torch.cuda.set_device(self.prev)
+    cur = torch.cuda.current_device()
+    if cur == dev.index:
+        check(fn(torch.cuda.current_stream(cur).cuda_stream, *args), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(torch.cuda.current_stream(dev).cuda_stream, *args), what)
 
 
 def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) -> torch.Tensor:
@@ -80,9 +69,13 @@ def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) ->
 def _pool(pool: torch.Tensor, table: torch.Tensor) -> tuple:
     """(pages, kv heads, page size, sequences, pages per sequence) after the checks."""
     dev = pool.device
-    _need(pool, "pool", torch.uint8, dev, (None, None, None, BLOCK))
-    _need(table, "page_table", torch.int32, dev, (None, None))
-    return pool.shape[0], pool.shape[1], pool.shape[2] * 16, table.shape[0], table.shape[1]
+    if pool.dim() != 4 or table.dim() != 2:
+        raise ValueError("pool must be [pages, kv heads, blocks, 2304] and page_table [sequences, pages]")
+    n_pages, hkv, per, _ = pool.shape
+    B, width = table.shape
+    _need(pool, "pool", torch.uint8, dev, (n_pages, hkv, per, BLOCK))
+    _need(table, "page_table", torch.int32, dev, (B, width))
+    return n_pages, hkv, per * 16, B, width
 
 
 def _rows(rows: int, B: int, seq: Optional[torch.Tensor], dev: torch.device) -> int:
@@ -137,15 +130,12 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, qkv: torch.Tensor, 
         return q_out
     if n_pages == 0 or width == 0 or hkv == 0 or page == 0:
         raise ValueError("the pool and the page table must not be empty")
-    with _Device(dev):
-        check(
-            lib().kvbp_kv4_append(
-                _on(dev), rows, per, _ptr(seq), B, n_heads, hkv, HEAD_DIM, page, n_pages, width, _ptr(qkv),
-                qkv.stride(0) if rows > 1 else qkv.shape[1], _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), _ptr(positions), _ptr(slots),
-                _ptr(page_table), _ptr(q_out) if n_heads else None, _ptr(pool), _ptr(dev_err),
-            ),
-            "kv4_append",
-        )
+    _launch(
+        lib().kvbp_kv4_append, "kv4_append", dev, rows, per, _ptr(seq), B, n_heads, hkv, HEAD_DIM, page, n_pages, width,
+        qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps,
+        _ptr(inv_freq), _ptr(positions), slots.data_ptr(), page_table.data_ptr(), q_out.data_ptr() if n_heads else None,
+        pool.data_ptr(), _ptr(dev_err),
+    )
     return q_out
 
 
@@ -156,8 +146,8 @@ def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor
     [rows, kv_heads, 128], or [kv_heads, rows, 128] (the prefill attention's layout) with
     ``heads_first``.  Rows of negative or out-of-range slots are zeros."""
     n_pages, hkv, page, B, width = _pool(pool, page_table)
-    dev, rows = pool.device, slots.shape[0] if slots.dim() == 1 else -1
-    _need(slots, "slots", torch.int32, dev, (rows,) if rows >= 0 else (None,))
+    dev, rows = pool.device, slots.numel()
+    _need(slots, "slots", torch.int32, dev, (rows,))
     per = _rows(rows, B, seq, dev)
     if dev_err is not None:
         _need(dev_err, "dev_err", torch.int32, dev, (1,))
@@ -169,14 +159,11 @@ def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor
     if n_pages == 0 or width == 0 or hkv == 0 or page == 0:
         raise ValueError("the pool and the page table must not be empty")
     row_stride, head_stride = (HEAD_DIM, rows * HEAD_DIM) if heads_first else (hkv * HEAD_DIM, HEAD_DIM)
-    with _Device(dev):
-        check(
-            lib().kvbp_kv4_gather(
-                _on(dev), rows, per, _ptr(seq), B, hkv, HEAD_DIM, page, n_pages, width, _ptr(slots), _ptr(page_table),
-                _ptr(pool), _ptr(k), _ptr(v), row_stride, head_stride, _ptr(dev_err),
-            ),
-            "kv4_gather",
-        )
+    _launch(
+        lib().kvbp_kv4_gather, "kv4_gather", dev, rows, per, _ptr(seq), B, hkv, HEAD_DIM, page, n_pages, width,
+        slots.data_ptr(), page_table.data_ptr(), pool.data_ptr(), k.data_ptr(), v.data_ptr(), row_stride, head_stride,
+        _ptr(dev_err),
+    )
     return k, v
 
 
@@ -192,15 +179,15 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
     n_pages, hkv, page, B, width = _pool(pool, page_table)
     dev = pool.device
     _need(lens, "lens", torch.int32, dev, (B,))
-    _need(q, "q", torch.bfloat16, dev, (B, None, HEAD_DIM))
-    hq = q.shape[1]
+    hq = q.shape[1] if q.dim() == 3 else 0
+    _need(q, "q", torch.bfloat16, dev, (B, hq, HEAD_DIM))
     if hkv == 0 or hq == 0 or hq % hkv or hq // hkv > 8:
         raise ValueError(f"{hq} query heads over {hkv} kv heads: whole groups of at most 8 are supported")
     S = 0
     for t, name, dt in ((slot_pos, "slot_pos", torch.int32), (step_score, "step_score", torch.float32)):
         if t is not None:
-            _need(t, name, dt, dev, (B, S or None))
-            S = t.shape[1]
+            S = S or (t.shape[1] if t.dim() == 2 else 0)
+            _need(t, name, dt, dev, (B, S))
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -215,15 +202,11 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
     limit = min(width * page, S) if S else width * page
     ws_bytes = L.kvbp_kv4_attn_workspace(B, hq, hkv, limit, step_score is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _Device(dev):
-        check(
-            L.kvbp_kv4_attn(
-                _on(dev), B, hq, hkv, HEAD_DIM, page, n_pages, width, _ptr(q), _ptr(pool), _ptr(page_table), _ptr(lens),
-                _ptr(slot_pos), S, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, _ptr(out), _ptr(step_score),
-                _ptr(ws), ws_bytes, _ptr(dev_err),
-            ),
-            "kv4_attn",
-        )
+    _launch(
+        L.kvbp_kv4_attn, "kv4_attn", dev, B, hq, hkv, HEAD_DIM, page, n_pages, width, q.data_ptr(), pool.data_ptr(),
+        page_table.data_ptr(), lens.data_ptr(), _ptr(slot_pos), S, _SCALE if scale is None else scale, out.data_ptr(),
+        _ptr(step_score), ws.data_ptr(), ws_bytes, _ptr(dev_err),
+    )
     return out
 
 
@@ -246,9 +229,8 @@ def int8_quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         rows, K, dtype=torch.int8, device=dev)
     s = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows and K:
-        with _Device(dev):
-            check(lib().kvbp_int8_quant_rows(_on(dev), rows, K, _ptr(x), x.stride(0) if rows > 1 else K, _ptr(q), pitch,
-                                             _ptr(s)), "int8_quant_rows")
+        _launch(lib().kvbp_int8_quant_rows, "int8_quant_rows", dev, rows, K, x.data_ptr(),
+                x.stride(0) if rows > 1 else K, q.data_ptr(), pitch, s.data_ptr())
     else:
         s.zero_()
     return q[:, :K], s
@@ -285,16 +267,9 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
         _need(dev_err, "dev_err", torch.int32, dev, (1,))
     if M == 0:
         return out
-    L = lib()
-    pitch = (K + 15) // 16 * 16
-    # codes and scales of x in one allocation (the scales behind the codes)
-    ws = torch.empty(M * pitch + 4 * M, dtype=torch.uint8, device=dev)
-    xq = ws.data_ptr()
-    xs = xq + M * pitch
-    with _Device(dev):
-        st = _on(dev)
-        check(L.kvbp_int8_quant_rows(st, M, K, x.data_ptr(), x.stride(0) if M > 1 else K, xq, pitch, xs),
-              "int8_quant_rows")
-        check(L.kvbp_int8_gemm(st, int(out_dtype is torch.float32), M, N, K, w.data_ptr(), ldw, w_scale.data_ptr(), xq,
-                               pitch, xs, _ptr(bias), out.data_ptr(), N, _ptr(dev_err)), "int8_gemm")
+    ws_bytes = M * ((K + 15) // 16 * 16 + 4)  # kvbp_int8_linear_workspace: the codes and scales of x
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _launch(lib().kvbp_int8_linear, "int8_linear", dev, out_dtype is torch.float32, M, N, K, w.data_ptr(), ldw,
+            w_scale.data_ptr(), x.data_ptr(), x.stride(0) if M > 1 else K, _ptr(bias), out.data_ptr(), N, ws.data_ptr(),
+            ws_bytes, _ptr(dev_err))
     return out

@@ -82,12 +82,12 @@ def attend(pool, table, lens, q, slot_pos, scale):
     (n / 128 + 16 additions, a block of 16 slots each, 8 warps, and the joins, cut at 2^-23 of
     sum p |v|), and the fp32 logits: 32 products of |q| and codes up to 7 a group and four
     groups, 2^-21 of their absolute sum for the rounding chain, which is an absolute error dl
-    of a logit and a relative one 2 dl of every probability.  The weights are carried in f16
-    as 2^15 p s relative to the largest p at most; where that falls below f16's normals it is
-    rounded at 2^-25, so each slot may add 7 * 2^-25 * 2^-15 (a code is at most 7, the weights'
-    sum at least 1): n * 7 * 2^-40."""
+    of a logit and a relative one 2 dl of every probability.  A weight is carried
+    in f16 as 2^e p s, p <= 1 the largest, e = min(15, 28 - X) and X at most the or of the V
+    scales' exponent fields; below f16's normals it is rounded at 2^-25, so each slot may add
+    7 * 2^-(25 + e) (a code is at most 7, the weights' sum at least 1)."""
     kv = values(pool)
-    sk = decode(pool)[0][1]
+    (_, sk), (_, sv) = decode(pool)
     B, hq, _ = q.shape
     hkv, page = pool.shape[1], pool.shape[2] * 16
     grp = hq // hkv
@@ -114,7 +114,9 @@ def attend(pool, table, lens, q, slot_pos, scale):
         big = 7 * torch.einsum("hgjd,nhj->hgn", qd[b].abs().reshape(hkv, grp, 4, 32), sk[pg, :, at % page])
         dl = 2.0 ** -21 * abs(scale) * big.amax()
         drel[b] = 2 * dl + 2.0 ** -20
-        bound[b] = (2.0 ** -8 * out[b].abs() + len(at) * 7 * 2.0 ** -40 +
+        field = int(np.bitwise_or.reduce(sv[pg, :, at % page].numpy().astype(np.float16).view(np.uint16).ravel())) >> 10 & 31
+        floor = 2.0 ** -(25 + min(15, 28 - field))
+        bound[b] = (2.0 ** -8 * out[b].abs() + len(at) * 7 * floor +
                     (2.0 ** -10 + (len(at) / 128 + 16) * 2.0 ** -23 + 2 * drel[b]) * mass)
         score[b, at] = p.amax((0, 1))
     return out.reshape(B, hq, 128), score, bound.reshape(B, hq, 128), drel

@@ -430,7 +430,7 @@ def test_quantize_rows_strided_and_misaligned_input():
 
 SIZES = [(1, 1, 1), (1, 129, 33), (2, 100, 128), (16, 256, 512), (17, 300, 1000), (32, 640, 2048), (33, 129, 255),
          (64, 384, 384), (65, 1000, 900), (127, 129, 4097), (128, 128, 128), (130, 513, 640), (257, 700, 96),
-         (300, 2560, 1024), (513, 257, 1281), (1000, 1153, 777), (4, 4608, 3584), (1, 20000, 256)]
+         (300, 2560, 1024), (513, 257, 1281), (1000, 1153, 777), (4, 4608, 3584), (1, 20000, 256), (4500, 1153, 300), (300, 20000, 640), (700, 25700, 200)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
