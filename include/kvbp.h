@@ -423,7 +423,8 @@ int kvbp_demote_int8(kvbp_stream_t stream, void* kcache, void* vcache, int32_t l
  * with q_out NULL), k and v once to their codes.  Row r belongs to sequence seq[r], or
  * r / rows_per_seq when seq is NULL, and goes to logical slot slots[r] (< 0: not stored).
  * The slots of one call must differ: of two rows for one slot either one's bytes may stay.
- * ldq a multiple of 4; qkv and q_out 8-byte aligned. */
+ * q_out is 16-byte aligned and does not overlap qkv (rows of qkv are fastest where they are
+ * 16-byte aligned). */
 int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, const int32_t* seq, int32_t B,
                     int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t max_pages,
                     const void* qkv, int32_t ldq, const void* bias, const void* q_norm_w, const void* k_norm_w,
@@ -431,7 +432,7 @@ int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, co
                     const int32_t* page_table, void* q_out, void* pool, int32_t* dev_err);
 
 /* Read-back of listed slots as bf16((code - 8) * scale): row r, head h to k_out / v_out +
- * r * row_stride + h * head_stride (elements; multiples of 4, outputs 8-byte aligned), e.g.
+ * r * row_stride + h * head_stride (elements; multiples of 8, outputs 16-byte aligned), e.g.
  * [rows][Hkv][128] or the prefill attention's [Hkv][rows][128].  Rows of a skipped or
  * negative slot are zeros. */
 int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, const int32_t* seq, int32_t B,
@@ -442,7 +443,7 @@ int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, co
 /* Attention of one token per sequence over the 4-bit pages, with the per-slot eviction
  * score: out[b] = softmax(scale * q . k) v over the live slots of sequence b -- logical
  * slots s < lens[b] (0 allowed) with slot_pos[b][s] >= 0 (slot_pos [B][S], or NULL: all).
- * q, out [B][Hq][128] bf16, 16-byte aligned; Hq / Hkv <= 8.  step_score [B][S] float (may be
+ * q, out [B][Hq][128] bf16, 16-byte aligned and apart; Hq / Hkv <= 8.  step_score [B][S] float (may be
  * NULL, non-negative on entry) is max-accumulated with each live slot's largest probability
  * over the heads, as kvbp_decode_attn_score does.  lens above max_pages * page_size (or S,
  * when slot_pos or step_score is given) is cut there and sets KVBP_DEV_INDEX.  A sequence

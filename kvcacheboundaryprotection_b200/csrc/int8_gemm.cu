@@ -99,9 +99,12 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t da, uint64_t db
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
       "l"(da), "l"(db), "r"(id), "r"(acc));
 }
-__device__ __forceinline__ int ld_dsmem_s32(uint32_t cluster_addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ int4 ld_dsmem_v4(uint32_t cluster_addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void store(const Args& a, int m, int n, int acc, float sx, float sw, float bias) {
@@ -261,16 +264,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (S > 1) {
     cluster_sync_all();
-    // this CTA's share of the tile's live elements
-    const int E = cols * 128, e1 = static_cast<int>(static_cast<long long>(rank + 1) * E / S);
+    // this CTA's share of the tile's live elements, four channels at a time
+    const int E = cols * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * E / S);
     if (all_ok)
       for (int e = static_cast<int>(static_cast<long long>(rank) * E / S) + tid; e < e1; e += kThreads) {
-        const uint32_t at = smem_u32(part + e);
-        int sum = 0;
+        const uint32_t at = smem_u32(part + 4 * e);
+        int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 8
-        for (int r = 0; r < S; ++r) sum += ld_dsmem_s32(mapa_u32(at, r));
-        const int m = m0 + (e >> 7), n = n0 + (e & 127);
-        if (n < a.N) store(a, m, n, sum, a.sx[m], a.sw[n], a.bias ? __bfloat162float(a.bias[n]) : 0.f);
+        for (int r = 0; r < S; ++r) {
+          const int4 v = ld_dsmem_v4(mapa_u32(at, r));
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const int m = m0 + (e >> 5), n = n0 + (e & 31) * 4, v[4] = {sum.x, sum.y, sum.z, sum.w};
+        const float sx = a.sx[m];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < a.N) store(a, m, n + i, v[i], sx, a.sw[n + i], a.bias ? __bfloat162float(a.bias[n + i]) : 0.f);
       }
     cluster_sync_all();  // no CTA leaves while a peer may still read its part
   }
@@ -508,7 +517,7 @@ static int gemm(cudaStream_t st, const Args& a, const void* w, long long ldw, co
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
   const long long tn = (a.N + 127) / 128;
   const int steps = (a.K + kBK - 1) / kBK;
-  const bool many = tn * ((a.M + kPN - 1) / kPN) >= sms;
+  const bool many = a.M > 128 && tn * ((a.M + kPN - 1) / kPN) >= sms;
   const int NT = many ? kPN : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
   const long long tm = (a.M + NT - 1) / NT;
   if (!many && tm > 65535) return fail(kStatusUnsupported, "int8_gemm: too many tiles");

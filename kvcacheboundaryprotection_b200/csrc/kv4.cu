@@ -59,173 +59,215 @@ struct Pool {
   __device__ __forceinline__ size_t hstride() const { return static_cast<size_t>(page / 16) * kBlock; }
 };
 
-// max|x| over the 8 lanes that share a group, as bits: a NaN's bits are the largest, so it
+// max|x| over the 4 lanes that share a group, as bits: a NaN's bits are the largest, so it
 // reaches the scale.
 __device__ __forceinline__ uint32_t group_max(uint32_t m) {
-#pragma unroll
-  for (int o = 4; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 __device__ __forceinline__ __half group_scale(uint32_t amax_bits) {
   if (amax_bits > 0x7f800000u) return __ushort_as_half(0x7fff);
   return __float2half_rn(fminf(__uint_as_float(amax_bits) / 7.0f, 65504.0f));
 }
-// four codes as one 16-bit word
-__device__ __forceinline__ uint32_t four_codes(const float (&x)[4], float scale) {
+// eight codes as one 32-bit word
+__device__ __forceinline__ uint32_t eight_codes(const float (&x)[8], float scale) {
   uint32_t w = 0;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
+  for (int n = 0; n < 8; ++n) {
     // scale 0 (all values below the smallest f16 step) and NaN: code 8, the value 0 * scale
     const float q = scale > 0.f ? fminf(fmaxf(rintf(x[n] / scale), -7.f), 7.f) : 0.f;
     w |= static_cast<uint32_t>(static_cast<int>(q) + 8) << (4 * n);
   }
   return w;
 }
+__device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[2 * k] = bf16lo(w[k]), x[2 * k + 1] = bf16hi(w[k]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+// x[0..7] from eight values p[0..7] of any alignment (the weights of norms and biases)
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+#pragma unroll
+  for (int n = 0; n < 8; ++n) x[n] = __bfloat162float(p[n]);
+}
 
-// Append.  One CTA per row; half-warp u finishes heads u, u + 16, ... of the row's Hq query,
-// Hkv key and Hkv value heads; lane l of the half-warp owns dims 4 l .. 4 l + 3 and
-// 64 + 4 l .. 64 + 4 l + 3, so the RoPE pairs (d, d + 64) are its own and a group of 32 dims
-// is 8 lanes.  Everything between the bf16 input and the stored value is fp32, rounded once
-// (q to bf16, k and v to their codes): the cache keeps 4 bits, so no bf16 step in between
-// is worth its error.  The angle pos * inv_freq is reduced in double: at position 4e5 an
-// fp32 product would be off by up to 2e-2 rad.
-// HBM-bound on a prompt: it reads qkv and writes q once, and 144 bytes per kv head.
-__global__ void __launch_bounds__(256) append_kernel(
-    const __nv_bfloat16* __restrict__ qkv, int ldq, const __nv_bfloat16* __restrict__ bias,
-    const __nv_bfloat16* __restrict__ qnw, const __nv_bfloat16* __restrict__ knw, float eps,
-    const float* __restrict__ inv_freq, const int* __restrict__ positions, const int* __restrict__ slots,
-    const int* __restrict__ seq, int rows_per_seq, int Hq, Pool pool, __nv_bfloat16* __restrict__ q_out, int* err) {
+struct AppendArgs {
+  const __nv_bfloat16* qkv;
+  const __nv_bfloat16* bias;
+  const __nv_bfloat16* qnw;
+  const __nv_bfloat16* knw;
+  const float* inv_freq;
+  const int* positions;
+  const int* slots;
+  const int* seq;
+  Pool pool;
+  __nv_bfloat16* q_out;
+  int* err;
+  int ldq, rows, rows_per_seq, Hq, wide;
+  float eps;
+};
+
+// Append.  A CTA takes R rows; a warp takes four heads of a row at a time, eight lanes each:
+// lane l of the eight owns dims 8 l .. 8 l + 7 and 64 + 8 l .. 64 + 8 l + 7 (16-byte loads),
+// so the RoPE pairs (d, d + 64) are its own, a group of 32 dims is four lanes and its eight
+// codes are one word of K.  Everything between the bf16 input and the stored value is fp32,
+// rounded once (q to bf16, k and v to their codes): the cache keeps 4 bits, so no bf16 step in
+// between is worth its error.  The angle pos * inv_freq is reduced in double: at position 4e5
+// an fp32 product would be off by up to 2e-2 rad.
+// Bound by HBM on a prompt (reads qkv, writes q, 144 bytes per kv head): eight rows per CTA
+// share one phase of angles, one per thread and half; with few rows one row per CTA spreads
+// them over the SMs (latency).
+template <int R>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float cs[64], sn[64];
-  const int r = blockIdx.x, tid = threadIdx.x, l = tid & 15;
-  if (inv_freq) {
-    if (tid < 64) {
-      const double turns = static_cast<double>(positions[r]) * static_cast<double>(inv_freq[tid]) * 0.15915494309189533577;
+  __shared__ float cs[R][64], sn[R][64];
+  const int r0 = blockIdx.x * R, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid & 7;
+  const int nr = min(R, a.rows - r0);
+  if (a.inv_freq) {
+    for (int i = tid; i < nr * 64; i += 256) {
+      const int r = i >> 6, f = i & 63;
+      const double turns =
+          static_cast<double>(a.positions[r0 + r]) * static_cast<double>(a.inv_freq[f]) * 0.15915494309189533577;
       float s, c;
       sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-      cs[tid] = c;
-      sn[tid] = s;
+      cs[r][f] = c;
+      sn[r][f] = s;
     }
     __syncthreads();
   }
-  const int slot = slots[r];
-  const int b = seq ? seq[r] : r / rows_per_seq;
-  uint8_t* blk = slot >= 0 ? pool.block_of(b, slot, err, tid == 0) : nullptr;
-  const int in = slot & 15;
-  const int nh = Hq + 2 * pool.Hkv;
-  // both halves of a warp run the same number of rounds: the shuffles are warp-wide
-  for (int h0 = (tid >> 5) * 2; h0 < nh; h0 += 16) {
-    const int hh = h0 + ((tid >> 4) & 1);
-    const bool live = hh < nh;
-    const int hc = live ? hh : nh - 1;
-    const __nv_bfloat16* src = qkv + static_cast<size_t>(r) * ldq + hc * 128 + 4 * l;
-    const uint2 a = *reinterpret_cast<const uint2*>(src), c = *reinterpret_cast<const uint2*>(src + 64);
-    float lo[4] = {bf16lo(a.x), bf16hi(a.x), bf16lo(a.y), bf16hi(a.y)};
-    float hi[4] = {bf16lo(c.x), bf16hi(c.x), bf16lo(c.y), bf16hi(c.y)};
-    if (bias) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        lo[n] += __bfloat162float(bias[hc * 128 + 4 * l + n]);
-        hi[n] += __bfloat162float(bias[hc * 128 + 64 + 4 * l + n]);
-      }
+  const int Hkv = a.pool.Hkv, nh = a.Hq + 2 * Hkv, quads = (nh + 3) >> 2;
+  for (int u = warp; u < nr * quads; u += 8) {
+    const int ri = u / quads, r = r0 + ri, h = 4 * (u - ri * quads) + (lane >> 3);
+    const bool live = h < nh;
+    const int hc = live ? h : nh - 1;  // lanes past the last head keep the shuffles whole
+    const __nv_bfloat16* src = a.qkv + static_cast<size_t>(r) * a.ldq + hc * 128 + 8 * l;
+    float lo[8], hi[8];
+    if (a.wide) {
+      const uint4 x = *reinterpret_cast<const uint4*>(src), y = *reinterpret_cast<const uint4*>(src + 64);
+      unpack8(x, lo);
+      unpack8(y, hi);
+    } else {
+      load8(src, lo);
+      load8(src + 64, hi);
     }
-    const bool is_q = hc < Hq, is_v = hc >= Hq + pool.Hkv;
-    const __nv_bfloat16* nw = is_q ? qnw : knw;
-    if (qnw || knw) {
+    const bool is_q = hc < a.Hq, is_v = hc >= a.Hq + Hkv;
+    if (a.bias) {
+      float bl[8], bh[8];
+      load8(a.bias + hc * 128 + 8 * l, bl);
+      load8(a.bias + hc * 128 + 64 + 8 * l, bh);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) lo[n] += bl[n], hi[n] += bh[n];
+    }
+    if (a.qnw || a.knw) {
       float ss = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) ss += lo[n] * lo[n] + hi[n] * hi[n];
+      for (int n = 0; n < 8; ++n) ss += lo[n] * lo[n] + hi[n] * hi[n];
 #pragma unroll
-      for (int o = 8; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      for (int o = 4; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const __nv_bfloat16* nw = is_q ? a.qnw : a.knw;
       if (!is_v && nw) {
-        const float rms = sqrtf(ss / 128.0f + eps);
+        const float inv = 1.0f / sqrtf(ss / 128.0f + a.eps);
+        float wl[8], wh[8];
+        load8(nw + 8 * l, wl);
+        load8(nw + 64 + 8 * l, wh);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          lo[n] = lo[n] / rms * __bfloat162float(nw[4 * l + n]);
-          hi[n] = hi[n] / rms * __bfloat162float(nw[64 + 4 * l + n]);
-        }
+        for (int n = 0; n < 8; ++n) lo[n] = lo[n] * inv * wl[n], hi[n] = hi[n] * inv * wh[n];
       }
     }
-    if (inv_freq && !is_v) {
+    if (a.inv_freq && !is_v) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float co = cs[4 * l + n], si = sn[4 * l + n];
+      for (int n = 0; n < 8; ++n) {
+        const float co = cs[ri][8 * l + n], si = sn[ri][8 * l + n];
         const float y = lo[n] * co - hi[n] * si;
         hi[n] = hi[n] * co + lo[n] * si;
         lo[n] = y;
       }
     }
-    if (is_q) {
-      if (live) {
-        __nv_bfloat16* dst = q_out + (static_cast<size_t>(r) * Hq + hc) * 128 + 4 * l;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-        *reinterpret_cast<uint2*>(dst + 64) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
-      }
+    if (is_q && live) {
+      __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(r) * a.Hq + hc) * 128 + 8 * l;
+      *reinterpret_cast<uint4*>(dst) = pack8(lo);
+      *reinterpret_cast<uint4*>(dst + 64) = pack8(hi);
     }
-    // every lane of the warp reduces (the other half-warp may hold a key)
+    if (__all_sync(0xffffffffu, is_q)) continue;
+    // every lane of the warp reduces (another eight may hold a key)
     uint32_t ml = 0, mh = 0;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < 8; ++n) {
       ml = max(ml, __float_as_uint(fabsf(lo[n])));
       mh = max(mh, __float_as_uint(fabsf(hi[n])));
     }
     ml = group_max(ml);
     mh = group_max(mh);
-    if (live && !is_q && blk) {
-      uint8_t* dst = blk + static_cast<size_t>(hc - Hq - (is_v ? pool.Hkv : 0)) * pool.hstride();
-      const __half sl = group_scale(ml), sh = group_scale(mh);
-      const uint32_t wl = four_codes(lo, __half2float(sl)), wh = four_codes(hi, __half2float(sh));
-      const int cl = is_v ? v_code_offset(in, l) : k_code_offset(in, l);
-      const int ch = is_v ? v_code_offset(in, l + 16) : k_code_offset(in, l + 16);
-      *reinterpret_cast<uint16_t*>(dst + cl) = static_cast<uint16_t>(wl);
-      *reinterpret_cast<uint16_t*>(dst + ch) = static_cast<uint16_t>(wh);
-      if ((l & 7) == 0) {
-        const int j = l >> 3;
-        *reinterpret_cast<__half*>(dst + (is_v ? v_scale_offset(in, j) : k_scale_offset(in, j))) = sl;
-        *reinterpret_cast<__half*>(dst + (is_v ? v_scale_offset(in, j + 2) : k_scale_offset(in, j + 2))) = sh;
-      }
+    const int slot = a.slots[r];
+    if (is_q || !live || slot < 0) continue;
+    const int b = a.seq ? a.seq[r] : r / a.rows_per_seq;
+    uint8_t* dst = a.pool.block_of(b, slot, a.err, l == 0);
+    if (!dst) continue;
+    dst += static_cast<size_t>(hc - a.Hq - (is_v ? Hkv : 0)) * a.pool.hstride();
+    const int in = slot & 15, j = l >> 2;
+    const __half sl = group_scale(ml), sh = group_scale(mh);
+    const uint32_t wl = eight_codes(lo, __half2float(sl)), wh = eight_codes(hi, __half2float(sh));
+    if (is_v) {
+      *reinterpret_cast<uint16_t*>(dst + v_code_offset(in, 2 * l)) = static_cast<uint16_t>(wl);
+      *reinterpret_cast<uint16_t*>(dst + v_code_offset(in, 2 * l + 1)) = static_cast<uint16_t>(wl >> 16);
+      *reinterpret_cast<uint16_t*>(dst + v_code_offset(in, 2 * l + 16)) = static_cast<uint16_t>(wh);
+      *reinterpret_cast<uint16_t*>(dst + v_code_offset(in, 2 * l + 17)) = static_cast<uint16_t>(wh >> 16);
+    } else {
+      *reinterpret_cast<uint32_t*>(dst + k_code_offset(in, 2 * l)) = wl;
+      *reinterpret_cast<uint32_t*>(dst + k_code_offset(in, 2 * l + 16)) = wh;
+    }
+    if ((l & 3) == 0) {
+      *reinterpret_cast<__half*>(dst + (is_v ? v_scale_offset(in, j) : k_scale_offset(in, j))) = sl;
+      *reinterpret_cast<__half*>(dst + (is_v ? v_scale_offset(in, j + 2) : k_scale_offset(in, j + 2))) = sh;
     }
   }
 }
 
-// Read-back of listed slots as bf16 rows.  One half-warp per (row, kv head).
+// Read-back of listed slots as bf16 rows: eight lanes per (row, kv head), as in the append.
 __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slots, const int* __restrict__ seq,
                                                      int rows_per_seq, long long n, Pool pool,
                                                      __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                                                      long long row_stride, long long head_stride, int* err) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long u = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const long long u = static_cast<long long>(blockIdx.x) * 32 + (threadIdx.x >> 3);
   if (u >= n) return;
-  const int l = threadIdx.x & 15;
+  const int l = threadIdx.x & 7;
   const long long r = u / pool.Hkv;
   const int h = static_cast<int>(u - r * pool.Hkv);
   const int slot = slots[r];
   const int b = seq ? seq[r] : static_cast<int>(r / rows_per_seq);
   const uint8_t* blk = slot >= 0 ? pool.block_of(b, slot, err, h == 0 && l == 0) : nullptr;
-  uint2 o[2][2] = {};
+  uint4 o[4] = {};
   if (blk) {
     blk += h * pool.hstride();
-    const int in = slot & 15;
+    const int in = slot & 15, j = l >> 2;
+    auto u16 = [&](int at) { return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(blk + at)); };
+    const uint32_t w[4] = {*reinterpret_cast<const uint32_t*>(blk + k_code_offset(in, 2 * l)),
+                           *reinterpret_cast<const uint32_t*>(blk + k_code_offset(in, 2 * l + 16)),
+                           u16(v_code_offset(in, 2 * l)) | u16(v_code_offset(in, 2 * l + 1)) << 16,
+                           u16(v_code_offset(in, 2 * l + 16)) | u16(v_code_offset(in, 2 * l + 17)) << 16};
+    const float s[4] = {__half2float(__ushort_as_half(u16(k_scale_offset(in, j)))),
+                        __half2float(__ushort_as_half(u16(k_scale_offset(in, j + 2)))),
+                        __half2float(__ushort_as_half(u16(v_scale_offset(in, j)))),
+                        __half2float(__ushort_as_half(u16(v_scale_offset(in, j + 2))))};
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int i = 0; i < 4; ++i) {
+      float x[8];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int L = l + 16 * half, j = L >> 3;
-        const uint32_t c = *reinterpret_cast<const uint16_t*>(blk + (w ? v_code_offset(in, L) : k_code_offset(in, L)));
-        const float s = __half2float(*reinterpret_cast<const __half*>(blk + (w ? v_scale_offset(in, j) : k_scale_offset(in, j))));
-        float x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = static_cast<float>(static_cast<int>((c >> (4 * k)) & 15u) - 8) * s;
-        o[w][half] = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-      }
+      for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(static_cast<int>((w[i] >> (4 * k)) & 15u) - 8) * s[i];
+      o[i] = pack8(x);
+    }
   }
-  const long long at = r * row_stride + h * head_stride + 4 * l;
-  *reinterpret_cast<uint2*>(k_out + at) = o[0][0];
-  *reinterpret_cast<uint2*>(k_out + at + 64) = o[0][1];
-  *reinterpret_cast<uint2*>(v_out + at) = o[1][0];
-  *reinterpret_cast<uint2*>(v_out + at + 64) = o[1][1];
+  const long long at = r * row_stride + h * head_stride + 8 * l;
+  *reinterpret_cast<uint4*>(k_out + at) = o[0];
+  *reinterpret_cast<uint4*>(k_out + at + 64) = o[1];
+  *reinterpret_cast<uint4*>(v_out + at) = o[2];
+  *reinterpret_cast<uint4*>(v_out + at + 64) = o[3];
 }
 
 // ---- attention of one token per sequence ------------------------------------------------
@@ -941,6 +983,11 @@ static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const vo
   return kStatusOk;
 }
 
+constexpr int kManyRows = 2048;  // from here on eight rows per CTA
+static bool overlap(const void* p, long long np, const void* q, long long nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Checks shared by the three entry points; fills ``p``.
@@ -979,13 +1026,17 @@ extern "C" int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_
   if (rows <= 0 || Hq < 0 || (!seq && rows_per_seq <= 0) || Hq > 65535 || Hkv > 65535 ||
       ldq < (static_cast<long long>(Hq) + 2 * Hkv) * 128)
     return fail(kvbp::kStatusArg, "kv4_append: bad size");
-  if (ldq % 4 || ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 7))
-    return fail(kvbp::kStatusArg, "kv4_append: qkv and q_out rows must be 8-byte aligned");
-  const cudaError_t e = kvbp::launch_pdl(
-      kv4::append_kernel, dim3(rows), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0),
-      static_cast<const __nv_bfloat16*>(qkv), ldq, static_cast<const __nv_bfloat16*>(bias),
-      static_cast<const __nv_bfloat16*>(q_norm_w), static_cast<const __nv_bfloat16*>(k_norm_w), eps, inv_freq,
-      positions, slots, seq, rows_per_seq, Hq, p, static_cast<__nv_bfloat16*>(q_out), dev_err);
+  if (!kv4::aligned16(q_out)) return fail(kvbp::kStatusArg, "kv4_append: q_out must be 16-byte aligned");
+  if (Hq > 0 && kv4::overlap(qkv, 2ll * ((rows - 1ll) * ldq + (Hq + 2ll * Hkv) * 128), q_out, 256ll * rows * Hq))
+    return fail(kvbp::kStatusArg, "kv4_append: q_out must not overlap qkv");
+  const kv4::AppendArgs a{static_cast<const __nv_bfloat16*>(qkv), static_cast<const __nv_bfloat16*>(bias),
+                          static_cast<const __nv_bfloat16*>(q_norm_w), static_cast<const __nv_bfloat16*>(k_norm_w),
+                          inv_freq, positions, slots, seq, p, static_cast<__nv_bfloat16*>(q_out), dev_err, ldq, rows,
+                          rows_per_seq, Hq, kv4::aligned16(qkv) && ldq % 8 == 0, eps};
+  const cudaError_t e =
+      rows >= kv4::kManyRows
+          ? kvbp::launch_pdl(kv4::append_kernel<8>, dim3((rows + 7) / 8), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0), a)
+          : kvbp::launch_pdl(kv4::append_kernel<1>, dim3(rows), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0), a);
   if (e != cudaSuccess) return fail(kvbp::kStatusCuda, "kv4_append launch: %s", cudaGetErrorString(e));
   return kvbp::kStatusOk;
 }
@@ -999,13 +1050,13 @@ extern "C" int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_
     return st;
   if (!slots || !k_out || !v_out) return fail(kvbp::kStatusArg, "kv4_gather: null pointer");
   if (rows <= 0 || (!seq && rows_per_seq <= 0)) return fail(kvbp::kStatusArg, "kv4_gather: bad size");
-  if (row_stride < 128 || head_stride < 128 || row_stride % 4 || head_stride % 4 ||
-      ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 7))
-    return fail(kvbp::kStatusArg, "kv4_gather: output rows must be 128 apart or more and 8-byte aligned");
+  if (row_stride < 128 || head_stride < 128 || row_stride % 8 || head_stride % 8 || !kv4::aligned16(k_out) ||
+      !kv4::aligned16(v_out))
+    return fail(kvbp::kStatusArg, "kv4_gather: output rows must be 128 apart or more and 16-byte aligned");
   const long long n = static_cast<long long>(rows) * Hkv;
-  if ((n + 15) / 16 > 0x7fffffffll) return fail(kvbp::kStatusArg, "kv4_gather: too many rows");
+  if ((n + 31) / 32 > 0x7fffffffll) return fail(kvbp::kStatusArg, "kv4_gather: too many rows");
   const cudaError_t e = kvbp::launch_pdl(
-      kv4::gather_kernel, dim3(static_cast<unsigned>((n + 15) / 16)), dim3(256), 0,
+      kv4::gather_kernel, dim3(static_cast<unsigned>((n + 31) / 32)), dim3(256), 0,
       reinterpret_cast<cudaStream_t>(stream), dim3(0), slots, seq, rows_per_seq, n, p,
       static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), static_cast<long long>(row_stride),
       static_cast<long long>(head_stride), dev_err);
@@ -1032,6 +1083,8 @@ extern "C" int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_
   if (S < 0 || ((slot_pos || step_score) && S == 0)) return fail(kvbp::kStatusArg, "kv4_attn: bad slot stride");
   if (!kv4::aligned16(q) || !kv4::aligned16(out) || !kv4::aligned16(workspace))
     return fail(kvbp::kStatusArg, "kv4_attn: q, out and the workspace must be 16-byte aligned");
+  if (kv4::overlap(q, 256ll * B * Hq, out, 256ll * B * Hq))
+    return fail(kvbp::kStatusArg, "kv4_attn: out must not overlap q");
   return kv4::attend(reinterpret_cast<cudaStream_t>(stream), B, Hq, p, q, lens, slot_pos, S, scale, out, step_score,
                      workspace, workspace_bytes, dev_err);
 }

@@ -16,6 +16,7 @@ out of range) set bits of ``dev_err``, an int32 tensor of one element, when one 
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -26,6 +27,8 @@ from .capi import check, lib
 BLOCK = 2304  # bytes of 16 slots of one kv head (KVBP_KV4_BLOCK)
 HEAD_DIM = 128
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+# the current stream's handle of a device index (torch.cuda.current_stream makes an object)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -48,12 +51,19 @@ def _launch(fn, what: str, dev: torch.device, *args) -> None:
     device."""
     if dev.type != "cuda":
         raise ValueError("the low-bit operators run on CUDA devices only")
-    cur = torch.cuda.current_device()
-    if cur == dev.index:
-        check(fn(torch.cuda.current_stream(cur).cuda_stream, *args), what)
+    idx = dev.index
+    if torch.cuda.current_device() == idx:
+        status = fn(_raw_stream(idx), *args)
     else:
-        with torch.cuda.device(dev):
-            check(fn(torch.cuda.current_stream(dev).cuda_stream, *args), what)
+        with torch.cuda.device(idx):
+            status = fn(_raw_stream(idx), *args)
+    if status:
+        check(status, what)
+
+
+@lru_cache(maxsize=1024)
+def _attn_workspace(B: int, hq: int, hkv: int, limit: int, score: bool) -> int:
+    return lib().kvbp_kv4_attn_workspace(B, hq, hkv, limit, score)
 
 
 def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) -> torch.Tensor:
@@ -198,12 +208,11 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
         return out
     if n_pages == 0 or width == 0 or page == 0 or ((slot_pos is not None or step_score is not None) and S == 0):
         raise ValueError("the pool, the page table, slot_pos and step_score must not be empty")
-    L = lib()
     limit = min(width * page, S) if S else width * page
-    ws_bytes = L.kvbp_kv4_attn_workspace(B, hq, hkv, limit, step_score is not None)
+    ws_bytes = _attn_workspace(B, hq, hkv, limit, step_score is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     _launch(
-        L.kvbp_kv4_attn, "kv4_attn", dev, B, hq, hkv, HEAD_DIM, page, n_pages, width, q.data_ptr(), pool.data_ptr(),
+        lib().kvbp_kv4_attn, "kv4_attn", dev, B, hq, hkv, HEAD_DIM, page, n_pages, width, q.data_ptr(), pool.data_ptr(),
         page_table.data_ptr(), lens.data_ptr(), _ptr(slot_pos), S, _SCALE if scale is None else scale, out.data_ptr(),
         _ptr(step_score), ws.data_ptr(), ws_bytes, _ptr(dev_err),
     )
