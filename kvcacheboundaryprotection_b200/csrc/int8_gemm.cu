@@ -52,13 +52,32 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
   const float top = __uint_as_float(m);
   const bool fine = m > 0 && m < 0x7f800000u;
   if (tid == 0) scale[r] = top / 127.0f;
-  auto code = [&](float v) -> uint32_t {
-    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * v / top))) & 255u : 0u;
+  // rint(127 x / top): x times the rounded factor plus 1.5 * 2^23 leaves the integer in the low
+  // mantissa bits.  The factor is off by 2^-24 of at most 127, so only what lies within 2^-8 of
+  // half-way can round wrongly: it is divided.
+  const float factor = fine ? 127.0f / top : 0.f;
+  auto code = [&](float v, float& worst) -> uint32_t {
+    const float s = fmaf(v, factor, 12582912.0f);
+    worst = fmaxf(worst, fabsf(fmaf(v, factor, 12582912.0f - s)));
+    return __float_as_uint(s);
+  };
+  auto exact = [&](float v) -> uint32_t {
+    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * v / top))) : 0u;
+  };
+  auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
   };
   auto emit = [&](const uint4 w, int i) {
-    *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(
-        code(bf16lo(w.x)) | code(bf16hi(w.x)) << 8 | code(bf16lo(w.y)) << 16 | code(bf16hi(w.y)) << 24,
-        code(bf16lo(w.z)) | code(bf16hi(w.z)) << 8 | code(bf16lo(w.w)) << 16 | code(bf16hi(w.w)) << 24);
+    float x[8] = {bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y), bf16lo(w.z), bf16hi(w.z), bf16lo(w.w), bf16hi(w.w)};
+    uint32_t c[8];
+    float worst = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = code(x[k], worst);
+    if (!fine || worst > 0.49609375f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) c[k] = exact(x[k]);
+    }
+    *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(bytes(c[0], c[1], c[2], c[3]), bytes(c[4], c[5], c[6], c[7]));
   };
 #pragma unroll
   for (int u = 0; u < kVec; ++u) {
@@ -66,7 +85,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
     if (i < nv) emit(keep[u], i);
   }
   for (int i = tid + 256 * kVec; i < nv; i += 256) emit(rv[i], i);
-  for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(code(__bfloat162float(row[i])));
+  for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(exact(__bfloat162float(row[i])));
 }
 
 // ---- the product on the 5th-generation tensor cores (tcgen05.mma kind::i8) -------------
@@ -82,6 +101,7 @@ struct Args {
   void* out;
   long long ldo;
   int M, N, K, f32;
+  int vec;    // four channels at a time are aligned
   int early;  // the weight is known to be complete before the kernel before this one ends
   int* err;
 };
@@ -114,6 +134,27 @@ __device__ __forceinline__ void store(const Args& a, int m, int n, int acc, floa
     static_cast<float*>(a.out)[at] = y;
   else
     static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+}
+// four channels from n on
+__device__ __forceinline__ void store4(const Args& a, int m, int n, int4 acc, float sx) {
+  if (a.vec && n < a.N) {  // N, ldo multiples of 4, pointers aligned
+    const float4 sw = *reinterpret_cast<const float4*>(a.sw + n);
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.bias) {
+      const uint2 w = *reinterpret_cast<const uint2*>(a.bias + n);
+      b = make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
+    }
+    const float4 y = make_float4(static_cast<float>(acc.x) * sx * sw.x + b.x, static_cast<float>(acc.y) * sx * sw.y + b.y,
+                                 static_cast<float>(acc.z) * sx * sw.z + b.z, static_cast<float>(acc.w) * sx * sw.w + b.w);
+    const size_t at = static_cast<size_t>(m) * a.ldo + n;
+    if (a.f32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = y;
+    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
+    return;
+  }
+  const int v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < a.N) store(a, m, n + i, v[i], sx, a.sw[n + i], a.bias ? __bfloat162float(a.bias[n + i]) : 0.f);
 }
 // Barrier among ``nthreads`` threads; true on all of them when ``v`` is on any.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool v) {
@@ -275,11 +316,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int4 v = ld_dsmem_v4(mapa_u32(at, r));
           sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-        const int m = m0 + (e >> 5), n = n0 + (e & 31) * 4, v[4] = {sum.x, sum.y, sum.z, sum.w};
-        const float sx = a.sx[m];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < a.N) store(a, m, n + i, v[i], sx, a.sw[n + i], a.bias ? __bfloat162float(a.bias[n + i]) : 0.f);
+        const int m = m0 + (e >> 5), n = n0 + (e & 31) * 4;
+        store4(a, m, n, sum, a.sx[m]);
       }
     cluster_sync_all();  // no CTA leaves while a peer may still read its part
   }
@@ -511,8 +549,9 @@ static int check(const Args& a, const void* w, long long ldw, const void* xq, lo
   return kStatusOk;
 }
 
-static int gemm(cudaStream_t st, const Args& a, const void* w, long long ldw, const void* xq, long long ldq) {
+static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const void* xq, long long ldq) {
   if (int bad = check(a, w, ldw, xq, ldq)) return bad;
+  a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.sw, 16) && !misaligned(a.bias, 8) && !misaligned(a.out, a.f32 ? 16 : 8);
   const int sms = prepare_device(reinterpret_cast<const void*>(persist_kernel), kPBytes);
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
   const long long tn = (a.N + 127) / 128;
@@ -554,7 +593,7 @@ extern "C" int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t 
 extern "C" int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
                               int64_t ldw, const float* w_scale, const void* xq, int64_t ldq, const float* x_scale,
                               const void* bias, void* out, int64_t ldo, int32_t* dev_err) {
-  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, dev_err};
+  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, 0, dev_err};
   return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, xq, ldq);
 }
 
@@ -571,7 +610,7 @@ extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t 
   const int64_t ldq = (static_cast<int64_t>(K) + 15) / 16 * 16;
   float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + ldq * M);
   // the product's arguments first: a refused call leaves the workspace alone
-  const kvbp::i8::Args a{w_scale, scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 1, dev_err};
+  const kvbp::i8::Args a{w_scale, scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, 1, dev_err};
   if (int st = kvbp::i8::check(a, w, ldw, workspace, ldq)) return st;
   if (int st = kvbp_int8_quant_rows(stream, M, K, x, ldx, workspace, ldq, scale)) return st;
   return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, workspace, ldq);

@@ -18,6 +18,8 @@
 //   2176  V scales: slot s = 4 t + 2 h + e, group i at 32 t + 16 h + 4 i + 2 e
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kvbp_internal.h"
 
@@ -69,14 +71,16 @@ __device__ __forceinline__ __half group_scale(uint32_t amax_bits) {
   if (amax_bits > 0x7f800000u) return __ushort_as_half(0x7fff);
   return __float2half_rn(fminf(__uint_as_float(amax_bits) / 7.0f, 65504.0f));
 }
-// eight codes as one 32-bit word
+// eight codes as one 32-bit word: clip(rint(x / scale), -7, 7) + 8 each.  The quotient is
+// rounded to an integer by adding 1.5 * 2^23, which leaves it in the low mantissa bits.
+// Scale 0 (all values below the smallest f16 step) and NaN: code 8, the value 0 * scale.
 __device__ __forceinline__ uint32_t eight_codes(const float (&x)[8], float scale) {
+  const float inv = scale > 0.f ? 1.0f / scale : 0.f;
   uint32_t w = 0;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    // scale 0 (all values below the smallest f16 step) and NaN: code 8, the value 0 * scale
-    const float q = scale > 0.f ? fminf(fmaxf(rintf(x[n] / scale), -7.f), 7.f) : 0.f;
-    w |= static_cast<uint32_t>(static_cast<int>(q) + 8) << (4 * n);
+    const float q = fminf(fmaxf(x[n] * inv, -7.f), 7.f) + (12582912.0f + 8.0f);
+    w |= (__float_as_uint(q) & 15u) << (4 * n);
   }
   return w;
 }
@@ -88,10 +92,14 @@ __device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
-// x[0..7] from eight values p[0..7] of any alignment (the weights of norms and biases)
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+// x[0..7] = p[0..7], one load where all of the call's rows are 16-byte aligned (``wide``)
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool wide, float (&x)[8]) {
+  if (wide) {
+    unpack8(*reinterpret_cast<const uint4*>(p), x);
+  } else {
 #pragma unroll
-  for (int n = 0; n < 8; ++n) x[n] = __bfloat162float(p[n]);
+    for (int n = 0; n < 8; ++n) x[n] = __bfloat162float(p[n]);
+  }
 }
 
 struct AppendArgs {
@@ -121,10 +129,10 @@ struct AppendArgs {
 // share one phase of angles, one per thread and half; with few rows one row per CTA spreads
 // them over the SMs (latency).
 template <int R>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, R > 1 ? 4 : 1) append_kernel(const AppendArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float cs[R][64], sn[R][64];
+  __shared__ __align__(16) float cs[R][64], sn[R][64];
   const int r0 = blockIdx.x * R, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid & 7;
   const int nr = min(R, a.rows - r0);
   if (a.inv_freq) {
@@ -140,25 +148,44 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     __syncthreads();
   }
   const int Hkv = a.pool.Hkv, nh = a.Hq + 2 * Hkv, quads = (nh + 3) >> 2;
-  for (int u = warp; u < nr * quads; u += 8) {
-    const int ri = u / quads, r = r0 + ri, h = 4 * (u - ri * quads) + (lane >> 3);
+  // the next unit's loads are in flight while one is finished
+  auto source = [&](int ri, int quad) {
+    return a.qkv + static_cast<size_t>(r0 + ri) * a.ldq + min(4 * quad + (lane >> 3), nh - 1) * 128 + 8 * l;
+  };
+  auto step = [&](int& ri, int& quad) {  // eight units on
+    for (quad += 8; quad >= quads; quad -= quads) ++ri;
+  };
+  uint4 xl = {}, xh = {};
+  int nri = 0, nquad = warp - 8;
+  step(nri, nquad);
+  if (a.wide && nri < nr) {
+    const __nv_bfloat16* src = source(nri, nquad);
+    xl = *reinterpret_cast<const uint4*>(src);
+    xh = *reinterpret_cast<const uint4*>(src + 64);
+  }
+  while (nri < nr) {
+    const int ri = nri, r = r0 + ri, quad = nquad, h = 4 * quad + (lane >> 3);
     const bool live = h < nh;
     const int hc = live ? h : nh - 1;  // lanes past the last head keep the shuffles whole
-    const __nv_bfloat16* src = a.qkv + static_cast<size_t>(r) * a.ldq + hc * 128 + 8 * l;
+    step(nri, nquad);
     float lo[8], hi[8];
     if (a.wide) {
-      const uint4 x = *reinterpret_cast<const uint4*>(src), y = *reinterpret_cast<const uint4*>(src + 64);
-      unpack8(x, lo);
-      unpack8(y, hi);
+      unpack8(xl, lo);
+      unpack8(xh, hi);
+      if (nri < nr) {
+        const __nv_bfloat16* src = source(nri, nquad);
+        xl = *reinterpret_cast<const uint4*>(src);
+        xh = *reinterpret_cast<const uint4*>(src + 64);
+      }
     } else {
-      load8(src, lo);
-      load8(src + 64, hi);
+      load8(source(ri, quad), false, lo);
+      load8(source(ri, quad) + 64, false, hi);
     }
     const bool is_q = hc < a.Hq, is_v = hc >= a.Hq + Hkv;
     if (a.bias) {
       float bl[8], bh[8];
-      load8(a.bias + hc * 128 + 8 * l, bl);
-      load8(a.bias + hc * 128 + 64 + 8 * l, bh);
+      load8(a.bias + hc * 128 + 8 * l, a.wide, bl);
+      load8(a.bias + hc * 128 + 64 + 8 * l, a.wide, bh);
 #pragma unroll
       for (int n = 0; n < 8; ++n) lo[n] += bl[n], hi[n] += bh[n];
     }
@@ -172,19 +199,24 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
       if (!is_v && nw) {
         const float inv = 1.0f / sqrtf(ss / 128.0f + a.eps);
         float wl[8], wh[8];
-        load8(nw + 8 * l, wl);
-        load8(nw + 64 + 8 * l, wh);
+        load8(nw + 8 * l, a.wide, wl);
+        load8(nw + 64 + 8 * l, a.wide, wh);
 #pragma unroll
         for (int n = 0; n < 8; ++n) lo[n] = lo[n] * inv * wl[n], hi[n] = hi[n] * inv * wh[n];
       }
     }
     if (a.inv_freq && !is_v) {
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float co = cs[ri][8 * l + n], si = sn[ri][8 * l + n];
-        const float y = lo[n] * co - hi[n] * si;
-        hi[n] = hi[n] * co + lo[n] * si;
-        lo[n] = y;
+      for (int n4 = 0; n4 < 8; n4 += 4) {
+        const float4 c4 = *reinterpret_cast<const float4*>(&cs[ri][8 * l + n4]);
+        const float4 s4 = *reinterpret_cast<const float4*>(&sn[ri][8 * l + n4]);
+        const float co[4] = {c4.x, c4.y, c4.z, c4.w}, si[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float y = lo[n4 + n] * co[n] - hi[n4 + n] * si[n];
+          hi[n4 + n] = hi[n4 + n] * co[n] + lo[n4 + n] * si[n];
+          lo[n4 + n] = y;
+        }
       }
     }
     if (is_q && live) {
@@ -229,18 +261,16 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 
 // Read-back of listed slots as bf16 rows: eight lanes per (row, kv head), as in the append.
 __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slots, const int* __restrict__ seq,
-                                                     int rows_per_seq, long long n, Pool pool,
+                                                     int rows_per_seq, int rows, Pool pool,
                                                      __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                                                      long long row_stride, long long head_stride, int* err) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long u = static_cast<long long>(blockIdx.x) * 32 + (threadIdx.x >> 3);
-  if (u >= n) return;
-  const int l = threadIdx.x & 7;
-  const long long r = u / pool.Hkv;
-  const int h = static_cast<int>(u - r * pool.Hkv);
+  const unsigned r = blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int l = threadIdx.x & 7, h = blockIdx.y;
+  if (r >= static_cast<unsigned>(rows)) return;
   const int slot = slots[r];
-  const int b = seq ? seq[r] : static_cast<int>(r / rows_per_seq);
+  const int b = seq ? seq[r] : static_cast<int>(r) / rows_per_seq;
   const uint8_t* blk = slot >= 0 ? pool.block_of(b, slot, err, h == 0 && l == 0) : nullptr;
   uint4 o[4] = {};
   if (blk) {
@@ -302,9 +332,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
 constexpr int kWarps = 8;
 constexpr int kStages = 2;       // per warp
 constexpr int kStageBlocks = 2;  // 16-slot blocks per stage
-constexpr int kMaxSeqs = 512;    // sequences per launch (their lengths live in shared memory)
+constexpr int kCtas = 2;         // per SM
+constexpr float kSlack = 5.f;    // how far (in bits) the running maximum may grow before a rescale
+constexpr int kMaxSeqs = 256;    // sequences per launch (their lengths live in shared memory)
 constexpr int kMaxCtas = 320;
-constexpr int kMinBlocks = 16;   // blocks per CTA at least
+constexpr int kMinBlocks = 2 * kWarps;  // blocks per CTA at least
 constexpr int kHeadPitch = 132;  // floats between heads of a partial O (conflict-free float4 stores)
 constexpr int kPart = 8 * 128 + 16;  // floats of one partial: O[8][128], ref[8], sum[8]
 
@@ -335,6 +367,8 @@ struct Smem {
   uint8_t ring[kWarps][kStages][kStageBlocks * kBlock];
   float part[kWarps][8][kHeadPitch];
   float ref[kWarps][8], sum[kWarps][8];
+  uint4 q[2][4][32];  // a head's B operands: [parity of the segment][group][lane]
+  float xs[2][8];     // and its logits per unit of the MMAs' sums
   uint64_t full[kWarps][kStages];
   uint32_t mask[kWarps][kStages];
   int first[kMaxSeqs + 1];  // first block of each sequence's first head
@@ -349,6 +383,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same with a zero accumulator
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -390,13 +432,15 @@ struct Segment {
     n = min(nsb - sb0, end - pos);
   }
   // blocks per stage: short segments are spread over all warps
-  __device__ __forceinline__ int per() const { return n <= kWarps ? 1 : kStageBlocks; }
+  __device__ __forceinline__ int per() const {
+    return n <= kWarps ? 1 : kStageBlocks;
+  }
 };
 
 // The lengths' prefix sums into shared memory; returns the number of blocks of all heads.
 __device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
   const int B = a.pool.B, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kEach = kMaxSeqs / (kWarps * 32);
+  constexpr int kEach = (kMaxSeqs + kWarps * 32 - 1) / (kWarps * 32);
   int v[kEach], t = 0;
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
@@ -434,7 +478,8 @@ __device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
   return total;
 }
 
-__global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a) {
+template <bool kScore>
+__global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -459,7 +504,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
   //    are not waited for; lane i < cnt follows the stage's block i (page index pi, block
   //    ``inner`` of the page), which moves by whole turns of the warps within a segment
   const int ppb = a.pool.page >> 4;  // blocks per page
-  const size_t page_bytes = static_cast<size_t>(Hkv) * ppb * kBlock;
   constexpr int kTurn = kWarps * kStageBlocks;
   const int turn_pages = kTurn / ppb, turn_inner = kTurn - turn_pages * ppb;
   Segment is;
@@ -474,26 +518,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
   }
   is.at(sm, Hkv, start, end);
   Segment cs = is;
-  int ipos = start, left = 0;  // left: blocks of the segment from this warp's next stage on
-  bool have = false, live = false;
-  int slot = 0, pi = 0, inner = 0, cnt = 0, page = -1, in_page = 0, is_len = 0;
-  const uint8_t* ihead = nullptr;
-  const uint8_t* iaddr = nullptr;
-  const int* itable = nullptr;
-  const int* islots = nullptr;
+  int ipos = start, left;  // left: blocks of the segment from this warp's stage on
+  bool have = true, live;
+  int slot, pi, inner, cnt, page;
   auto enter = [&]() {  // this warp's first stage of segment ``is``
-    const int per = is.per(), k = warp * per;
+    const int k = warp * is.per();
     left = is.n - k;
     slot = (is.sb0 + k) * 16 + lane;
     const int blk = is.sb0 + k + (lane < kStageBlocks ? lane : 0);
     pi = blk / ppb;
     inner = blk - pi * ppb;
-    is_len = sm.len[is.b];
-    ihead = a.pool.base + static_cast<size_t>(is.h) * ppb * kBlock;
-    itable = a.pool.table + static_cast<size_t>(is.b) * a.pool.max_pages;
-    islots = a.slot_pos ? a.slot_pos + static_cast<size_t>(is.b) * a.S : nullptr;
   };
-  auto fetch = [&]() {
+  auto look = [&]() {  // at the stage ``left`` points to, or the next segment's first
     while (left <= 0) {
       ipos += is.n;
       if (ipos >= end) {
@@ -503,94 +539,95 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
       is.at(sm, Hkv, ipos, end);
       enter();
     }
-    const int per = is.per();
-    cnt = min(per, left);
-    live = lane < cnt * 16 && slot < is_len;
-    if (live && islots) live = islots[slot] >= 0;
-    page = lane < cnt ? itable[pi] : -1;
-    in_page = inner;
-    iaddr = ihead;
-    have = true;
-    left -= kWarps * per;  // a segment of one-block stages has one turn only
-    slot += kTurn * 16;
-    pi += turn_pages;
-    inner += turn_inner;
-    if (inner >= ppb) inner -= ppb, ++pi;
+    cnt = min(is.per(), left);
+    live = lane < cnt * 16 && slot < sm.len[is.b];
+    if (a.slot_pos && live) live = a.slot_pos[static_cast<size_t>(is.b) * a.S + slot] >= 0;
+    page = lane < cnt ? a.pool.table[static_cast<size_t>(is.b) * a.pool.max_pages + pi] : -1;
   };
-  auto issue = [&](int st) {
+  auto issue = [&](int st) {  // the stage last looked at, and on to the next
     if (!have) return;
     const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.n_pages);
     const uint32_t okm = __ballot_sync(0xffffffffu, ok);
-    if (okm != (1u << cnt) - 1u && lane < cnt && !ok) set_err(a.err, kErrIndex);
-    const uint32_t mask = __ballot_sync(0xffffffffu, live && ((okm >> (lane >> 4)) & 1u));
+    uint32_t mask = __ballot_sync(0xffffffffu, live);
+    if (okm != (1u << cnt) - 1u) {  // a page out of range: its slots are masked
+      if (lane < cnt && !ok) set_err(a.err, kErrIndex);
+      mask &= (okm & 1u ? 0x0000ffffu : 0u) | (okm & 2u ? 0xffff0000u : 0u);
+    }
     if (lane == 0) {
       sm.mask[warp][st] = mask;
       mbar_expect_tx(&sm.full[warp][st], __popc(okm) * kBlock);
     }
     __syncwarp();
     if (ok)
-      bulk_load(sm.ring[warp][st] + lane * kBlock, iaddr + page * page_bytes + in_page * kBlock, kBlock,
+      bulk_load(sm.ring[warp][st] + lane * kBlock,
+                a.pool.base + ((static_cast<size_t>(page) * Hkv + is.h) * ppb + inner) * kBlock, kBlock,
                 &sm.full[warp][st]);
+    left -= kWarps * is.per();  // a segment of smaller stages has one turn only
+    slot += kTurn * 16;
+    pi += turn_pages;
+    inner += turn_inner;
+    if (inner >= ppb) inner -= ppb, ++pi;
+    look();
   };
   enter();
-  fetch();
+  look();
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) {
-    issue(s);
-    if (have) fetch();
-  }
+  for (int s = 0; s < kStages; ++s) issue(s);
 
-  int st = 0, phase = 0;  // the stage consumed next
-  bool dead = false;      // a copy never arrived: stop streaming, keep the barriers
+  // q of a segment's head as the MMA's B operands, heads on the columns: one warp's work
+  auto prepare_q = [&](const Segment& s, int buf) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(s.b) * a.Hq + s.h * group + g) * 128);
+    uint4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = g < group ? src[4 * j + t] : make_uint4(0, 0, 0, 0);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, max((ws[k] >> 16) & 0x7fffu, ws[k] & 0x7fffu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^up brings the head's largest |q| to [2^14, 2^15)
+    const int up = min(14 + 127 - static_cast<int>(top >> 7), 126);
+    const float f = __int_as_float((up + 127) << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d[8] = {bf16lo(w[j].x) * f, bf16hi(w[j].x) * f, bf16lo(w[j].y) * f, bf16hi(w[j].y) * f,
+                          bf16lo(w[j].z) * f, bf16hi(w[j].z) * f, bf16lo(w[j].w) * f, bf16hi(w[j].w) * f};
+      sm.q[buf][j][lane] = make_uint4(half2_bits(__floats2half2_rn(d[0], d[4])), half2_bits(__floats2half2_rn(d[1], d[5])),
+                                      half2_bits(__floats2half2_rn(d[2], d[6])), half2_bits(__floats2half2_rn(d[3], d[7])));
+    }
+    // logits in units of ln 2 per unit of the sums: scale log2(e) / 2^up, in two factors
+    // (2^-up alone can overflow)
+    if (t == 0)
+      sm.xs[buf][g] = a.scale * 1.4426950408889634f * __int_as_float((127 - (up >> 1)) << 23) *
+                      __int_as_float((127 - (up - (up >> 1))) << 23);
+  };
+  if (warp == kWarps - 1) prepare_q(cs, 0);
+  __syncthreads();
+
+  int st = 0, phase = 0, buf = 0;  // the stage consumed next; the segment's q
+  bool dead = false;               // a copy never arrived: stop streaming, keep the barriers
   const int sg = 4 * (g >> 1) + (g & 1);  // slot (of 16) of MMA row g; row g + 8 is slot sg + 2
   for (int pos = start; pos < end;) {
-    // q of this head as the MMA's B operand [group j][step u][2], heads on the columns
-    uint32_t qf[4][2][2];
-    float xs[2];
-    {
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(cs.b) * a.Hq + cs.h * group + g) * 128);
-      uint4 w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = g < group ? src[4 * j + t] : make_uint4(0, 0, 0, 0);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max((ws[k] >> 16) & 0x7fffu, ws[k] & 0x7fffu));
-      }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^up brings the head's largest |q| to [2^14, 2^15)
-      const int up = min(14 + 127 - static_cast<int>(top >> 7), 126);
-      const float f = __int_as_float((up + 127) << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float d[8] = {bf16lo(w[j].x) * f, bf16hi(w[j].x) * f, bf16lo(w[j].y) * f, bf16hi(w[j].y) * f,
-                            bf16lo(w[j].z) * f, bf16hi(w[j].z) * f, bf16lo(w[j].w) * f, bf16hi(w[j].w) * f};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            qf[j][u][e] = half2_bits(__floats2half2_rn(d[2 * u + e], d[2 * u + e + 4]));
-      }
-      // a thread's C columns are heads 2 t and 2 t + 1: logits in units of ln 2 per unit of
-      // their sums, scale log2(e) / 2^up, in two factors (2^-up alone can overflow)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int upe = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
-        xs[e] = a.scale * 1.4426950408889634f * __int_as_float((127 - (upe >> 1)) << 23) *
-                __int_as_float((127 - (upe - (upe >> 1))) << 23);
-      }
+    Segment next = cs;
+    if (pos + cs.n < end) {
+      next.at(sm, Hkv, pos + cs.n, end);
+      if (warp == kWarps - 1) prepare_q(next, buf ^ 1);
     }
+    const float xs[2] = {sm.xs[buf][2 * t], sm.xs[buf][2 * t + 1]};
     float o[8][4], l[2] = {0.f, 0.f}, ref[2] = {-INFINITY, -INFINITY};
+    float lim[2] = {-INFINITY, -INFINITY};  // ref + e: the largest logit that needs no rescale
+    uint32_t fields = 0;                    // or of the V scales' exponent fields so far
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
 
     const int per = cs.per();
-    float* lg = a.logits && 2 * t < a.gs
+    float* lg = kScore && 2 * t < a.gs
                     ? a.logits + (static_cast<size_t>(cs.b * Hkv + cs.h) * a.s16 + cs.sb0 * 16 + sg) * a.gs + 2 * t
                     : nullptr;
     for (int k = warp * per; k < cs.n; k += kWarps * per) {
@@ -604,11 +641,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
       }
       const uint32_t mask = dead ? 0u : sm.mask[warp][st];
       const uint8_t* base = sm.ring[warp][st];
-      float x[kStageBlocks][4];
-      const bool all = mask == 0xffffffffu;  // every slot of a whole stage is live
+      auto process = [&](auto full_stage) {
+        constexpr bool kFull = decltype(full_stage)::value;  // no mask, no missing block
+        // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3) of a block, zero
+        // where masked (the memory may hold anything)
+        auto v_scales = [&](int bl, int h) {
+          uint4 v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
+          if (!kFull) {
+            const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
+            const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+            v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
+          }
+          return v;
+        };
+        float x[kStageBlocks][4], top[2] = {-INFINITY, -INFINITY};
+        uint32_t bits = 0;
 #pragma unroll
-      for (int bl = 0; bl < kStageBlocks; ++bl) {
-        if (bl < nb) {
+        for (int bl = 0; bl < kStageBlocks; ++bl) {
+          if (!kFull && bl >= nb) break;
           const uint8_t* blk = base + bl * kBlock;
           const uint4 k0 = *reinterpret_cast<const uint4*>(blk + 64 * sg + 16 * t);
           const uint4 k1 = *reinterpret_cast<const uint4*>(blk + 64 * (sg + 2) + 16 * t);
@@ -617,104 +667,91 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
           const float2 f0[2] = {__half22float2(bits_half2(s0.x)), __half22float2(bits_half2(s0.y))};
           const float2 f1[2] = {__half22float2(bits_half2(s1.x)), __half22float2(bits_half2(s1.y))};
-          float y[4] = {0.f, 0.f, 0.f, 0.f};
+          float y[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            float c[4];
+            const uint4 qf = sm.q[buf][j][lane];
             const uint32_t u0 = w0[j] >> 8, u1 = w1[j] >> 8;
-            mma_f16(c, code_pair(w0[j]), code_pair(w1[j]), code_pair_hi(w0[j]), code_pair_hi(w1[j]), qf[j][0][0],
-                    qf[j][0][1]);
-            mma_f16(c, code_pair(u0), code_pair(u1), code_pair_hi(u0), code_pair_hi(u1), qf[j][1][0], qf[j][1][1]);
+            mma_f16_new(c, code_pair(w0[j]), code_pair(w1[j]), code_pair_hi(w0[j]), code_pair_hi(w1[j]), qf.x,
+                        qf.y);
+            mma_f16(c, code_pair(u0), code_pair(u1), code_pair_hi(u0), code_pair_hi(u1), qf.z, qf.w);
             const float a0 = j & 1 ? f0[j >> 1].y : f0[j >> 1].x, a1 = j & 1 ? f1[j >> 1].y : f1[j >> 1].x;
-            y[0] += a0 * c[0];
-            y[1] += a0 * c[1];
-            y[2] += a1 * c[2];
-            y[3] += a1 * c[3];
+            y[0] = j ? y[0] + a0 * c[0] : a0 * c[0];
+            y[1] = j ? y[1] + a0 * c[1] : a0 * c[1];
+            y[2] = j ? y[2] + a1 * c[2] : a1 * c[2];
+            y[3] = j ? y[3] + a1 * c[3] : a1 * c[3];
           }
           x[bl][0] = y[0] * xs[0];
           x[bl][1] = y[1] * xs[1];
           x[bl][2] = y[2] * xs[0];
           x[bl][3] = y[3] * xs[1];
-          if (!all) {
+          if (!kFull) {
             const uint32_t m = mask >> (16 * bl + sg);
             if (!(m & 1u)) x[bl][0] = x[bl][1] = -INFINITY;
             if (!(m & 4u)) x[bl][2] = x[bl][3] = -INFINITY;
           }
-          if (lg) {
+          if (kScore && lg) {
             float* to = lg + (k + bl) * 16 * a.gs;
             *reinterpret_cast<float2*>(to) = make_float2(x[bl][0], x[bl][1]);
             *reinterpret_cast<float2*>(to + 2 * a.gs) = make_float2(x[bl][2], x[bl][3]);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[bl][e] = -INFINITY;
+          top[0] = fmaxf(top[0], fmaxf(x[bl][0], x[bl][2]));
+          top[1] = fmaxf(top[1], fmaxf(x[bl][1], x[bl][3]));
+          const uint4 v0 = v_scales(bl, 0), v1 = v_scales(bl, 1);
+          bits |= v0.x | v0.y | v0.z | v0.w | v1.x | v1.y | v1.z | v1.w;
         }
-      }
-      // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3), zero where
-      // masked (the memory may hold anything).  Their exponent fields or-ed together are at
-      // least the largest: e only has to be small enough, and it stays above -4.
-      uint4 sv[kStageBlocks][2];
-      uint32_t bits = 0;
+        // Rescale where a weight would pass 2^e, then with kSlack bits to spare: most stages only
+        // vote.  e keeps P * scale below 2^14 through the V scales' exponent fields or-ed
+        // together (at least the largest; it has to be small enough only, and stays above -4).
+        bits &= 0x7c007c00u;
+        if (__any_sync(0xffffffffu, (bits & ~fields) || top[0] > lim[0] || top[1] > lim[1])) {
+          fields |= __reduce_or_sync(0xffffffffu, bits);
+          fields |= fields >> 16 | fields << 16;
+          const float e = static_cast<float>(min(15, 28 - static_cast<int>(fields >> 26)));
+          float f[2];
 #pragma unroll
-      for (int bl = 0; bl < kStageBlocks; ++bl)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (bl < nb) v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
-          if (!all) {
-            const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
-            const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-            v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
+          for (int c = 0; c < 2; ++c) {
+            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+            const float r = top[c] - e > ref[c] ? top[c] - e + kSlack : ref[c];
+            f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
+            ref[c] = r;
+            lim[c] = r + e;
+            l[c] *= f[c];
           }
-          sv[bl][h] = v;
-          bits |= v.x | v.y | v.z | v.w;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
         }
-      bits = __reduce_or_sync(0xffffffffu, bits);
-      const int e = min(15, 28 - static_cast<int>(((bits | bits >> 16) >> 10) & 31u));  // P * scale < 2^14
-      float f[2];
+        const float r0 = ref[0] == -INFINITY ? 0.f : ref[0], r1 = ref[1] == -INFINITY ? 0.f : ref[1];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float m = fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        const float r = fmaxf(ref[c], m - static_cast<float>(e));
-        f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
-        ref[c] = r;
-        l[c] *= f[c];
-      }
-      if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+        for (int bl = 0; bl < kStageBlocks; ++bl) {
+          if (!kFull && bl >= nb) break;
+          const uint8_t* blk = base + bl * kBlock;
+          const float p0 = ex2(x[bl][0] - r0), p1 = ex2(x[bl][1] - r1), p2 = ex2(x[bl][2] - r0), p3 = ex2(x[bl][3] - r1);
+          l[0] += p0 + p2;
+          l[1] += p1 + p3;
+          const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
+          const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
+          const uint4 s0 = v_scales(bl, 0), s1 = v_scales(bl, 1);
+          const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t);
+          const uint4 v1 = *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t);
+          const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb[4] = {s1.x, s1.y, s1.z, s1.w};
+          const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
-      }
-      const float r0 = ref[0] == -INFINITY ? 0.f : ref[0], r1 = ref[1] == -INFINITY ? 0.f : ref[1];
-#pragma unroll
-      for (int bl = 0; bl < kStageBlocks; ++bl) {
-        if (bl >= nb) continue;
-        const uint8_t* blk = base + bl * kBlock;
-        const float p0 = ex2(x[bl][0] - r0), p1 = ex2(x[bl][1] - r1), p2 = ex2(x[bl][2] - r0), p3 = ex2(x[bl][3] - r1);
-        l[0] += p0 + p2;
-        l[1] += p1 + p3;
-        const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
-        const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
-        const uint4 s0 = sv[bl][0], s1 = sv[bl][1];
-        const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t);
-        const uint4 v1 = *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t);
-        const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb4[4] = {s1.x, s1.y, s1.z, s1.w};
-        const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t c0 = half2_bits(__hmul2(b0, bits_half2(sa[i]))), c1 = half2_bits(__hmul2(b1, bits_half2(sb4[i])));
-          const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
-          mma_f16(o[2 * i], code_pair(w0[i]), code_pair_hi(w0[i]), code_pair(w1[i]), code_pair_hi(w1[i]), c0, c1);
-          mma_f16(o[2 * i + 1], code_pair(u0), code_pair_hi(u0), code_pair(u1), code_pair_hi(u1), c0, c1);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t c0 = half2_bits(__hmul2(b0, bits_half2(sa[i]))), c1 = half2_bits(__hmul2(b1, bits_half2(sb[i])));
+            const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
+            mma_f16(o[2 * i], code_pair(w0[i]), code_pair_hi(w0[i]), code_pair(w1[i]), code_pair_hi(w1[i]), c0, c1);
+            mma_f16(o[2 * i + 1], code_pair(u0), code_pair_hi(u0), code_pair(u1), code_pair_hi(u1), c0, c1);
+          }
         }
-      }
+      };
+      if (mask == 0xffffffffu) process(std::true_type{});  // every slot of a whole stage is live
+      else process(std::false_type{});
       __syncwarp();
-      if (!dead) {
-        issue(st);
-        if (have) fetch();
-      }
+      if (!dead) issue(st);
       if (++st == kStages) st = 0, phase ^= 1;
     }
 
@@ -774,21 +811,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_kernel(const AttnArgs a
       }
     }
     pos += cs.n;
-    if (pos < end) {
-      cs.at(sm, Hkv, pos, end);
-      __syncthreads();  // the parts have been read: the next segment may write its own
-    }
+    cs = next;
+    buf ^= 1;
+    // the parts have been read, so the next segment may write its own; its q is in place
+    if (pos < end) __syncthreads();
   }
 }
 
-// Finishes what the streaming kernel left: CTAs x < Hkv join the parts of head (x, sequence)
-// (or write zeros for an empty sequence); the others form the eviction score of 256 slots of
-// a sequence from the logits and the final (ref, sum) of its heads.  One launch for both:
-// they are short and latency-bound, so loads are issued as early and as many as possible.
+// Finishes what the streaming kernel left: CTAs x < ceil(Hq / 2) join the parts of two query
+// heads of a sequence (or write zeros for an empty one), four warps a head with a quarter of
+// the parts each; the others form the eviction score of 256 slots of a sequence from the
+// logits and the final (ref, sum) of its heads.  One launch for both: they are short and
+// latency-bound, so loads are issued as early and as many as possible.
 __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ float2 fin[];  // (ref, 1 / sum) of every query head of the sequence
+  __shared__ float4 quarter[8][32];
+  __shared__ float qsum[8];
   const int Hkv = a.pool.Hkv, group = a.Hq / Hkv, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int R = a.header[0], first = a.header[2 + b], nsb = (a.header[2 + b + 1] - first) / Hkv;
   // the part of head (b, h), first block s0, that CTA c left: in the CTA's first place where
@@ -801,57 +841,57 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
     L = L * (M == top ? 1.0f : ex2(M - top)) + l * (m == top ? 1.0f : ex2(m - top));
     M = top;
   };
-  if (static_cast<int>(blockIdx.x) < Hkv) {
-    const int h = blockIdx.x;
-    if (warp >= group) return;  // one query head per warp, four dims per lane
-    __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + h * group + warp) * 128 + 4 * lane;
-    if (nsb == 0) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
-      return;
-    }
-    const int s0 = first + h * nsb, c0 = s0 / R, c1 = (s0 + nsb - 1) / R;
-    if (c0 == c1) return;
+  const int pairs = (a.Hq + 1) >> 1;
+  if (static_cast<int>(blockIdx.x) < pairs) {
+    const int q = min(2 * static_cast<int>(blockIdx.x) + (warp >> 2), a.Hq - 1), mine = warp & 3;
+    const int h = q / group, w = q - h * group;
+    const int s0 = first + h * nsb, c0 = nsb ? s0 / R : 0, c1 = nsb ? (s0 + nsb - 1) / R : 0;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts at a time: lane i the (ref, sum) of part i
-      const int nc = min(32, c1 - cb + 1);
-      float rw = -INFINITY, lw = 0.f;
-      if (lane < nc) {
-        const float* p = part_of(cb + lane, s0);
-        rw = p[1024 + warp], lw = p[1032 + warp];
-      }
-      float top = fmaxf(M, rw);
+    if (c0 < c1) {
+      for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, part_of(c, s0)[1024 + w]);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float f = M == top ? 1.0f : ex2(M - top);
-      M = top;
-      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-      const float fw = rw == top ? 1.0f : ex2(rw - top);
-      float add = lw * fw;
+      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      for (int cb = c0 + mine; cb <= c1; cb += 16) {
+        float4 v[4];
+        float rw[4], lw[4];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
-      L = L * f + add;
-      for (int i = 0; i < nc; i += 8) {
-        float4 v[8];
+        for (int u = 0; u < 4; ++u) {
+          const int c = cb + 4 * u;
+          const float* p = part_of(min(c, c1), s0);
+          v[u] = *reinterpret_cast<const float4*>(p + w * 128 + 4 * lane);
+          rw[u] = p[1024 + w];
+          lw[u] = p[1032 + w];
+        }
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          v[u] = i + u < nc ? *reinterpret_cast<const float4*>(part_of(cb + i + u, s0) + warp * 128 + 4 * lane)
-                            : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float g = __shfl_sync(0xffffffffu, fw, (i + u) & 31);
-          if (i + u < nc) acc.x += v[u].x * g, acc.y += v[u].y * g, acc.z += v[u].z * g, acc.w += v[u].w * g;
+        for (int u = 0; u < 4; ++u) {
+          if (cb + 4 * u > c1) break;
+          const float f = rw[u] == M ? 1.0f : ex2(rw[u] - M);
+          L += lw[u] * f;
+          acc.x += v[u].x * f, acc.y += v[u].y * f, acc.z += v[u].z * f, acc.w += v[u].w * f;
         }
       }
     }
+    quarter[warp][lane] = acc;
+    if (lane == 0) qsum[warp] = L;
+    __syncthreads();
+    // written by the streaming kernel where one CTA had the whole head; the last head's twin
+    // of an odd count writes what the head itself writes
+    if (mine || (nsb && c0 == c1)) return;
+    for (int u = 1; u < 4; ++u) {
+      const float4 v = quarter[warp + u][lane];
+      L += qsum[warp + u];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    }
     const bool none = L == 0.f;
     const float r = none ? 0.f : 1.0f / L;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
-    if (none && lane == 0) set_err(a.err, kErrNoValidSlot);
+    __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + q) * 128 + 4 * lane;
+    *reinterpret_cast<uint2*>(dst) = none ? make_uint2(0, 0) : make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
+    if (none && nsb && lane == 0) set_err(a.err, kErrNoValidSlot);
     return;
   }
-  const int s = (blockIdx.x - Hkv) * 256 + threadIdx.x;
-  if (static_cast<int>(blockIdx.x - Hkv) * 256 >= nsb * 16) return;
+  const int s = (blockIdx.x - pairs) * 256 + threadIdx.x;
+  if (static_cast<int>(blockIdx.x - pairs) * 256 >= nsb * 16) return;
   const bool mine = s < nsb * 16 && s < a.S;
   // eight threads per query head, the parts over them
   const int sub = threadIdx.x & 7;
@@ -936,7 +976,8 @@ static long long workspace_bytes(int B, int Hq, int Hkv, int limit, bool score) 
 static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const void* q, const int* lens,
                   const int* slot_pos, int S, float scale, void* out, float* step_score, void* ws, long long ws_bytes,
                   int* err) {
-  const int sms = prepare_device(reinterpret_cast<const void*>(attend_kernel), sizeof(Smem));
+  auto kernel = step_score ? attend_kernel<true> : attend_kernel<false>;
+  const int sms = prepare_device(reinterpret_cast<const void*>(kernel), sizeof(Smem));
   if (sms <= 0) return fail(kStatusCuda, "kv4_attn: no usable CUDA device");
   cudaError_t e;
   const int Hkv = pool.Hkv, group = Hq / Hkv;
@@ -971,12 +1012,12 @@ static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const vo
     a.gs = floats_per_row(group);
     const long long line = static_cast<long long>(a.pool.B) * Hkv * nsb;
     long long grid = (line + kMinBlocks - 1) / kMinBlocks;
-    const int most = 2 * sms < kMaxCtas ? 2 * sms : kMaxCtas;
+    const int most = kCtas * sms < kMaxCtas ? kCtas * sms : kMaxCtas;
     grid = grid < 1 ? 1 : grid > most ? most : grid;
-    e = launch_pdl(attend_kernel, dim3(static_cast<unsigned>(grid)), dim3(kWarps * 32), sizeof(Smem), stream, dim3(0), a);
+    e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kWarps * 32), sizeof(Smem), stream, dim3(0), a);
     if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
     const int chunks = step_score ? (nsb * 16 + 255) / 256 : 0;
-    e = launch_pdl(combine_kernel, dim3(Hkv + chunks, a.pool.B), dim3(256), step_score ? Hq * sizeof(float2) : 0, stream,
+    e = launch_pdl(combine_kernel, dim3((Hq + 1) / 2 + chunks, a.pool.B), dim3(256), step_score ? Hq * sizeof(float2) : 0, stream,
                    dim3(0), a);
     if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
   }
@@ -1032,10 +1073,11 @@ extern "C" int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_
   const kv4::AppendArgs a{static_cast<const __nv_bfloat16*>(qkv), static_cast<const __nv_bfloat16*>(bias),
                           static_cast<const __nv_bfloat16*>(q_norm_w), static_cast<const __nv_bfloat16*>(k_norm_w),
                           inv_freq, positions, slots, seq, p, static_cast<__nv_bfloat16*>(q_out), dev_err, ldq, rows,
-                          rows_per_seq, Hq, kv4::aligned16(qkv) && ldq % 8 == 0, eps};
+                          rows_per_seq, Hq,
+                          kv4::aligned16(qkv) && ldq % 8 == 0 && kv4::aligned16(bias) && kv4::aligned16(q_norm_w) && kv4::aligned16(k_norm_w), eps};
   const cudaError_t e =
       rows >= kv4::kManyRows
-          ? kvbp::launch_pdl(kv4::append_kernel<8>, dim3((rows + 7) / 8), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0), a)
+          ? kvbp::launch_pdl(kv4::append_kernel<8>, dim3((static_cast<unsigned>(rows) + 7) / 8), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0), a)
           : kvbp::launch_pdl(kv4::append_kernel<1>, dim3(rows), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), dim3(0), a);
   if (e != cudaSuccess) return fail(kvbp::kStatusCuda, "kv4_append launch: %s", cudaGetErrorString(e));
   return kvbp::kStatusOk;
@@ -1053,11 +1095,10 @@ extern "C" int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_
   if (row_stride < 128 || head_stride < 128 || row_stride % 8 || head_stride % 8 || !kv4::aligned16(k_out) ||
       !kv4::aligned16(v_out))
     return fail(kvbp::kStatusArg, "kv4_gather: output rows must be 128 apart or more and 16-byte aligned");
-  const long long n = static_cast<long long>(rows) * Hkv;
-  if ((n + 31) / 32 > 0x7fffffffll) return fail(kvbp::kStatusArg, "kv4_gather: too many rows");
+  if (Hkv > 65535) return fail(kvbp::kStatusArg, "kv4_gather: bad size");
   const cudaError_t e = kvbp::launch_pdl(
-      kv4::gather_kernel, dim3(static_cast<unsigned>((n + 31) / 32)), dim3(256), 0,
-      reinterpret_cast<cudaStream_t>(stream), dim3(0), slots, seq, rows_per_seq, n, p,
+      kv4::gather_kernel, dim3((static_cast<unsigned>(rows) + 31) / 32, Hkv), dim3(256), 0,
+      reinterpret_cast<cudaStream_t>(stream), dim3(0), slots, seq, rows_per_seq, rows, p,
       static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), static_cast<long long>(row_stride),
       static_cast<long long>(head_stride), dev_err);
   if (e != cudaSuccess) return fail(kvbp::kStatusCuda, "kv4_gather launch: %s", cudaGetErrorString(e));

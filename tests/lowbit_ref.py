@@ -83,9 +83,10 @@ def attend(pool, table, lens, q, slot_pos, scale):
     sum p |v|), and the fp32 logits: 32 products of |q| and codes up to 7 a group and four
     groups, 2^-21 of their absolute sum for the rounding chain, which is an absolute error dl
     of a logit and a relative one 2 dl of every probability.  A weight is carried
-    in f16 as 2^e p s, p <= 1 the largest, e = min(15, 28 - X) and X at most the or of the V
-    scales' exponent fields; below f16's normals it is rounded at 2^-25, so each slot may add
-    7 * 2^-(25 + e) (a code is at most 7, the weights' sum at least 1)."""
+    in f16 as at least 2^(e - 5) p s, p <= 1 the largest, e = min(15, 28 - X) and X at most the
+    or of the V scales' exponent fields (5 bits are kept for the maximum to grow); below f16's normals it is rounded at 2^-25, before (then times s) and
+    after the product, so each slot may add (1 + s) * 7 * 2^-(20 + e) (a code is at most 7, the
+    weights' sum at least 1)."""
     kv = values(pool)
     (_, sk), (_, sv) = decode(pool)
     B, hq, _ = q.shape
@@ -115,7 +116,7 @@ def attend(pool, table, lens, q, slot_pos, scale):
         dl = 2.0 ** -21 * abs(scale) * big.amax()
         drel[b] = 2 * dl + 2.0 ** -20
         field = int(np.bitwise_or.reduce(sv[pg, :, at % page].numpy().astype(np.float16).view(np.uint16).ravel())) >> 10 & 31
-        floor = 2.0 ** -(25 + min(15, 28 - field))
+        floor = (1 + sv[pg, :, at % page].max()) * 2.0 ** -(20 + min(15, 28 - field))
         bound[b] = (2.0 ** -8 * out[b].abs() + len(at) * 7 * floor +
                     (2.0 ** -10 + (len(at) / 128 + 16) * 2.0 ** -23 + 2 * drel[b]) * mass)
         score[b, at] = p.amax((0, 1))
