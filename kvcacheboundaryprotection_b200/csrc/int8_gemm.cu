@@ -11,9 +11,9 @@ namespace i8 {
 // fp32, so half-way values are half-way in any precision; a zero row gives zeros and scale
 // 0).  A row with a NaN or an infinity gets a scale that is not finite, and codes 0: every
 // output of that token is then NaN.  One CTA per row, the row kept in registers between the
-// maximum and the codes (kVec 16-byte vectors per thread cover K <= 16384; longer rows are
-// read again, from L2).
-constexpr int kVec = 8;
+// maximum and the codes (kVec 16-byte vectors per thread: K <= 2048 kVec; longer rows are read
+// again, from L2).  Latency-bound: few registers let many rows share an SM.
+template <int kVec>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int K,
                                                          int vec, int8_t* __restrict__ q, long long ldq,
                                                          float* __restrict__ scale) {
@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
   const bool fine = m > 0 && m < 0x7f800000u;
   if (tid == 0) scale[r] = top / 127.0f;
   // rint(127 x / top): x times the rounded factor plus 1.5 * 2^23 leaves the integer in the low
-  // mantissa bits.  The factor is off by 2^-24 of at most 127, so only what lies within 2^-8 of
-  // half-way can round wrongly: it is divided.
+  // mantissa bits.  The factor is off by 2^-24 of it, so a quotient (at most 127) by 8e-6: only
+  // what lies within 1e-4 of half-way can round wrongly, and is divided.
   const float factor = fine ? 127.0f / top : 0.f;
   auto code = [&](float v, float& worst) -> uint32_t {
     const float s = fmaf(v, factor, 12582912.0f);
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
     float worst = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) c[k] = code(x[k], worst);
-    if (!fine || worst > 0.49609375f) {
+    if (!fine || worst > 0.4999f) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) c[k] = exact(x[k]);
     }
@@ -108,6 +108,7 @@ struct Args {
 
 constexpr int kBK = 128;               // bytes (= codes) of K per stage: one swizzle atom
 constexpr int kTileW = 128 * kBK;      // weight tile
+constexpr int kMaxSplits = 8;          // a portable cluster
 constexpr int kThreads = 6 * 32;       // producer, MMA, four epilogue warps
 
 __host__ __device__ constexpr uint32_t idesc_i8(int N) {  // D s32, A and B s8, both K-major, M = 128
@@ -127,35 +128,35 @@ __device__ __forceinline__ int4 ld_dsmem_v4(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ void store(const Args& a, int m, int n, int acc, float sx, float sw, float bias) {
-  const float y = static_cast<float>(acc) * sx * sw + bias;
-  const size_t at = static_cast<size_t>(m) * a.ldo + n;
-  if (a.f32)
-    static_cast<float*>(a.out)[at] = y;
-  else
-    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-}
-// four channels from n on
-__device__ __forceinline__ void store4(const Args& a, int m, int n, int4 acc, float sx) {
-  if (a.vec && n < a.N) {  // N, ldo multiples of 4, pointers aligned
-    const float4 sw = *reinterpret_cast<const float4*>(a.sw + n);
-    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.bias) {
-      const uint2 w = *reinterpret_cast<const uint2*>(a.bias + n);
-      b = make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
-    }
-    const float4 y = make_float4(static_cast<float>(acc.x) * sx * sw.x + b.x, static_cast<float>(acc.y) * sx * sw.y + b.y,
-                                 static_cast<float>(acc.z) * sx * sw.z + b.z, static_cast<float>(acc.w) * sx * sw.w + b.w);
-    const size_t at = static_cast<size_t>(m) * a.ldo + n;
-    if (a.f32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = y;
-    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
-    return;
-  }
-  const int v[4] = {acc.x, acc.y, acc.z, acc.w};
+// scales and biases of channels n .. n + 3 (those below N)
+struct Four {
+  float sw[4], b[4];
+  __device__ __forceinline__ void load(const Args& a, int n) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (n + i < a.N) store(a, m, n + i, v[i], sx, a.sw[n + i], a.bias ? __bfloat162float(a.bias[n + i]) : 0.f);
-}
+    for (int i = 0; i < 4; ++i) {
+      sw[i] = n + i < a.N ? a.sw[n + i] : 0.f;
+      b[i] = a.bias && n + i < a.N ? __bfloat162float(a.bias[n + i]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(const Args& a, int m, int n, int4 acc, float sx) const {
+    const float y[4] = {static_cast<float>(acc.x) * sx * sw[0] + b[0], static_cast<float>(acc.y) * sx * sw[1] + b[1],
+                        static_cast<float>(acc.z) * sx * sw[2] + b[2], static_cast<float>(acc.w) * sx * sw[3] + b[3]};
+    const size_t at = static_cast<size_t>(m) * a.ldo + n;
+    float* f = static_cast<float*>(a.out) + at;
+    __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a.out) + at;
+    if (a.vec && n < a.N) {  // N, ldo multiples of 4, the output aligned
+      if (a.f32) *reinterpret_cast<float4*>(f) = make_float4(y[0], y[1], y[2], y[3]);
+      else *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) {
+        if (a.f32) f[i] = y[i];
+        else h[i] = __float2bfloat16_rn(y[i]);
+      }
+  }
+};
 // Barrier among ``nthreads`` threads; true on all of them when ``v`` is on any.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool v) {
   uint32_t r;
@@ -184,7 +185,7 @@ template <int NT>
 struct Ring {
   static constexpr int kStage = kTileW + NT * kBK;
   static constexpr int kStages = (NT <= 32 ? 5 : NT == 64 ? 4 : 3);
-  static constexpr int kBytes = kStages * kStage + 1024 + 256;
+  static constexpr int kBytes = kStages * kStage + 1024 + 256 + NT * 4;
   static_assert(kStages * kStage >= NT * 128 * 4, "the partial tile reuses the ring");
 };
 
@@ -200,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* done = empty + R::kStages;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
   int* bad = reinterpret_cast<int*>(tslot + 1);
+  float* sxs = reinterpret_cast<float*>(bad + 1);  // the tokens' scales
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = gridDim.x, rank = blockIdx.x;
   const int n0 = blockIdx.y * 128, m0 = blockIdx.z * NT;
@@ -281,46 +283,52 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool ok = wait_or_fail(done, 0) && healthy();
   tc_after();
   pdl_wait();  // before the scales are read and anything is written
-  const bool all_ok = !__syncthreads_or(!ok);
   const int cols = min(NT, a.M - m0);  // live tokens of the tile
-  int* part = reinterpret_cast<int*>(base);  // [token][128 channels], over the drained ring
+  if (tid < cols) sxs[tid] = a.sx[m0 + tid];
+  const bool all_ok = !__syncthreads_or(!ok);
+  // The accumulator goes through shared memory (the drained ring), [token][128 channels], so
+  // that the stores are 8 or 16 bytes a thread and run along the channels.  (Stored straight
+  // from TMEM, one channel a lane, the 128-token tile took 11 us for its 16 KiB.)
+  int* part = reinterpret_cast<int*>(base);
   if (warp >= 2 && all_ok) {
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const int ch = q * 32 + lane, n = n0 + ch;
+    int* mine = part + q * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
     constexpr int C = NT < 32 ? 16 : 32;
-    const float sw = n < a.N ? a.sw[n] : 0.f;
-    const float bias = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
 #pragma unroll 1
-    for (int c = 0; c < NT && c < cols; c += C) {
+    for (int c = 0; c < cols; c += C) {
       int v[C];
       ld_acc<C>(acc + c, v);
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        if (c + i >= cols) break;
-        if (S > 1) part[(c + i) * 128 + ch] = v[i];
-        else if (n < a.N) store(a, m0 + c + i, n, v[i], a.sx[m0 + c + i], sw, bias);
-      }
+      for (int i = 0; i < C; ++i) mine[(c + i) * 128] = v[i];
     }
   }
-  if (S > 1) {
-    cluster_sync_all();
-    // this CTA's share of the tile's live elements, four channels at a time
-    const int E = cols * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * E / S);
-    if (all_ok)
-      for (int e = static_cast<int>(static_cast<long long>(rank) * E / S) + tid; e < e1; e += kThreads) {
+  if (S > 1) cluster_sync_all();
+  else __syncthreads();
+  // this CTA's share of the tile's live elements, four channels at a time
+  const int E = cols * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * E / S);
+  if (all_ok) {
+    const int e0 = static_cast<int>(static_cast<long long>(rank) * E / S) + tid;
+    const int n = n0 + (e0 & 31) * 4;  // the same in every turn: kThreads is a multiple of 32
+    Four four;
+    four.load(a, n);
+#pragma unroll 2
+    for (int e = e0; e < e1; e += kThreads) {
+      int4 sum = make_int4(0, 0, 0, 0);
+      if (S > 1) {
         const uint32_t at = smem_u32(part + 4 * e);
-        int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 8
-        for (int r = 0; r < S; ++r) {
-          const int4 v = ld_dsmem_v4(mapa_u32(at, r));
-          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-        }
-        const int m = m0 + (e >> 5), n = n0 + (e & 31) * 4;
-        store4(a, m, n, sum, a.sx[m]);
+        int4 v[kMaxSplits];  // all peers' values before the first addition
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) v[r] = r < S ? ld_dsmem_v4(mapa_u32(at, r)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+      } else {
+        sum = *reinterpret_cast<const int4*>(part + 4 * e);
       }
-    cluster_sync_all();  // no CTA leaves while a peer may still read its part
+      four.store(a, m0 + (e >> 5), n, sum, sxs[e >> 5]);
+    }
   }
+  if (S > 1) cluster_sync_all();  // no CTA leaves while a peer may still read its part
   tc_before();
   __syncthreads();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
@@ -523,8 +531,9 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
   if (misaligned(q, 16) || ldq % 16) return fail(kStatusArg, "int8_quant_rows: q rows must be 16-byte aligned");
   // 16-byte loads where x's rows allow them, else one value at a time
   const int vec = !misaligned(x, 16) && ldx % 8 == 0;
-  const cudaError_t e = launch_pdl(quant_rows_kernel, dim3(rows), dim3(256), 0, st, dim3(0),
-                                   static_cast<const __nv_bfloat16*>(x), ldx, K, vec, static_cast<int8_t*>(q), ldq, scale);
+  auto kernel = K <= 4096 ? quant_rows_kernel<2> : K <= 10240 ? quant_rows_kernel<5> : quant_rows_kernel<8>;
+  const cudaError_t e = launch_pdl(kernel, dim3(rows), dim3(256), 0, st, dim3(0), static_cast<const __nv_bfloat16*>(x),
+                                   ldx, K, vec, static_cast<int8_t*>(q), ldq, scale);
   if (e != cudaSuccess) return fail(kStatusCuda, "int8_quant_rows launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
@@ -534,7 +543,7 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
 static int splits(long long tiles, int steps, int sms) {
   long long s = 2ll * sms / tiles;
   if (s > steps / 4) s = steps / 4;
-  return s < 1 ? 1 : s > 8 ? 8 : static_cast<int>(s);
+  return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : static_cast<int>(s);
 }
 
 static int check(const Args& a, const void* w, long long ldw, const void* xq, long long ldq) {
@@ -551,7 +560,7 @@ static int check(const Args& a, const void* w, long long ldw, const void* xq, lo
 
 static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const void* xq, long long ldq) {
   if (int bad = check(a, w, ldw, xq, ldq)) return bad;
-  a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.sw, 16) && !misaligned(a.bias, 8) && !misaligned(a.out, a.f32 ? 16 : 8);
+  a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
   const int sms = prepare_device(reinterpret_cast<const void*>(persist_kernel), kPBytes);
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
   const long long tn = (a.N + 127) / 128;
