@@ -71,16 +71,27 @@ __device__ __forceinline__ __half group_scale(uint32_t amax_bits) {
   if (amax_bits > 0x7f800000u) return __ushort_as_half(0x7fff);
   return __float2half_rn(fminf(__uint_as_float(amax_bits) / 7.0f, 65504.0f));
 }
-// eight codes as one 32-bit word: clip(rint(x / scale), -7, 7) + 8 each.  The quotient is
-// rounded to an integer by adding 1.5 * 2^23, which leaves it in the low mantissa bits.
-// Scale 0 (all values below the smallest f16 step) and NaN: code 8, the value 0 * scale.
+// eight codes as one 32-bit word: clip(rint(x / scale), -7, 7) + 8 each.  x times the rounded
+// reciprocal plus 1.5 * 2^23 leaves the integer in the low mantissa bits; only what lies within
+// 1e-4 of half-way can round wrongly (bf16 values over an f16 scale often are half-way), and is
+// divided.  Scale 0 (all values below the smallest f16 step) and NaN: code 8.
 __device__ __forceinline__ uint32_t eight_codes(const float (&x)[8], float scale) {
   const float inv = scale > 0.f ? 1.0f / scale : 0.f;
   uint32_t w = 0;
+  float worst = 0.f;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    const float q = fminf(fmaxf(x[n] * inv, -7.f), 7.f) + (12582912.0f + 8.0f);
+    const float v = fminf(fmaxf(x[n] * inv, -7.f), 7.f), q = v + (12582912.0f + 8.0f);
+    worst = fmaxf(worst, fabsf(v - (q - (12582912.0f + 8.0f))));
     w |= (__float_as_uint(q) & 15u) << (4 * n);
+  }
+  if (worst > 0.4999f) {
+    w = 0;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float q = scale > 0.f ? fminf(fmaxf(rintf(x[n] / scale), -7.f), 7.f) : 0.f;
+      w |= static_cast<uint32_t>(static_cast<int>(q) + 8) << (4 * n);
+    }
   }
   return w;
 }
@@ -123,8 +134,10 @@ struct AppendArgs {
 // so the RoPE pairs (d, d + 64) are its own, a group of 32 dims is four lanes and its eight
 // codes are one word of K.  Everything between the bf16 input and the stored value is fp32,
 // rounded once (q to bf16, k and v to their codes): the cache keeps 4 bits, so no bf16 step in
-// between is worth its error.  The angle pos * inv_freq is reduced in double: at position 4e5
-// an fp32 product would be off by up to 2e-2 rad.
+// between is worth its error.  Every product, sum and quotient is rounded by itself (no fused
+// multiply-add) and the angle pos * inv_freq and its cosine are double: the fp32 values, and so
+// the codes of those that sit at a code's border, are the ones that the formula gives step by
+// step.  (An fp32 angle would be off by up to 2e-2 rad at position 4e5.)
 // Bound by HBM on a prompt (reads qkv, writes q, 144 bytes per kv head): eight rows per CTA
 // share one phase of angles, one per thread and half; with few rows one row per CTA spreads
 // them over the SMs (latency).
@@ -140,10 +153,10 @@ __global__ void __launch_bounds__(256, R > 1 ? 4 : 1) append_kernel(const Append
       const int r = i >> 6, f = i & 63;
       const double turns =
           static_cast<double>(a.positions[r0 + r]) * static_cast<double>(a.inv_freq[f]) * 0.15915494309189533577;
-      float s, c;
-      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-      cs[r][f] = c;
-      sn[r][f] = s;
+      double s, c;
+      sincospi(2.0 * (turns - rint(turns)), &s, &c);
+      cs[r][f] = static_cast<float>(c);
+      sn[r][f] = static_cast<float>(s);
     }
     __syncthreads();
   }
@@ -190,19 +203,32 @@ __global__ void __launch_bounds__(256, R > 1 ? 4 : 1) append_kernel(const Append
       for (int n = 0; n < 8; ++n) lo[n] += bl[n], hi[n] += bh[n];
     }
     if (a.qnw || a.knw) {
-      float ss = 0.f;
+      // pairwise sum of squares: fours of dims, then halves of what is left onto each other
+      float f[2];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) ss += lo[n] * lo[n] + hi[n] * hi[n];
+      for (int k = 0; k < 2; ++k) {
+        float p = __fmul_rn(lo[4 * k], lo[4 * k]), q = __fmul_rn(hi[4 * k], hi[4 * k]);
 #pragma unroll
-      for (int o = 4; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        for (int n = 4 * k + 1; n < 4 * k + 4; ++n) {
+          p = __fadd_rn(p, __fmul_rn(lo[n], lo[n]));
+          q = __fadd_rn(q, __fmul_rn(hi[n], hi[n]));
+        }
+        f[k] = __fadd_rn(p, q);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) f[k] = __fadd_rn(f[k], __shfl_xor_sync(0xffffffffu, f[k], o));
+      }
+      const float ss = __fadd_rn(f[0], f[1]);
       const __nv_bfloat16* nw = is_q ? a.qnw : a.knw;
       if (!is_v && nw) {
-        const float inv = 1.0f / sqrtf(ss / 128.0f + a.eps);
+        const float rms = sqrtf(__fadd_rn(ss / 128.0f, a.eps)), inv = 1.0f / rms;
         float wl[8], wh[8];
         load8(nw + 8 * l, a.wide, wl);
         load8(nw + 64 + 8 * l, a.wide, wh);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) lo[n] = lo[n] * inv * wl[n], hi[n] = hi[n] * inv * wh[n];
+        for (int n = 0; n < 8; ++n) {  // keys become codes: their quotients are exact, q's within an ulp
+          lo[n] = __fmul_rn(is_q ? lo[n] * inv : lo[n] / rms, wl[n]);
+          hi[n] = __fmul_rn(is_q ? hi[n] * inv : hi[n] / rms, wh[n]);
+        }
       }
     }
     if (a.inv_freq && !is_v) {
@@ -213,8 +239,8 @@ __global__ void __launch_bounds__(256, R > 1 ? 4 : 1) append_kernel(const Append
         const float co[4] = {c4.x, c4.y, c4.z, c4.w}, si[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const float y = lo[n4 + n] * co[n] - hi[n4 + n] * si[n];
-          hi[n4 + n] = hi[n4 + n] * co[n] + lo[n4 + n] * si[n];
+          const float y = __fsub_rn(__fmul_rn(lo[n4 + n], co[n]), __fmul_rn(hi[n4 + n], si[n]));
+          hi[n4 + n] = __fadd_rn(__fmul_rn(hi[n4 + n], co[n]), __fmul_rn(lo[n4 + n], si[n]));
           lo[n4 + n] = y;
         }
       }
