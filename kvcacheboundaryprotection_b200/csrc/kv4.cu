@@ -396,7 +396,6 @@ struct Smem {
   uint4 q[2][4][32];  // a head's B operands: [parity of the segment][group][lane]
   float xs[2][8];     // and its logits per unit of the MMAs' sums
   uint64_t full[kWarps][kStages];
-  uint32_t mask[kWarps][kStages];
   int first[kMaxSeqs + 1];  // first block of each sequence's first head
   int len[kMaxSeqs];
   int wsum[kWarps];
@@ -547,6 +546,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
   int ipos = start, left;  // left: blocks of the segment from this warp's stage on
   bool have = true, live;
   int slot, pi, inner, cnt, page;
+  uint32_t masks[kStages];  // live slots of the stages in the ring
   auto enter = [&]() {  // this warp's first stage of segment ``is``
     const int k = warp * is.per();
     left = is.n - k;
@@ -579,10 +579,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
       if (lane < cnt && !ok) set_err(a.err, kErrIndex);
       mask &= (okm & 1u ? 0x0000ffffu : 0u) | (okm & 2u ? 0xffff0000u : 0u);
     }
-    if (lane == 0) {
-      sm.mask[warp][st] = mask;
-      mbar_expect_tx(&sm.full[warp][st], __popc(okm) * kBlock);
-    }
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) masks[s] = s == st ? mask : masks[s];
+    if (lane == 0) mbar_expect_tx(&sm.full[warp][st], __popc(okm) * kBlock);
     __syncwarp();
     if (ok)
       bulk_load(sm.ring[warp][st] + lane * kBlock,
@@ -665,7 +664,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
           mbar_wait_bounded(&sm.full[warp][(st + s) % kStages], phase ^ (st + s >= kStages), 1u << 16);
         __syncwarp();
       }
-      const uint32_t mask = dead ? 0u : sm.mask[warp][st];
+      uint32_t mask = masks[0];
+#pragma unroll
+      for (int s = 1; s < kStages; ++s) mask = s == st ? masks[s] : mask;
+      if (dead) mask = 0;
       const uint8_t* base = sm.ring[warp][st];
       auto process = [&](auto full_stage) {
         constexpr bool kFull = decltype(full_stage)::value;  // no mask, no missing block
@@ -854,7 +856,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
   pdl_wait();
   extern __shared__ float2 fin[];  // (ref, 1 / sum) of every query head of the sequence
   __shared__ float4 quarter[8][32];
-  __shared__ float qsum[8];
+  __shared__ float2 qsum[8];
   const int Hkv = a.pool.Hkv, group = a.Hq / Hkv, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int R = a.header[0], first = a.header[2 + b], nsb = (a.header[2 + b + 1] - first) / Hkv;
   // the part of head (b, h), first block s0, that CTA c left: in the CTA's first place where
@@ -874,41 +876,35 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
     const int s0 = first + h * nsb, c0 = nsb ? s0 / R : 0, c1 = nsb ? (s0 + nsb - 1) / R : 0;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto fold = [&](const float4 v, float m, float l) {
+      const float top = fmaxf(M, m), f = M == top ? 1.0f : ex2(M - top), g = m == top ? 1.0f : ex2(m - top);
+      M = top;
+      L = L * f + l * g;
+      acc.x = acc.x * f + v.x * g, acc.y = acc.y * f + v.y * g, acc.z = acc.z * f + v.z * g, acc.w = acc.w * f + v.w * g;
+    };
     if (c0 < c1) {
-      for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, part_of(c, s0)[1024 + w]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       for (int cb = c0 + mine; cb <= c1; cb += 16) {
         float4 v[4];
         float rw[4], lw[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int c = cb + 4 * u;
-          const float* p = part_of(min(c, c1), s0);
+          const float* p = part_of(min(cb + 4 * u, c1), s0);
           v[u] = *reinterpret_cast<const float4*>(p + w * 128 + 4 * lane);
           rw[u] = p[1024 + w];
           lw[u] = p[1032 + w];
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (cb + 4 * u > c1) break;
-          const float f = rw[u] == M ? 1.0f : ex2(rw[u] - M);
-          L += lw[u] * f;
-          acc.x += v[u].x * f, acc.y += v[u].y * f, acc.z += v[u].z * f, acc.w += v[u].w * f;
-        }
+        for (int u = 0; u < 4; ++u)
+          if (cb + 4 * u <= c1) fold(v[u], rw[u], lw[u]);
       }
     }
     quarter[warp][lane] = acc;
-    if (lane == 0) qsum[warp] = L;
+    if (lane == 0) qsum[warp] = make_float2(M, L);
     __syncthreads();
     // written by the streaming kernel where one CTA had the whole head; the last head's twin
     // of an odd count writes what the head itself writes
     if (mine || (nsb && c0 == c1)) return;
-    for (int u = 1; u < 4; ++u) {
-      const float4 v = quarter[warp + u][lane];
-      L += qsum[warp + u];
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    }
+    for (int u = 1; u < 4; ++u) fold(quarter[warp + u][lane], qsum[warp + u].x, qsum[warp + u].y);
     const bool none = L == 0.f;
     const float r = none ? 0.f : 1.0f / L;
     __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + q) * 128 + 4 * lane;

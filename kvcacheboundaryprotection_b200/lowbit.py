@@ -27,6 +27,7 @@ from .capi import check, lib
 BLOCK = 2304  # bytes of 16 slots of one kv head (KVBP_KV4_BLOCK)
 HEAD_DIM = 128
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_U8, _I8, _I32, _F32, _BF16 = torch.uint8, torch.int8, torch.int32, torch.float32, torch.bfloat16
 # the current stream's handle of a device index (torch.cuda.current_stream makes an object)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -72,26 +73,25 @@ def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) ->
         raise ValueError(f"page_size {page_size} is not a multiple of 16")
     if n_pages <= 0 or n_kv_heads <= 0:
         raise ValueError("n_pages and n_kv_heads must be > 0")
-    return torch.zeros(n_pages, n_kv_heads, page_size // 16, BLOCK, dtype=torch.uint8,
+    return torch.zeros(n_pages, n_kv_heads, page_size // 16, BLOCK, dtype=_U8,
                        device=torch.device("cuda") if device is None else device)
 
 
 def _pool(pool: torch.Tensor, table: torch.Tensor) -> tuple:
-    """(pages, kv heads, page size, sequences, pages per sequence) after the checks."""
-    dev = pool.device
-    if pool.dim() != 4 or table.dim() != 2:
+    """(pages, kv heads, page size, sequences, pages per sequence, device) after the checks."""
+    shape, tshape, dev = pool.shape, table.shape, pool.device
+    if len(shape) != 4 or len(tshape) != 2:
         raise ValueError("pool must be [pages, kv heads, blocks, 2304] and page_table [sequences, pages]")
-    n_pages, hkv, per, _ = pool.shape
-    B, width = table.shape
-    _need(pool, "pool", torch.uint8, dev, (n_pages, hkv, per, BLOCK))
-    _need(table, "page_table", torch.int32, dev, (B, width))
-    return n_pages, hkv, per * 16, B, width
+    n_pages, hkv, per, _ = shape
+    _need(pool, "pool", _U8, dev, (n_pages, hkv, per, BLOCK))
+    _need(table, "page_table", _I32, dev, tshape)
+    return n_pages, hkv, per * 16, tshape[0], tshape[1], dev
 
 
 def _rows(rows: int, B: int, seq: Optional[torch.Tensor], dev: torch.device) -> int:
     """Rows per sequence when no ``seq`` names each row's sequence."""
     if seq is not None:
-        _need(seq, "seq", torch.int32, dev, (rows,))
+        _need(seq, "seq", _I32, dev, (rows,))
         return 1
     if B == 0 or rows % B:
         raise ValueError(f"{rows} rows do not divide over {B} sequences: pass seq")
@@ -109,40 +109,44 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, qkv: torch.Tensor, 
     logical slot ``slots[r]`` (negative: not stored) of sequence ``seq[r]`` (default: the
     rows divide evenly over the page table's sequences).  With ``inv_freq`` [64] float32,
     q and k are rotated by ``positions[r]``.  Returns q [rows, n_heads, 128] bf16."""
-    n_pages, hkv, page, B, width = _pool(pool, page_table)
-    dev = pool.device
-    if qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.dim() != 2:
+    n_pages, hkv, page, B, width, dev = _pool(pool, page_table)
+    if qkv.dtype is not _BF16 or qkv.device != dev or qkv.dim() != 2:
         raise ValueError("qkv must be a bfloat16 matrix on the pool's device")
-    rows, nh = qkv.shape[0], n_heads + 2 * hkv
-    if n_heads < 0 or qkv.shape[1] != nh * HEAD_DIM:
-        raise ValueError(f"qkv has {qkv.shape[1]} columns, {n_heads} + 2 * {hkv} heads need {nh * HEAD_DIM}")
-    if rows and (qkv.stride(1) != 1 or (rows > 1 and qkv.stride(0) < qkv.shape[1])):
+    rows, cols = qkv.shape
+    nh = n_heads + 2 * hkv
+    if n_heads < 0 or cols != nh * HEAD_DIM:
+        raise ValueError(f"qkv has {cols} columns, {n_heads} + 2 * {hkv} heads need {nh * HEAD_DIM}")
+    ldq, step = qkv.stride()
+    if rows <= 1:
+        ldq = cols
+    if rows and cols and (step != 1 or ldq < cols):
         raise ValueError("qkv's columns must be contiguous and its rows must not overlap")
-    _need(slots, "slots", torch.int32, dev, (rows,))
+    _need(slots, "slots", _I32, dev, (rows,))
     per = _rows(rows, B, seq, dev)
     if (inv_freq is None) != (positions is None):
         raise ValueError("positions and inv_freq go together")
     if inv_freq is not None:
-        _need(inv_freq, "inv_freq", torch.float32, dev, (HEAD_DIM // 2,))
-        _need(positions, "positions", torch.int32, dev, (rows,))
+        _need(inv_freq, "inv_freq", _F32, dev, (HEAD_DIM // 2,))
+        _need(positions, "positions", _I32, dev, (rows,))
     if bias is not None:
-        _need(bias, "bias", torch.bfloat16, dev, (nh * HEAD_DIM,))
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _need(t, name, torch.bfloat16, dev, (HEAD_DIM,))
+        _need(bias, "bias", _BF16, dev, (nh * HEAD_DIM,))
+    if q_norm is not None:
+        _need(q_norm, "q_norm", _BF16, dev, (HEAD_DIM,))
+    if k_norm is not None:
+        _need(k_norm, "k_norm", _BF16, dev, (HEAD_DIM,))
     if q_out is None:
-        q_out = torch.empty(rows, n_heads, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+        q_out = qkv.new_empty((rows, n_heads, HEAD_DIM))
     else:
-        _need(q_out, "q_out", torch.bfloat16, dev, (rows, n_heads, HEAD_DIM))
+        _need(q_out, "q_out", _BF16, dev, (rows, n_heads, HEAD_DIM))
     if dev_err is not None:
-        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+        _need(dev_err, "dev_err", _I32, dev, (1,))
     if rows == 0:
         return q_out
     if n_pages == 0 or width == 0 or hkv == 0 or page == 0:
         raise ValueError("the pool and the page table must not be empty")
     _launch(
         lib().kvbp_kv4_append, "kv4_append", dev, rows, per, _ptr(seq), B, n_heads, hkv, HEAD_DIM, page, n_pages, width,
-        qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps,
+        qkv.data_ptr(), ldq, _ptr(bias), _ptr(q_norm), _ptr(k_norm), eps,
         _ptr(inv_freq), _ptr(positions), slots.data_ptr(), page_table.data_ptr(), q_out.data_ptr() if n_heads else None,
         pool.data_ptr(), _ptr(dev_err),
     )
@@ -155,14 +159,14 @@ def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor
     """K and V of the listed slots as the bf16 values their codes stand for: two tensors
     [rows, kv_heads, 128], or [kv_heads, rows, 128] (the prefill attention's layout) with
     ``heads_first``.  Rows of negative or out-of-range slots are zeros."""
-    n_pages, hkv, page, B, width = _pool(pool, page_table)
-    dev, rows = pool.device, slots.numel()
-    _need(slots, "slots", torch.int32, dev, (rows,))
+    n_pages, hkv, page, B, width, dev = _pool(pool, page_table)
+    rows = slots.numel()
+    _need(slots, "slots", _I32, dev, (rows,))
     per = _rows(rows, B, seq, dev)
     if dev_err is not None:
-        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+        _need(dev_err, "dev_err", _I32, dev, (1,))
     shape = (hkv, rows, HEAD_DIM) if heads_first else (rows, hkv, HEAD_DIM)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    k = torch.empty(shape, dtype=_BF16, device=dev)
     v = torch.empty_like(k)
     if rows == 0:
         return k, v
@@ -186,31 +190,32 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
     ``step_score`` [B, S] float32 is max-accumulated with every live slot's largest
     probability over the heads.  ``scale`` defaults to 1 / sqrt(128).  Returns out
     [B, heads, 128] bf16; a sequence without a live slot gives zeros."""
-    n_pages, hkv, page, B, width = _pool(pool, page_table)
-    dev = pool.device
-    _need(lens, "lens", torch.int32, dev, (B,))
+    n_pages, hkv, page, B, width, dev = _pool(pool, page_table)
+    _need(lens, "lens", _I32, dev, (B,))
     hq = q.shape[1] if q.dim() == 3 else 0
-    _need(q, "q", torch.bfloat16, dev, (B, hq, HEAD_DIM))
+    _need(q, "q", _BF16, dev, (B, hq, HEAD_DIM))
     if hkv == 0 or hq == 0 or hq % hkv or hq // hkv > 8:
         raise ValueError(f"{hq} query heads over {hkv} kv heads: whole groups of at most 8 are supported")
     S = 0
-    for t, name, dt in ((slot_pos, "slot_pos", torch.int32), (step_score, "step_score", torch.float32)):
-        if t is not None:
-            S = S or (t.shape[1] if t.dim() == 2 else 0)
-            _need(t, name, dt, dev, (B, S))
+    if slot_pos is not None:
+        S = slot_pos.shape[-1] if slot_pos.dim() else 0
+        _need(slot_pos, "slot_pos", _I32, dev, (B, S))
+    if step_score is not None:
+        S = S if slot_pos is not None else step_score.shape[-1] if step_score.dim() else 0
+        _need(step_score, "step_score", _F32, dev, (B, S))
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need(out, "out", torch.bfloat16, dev, (B, hq, HEAD_DIM))
+        _need(out, "out", _BF16, dev, (B, hq, HEAD_DIM))
     if dev_err is not None:
-        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+        _need(dev_err, "dev_err", _I32, dev, (1,))
     if B == 0:
         return out
     if n_pages == 0 or width == 0 or page == 0 or ((slot_pos is not None or step_score is not None) and S == 0):
         raise ValueError("the pool, the page table, slot_pos and step_score must not be empty")
     limit = min(width * page, S) if S else width * page
     ws_bytes = _attn_workspace(B, hq, hkv, limit, step_score is not None)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = pool.new_empty(ws_bytes)
     _launch(
         lib().kvbp_kv4_attn, "kv4_attn", dev, B, hq, hkv, HEAD_DIM, page, n_pages, width, q.data_ptr(), pool.data_ptr(),
         page_table.data_ptr(), lens.data_ptr(), _ptr(slot_pos), S, _SCALE if scale is None else scale, out.data_ptr(),
@@ -219,27 +224,32 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
     return out
 
 
-def _matrix(x: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    if x.dim() != 2 or x.dtype is not dtype:
+def _matrix(x: torch.Tensor, name: str, dtype: torch.dtype) -> tuple:
+    """(rows, columns, row stride) of a matrix with dense columns and rows apart."""
+    if x.dtype is not dtype or x.dim() != 2:
         raise ValueError(f"{name} must be a {dtype} matrix")
-    if x.shape[0] and x.shape[1] and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+    rows, cols = x.shape
+    ld, step = x.stride()
+    if rows <= 1:
+        ld = cols
+    if rows and cols and (step != 1 or ld < cols):
         raise ValueError(f"{name}'s columns must be contiguous and its rows must not overlap")
+    return rows, cols, ld
 
 
 def int8_quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows of a bf16 matrix in 8 bits: codes int8 [rows, K] (a view of storage whose rows
     start on 16-byte boundaries, as ``int8_linear`` wants its weight) and scales float32
     [rows]; x is about codes * scale."""
-    _matrix(x, "x", torch.bfloat16)
-    rows, K = x.shape
+    rows, K, ldx = _matrix(x, "x", _BF16)
     dev = x.device
     pitch = (K + 15) // 16 * 16
-    q = torch.zeros(rows, pitch, dtype=torch.int8, device=dev) if pitch != K else torch.empty(
-        rows, K, dtype=torch.int8, device=dev)
-    s = torch.empty(rows, dtype=torch.float32, device=dev)
+    q = torch.zeros(rows, pitch, dtype=_I8, device=dev) if pitch != K else torch.empty(
+        rows, K, dtype=_I8, device=dev)
+    s = torch.empty(rows, dtype=_F32, device=dev)
     if rows and K:
-        _launch(lib().kvbp_int8_quant_rows, "int8_quant_rows", dev, rows, K, x.data_ptr(),
-                x.stride(0) if rows > 1 else K, q.data_ptr(), pitch, s.data_ptr())
+        _launch(lib().kvbp_int8_quant_rows, "int8_quant_rows", dev, rows, K, x.data_ptr(), ldx, q.data_ptr(),
+                pitch, s.data_ptr())
     else:
         s.zero_()
     return q[:, :K], s
@@ -252,33 +262,33 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
     bias [N] bf16: each row of x is rounded to 8 bits with its own scale, the sums are exact
     32-bit integers, and y = sum * x_scale * w_scale + bias is rounded once to ``out_dtype``
     (bfloat16 or float32)."""
-    _matrix(x, "x", torch.bfloat16)
-    _matrix(w, "w", torch.int8)
-    M, K = x.shape
-    N, dev = w.shape[0], x.device
-    if w.device != dev or w.shape[1] != K:
+    M, K, ldx = _matrix(x, "x", _BF16)
+    N, Kw, ldw = _matrix(w, "w", _I8)
+    dev, pitch = x.device, (K + 15) // 16 * 16
+    if w.device != dev or Kw != K:
         raise ValueError(f"w must be [N, {K}] on {dev}, got {tuple(w.shape)} on {w.device}")
     if K == 0 or N == 0:
         raise ValueError("int8_linear needs at least one input and one output feature")
-    ldw = w.stride(0) if N > 1 else (K + 15) // 16 * 16
+    if N == 1:
+        ldw = pitch
     if ldw % 16 or w.data_ptr() % 16:
         raise ValueError("w's rows must start on 16-byte boundaries (int8_quantize_rows makes such weights)")
-    _need(w_scale, "w_scale", torch.float32, dev, (N,))
+    _need(w_scale, "w_scale", _F32, dev, (N,))
     if bias is not None:
-        _need(bias, "bias", torch.bfloat16, dev, (N,))
-    if out_dtype not in (torch.bfloat16, torch.float32):
+        _need(bias, "bias", _BF16, dev, (N,))
+    if out_dtype is not _BF16 and out_dtype is not _F32:
         raise ValueError("out_dtype must be bfloat16 or float32")
     if out is None:
         out = torch.empty(M, N, dtype=out_dtype, device=dev)
     else:
         _need(out, "out", out_dtype, dev, (M, N))
     if dev_err is not None:
-        _need(dev_err, "dev_err", torch.int32, dev, (1,))
+        _need(dev_err, "dev_err", _I32, dev, (1,))
     if M == 0:
         return out
-    ws_bytes = M * ((K + 15) // 16 * 16 + 4)  # kvbp_int8_linear_workspace: the codes and scales of x
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _launch(lib().kvbp_int8_linear, "int8_linear", dev, out_dtype is torch.float32, M, N, K, w.data_ptr(), ldw,
-            w_scale.data_ptr(), x.data_ptr(), x.stride(0) if M > 1 else K, _ptr(bias), out.data_ptr(), N, ws.data_ptr(),
+    ws_bytes = M * (pitch + 4)  # kvbp_int8_linear_workspace: the codes and scales of x
+    ws = w.new_empty(ws_bytes)
+    _launch(lib().kvbp_int8_linear, "int8_linear", dev, out_dtype is _F32, M, N, K, w.data_ptr(), ldw,
+            w_scale.data_ptr(), x.data_ptr(), ldx, _ptr(bias), out.data_ptr(), N, ws.data_ptr(),
             ws_bytes, _ptr(dev_err))
     return out
