@@ -7,10 +7,57 @@
 namespace kvbp {
 namespace i8 {
 
-// Per-token quantisation: sx = max|x| / 127, xq = rint(127 x / max|x|) (127 x is exact in
-// fp32, so half-way values are half-way in any precision; a zero row gives zeros and scale
-// 0).  A row with a NaN or an infinity gets a scale that is not finite, and codes 0: every
-// output of that token is then NaN.  One CTA per row, the row kept in registers between the
+// A row's codes from the bits m of its max|x|: rint(127 x / max|x|) (127 x is exact in fp32, so
+// half-way values are half-way in any precision).
+struct RowQuant {
+  float top, factor;
+  bool fine;  // not zero, infinite or NaN: else every code is 0
+  __device__ __forceinline__ explicit RowQuant(uint32_t m) {
+    top = __uint_as_float(m);
+    fine = m > 0 && m < 0x7f800000u;
+    factor = fine ? 127.0f / top : 0.f;
+  }
+  __device__ __forceinline__ float scale() const { return top / 127.0f; }
+  __device__ __forceinline__ uint32_t exact(float v) const {
+    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * v / top))) : 0u;
+  }
+  // x times the rounded factor plus 1.5 * 2^23 leaves the integer in the low mantissa bits.  The
+  // factor is off by 2^-24 of it, so a quotient (at most 127) by 8e-6: only what lies within
+  // 1e-4 of half-way can round wrongly, and is divided.
+  __device__ __forceinline__ uint2 eight(const uint4 w) const {
+    const float x[8] = {bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y), bf16lo(w.z), bf16hi(w.z), bf16lo(w.w), bf16hi(w.w)};
+    uint32_t c[8];
+    float worst = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float s = fmaf(x[k], factor, 12582912.0f);
+      worst = fmaxf(worst, fabsf(fmaf(x[k], factor, 12582912.0f - s)));
+      c[k] = __float_as_uint(s);
+    }
+    if (!fine || worst > 0.4999f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) c[k] = exact(x[k]);
+    }
+    auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    };
+    return make_uint2(bytes(c[0], c[1], c[2], c[3]), bytes(c[4], c[5], c[6], c[7]));
+  }
+};
+// m = max(m, max|x| of eight values) as bits: a NaN's bits are the largest
+__device__ __forceinline__ uint32_t fold_max(uint32_t m, const uint4 w) {
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) m = max(m, max((ws[k] << 16) & 0x7fffffffu, ws[k] & 0x7fff0000u));
+  return m;
+}
+__device__ __forceinline__ uint32_t abs_bits(const __nv_bfloat16 x) {
+  return __float_as_uint(__bfloat162float(x)) & 0x7fffffffu;
+}
+
+// Per-token quantisation: sx = max|x| / 127 and the codes above (a zero row gives zeros and
+// scale 0).  A row with a NaN or an infinity gets a scale that is not finite, and codes 0:
+// every output of that token is then NaN.  One CTA per row, the row kept in registers between the
 // maximum and the codes (kVec 16-byte vectors per thread: K <= 2048 kVec; longer rows are read
 // again, from L2).  Latency-bound: few registers let many rows share an SM.
 template <int kVec>
@@ -30,62 +77,30 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
   const uint4* rv = reinterpret_cast<const uint4*>(row);
   uint4 keep[kVec];
   uint32_t m = 0;  // max|x| as bits: a NaN's bits are the largest
-  auto fold = [&](const uint4 w) {
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) m = max(m, max((ws[k] << 16) & 0x7fffffffu, ws[k] & 0x7fff0000u));
-  };
 #pragma unroll
   for (int u = 0; u < kVec; ++u) {
     const int i = tid + 256 * u;
     keep[u] = i < nv ? rv[i] : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int u = 0; u < kVec; ++u) fold(keep[u]);
-  for (int i = tid + 256 * kVec; i < nv; i += 256) fold(rv[i]);
-  for (int i = nv * 8 + tid; i < K; i += 256) m = max(m, __float_as_uint(__bfloat162float(row[i])) & 0x7fffffffu);
+  for (int u = 0; u < kVec; ++u) m = fold_max(m, keep[u]);
+  for (int i = tid + 256 * kVec; i < nv; i += 256) m = fold_max(m, rv[i]);
+  for (int i = nv * 8 + tid; i < K; i += 256) m = max(m, abs_bits(row[i]));
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = max(m, red[w]);
-  const float top = __uint_as_float(m);
-  const bool fine = m > 0 && m < 0x7f800000u;
-  if (tid == 0) scale[r] = top / 127.0f;
-  // rint(127 x / top): x times the rounded factor plus 1.5 * 2^23 leaves the integer in the low
-  // mantissa bits.  The factor is off by 2^-24 of it, so a quotient (at most 127) by 8e-6: only
-  // what lies within 1e-4 of half-way can round wrongly, and is divided.
-  const float factor = fine ? 127.0f / top : 0.f;
-  auto code = [&](float v, float& worst) -> uint32_t {
-    const float s = fmaf(v, factor, 12582912.0f);
-    worst = fmaxf(worst, fabsf(fmaf(v, factor, 12582912.0f - s)));
-    return __float_as_uint(s);
-  };
-  auto exact = [&](float v) -> uint32_t {
-    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * v / top))) : 0u;
-  };
-  auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-  };
-  auto emit = [&](const uint4 w, int i) {
-    float x[8] = {bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y), bf16lo(w.z), bf16hi(w.z), bf16lo(w.w), bf16hi(w.w)};
-    uint32_t c[8];
-    float worst = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) c[k] = code(x[k], worst);
-    if (!fine || worst > 0.4999f) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) c[k] = exact(x[k]);
-    }
-    *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(bytes(c[0], c[1], c[2], c[3]), bytes(c[4], c[5], c[6], c[7]));
-  };
+  const RowQuant rq(m);
+  if (tid == 0) scale[r] = rq.scale();
+  auto emit = [&](const uint4 w, int i) { *reinterpret_cast<uint2*>(dst + 8 * i) = rq.eight(w); };
 #pragma unroll
   for (int u = 0; u < kVec; ++u) {
     const int i = tid + 256 * u;
     if (i < nv) emit(keep[u], i);
   }
   for (int i = tid + 256 * kVec; i < nv; i += 256) emit(rv[i], i);
-  for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(exact(__bfloat162float(row[i])));
+  for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(rq.exact(__bfloat162float(row[i])));
 }
 
 // ---- the product on the 5th-generation tensor cores (tcgen05.mma kind::i8) -------------
@@ -101,6 +116,9 @@ struct Args {
   void* out;
   long long ldo;
   int M, N, K, f32;
+  const __nv_bfloat16* x;  // fused quantisation: the tokens themselves
+  long long ldx;
+  int vec_x;  // its rows are 16-byte aligned
   int vec;    // four channels at a time are aligned
   int early;  // the weight is known to be complete before the kernel before this one ends
   int* err;
@@ -181,25 +199,35 @@ __device__ __forceinline__ void ld_acc(uint32_t taddr, int (&v)[C]) {
 // One output tile (128 channels x NT tokens) per cluster; the cluster's CTAs share the tile's
 // K range (gridDim.x = cluster size) and join their int32 partial tiles over distributed shared
 // memory.  Bound by the weight stream when tokens are few: stages are sized for two CTAs per SM.
-template <int NT>
+// With kFuse (a few tokens) the epilogue warps quantise the tokens themselves while the first
+// weights are under way: each CTA reads all of x for the rows' maxima (a few KB from L2) and
+// puts its own K range's codes into shared memory as the MMA's operand.  That saves a launch,
+// which is as long as the product of one token.
+constexpr int kFuseTokens = 4;
+constexpr int kFuseSteps = 30;  // stages of K per CTA whose codes fit beside three of weights
+template <int NT, bool kFuse>
 struct Ring {
-  static constexpr int kStage = kTileW + NT * kBK;
-  static constexpr int kStages = (NT <= 32 ? 5 : NT == 64 ? 4 : 3);
-  static constexpr int kBytes = kStages * kStage + 1024 + 256 + NT * 4;
+  static constexpr int kStage = kTileW + (kFuse ? 0 : NT * kBK);
+  static constexpr int kStages = kFuse ? 3 : NT <= 32 ? 5 : NT == 64 ? 4 : 3;
+  static constexpr int kTokens = kFuse ? kFuseSteps * NT * kBK : 0;
+  static constexpr int kBytes = kStages * kStage + kTokens + 1024 + 256 + NT * 4 + 16 * kFuseTokens;
   static_assert(kStages * kStage >= NT * 128 * 4, "the partial tile reuses the ring");
+  static_assert(kBytes <= 115712, "two CTAs per SM");
 };
 
-template <int NT>
+template <int NT, bool kFuse>
 __global__ void __launch_bounds__(kThreads, 2)
     split_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a) {
-  using R = Ring<NT>;
+  using R = Ring<NT, kFuse>;
   constexpr int kCols = NT < 32 ? 32 : NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(base + R::kStages * R::kStage);
+  uint8_t* tokens = base + R::kStages * R::kStage;  // kFuse: [step][16 tokens][128], swizzled
+  uint64_t* full = reinterpret_cast<uint64_t*>(tokens + R::kTokens);
   uint64_t* empty = full + R::kStages;
   uint64_t* done = empty + R::kStages;
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* ready = done + 1;  // kFuse: the tokens' codes are in place
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(ready + 1);
   int* bad = reinterpret_cast<int*>(tslot + 1);
   float* sxs = reinterpret_cast<float*>(bad + 1);  // the tokens' scales
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -215,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
+    mbar_init(ready, 128);
     *bad = 0;
     fence_barrier_init();
   }
@@ -237,20 +266,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 0) {
     if (lane == 0) {
       prefetch_tmap(&wmap);
-      prefetch_tmap(&xmap);
-      if (!a.early) pdl_wait();
+      if (!kFuse) prefetch_tmap(&xmap);
+      if (kFuse || !a.early) pdl_wait();
       auto load_w = [&](int u) {
         const int st = u % R::kStages;
         mbar_expect_tx(&full[st], R::kStage);
         tma_load_2d(base + st * R::kStage, &wmap, &full[st], (k0 + u) * kBK, n0);
       };
       auto load_x = [&](int u) {
+        if (kFuse) return;
         const int st = u % R::kStages;
         tma_load_2d(base + st * R::kStage + kTileW, &xmap, &full[st], (k0 + u) * kBK, m0);
       };
       const int first = nk < R::kStages ? nk : R::kStages;
       for (int u = 0; u < first; ++u) load_w(u);
-      if (a.early) pdl_wait();  // the tokens' codes come from the kernel before this one
+      if (!kFuse && a.early) pdl_wait();  // the tokens' codes come from the kernel before this one
       for (int u = 0; u < first; ++u) load_x(u);
       int issued = first;
       for (int u = first; u < nk && healthy(); ++u, ++issued) {
@@ -266,11 +296,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      for (int u = 0; u < nk && healthy(); ++u) {
+      bool go = true;
+      if (kFuse) {
+        go = wait_or_fail(ready, 0);
+        tc_after();
+      }
+      for (int u = 0; u < nk && go && healthy(); ++u) {
         const int st = u % R::kStages;
         if (!wait_or_fail(&full[st], static_cast<uint32_t>(u / R::kStages) & 1)) break;
         tc_after();
-        const uint32_t sw = smem_u32(base + st * R::kStage), sx = sw + kTileW;
+        const uint32_t sw = smem_u32(base + st * R::kStage);
+        const uint32_t sx = kFuse ? smem_u32(tokens) + u * (NT * kBK) : sw + kTileW;
 #pragma unroll
         for (int ks = 0; ks < kBK / 32; ++ks)
           mma_i8(tmem, tc_sdesc(sw + ks * 32), tc_sdesc(sx + ks * 32), idesc_i8(NT), (u > 0 || ks > 0) ? 1u : 0u);
@@ -279,12 +315,55 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc_commit(done);
     }
     __syncwarp();
+  } else if (kFuse) {
+    pdl_wait();
+    uint32_t* red = reinterpret_cast<uint32_t*>(sxs + NT);  // the four warps' maxima
+    const int et = tid - 64, nv = a.vec_x ? a.K / 8 : 0;
+    uint32_t m[kFuseTokens] = {};
+    for (int i = et; i < nv; i += 128)
+#pragma unroll
+      for (int r = 0; r < kFuseTokens; ++r)
+        if (r < a.M) m[r] = fold_max(m[r], reinterpret_cast<const uint4*>(a.x + r * a.ldx)[i]);
+    for (int i = nv * 8 + et; i < a.K; i += 128)
+#pragma unroll
+      for (int r = 0; r < kFuseTokens; ++r)
+        if (r < a.M) m[r] = max(m[r], abs_bits(a.x[r * a.ldx + i]));
+#pragma unroll
+    for (int r = 0; r < kFuseTokens; ++r) {
+      m[r] = __reduce_max_sync(0xffffffffu, m[r]);
+      if (lane == 0) red[(warp - 2) * kFuseTokens + r] = m[r];
+    }
+    named_bar(1, 128);
+    for (int r = 0; r < a.M; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = max(top, red[w * kFuseTokens + r]);
+      const RowQuant rq(top);
+      if (et == 0) sxs[r] = rq.scale();
+      const __nv_bfloat16* row = a.x + r * a.ldx;
+      for (int c = et; c < nk * 16; c += 128) {  // eight codes at a time of this CTA's K range
+        const int k = k0 * kBK + 8 * c;          // columns past K meet zero weights
+        uint2 codes = make_uint2(0, 0);
+        if (8 * (k / 8 + 1) <= nv * 8) {
+          codes = rq.eight(reinterpret_cast<const uint4*>(row)[k / 8]);
+        } else if (k < a.K) {
+          uint32_t b[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] = k + i < a.K ? rq.exact(__bfloat162float(row[k + i])) & 255u : 0u;
+          codes = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+        }
+        const int chunk = (c & 15) >> 1;  // 16-byte chunk of the row's 128, swizzled by row
+        *reinterpret_cast<uint2*>(tokens + (c >> 4) * (NT * kBK) + r * kBK + ((chunk ^ (r & 7)) << 4) + (c & 1) * 8) = codes;
+      }
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(ready);
   }
   const bool ok = wait_or_fail(done, 0) && healthy();
   tc_after();
   pdl_wait();  // before the scales are read and anything is written
   const int cols = min(NT, a.M - m0);  // live tokens of the tile
-  if (tid < cols) sxs[tid] = a.sx[m0 + tid];
+  if (!kFuse && tid < cols) sxs[tid] = a.sx[m0 + tid];
   const bool all_ok = !__syncthreads_or(!ok);
   // The accumulator goes through shared memory (the drained ring), [token][128 channels], so
   // that the stores are 8 or 16 bytes a thread and run along the channels.  (Stored straight
@@ -516,11 +595,12 @@ static CUresult tile_map(CUtensorMap* map, const void* p, int rows, int K, long 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-template <int NT>
+template <int NT, bool kFuse>
 static cudaError_t launch_split(cudaStream_t st, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, int S) {
-  if (prepare_device(reinterpret_cast<const void*>(split_kernel<NT>), Ring<NT>::kBytes) <= 0) return cudaErrorNoDevice;
+  constexpr int smem = Ring<NT, kFuse>::kBytes;
+  if (prepare_device(reinterpret_cast<const void*>(split_kernel<NT, kFuse>), smem) <= 0) return cudaErrorNoDevice;
   const dim3 grid(S, (a.N + 127) / 128, (a.M + NT - 1) / NT);
-  return launch_pdl(split_kernel<NT>, grid, dim3(kThreads), Ring<NT>::kBytes, st, S > 1 ? dim3(S, 1, 1) : dim3(0), wm, xm, a);
+  return launch_pdl(split_kernel<NT, kFuse>, grid, dim3(kThreads), smem, st, S > 1 ? dim3(S, 1, 1) : dim3(0), wm, xm, a);
 }
 
 static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
@@ -546,20 +626,23 @@ static int splits(long long tiles, int steps, int sms) {
   return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : static_cast<int>(s);
 }
 
-static int check(const Args& a, const void* w, long long ldw, const void* xq, long long ldq) {
-  if (!w || !a.sw || !xq || !a.sx || !a.out) return fail(kStatusArg, "int8_gemm: null pointer");
-  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || ldw < a.K || ldq < a.K || a.ldo < a.N) return fail(kStatusArg, "int8_gemm: bad size");
+// Checks of all but the tokens.
+static int check(const Args& a, const void* w, long long ldw) {
+  if (!w || !a.sw || !a.out) return fail(kStatusArg, "int8_gemm: null pointer");
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0 || ldw < a.K || a.ldo < a.N) return fail(kStatusArg, "int8_gemm: bad size");
   // the sum of K products of up to 127 * 128 stays in 32 bits
   if (a.K > 131071) return fail(kStatusUnsupported, "int8_gemm: K %d > 131071 could overflow the 32-bit sums", a.K);
-  if (misaligned(w, 16) || misaligned(xq, 16) || ldw % 16 || ldq % 16)
-    return fail(kStatusArg, "int8_gemm: w and xq rows must be 16-byte aligned");
+  if (misaligned(w, 16) || ldw % 16) return fail(kStatusArg, "int8_gemm: w's rows must be 16-byte aligned");
   if (misaligned(a.out, a.f32 ? 4 : 2)) return fail(kStatusArg, "int8_gemm: misaligned output");
   if ((a.N + 127) / 128 > 65535) return fail(kStatusUnsupported, "int8_gemm: N %d is too large", a.N);
   return kStatusOk;
 }
 
 static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const void* xq, long long ldq) {
-  if (int bad = check(a, w, ldw, xq, ldq)) return bad;
+  if (int bad = check(a, w, ldw)) return bad;
+  if (!xq || !a.sx) return fail(kStatusArg, "int8_gemm: null pointer");
+  if (ldq < a.K) return fail(kStatusArg, "int8_gemm: bad size");
+  if (misaligned(xq, 16) || ldq % 16) return fail(kStatusArg, "int8_gemm: xq's rows must be 16-byte aligned");
   a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
   const int sms = prepare_device(reinterpret_cast<const void*>(persist_kernel), kPBytes);
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
@@ -578,14 +661,35 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
   if (many)
     e = launch_pdl(persist_kernel, dim3(static_cast<unsigned>(tn * tm < sms ? tn * tm : sms)), dim3(kThreads), kPBytes, st, dim3(0), wm, xm, a);
   else if (NT == 16)
-    e = launch_split<16>(st, wm, xm, a, S);
+    e = launch_split<16, false>(st, wm, xm, a, S);
   else if (NT == 32)
-    e = launch_split<32>(st, wm, xm, a, S);
+    e = launch_split<32, false>(st, wm, xm, a, S);
   else if (NT == 64)
-    e = launch_split<64>(st, wm, xm, a, S);
+    e = launch_split<64, false>(st, wm, xm, a, S);
   else
-    e = launch_split<128>(st, wm, xm, a, S);
+    e = launch_split<128, false>(st, wm, xm, a, S);
   if (e != cudaSuccess) return fail(kStatusCuda, "int8_gemm launch: %s", cudaGetErrorString(e));
+  return kStatusOk;
+}
+
+// Up to four tokens straight from bf16: quantisation and product in one kernel.
+static bool fused(int M, int K) { return M <= kFuseTokens && K <= kFuseSteps * kMaxSplits * kBK; }
+
+static int gemm_fused(cudaStream_t st, Args a, const void* w, long long ldw) {
+  if (int bad = check(a, w, ldw)) return bad;
+  if (!a.x) return fail(kStatusArg, "int8_linear: null pointer");
+  if (a.ldx < a.K) return fail(kStatusArg, "int8_linear: bad size");
+  a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
+  a.vec_x = !misaligned(a.x, 16) && a.ldx % 8 == 0;
+  const int sms = prepare_device(reinterpret_cast<const void*>(split_kernel<16, true>), Ring<16, true>::kBytes);
+  if (sms <= 0) return fail(kStatusCuda, "int8_linear: no usable CUDA device");
+  CUtensorMap wm;
+  const CUresult r = tile_map(&wm, w, a.N, a.K, ldw, 128);
+  if (r != CUDA_SUCCESS) return fail(kStatusCuda, "int8_linear: tensor map failed (%d)", static_cast<int>(r));
+  const int steps = (a.K + kBK - 1) / kBK, least = (steps + kFuseSteps - 1) / kFuseSteps;
+  const int S = splits((a.N + 127) / 128, steps, sms);
+  const cudaError_t e = launch_split<16, true>(st, wm, wm, a, S < least ? least : S);
+  if (e != cudaSuccess) return fail(kStatusCuda, "int8_linear launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
 
@@ -602,25 +706,29 @@ extern "C" int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t 
 extern "C" int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
                               int64_t ldw, const float* w_scale, const void* xq, int64_t ldq, const float* x_scale,
                               const void* bias, void* out, int64_t ldo, int32_t* dev_err) {
-  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, 0, dev_err};
+  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, nullptr, 0, 0, 0, 0, dev_err};
   return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, xq, ldq);
 }
 
 extern "C" int64_t kvbp_int8_linear_workspace(int32_t M, int32_t K) {
-  return M <= 0 || K <= 0 ? 0 : static_cast<int64_t>(M) * ((K + 15) / 16 * 16) + 4ll * M;
+  if (M <= 0 || K <= 0 || kvbp::i8::fused(M, K)) return 0;
+  return static_cast<int64_t>(M) * ((static_cast<int64_t>(K) + 15) / 16 * 16) + 4ll * M;
 }
 
 extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
                                 int64_t ldw, const float* w_scale, const void* x, int64_t ldx, const void* bias,
                                 void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, int32_t* dev_err) {
-  if (!workspace) return kvbp::fail(kvbp::kStatusArg, "int8_linear: null pointer");
+  kvbp::i8::Args a{w_scale, nullptr, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0,
+                   static_cast<const __nv_bfloat16*>(x), ldx, 0, 0, 1, dev_err};
+  // the product's arguments first: a refused call leaves the workspace alone
+  if (int st = kvbp::i8::check(a, w, ldw)) return st;
+  if (kvbp::i8::fused(M, K)) return kvbp::i8::gemm_fused(reinterpret_cast<cudaStream_t>(stream), a, w, ldw);
+  if (!workspace || kvbp::i8::misaligned(workspace, 16)) return kvbp::fail(kvbp::kStatusArg, "int8_linear: no aligned workspace");
   if (workspace_bytes < kvbp_int8_linear_workspace(M, K))
     return kvbp::fail(kvbp::kStatusArg, "int8_linear: workspace of %lld bytes is too small", static_cast<long long>(workspace_bytes));
   const int64_t ldq = (static_cast<int64_t>(K) + 15) / 16 * 16;
   float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + ldq * M);
-  // the product's arguments first: a refused call leaves the workspace alone
-  const kvbp::i8::Args a{w_scale, scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, 0, 1, dev_err};
-  if (int st = kvbp::i8::check(a, w, ldw, workspace, ldq)) return st;
   if (int st = kvbp_int8_quant_rows(stream, M, K, x, ldx, workspace, ldq, scale)) return st;
+  a.sx = scale;
   return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, workspace, ldq);
 }

@@ -67,6 +67,11 @@ def _attn_workspace(B: int, hq: int, hkv: int, limit: int, score: bool) -> int:
     return lib().kvbp_kv4_attn_workspace(B, hq, hkv, limit, score)
 
 
+@lru_cache(maxsize=1024)
+def _linear_workspace(M: int, K: int) -> int:
+    return lib().kvbp_int8_linear_workspace(M, K)
+
+
 def kv4_pool(n_pages: int, n_kv_heads: int, page_size: int = 64, device=None) -> torch.Tensor:
     """A pool of ``n_pages`` zeroed pages: uint8 [n_pages, n_kv_heads, page_size / 16, 2304]."""
     if page_size <= 0 or page_size % 16:
@@ -286,9 +291,8 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
         _need(dev_err, "dev_err", _I32, dev, (1,))
     if M == 0:
         return out
-    ws_bytes = M * (pitch + 4)  # kvbp_int8_linear_workspace: the codes and scales of x
-    ws = w.new_empty(ws_bytes)
+    ws_bytes = _linear_workspace(M, K)  # the codes and scales of x, unless there are only a few rows
+    ws = w.new_empty(ws_bytes) if ws_bytes else None
     _launch(lib().kvbp_int8_linear, "int8_linear", dev, out_dtype is _F32, M, N, K, w.data_ptr(), ldw,
-            w_scale.data_ptr(), x.data_ptr(), ldx, _ptr(bias), out.data_ptr(), N, ws.data_ptr(),
-            ws_bytes, _ptr(dev_err))
+            w_scale.data_ptr(), x.data_ptr(), ldx, _ptr(bias), out.data_ptr(), N, _ptr(ws), ws_bytes, _ptr(dev_err))
     return out

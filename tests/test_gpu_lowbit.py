@@ -428,7 +428,7 @@ def test_quantize_rows_strided_and_misaligned_input():
         assert torch.equal(q.cpu().double(), _codes64(view)[0])
 
 
-SIZES = [(1, 1, 1), (1, 129, 33), (2, 100, 128), (16, 256, 512), (17, 300, 1000), (32, 640, 2048), (33, 129, 255),
+SIZES = [(1, 1, 1), (1, 129, 33), (3, 1000, 4001), (4, 260, 30720), (4, 129, 30721), (2, 38000, 3590), (5, 300, 1000), (2, 100, 128), (16, 256, 512), (17, 300, 1000), (32, 640, 2048), (33, 129, 255),
          (64, 384, 384), (65, 1000, 900), (127, 129, 4097), (128, 128, 128), (130, 513, 640), (257, 700, 96),
          (300, 2560, 1024), (513, 257, 1281), (1000, 1153, 777), (4, 4608, 3584), (1, 20000, 256), (4500, 1153, 300), (300, 20000, 640), (700, 25700, 200)]
 
@@ -456,15 +456,31 @@ def test_int8_linear(M, N, K, dt):
 
 
 def test_int8_linear_rows_that_are_zero_or_not_finite():
-    x, w, b = _int8_case(40, 200, 300, 5, True)
-    x[3] = 0
-    x[7, 11] = math.nan
-    x[21, 0] = -math.inf
+    for rows, zero, nan, inf in ((40, 3, 7, 21), (4, 0, 1, 3)):
+        x, w, b = _int8_case(rows, 200, 300, 5, True)
+        x[zero] = 0
+        x[nan, 11] = math.nan
+        x[inf, 0] = -math.inf
+        wq, ws = lowbit.int8_quantize_rows(w.cuda())
+        y = lowbit.int8_linear(x.cuda(), wq, ws, b.cuda()).cpu()
+        assert torch.equal(y[zero], b) and torch.isnan(y[nan]).all() and torch.isnan(y[inf]).all()
+        rest = [r for r in range(rows) if r not in (nan, inf)]
+        assert torch.isfinite(y[rest]).all()
+
+
+@pytest.mark.parametrize("M", [1, 4, 6])
+def test_int8_linear_strided_and_misaligned_rows(M):
+    """The few-token kernel and the two-kernel path take rows at any stride and offset."""
+    x, w, b = _int8_case(2 * M, 300, 520, 8, True)
     wq, ws = lowbit.int8_quantize_rows(w.cuda())
-    y = lowbit.int8_linear(x.cuda(), wq, ws, b.cuda()).cpu()
-    assert torch.equal(y[3], b) and torch.isnan(y[7]).all() and torch.isnan(y[21]).all()
-    rest = [r for r in range(40) if r not in (7, 21)]
-    assert torch.isfinite(y[rest]).all()
+    for rows, first, K in ((2, 0, 520), (1, 3, 501), (2, 1, 517), (1, 8, 512)):
+        view = x.cuda()[::rows][:M, first:first + K]
+        wv = lowbit.int8_quantize_rows(w[:, :K].contiguous().cuda())
+        y = lowbit.int8_linear(view, *wv, b.cuda())
+        assert torch.equal(y, lowbit.int8_linear(view.contiguous(), *wv, b.cuda()))
+        q, s = lowbit.int8_quantize_rows(view)  # the same codes: exact sums, one rounding
+        want = (q.double() @ wv[0].double().t()) * s.double()[:, None] * wv[1].double() + b.cuda().double()
+        assert ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() * (1 + 2.0 ** -8) + 8 * 2.0 ** -24 * (want - b.cuda().double()).abs()).all()
 
 
 def test_int8_linear_extreme_codes_do_not_overflow():
