@@ -472,8 +472,8 @@ int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N,
                    const float* w_scale, const void* xq, int64_t ldq, const float* x_scale, const void* bias,
                    void* out, int64_t ldo, int32_t* dev_err);
 
-/* kvbp_int8_quant_rows of x [M][ldx] bf16 and kvbp_int8_gemm in one call (one kernel for up to
- * four rows).  workspace (16-byte aligned, kvbp_int8_linear_workspace bytes; NULL where that is
+/* kvbp_int8_quant_rows of x [M][ldx] bf16 and kvbp_int8_gemm in one call (one kernel for a
+ * single row).  workspace (16-byte aligned, kvbp_int8_linear_workspace bytes; NULL where that is
  * 0) holds the codes and scales between the two; the next call on the same stream may reuse
  * it, calls that may overlap need one each. */
 int64_t kvbp_int8_linear_workspace(int32_t M, int32_t K);

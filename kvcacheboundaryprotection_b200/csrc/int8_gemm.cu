@@ -199,11 +199,13 @@ __device__ __forceinline__ void ld_acc(uint32_t taddr, int (&v)[C]) {
 // One output tile (128 channels x NT tokens) per cluster; the cluster's CTAs share the tile's
 // K range (gridDim.x = cluster size) and join their int32 partial tiles over distributed shared
 // memory.  Bound by the weight stream when tokens are few: stages are sized for two CTAs per SM.
-// With kFuse (a few tokens) the epilogue warps quantise the tokens themselves while the first
-// weights are under way: each CTA reads all of x for the rows' maxima (a few KB from L2) and
-// puts its own K range's codes into shared memory as the MMA's operand.  That saves a launch,
-// which is as long as the product of one token.
-constexpr int kFuseTokens = 4;
+// With kFuse (one token) the epilogue warps quantise the token themselves while the first
+// weights are under way: each CTA reads all of x for its maximum (a few KB from L2) and puts its
+// own K range's codes into shared memory as the MMA's operand.  That saves a launch: the GPU
+// time is the same (6.9 against 7.4 us at 6144 x 2560, 27.7 against 26.5 at 37888 x 3584), the
+// host's a third less.  With four tokens the CTAs' repeated work costs more than the
+// launch (8.9 and 33.4 us).
+constexpr int kFuseTokens = 1;
 constexpr int kFuseSteps = 30;  // stages of K per CTA whose codes fit beside three of weights
 template <int NT, bool kFuse>
 struct Ring {
@@ -672,7 +674,7 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
   return kStatusOk;
 }
 
-// Up to four tokens straight from bf16: quantisation and product in one kernel.
+// One token straight from bf16: quantisation and product in one kernel.
 static bool fused(int M, int K) { return M <= kFuseTokens && K <= kFuseSteps * kMaxSplits * kBK; }
 
 static int gemm_fused(cudaStream_t st, Args a, const void* w, long long ldw) {

@@ -291,7 +291,7 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
         _need(dev_err, "dev_err", _I32, dev, (1,))
     if M == 0:
         return out
-    ws_bytes = _linear_workspace(M, K)  # the codes and scales of x, unless there are only a few rows
+    ws_bytes = _linear_workspace(M, K)  # the codes and scales of x, unless it is one row
     ws = w.new_empty(ws_bytes) if ws_bytes else None
     _launch(lib().kvbp_int8_linear, "int8_linear", dev, out_dtype is _F32, M, N, K, w.data_ptr(), ldw,
             w_scale.data_ptr(), x.data_ptr(), ldx, _ptr(bias), out.data_ptr(), N, _ptr(ws), ws_bytes, _ptr(dev_err))

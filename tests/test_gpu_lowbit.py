@@ -428,7 +428,7 @@ def test_quantize_rows_strided_and_misaligned_input():
         assert torch.equal(q.cpu().double(), _codes64(view)[0])
 
 
-SIZES = [(1, 1, 1), (1, 129, 33), (3, 1000, 4001), (4, 260, 30720), (4, 129, 30721), (2, 38000, 3590), (5, 300, 1000), (2, 100, 128), (16, 256, 512), (17, 300, 1000), (32, 640, 2048), (33, 129, 255),
+SIZES = [(1, 1, 1), (1, 129, 33), (1, 1000, 4001), (1, 260, 30720), (1, 129, 30721), (1, 38000, 3590), (2, 1000, 4001), (5, 300, 1000), (2, 100, 128), (16, 256, 512), (17, 300, 1000), (32, 640, 2048), (33, 129, 255),
          (64, 384, 384), (65, 1000, 900), (127, 129, 4097), (128, 128, 128), (130, 513, 640), (257, 700, 96),
          (300, 2560, 1024), (513, 257, 1281), (1000, 1153, 777), (4, 4608, 3584), (1, 20000, 256), (4500, 1153, 300), (300, 20000, 640), (700, 25700, 200)]
 
@@ -466,11 +466,14 @@ def test_int8_linear_rows_that_are_zero_or_not_finite():
         assert torch.equal(y[zero], b) and torch.isnan(y[nan]).all() and torch.isnan(y[inf]).all()
         rest = [r for r in range(rows) if r not in (nan, inf)]
         assert torch.isfinite(y[rest]).all()
+        for r in range(4):  # a single row takes its own kernel
+            alone = lowbit.int8_linear(x[r:r + 1].cuda(), wq, ws, b.cuda()).cpu()
+            assert torch.equal(torch.nan_to_num(alone[0], nan=-1e4), torch.nan_to_num(y[r], nan=-1e4))
 
 
 @pytest.mark.parametrize("M", [1, 4, 6])
 def test_int8_linear_strided_and_misaligned_rows(M):
-    """The few-token kernel and the two-kernel path take rows at any stride and offset."""
+    """The one-token kernel and the two-kernel path take rows at any stride and offset."""
     x, w, b = _int8_case(2 * M, 300, 520, 8, True)
     wq, ws = lowbit.int8_quantize_rows(w.cuda())
     for rows, first, K in ((2, 0, 520), (1, 3, 501), (2, 1, 517), (1, 8, 512)):
