@@ -449,8 +449,10 @@ int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, co
  * when slot_pos or step_score is given) is cut there and sets KVBP_DEV_INDEX.  A sequence
  * without a live slot gives zeros (and KVBP_DEV_NO_VALID_SLOT when lens[b] > 0).  Softmax
  * statistics and sums are fp32; values in free slots and past lens never reach the result.
- * workspace: kvbp_kv4_attn_workspace bytes, 16-byte aligned, free to reuse by the next call
- * on the same stream (calls that may overlap need one each); nothing is kept in it. */
+ * workspace: kvbp_kv4_attn_workspace bytes for max_slots = the smaller of max_pages * page_size
+ * and (when slot_pos or step_score is given) S, 16-byte aligned, or NULL where that is 0 (short
+ * sequences); free to reuse by the next call on the same stream (calls that may overlap need
+ * one each); nothing is kept in it. */
 int64_t kvbp_kv4_attn_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t max_slots, int32_t with_score);
 int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t page_size,
                   int32_t n_pages, int32_t max_pages, const void* q, const void* pool, const int32_t* page_table,

@@ -398,7 +398,7 @@ struct Smem {
   uint64_t full[kWarps][kStages];
   int first[kMaxSeqs + 1];  // first block of each sequence's first head
   int len[kMaxSeqs];
-  int wsum[kWarps];
+  int wsum[kWarps], wmax[kWarps];
 };
 static_assert(sizeof(Smem) <= 115712 - 16, "two CTAs per SM");
 
@@ -445,6 +445,150 @@ __device__ __forceinline__ uint32_t code_pair_hi(uint32_t w) {
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
+// What a warp has of its slots' softmax: per query head (columns 2 t, 2 t + 1 of the MMAs) the
+// reference exponent and this thread's share of the sum, and O in the MMAs' layout: thread
+// (g, t) holds dims 32 i + 4 g + {0, 1, 2, 3} of the two heads in o[2 i][0, 1], o[2 i][2, 3],
+// o[2 i + 1][0, 1], o[2 i + 1][2, 3].
+struct Sums {
+  float o[8][4], l[2], ref[2];
+  float lim[2];     // ref + e: the largest logit that needs no rescale
+  uint32_t fields;  // or of the V scales' exponent fields so far
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+    l[0] = l[1] = 0.f;
+    ref[0] = ref[1] = lim[0] = lim[1] = -INFINITY;
+    fields = 0;
+  }
+  // Rescale where a weight would pass 2^e, then with kSlack bits to spare: most stages only
+  // vote.  e keeps P * scale below 2^14 through the V scales' exponent fields or-ed together
+  // (at least the largest; it has to be small enough only, and stays above -4).
+  __device__ __forceinline__ void vote(float (&top)[2], uint32_t bits) {
+    bits &= 0x7c007c00u;
+    if (!__any_sync(0xffffffffu, (bits & ~fields) || top[0] > lim[0] || top[1] > lim[1])) return;
+    fields |= __reduce_or_sync(0xffffffffu, bits);
+    fields |= fields >> 16 | fields << 16;
+    const float e = static_cast<float>(min(15, 28 - static_cast<int>(fields >> 26)));
+    float f[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+      const float r = top[c] - e > ref[c] ? top[c] - e + kSlack : ref[c];
+      f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
+      ref[c] = r;
+      lim[c] = r + e;
+      l[c] *= f[c];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
+  }
+  // O += P V of a block: its logits x, V codes (v0, v1) and V scales (s0, s1) of the slot pairs
+  __device__ __forceinline__ void weigh(const float (&x)[4], const uint4 v0, const uint4 v1, const uint4 s0, const uint4 s1) {
+    const float r0 = ref[0] == -INFINITY ? 0.f : ref[0], r1 = ref[1] == -INFINITY ? 0.f : ref[1];
+    const float p0 = ex2(x[0] - r0), p1 = ex2(x[1] - r1), p2 = ex2(x[2] - r0), p3 = ex2(x[3] - r1);
+    l[0] += p0 + p2;
+    l[1] += p1 + p3;
+    const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
+    const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
+    const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb[4] = {s1.x, s1.y, s1.z, s1.w};
+    const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c0 = half2_bits(__hmul2(b0, bits_half2(sa[i]))), c1 = half2_bits(__hmul2(b1, bits_half2(sb[i])));
+      const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
+      mma_f16(o[2 * i], code_pair(w0[i]), code_pair_hi(w0[i]), code_pair(w1[i]), code_pair_hi(w1[i]), c0, c1);
+      mma_f16(o[2 * i + 1], code_pair(u0), code_pair_hi(u0), code_pair(u1), code_pair_hi(u1), c0, c1);
+    }
+  }
+  // the warp's sums to shared memory: ref and sum [8], O [8][kHeadPitch] of the live heads
+  __device__ __forceinline__ void leave(float* to_ref, float* to_sum, float (*to_o)[kHeadPitch], int group, bool any, int g, int t) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
+      if (g == 0) to_ref[2 * t + c] = ref[c], to_sum[2 * t + c] = l[c];
+      if (any && 2 * t + c < group) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(&to_o[2 * t + c][32 * i + 4 * g]) =
+              make_float4(o[2 * i][c], o[2 * i][c + 2], o[2 * i + 1][c], o[2 * i + 1][c + 2]);
+      }
+    }
+  }
+};
+// Logits (in units of ln 2) of a block's slots sg (x[0, 1]) and sg + 2 (x[2, 3]) for heads 2 t,
+// 2 t + 1: K codes and scales of the two slots; q(j) is group j's B operand.
+template <typename Q>
+__device__ __forceinline__ void block_logits(const uint4 k0, const uint4 k1, const uint2 s0, const uint2 s1, Q q,
+                                             const float (&xs)[2], float (&x)[4]) {
+  const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+  const float2 f0[2] = {__half22float2(bits_half2(s0.x)), __half22float2(bits_half2(s0.y))};
+  const float2 f1[2] = {__half22float2(bits_half2(s1.x)), __half22float2(bits_half2(s1.y))};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float c[4];
+    const uint4 qf = q(j);
+    const uint32_t u0 = w0[j] >> 8, u1 = w1[j] >> 8;
+    mma_f16_new(c, code_pair(w0[j]), code_pair(w1[j]), code_pair_hi(w0[j]), code_pair_hi(w1[j]), qf.x, qf.y);
+    mma_f16(c, code_pair(u0), code_pair(u1), code_pair_hi(u0), code_pair_hi(u1), qf.z, qf.w);
+    const float a0 = j & 1 ? f0[j >> 1].y : f0[j >> 1].x, a1 = j & 1 ? f1[j >> 1].y : f1[j >> 1].x;
+    x[0] = j ? x[0] + a0 * c[0] : a0 * c[0];
+    x[1] = j ? x[1] + a0 * c[1] : a0 * c[1];
+    x[2] = j ? x[2] + a1 * c[2] : a1 * c[2];
+    x[3] = j ? x[3] + a1 * c[3] : a1 * c[3];
+  }
+  x[0] *= xs[0];
+  x[1] *= xs[1];
+  x[2] *= xs[0];
+  x[3] *= xs[1];
+}
+// -inf for the masked ones of slots sg and sg + 2 (bits 0 and 2 of m)
+__device__ __forceinline__ void mask_logits(float (&x)[4], uint32_t m) {
+  if (!(m & 1u)) x[0] = x[1] = -INFINITY;
+  if (!(m & 4u)) x[2] = x[3] = -INFINITY;
+}
+// the V scales of a slot pair, zero where masked (the memory may hold anything)
+__device__ __forceinline__ uint4 mask_scales(uint4 v, uint32_t two) {
+  const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+  v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
+  return v;
+}
+__device__ __forceinline__ uint32_t or4(const uint4 v) { return v.x | v.y | v.z | v.w; }
+// q of head g (zeros where not live) as the MMA's B operands, group j in qf[j], brought to
+// [2^14, 2^15) by 2^up; returns the head's logits in units of ln 2 per unit of the MMAs' sums:
+// scale log2(e) / 2^up, in two factors (2^-up alone can overflow).
+__device__ __forceinline__ float load_query(const __nv_bfloat16* head, bool live, float scale, int t, uint4 (&qf)[4]) {
+  const uint4* src = reinterpret_cast<const uint4*>(head);
+  uint4 w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = live ? src[4 * j + t] : make_uint4(0, 0, 0, 0);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = max(top, max((ws[k] >> 16) & 0x7fffu, ws[k] & 0x7fffu));
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int up = min(14 + 127 - static_cast<int>(top >> 7), 126);
+  const float f = __int_as_float((up + 127) << 23);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float d[8] = {bf16lo(w[j].x) * f, bf16hi(w[j].x) * f, bf16lo(w[j].y) * f, bf16hi(w[j].y) * f,
+                        bf16lo(w[j].z) * f, bf16hi(w[j].z) * f, bf16lo(w[j].w) * f, bf16hi(w[j].w) * f};
+    qf[j] = make_uint4(half2_bits(__floats2half2_rn(d[0], d[4])), half2_bits(__floats2half2_rn(d[1], d[5])),
+                       half2_bits(__floats2half2_rn(d[2], d[6])), half2_bits(__floats2half2_rn(d[3], d[7])));
+  }
+  return scale * 1.4426950408889634f * __int_as_float((127 - (up >> 1)) << 23) *
+         __int_as_float((127 - (up - (up >> 1))) << 23);
+}
+
 // A range's part of one (sequence, kv head): blocks [sb0, sb0 + n) of the head's nsb.
 struct Segment {
   int b, h, sb0, n, nsb;
@@ -462,11 +606,12 @@ struct Segment {
   }
 };
 
-// The lengths' prefix sums into shared memory; returns the number of blocks of all heads.
-__device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
+// The lengths' prefix sums into shared memory; returns the number of blocks of all heads, and
+// of the longest one.
+__device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report, int& longest) {
   const int B = a.pool.B, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kEach = (kMaxSeqs + kWarps * 32 - 1) / (kWarps * 32);
-  int v[kEach], t = 0;
+  int v[kEach], t = 0, most = 0;
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
     const int b = tid * kEach + u;
@@ -478,6 +623,7 @@ __device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
     if (b < B) sm.len[b] = n;
     v[u] = t;
     t += ((n + 15) >> 4) * a.pool.Hkv;
+    most = max(most, (n + 15) >> 4);
   }
   int inc = t;
 #pragma unroll
@@ -485,11 +631,14 @@ __device__ __forceinline__ int plan(const AttnArgs& a, Smem& sm, bool report) {
     const int y = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += y;
   }
-  if (lane == 31) sm.wsum[warp] = inc;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) sm.wsum[warp] = inc, sm.wmax[warp] = most;
   __syncthreads();
   int before = 0, total = 0;
+  longest = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
+    longest = max(longest, sm.wmax[w]);
     if (w < warp) before += sm.wsum[w];
     total += sm.wsum[w];
   }
@@ -514,9 +663,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
   fence_barrier_init();
   pdl_launch_dependents();
   pdl_wait();
-  const int total = plan(a, sm, blockIdx.x == 0);
-  int R = (total + gridDim.x - 1) / gridDim.x;
-  if (R < kMinBlocks) R = kMinBlocks;
+  int longest;
+  const int total = plan(a, sm, blockIdx.x == 0, longest);
+  // at least kMinBlocks of a head, or short heads one after the other would wait in few CTAs
+  const int R = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), min(kMinBlocks, longest));
   if (blockIdx.x == 0) {
     if (tid == 0) a.header[0] = R;
     for (int b = tid; b <= a.pool.B; b += kWarps * 32) a.header[2 + b] = sm.first[b];
@@ -599,36 +749,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
 #pragma unroll
   for (int s = 0; s < kStages; ++s) issue(s);
 
-  // q of a segment's head as the MMA's B operands, heads on the columns: one warp's work
-  auto prepare_q = [&](const Segment& s, int buf) {
-    const uint4* src = reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(s.b) * a.Hq + s.h * group + g) * 128);
-    uint4 w[4];
+  auto prepare_q = [&](const Segment& s, int buf) {  // q of a segment's head: one warp's work
+    uint4 qf[4];
+    const float unit = load_query(a.q + (static_cast<size_t>(s.b) * a.Hq + s.h * group + g) * 128, g < group, a.scale, t, qf);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = g < group ? src[4 * j + t] : make_uint4(0, 0, 0, 0);
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top = max(top, max((ws[k] >> 16) & 0x7fffu, ws[k] & 0x7fffu));
-    }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^up brings the head's largest |q| to [2^14, 2^15)
-    const int up = min(14 + 127 - static_cast<int>(top >> 7), 126);
-    const float f = __int_as_float((up + 127) << 23);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d[8] = {bf16lo(w[j].x) * f, bf16hi(w[j].x) * f, bf16lo(w[j].y) * f, bf16hi(w[j].y) * f,
-                          bf16lo(w[j].z) * f, bf16hi(w[j].z) * f, bf16lo(w[j].w) * f, bf16hi(w[j].w) * f};
-      sm.q[buf][j][lane] = make_uint4(half2_bits(__floats2half2_rn(d[0], d[4])), half2_bits(__floats2half2_rn(d[1], d[5])),
-                                      half2_bits(__floats2half2_rn(d[2], d[6])), half2_bits(__floats2half2_rn(d[3], d[7])));
-    }
-    // logits in units of ln 2 per unit of the sums: scale log2(e) / 2^up, in two factors
-    // (2^-up alone can overflow)
-    if (t == 0)
-      sm.xs[buf][g] = a.scale * 1.4426950408889634f * __int_as_float((127 - (up >> 1)) << 23) *
-                      __int_as_float((127 - (up - (up >> 1))) << 23);
+    for (int j = 0; j < 4; ++j) sm.q[buf][j][lane] = qf[j];
+    if (t == 0) sm.xs[buf][g] = unit;
   };
   if (warp == kWarps - 1) prepare_q(cs, 0);
   __syncthreads();
@@ -643,13 +769,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
       if (warp == kWarps - 1) prepare_q(next, buf ^ 1);
     }
     const float xs[2] = {sm.xs[buf][2 * t], sm.xs[buf][2 * t + 1]};
-    float o[8][4], l[2] = {0.f, 0.f}, ref[2] = {-INFINITY, -INFINITY};
-    float lim[2] = {-INFINITY, -INFINITY};  // ref + e: the largest logit that needs no rescale
-    uint32_t fields = 0;                    // or of the V scales' exponent fields so far
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+    Sums sums;
+    sums.clear();
+    auto q_of = [&](int j) { return sm.q[buf][j][lane]; };
 
     const int per = cs.per();
     float* lg = kScore && 2 * t < a.gs
@@ -671,16 +793,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
       const uint8_t* base = sm.ring[warp][st];
       auto process = [&](auto full_stage) {
         constexpr bool kFull = decltype(full_stage)::value;  // no mask, no missing block
-        // V scales of this thread's slot pairs (4 t, 4 t + 1), (4 t + 2, 4 t + 3) of a block, zero
-        // where masked (the memory may hold anything)
-        auto v_scales = [&](int bl, int h) {
-          uint4 v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
-          if (!kFull) {
-            const uint32_t two = mask >> (16 * bl + 4 * t + 2 * h);
-            const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-            v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
-          }
-          return v;
+        auto v_scales = [&](int bl, int h) {  // of this thread's slot pair 4 t + 2 h
+          const uint4 v = *reinterpret_cast<const uint4*>(base + bl * kBlock + kVScale + 32 * t + 16 * h);
+          return kFull ? v : mask_scales(v, mask >> (16 * bl + 4 * t + 2 * h));
         };
         float x[kStageBlocks][4], top[2] = {-INFINITY, -INFINITY};
         uint32_t bits = 0;
@@ -688,37 +803,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
         for (int bl = 0; bl < kStageBlocks; ++bl) {
           if (!kFull && bl >= nb) break;
           const uint8_t* blk = base + bl * kBlock;
-          const uint4 k0 = *reinterpret_cast<const uint4*>(blk + 64 * sg + 16 * t);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(blk + 64 * (sg + 2) + 16 * t);
-          const uint2 s0 = *reinterpret_cast<const uint2*>(blk + kKScale + 8 * sg);
-          const uint2 s1 = *reinterpret_cast<const uint2*>(blk + kKScale + 8 * (sg + 2));
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-          const float2 f0[2] = {__half22float2(bits_half2(s0.x)), __half22float2(bits_half2(s0.y))};
-          const float2 f1[2] = {__half22float2(bits_half2(s1.x)), __half22float2(bits_half2(s1.y))};
-          float y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float c[4];
-            const uint4 qf = sm.q[buf][j][lane];
-            const uint32_t u0 = w0[j] >> 8, u1 = w1[j] >> 8;
-            mma_f16_new(c, code_pair(w0[j]), code_pair(w1[j]), code_pair_hi(w0[j]), code_pair_hi(w1[j]), qf.x,
-                        qf.y);
-            mma_f16(c, code_pair(u0), code_pair(u1), code_pair_hi(u0), code_pair_hi(u1), qf.z, qf.w);
-            const float a0 = j & 1 ? f0[j >> 1].y : f0[j >> 1].x, a1 = j & 1 ? f1[j >> 1].y : f1[j >> 1].x;
-            y[0] = j ? y[0] + a0 * c[0] : a0 * c[0];
-            y[1] = j ? y[1] + a0 * c[1] : a0 * c[1];
-            y[2] = j ? y[2] + a1 * c[2] : a1 * c[2];
-            y[3] = j ? y[3] + a1 * c[3] : a1 * c[3];
-          }
-          x[bl][0] = y[0] * xs[0];
-          x[bl][1] = y[1] * xs[1];
-          x[bl][2] = y[2] * xs[0];
-          x[bl][3] = y[3] * xs[1];
-          if (!kFull) {
-            const uint32_t m = mask >> (16 * bl + sg);
-            if (!(m & 1u)) x[bl][0] = x[bl][1] = -INFINITY;
-            if (!(m & 4u)) x[bl][2] = x[bl][3] = -INFINITY;
-          }
+          block_logits(*reinterpret_cast<const uint4*>(blk + 64 * sg + 16 * t),
+                       *reinterpret_cast<const uint4*>(blk + 64 * (sg + 2) + 16 * t),
+                       *reinterpret_cast<const uint2*>(blk + kKScale + 8 * sg),
+                       *reinterpret_cast<const uint2*>(blk + kKScale + 8 * (sg + 2)), q_of, xs, x[bl]);
+          if (!kFull) mask_logits(x[bl], mask >> (16 * bl + sg));
           if (kScore && lg) {
             float* to = lg + (k + bl) * 16 * a.gs;
             *reinterpret_cast<float2*>(to) = make_float2(x[bl][0], x[bl][1]);
@@ -726,54 +815,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
           }
           top[0] = fmaxf(top[0], fmaxf(x[bl][0], x[bl][2]));
           top[1] = fmaxf(top[1], fmaxf(x[bl][1], x[bl][3]));
-          const uint4 v0 = v_scales(bl, 0), v1 = v_scales(bl, 1);
-          bits |= v0.x | v0.y | v0.z | v0.w | v1.x | v1.y | v1.z | v1.w;
+          bits |= or4(v_scales(bl, 0)) | or4(v_scales(bl, 1));
         }
-        // Rescale where a weight would pass 2^e, then with kSlack bits to spare: most stages only
-        // vote.  e keeps P * scale below 2^14 through the V scales' exponent fields or-ed
-        // together (at least the largest; it has to be small enough only, and stays above -4).
-        bits &= 0x7c007c00u;
-        if (__any_sync(0xffffffffu, (bits & ~fields) || top[0] > lim[0] || top[1] > lim[1])) {
-          fields |= __reduce_or_sync(0xffffffffu, bits);
-          fields |= fields >> 16 | fields << 16;
-          const float e = static_cast<float>(min(15, 28 - static_cast<int>(fields >> 26)));
-          float f[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-            top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-            const float r = top[c] - e > ref[c] ? top[c] - e + kSlack : ref[c];
-            f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
-            ref[c] = r;
-            lim[c] = r + e;
-            l[c] *= f[c];
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
-        }
-        const float r0 = ref[0] == -INFINITY ? 0.f : ref[0], r1 = ref[1] == -INFINITY ? 0.f : ref[1];
+        sums.vote(top, bits);
 #pragma unroll
         for (int bl = 0; bl < kStageBlocks; ++bl) {
           if (!kFull && bl >= nb) break;
           const uint8_t* blk = base + bl * kBlock;
-          const float p0 = ex2(x[bl][0] - r0), p1 = ex2(x[bl][1] - r1), p2 = ex2(x[bl][2] - r0), p3 = ex2(x[bl][3] - r1);
-          l[0] += p0 + p2;
-          l[1] += p1 + p3;
-          const __half2 b0 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p0, p1))));
-          const __half2 b1 = bits_half2(transpose8x8(half2_bits(__floats2half2_rn(p2, p3))));
-          const uint4 s0 = v_scales(bl, 0), s1 = v_scales(bl, 1);
-          const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t);
-          const uint4 v1 = *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t);
-          const uint32_t sa[4] = {s0.x, s0.y, s0.z, s0.w}, sb[4] = {s1.x, s1.y, s1.z, s1.w};
-          const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t c0 = half2_bits(__hmul2(b0, bits_half2(sa[i]))), c1 = half2_bits(__hmul2(b1, bits_half2(sb[i])));
-            const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
-            mma_f16(o[2 * i], code_pair(w0[i]), code_pair_hi(w0[i]), code_pair(w1[i]), code_pair_hi(w1[i]), c0, c1);
-            mma_f16(o[2 * i + 1], code_pair(u0), code_pair_hi(u0), code_pair(u1), code_pair_hi(u1), c0, c1);
-          }
+          sums.weigh(x[bl], *reinterpret_cast<const uint4*>(blk + 1024 + 64 * g + 16 * t),
+                     *reinterpret_cast<const uint4*>(blk + 1536 + 64 * g + 16 * t), v_scales(bl, 0), v_scales(bl, 1));
         }
       };
       if (mask == 0xffffffffu) process(std::true_type{});  // every slot of a whole stage is live
@@ -784,23 +834,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
     }
 
     // -- the warps' parts of this segment meet
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
-      if (g == 0) sm.ref[warp][2 * t + c] = ref[c], sm.sum[warp][2 * t + c] = l[c];
-    }
-    if (warp * per < cs.n) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (2 * t + c < group) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(&sm.part[warp][2 * t + c][32 * i + 4 * g]) =
-                make_float4(o[2 * i][c], o[2 * i][c + 2], o[2 * i + 1][c], o[2 * i + 1][c + 2]);
-        }
-    }
+    sums.leave(sm.ref[warp], sm.sum[warp], sm.part[warp], group, warp * per < cs.n, g, t);
     __syncthreads();
     const bool whole = cs.n == cs.nsb;
     if (warp < group) {  // one query head per warp, four dims per lane
@@ -975,6 +1009,156 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
   if (top > before) *dst = top;
 }
 
+// Attention over short sequences in one launch: W warps of a CTA share a (sequence, kv head), so
+// nothing is left to join between CTAs and the logits for the score stay in shared memory.
+// Bound by latency: lengths, pages, one block's loads, two or three blocks of arithmetic a warp;
+// blocks come straight into registers, the next one's loads in flight (W = 16 has no registers
+// for that, and few blocks a warp).
+constexpr int kShortBlocks = 128;      // blocks of a head at most (2048 slots)
+constexpr int kShortSmem = 168 * 1024;
+constexpr long long kShortTotal = 8192;   // blocks of all heads at most
+constexpr int kShortSpread = 148 * 16;    // warps wanted
+
+template <int W, bool kScore>
+__global__ void __launch_bounds__(W > 8 ? 512 : 256) short_kernel(const AttnArgs a) {
+  constexpr int kTeam = W > 8 ? 16 : 8, kHeads = kTeam / W;  // warps and heads of a CTA
+  extern __shared__ __align__(16) float smem_f[];
+  auto part = reinterpret_cast<float(*)[8][kHeadPitch]>(smem_f);  // [kTeam]
+  float* logits = smem_f + kTeam * 8 * kHeadPitch;               // [kHeads][s16][gs]
+  __shared__ float ref[kTeam][8], sum[kTeam][8];
+  __shared__ float2 fin[kHeads][8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int Hkv = a.pool.Hkv, group = a.Hq / Hkv, slot = warp / W, wi = warp % W;
+  const int hid = blockIdx.x * kHeads + slot;
+  const bool mine = hid < a.pool.B * Hkv;
+  const int b = mine ? hid / Hkv : 0, h = mine ? hid - b * Hkv : 0;
+  int n = mine ? a.lens[b] : 0;
+  if (n < 0 || n > a.limit) {
+    if (h == 0 && wi == 0 && lane == 0) set_err(a.err, kErrIndex);
+    n = n < 0 ? 0 : a.limit;
+  }
+  const int nsb = (n + 15) >> 4, ppb = a.pool.page >> 4;
+  float* lg = logits + static_cast<size_t>(slot) * a.s16 * a.gs;
+  Sums sums;
+  sums.clear();
+  if (wi < nsb) {
+    // pages of this warp's blocks wi, wi + W, ...: lane i the i-th
+    const int my_blk = wi + W * lane;
+    int page = -1;
+    if (my_blk < nsb) page = a.pool.table[static_cast<size_t>(b) * a.pool.max_pages + my_blk / ppb];
+    uint4 qf[4];
+    const float unit = load_query(a.q + (static_cast<size_t>(b) * a.Hq + h * group + g) * 128, g < group, a.scale, t, qf);
+    const float xs[2] = {__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4)};
+    auto q_of = [&](int j) { return qf[j]; };
+    const bool ok_page = static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.n_pages);
+    if (my_blk < nsb && !ok_page) set_err(a.err, kErrIndex);
+    const uint32_t oks = __ballot_sync(0xffffffffu, ok_page);
+    const int sg = 4 * (g >> 1) + (g & 1);
+    struct Raw {
+      uint4 k0, k1, v0, v1, s0, s1;
+      uint2 f0, f1;
+      int pos;
+    };
+    auto fetch = [&](int i, Raw& r) {  // this warp's i-th block
+      const int blk = wi + W * i, s = blk * 16 + (lane & 15);
+      r.pos = s < n ? (a.slot_pos ? a.slot_pos[static_cast<size_t>(b) * a.S + s] : 0) : -1;
+      const int pg = __shfl_sync(0xffffffffu, page, i);
+      if (!(oks >> i & 1u)) {
+        r = Raw{};
+        r.pos = -1;
+        return;
+      }
+      const uint8_t* p = a.pool.base + ((static_cast<size_t>(pg) * Hkv + h) * ppb + blk % ppb) * kBlock;
+      r.k0 = *reinterpret_cast<const uint4*>(p + 64 * sg + 16 * t);
+      r.k1 = *reinterpret_cast<const uint4*>(p + 64 * (sg + 2) + 16 * t);
+      r.f0 = *reinterpret_cast<const uint2*>(p + kKScale + 8 * sg);
+      r.f1 = *reinterpret_cast<const uint2*>(p + kKScale + 8 * (sg + 2));
+      r.v0 = *reinterpret_cast<const uint4*>(p + 1024 + 64 * g + 16 * t);
+      r.v1 = *reinterpret_cast<const uint4*>(p + 1536 + 64 * g + 16 * t);
+      r.s0 = *reinterpret_cast<const uint4*>(p + kVScale + 32 * t);
+      r.s1 = *reinterpret_cast<const uint4*>(p + kVScale + 32 * t + 16);
+    };
+    auto process = [&](const Raw& r, int blk) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, r.pos >= 0);  // both halves hold the 16 slots
+      float x[4];
+      block_logits(r.k0, r.k1, r.f0, r.f1, q_of, xs, x);
+      mask_logits(x, mask >> sg);
+      if (kScore && 2 * t < a.gs) {
+        float* to = lg + (blk * 16 + sg) * a.gs + 2 * t;
+        *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+        *reinterpret_cast<float2*>(to + 2 * a.gs) = make_float2(x[2], x[3]);
+      }
+      const uint4 s0 = mask_scales(r.s0, mask >> (4 * t)), s1 = mask_scales(r.s1, mask >> (4 * t + 2));
+      float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+      sums.vote(top, or4(s0) | or4(s1));
+      sums.weigh(x, r.v0, r.v1, s0, s1);
+    };
+    const int count = (nsb - wi + W - 1) / W;
+    Raw cur;
+    fetch(0, cur);
+    for (int i = 0; i < count; ++i) {
+      if (W <= 8) {
+        Raw next;
+        if (i + 1 < count) fetch(i + 1, next);
+        process(cur, wi + W * i);
+        cur = next;
+      } else {
+        process(cur, wi + W * i);
+        if (i + 1 < count) fetch(i + 1, cur);
+      }
+    }
+  }
+  sums.leave(ref[warp], sum[warp], part[warp], group, wi < nsb, g, t);
+  __syncthreads();
+  for (int q = wi; q < group && mine; q += W) {  // one query head per warp, four dims per lane
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, ref[slot * W + w][q]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float rw = ref[slot * W + w][q], lw = sum[slot * W + w][q];
+      if (rw > -INFINITY || lw != 0.f) {  // also a NaN sum
+        const float fw = rw == M ? 1.0f : ex2(rw - M);
+        const float4 v = *reinterpret_cast<const float4*>(&part[slot * W + w][q][4 * lane]);
+        L += lw * fw;
+        acc.x += v.x * fw, acc.y += v.y * fw, acc.z += v.z * fw, acc.w += v.w * fw;
+      }
+    }
+    const bool none = L == 0.f;
+    const float r = none ? 0.f : 1.0f / L;
+    __nv_bfloat16* dst = a.out + (static_cast<size_t>(b) * a.Hq + h * group + q) * 128 + 4 * lane;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
+    if (lane == 0) {
+      fin[slot][q] = make_float2(M > -INFINITY ? M : 0.f, r);
+      if (none && n > 0) set_err(a.err, kErrNoValidSlot);
+    }
+  }
+  if (!kScore) return;
+  __syncthreads();
+  for (int s = wi * 32 + lane; s < nsb * 16 && s < a.S; s += W * 32) {
+    float top = 0.f;
+    bool nan = false;
+    for (int q = 0; q < group; ++q) {
+      const float2 f = fin[slot][q];
+      const float p = ex2(lg[s * a.gs + q] - f.x) * f.y;
+      nan |= p != p;
+      top = fmaxf(top, p);
+    }
+    if (nan) set_err(a.err, kErrNanScore);
+    // the kv heads' CTAs meet here; non-negative floats order like their bits
+    if (top > 0.f) atomicMax(reinterpret_cast<int*>(a.step_score + static_cast<size_t>(b) * a.S + s), __float_as_int(top));
+  }
+}
+
+static bool overlap(const void* p, long long np, const void* q, long long nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 static int floats_per_row(int group) { return group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 
 // Sequences per launch: their lengths fit shared memory and the line of blocks 32 bits.
@@ -985,8 +1169,17 @@ static int seqs_per_launch(int B, int Hkv, int limit) {
   return static_cast<int>(n < B ? n : B);
 }
 
+// Warps per head of the one-launch form, 0 where the streaming form is the faster one.
+static int short_warps(int B, int Hkv, int limit) {
+  const long long heads = static_cast<long long>(B) * Hkv, nsb = (limit + 15) / 16;
+  if (nsb > kShortBlocks || heads * nsb > kShortTotal) return 0;
+  int W = 1;  // a lane keeps one block's page, and every SM gets its warps
+  while (W < 16 && (32 * W < nsb || (W < nsb && heads * W < kShortSpread))) W *= 2;
+  return W;
+}
+
 static long long workspace_bytes(int B, int Hq, int Hkv, int limit, bool score) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || limit < 0) return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || limit < 0 || short_warps(B, Hkv, limit)) return 0;
   long long n = kHeaderBytes + kPartBytes;
   if (score) {
     const long long pairs = static_cast<long long>(seqs_per_launch(B, Hkv, limit)) * Hkv;
@@ -995,20 +1188,61 @@ static long long workspace_bytes(int B, int Hq, int Hkv, int limit, bool score) 
   return n;
 }
 
+static long long limit_of(const Pool& pool, bool bounded, int S) {  // slots of a sequence at most
+  const long long n = static_cast<long long>(pool.max_pages) * pool.page;
+  return bounded && S < n ? S : n;
+}
+
+template <int W>
+static int launch_short(cudaStream_t stream, const AttnArgs& a) {
+  constexpr int kTeam = W > 8 ? 16 : 8;
+  auto kernel = a.step_score ? short_kernel<W, true> : short_kernel<W, false>;
+  if (prepare_device(reinterpret_cast<const void*>(kernel), kShortSmem) <= 0)
+    return fail(kStatusCuda, "kv4_attn: no usable CUDA device");
+  const size_t smem = (kTeam * 8 * kHeadPitch + (a.step_score ? kTeam / W * a.s16 * a.gs : 0)) * sizeof(float);
+  const int heads = a.pool.B * a.pool.Hkv, per = kTeam / W;
+  const cudaError_t e = launch_pdl(kernel, dim3((heads + per - 1) / per), dim3(kTeam * 32), smem, stream, dim3(0), a);
+  if (e != cudaSuccess) return fail(kStatusCuda, "kv4_attn launch: %s", cudaGetErrorString(e));
+  return kStatusOk;
+}
+
 static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const void* q, const int* lens,
                   const int* slot_pos, int S, float scale, void* out, float* step_score, void* ws, long long ws_bytes,
                   int* err) {
-  auto kernel = step_score ? attend_kernel<true> : attend_kernel<false>;
-  const int sms = prepare_device(reinterpret_cast<const void*>(kernel), sizeof(Smem));
-  if (sms <= 0) return fail(kStatusCuda, "kv4_attn: no usable CUDA device");
-  cudaError_t e;
+  if (const int W = short_warps(B, pool.Hkv, static_cast<int>(limit_of(pool, slot_pos || step_score, S)))) {
+    AttnArgs a{};
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.pool = pool;
+    a.lens = lens;
+    a.slot_pos = slot_pos;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.step_score = step_score;
+    a.err = err;
+    a.scale = scale;
+    a.Hq = Hq;
+    a.S = S;
+    a.limit = static_cast<int>(limit_of(pool, slot_pos || step_score, S));
+    a.s16 = (a.limit + 15) / 16 * 16;
+    a.gs = floats_per_row(Hq / pool.Hkv);
+    switch (W) {
+      case 1: return launch_short<1>(stream, a);
+      case 2: return launch_short<2>(stream, a);
+      case 4: return launch_short<4>(stream, a);
+      case 8: return launch_short<8>(stream, a);
+      default: return launch_short<16>(stream, a);
+    }
+  }
+  if (!ws || !aligned16(ws)) return fail(kStatusArg, "kv4_attn: no aligned workspace");
   const int Hkv = pool.Hkv, group = Hq / Hkv;
-  long long limit = static_cast<long long>(pool.max_pages) * pool.page;
-  if ((slot_pos || step_score) && S < limit) limit = S;
+  const long long limit = limit_of(pool, slot_pos || step_score, S);
   const int each = seqs_per_launch(B, Hkv, static_cast<int>(limit));
   if (each <= 0) return fail(kStatusUnsupported, "kv4_attn: too many heads and slots");
   if (ws_bytes < workspace_bytes(B, Hq, Hkv, static_cast<int>(limit), step_score != nullptr))
     return fail(kStatusArg, "kv4_attn: workspace of %lld bytes is too small", ws_bytes);
+  auto kernel = step_score ? attend_kernel<true> : attend_kernel<false>;
+  const int sms = prepare_device(reinterpret_cast<const void*>(kernel), sizeof(Smem));
+  if (sms <= 0) return fail(kStatusCuda, "kv4_attn: no usable CUDA device");
+  cudaError_t e;
   const int nsb = static_cast<int>((limit + 15) / 16);
   for (int b0 = 0; b0 < B; b0 += each) {
     AttnArgs a;
@@ -1033,7 +1267,8 @@ static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const vo
     a.s16 = nsb * 16;
     a.gs = floats_per_row(group);
     const long long line = static_cast<long long>(a.pool.B) * Hkv * nsb;
-    long long grid = (line + kMinBlocks - 1) / kMinBlocks;
+    const int least = nsb < kMinBlocks ? nsb : kMinBlocks;
+    long long grid = (line + least - 1) / least;
     const int most = kCtas * sms < kMaxCtas ? kCtas * sms : kMaxCtas;
     grid = grid < 1 ? 1 : grid > most ? most : grid;
     e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kWarps * 32), sizeof(Smem), stream, dim3(0), a);
@@ -1047,11 +1282,6 @@ static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const vo
 }
 
 constexpr int kManyRows = 2048;  // from here on eight rows per CTA
-static bool overlap(const void* p, long long np, const void* q, long long nq) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a < b + nq && b < a + np;
-}
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Checks shared by the three entry points; fills ``p``.
 static int make_pool(const char* what, int B, int Hkv, int D, int page, int n_pages, int max_pages, const void* pool,
@@ -1139,13 +1369,13 @@ extern "C" int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_
   kv4::Pool p;
   if (int st = kv4::make_pool("kv4_attn", B, Hkv, head_dim, page_size, n_pages, max_pages, pool, page_table, &p))
     return st;
-  if (!q || !lens || !out || !workspace) return fail(kvbp::kStatusArg, "kv4_attn: null pointer");
+  if (!q || !lens || !out) return fail(kvbp::kStatusArg, "kv4_attn: null pointer");
   if (Hq <= 0 || Hq % Hkv) return fail(kvbp::kStatusArg, "kv4_attn: Hq must be a multiple of Hkv");
   if (Hq / Hkv > 8) return fail(kvbp::kStatusUnsupported, "kv4_attn: query group %d > 8", Hq / Hkv);
   if (Hq > 4096) return fail(kvbp::kStatusUnsupported, "kv4_attn: %d query heads > 4096", Hq);
   if (S < 0 || ((slot_pos || step_score) && S == 0)) return fail(kvbp::kStatusArg, "kv4_attn: bad slot stride");
-  if (!kv4::aligned16(q) || !kv4::aligned16(out) || !kv4::aligned16(workspace))
-    return fail(kvbp::kStatusArg, "kv4_attn: q, out and the workspace must be 16-byte aligned");
+  if (!kv4::aligned16(q) || !kv4::aligned16(out))
+    return fail(kvbp::kStatusArg, "kv4_attn: q and out must be 16-byte aligned");
   if (kv4::overlap(q, 256ll * B * Hq, out, 256ll * B * Hq))
     return fail(kvbp::kStatusArg, "kv4_attn: out must not overlap q");
   return kv4::attend(reinterpret_cast<cudaStream_t>(stream), B, Hq, p, q, lens, slot_pos, S, scale, out, step_score,

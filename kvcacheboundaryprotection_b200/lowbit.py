@@ -220,11 +220,11 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
         raise ValueError("the pool, the page table, slot_pos and step_score must not be empty")
     limit = min(width * page, S) if S else width * page
     ws_bytes = _attn_workspace(B, hq, hkv, limit, step_score is not None)
-    ws = pool.new_empty(ws_bytes)
+    ws = pool.new_empty(ws_bytes) if ws_bytes else None  # short sequences need none
     _launch(
         lib().kvbp_kv4_attn, "kv4_attn", dev, B, hq, hkv, HEAD_DIM, page, n_pages, width, q.data_ptr(), pool.data_ptr(),
         page_table.data_ptr(), lens.data_ptr(), _ptr(slot_pos), S, _SCALE if scale is None else scale, out.data_ptr(),
-        _ptr(step_score), ws.data_ptr(), ws_bytes, _ptr(dev_err),
+        _ptr(step_score), _ptr(ws), ws_bytes, _ptr(dev_err),
     )
     return out
 

@@ -195,11 +195,14 @@ def test_append_and_gather_out_of_range_slots_and_pages_are_skipped():
 
 
 # ------------------------------------------------------------------------------- attend
-def _attend_case(lens, hq, hkv, page, masked, seed, loud=1.0, width=None):
+def _attend_case(lens, hq, hkv, page, masked, seed, loud=1.0, width=None, wide=False):
+    """``wide``: a page table for more than 2048 slots, which the streaming kernel takes whatever
+    the lengths; without it short sequences take the one-launch kernel."""
     g = _gen(seed)
     B = len(lens)
     need = [(n + page - 1) // page for n in lens]
     w = max(1, max(need)) + 1 if width is None else width
+    w = max(w, 2100 // page + 2) if wide else w
     n_pages = sum(need) + 2
     k = torch.randn(n_pages, hkv, page, 128, generator=g).double()
     k[..., ::17] *= 6
@@ -255,15 +258,31 @@ def _check_attend(c, score=None, scale=None, dev_err_want=0):
 
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 1), (6, 2), (4, 1), (28, 4), (8, 1), (32, 8), (5, 5)])
 @pytest.mark.parametrize("page", [16, 48, 64])
-def test_attend_lengths_around_every_edge(hq, hkv, page):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_lengths_around_every_edge(hq, hkv, page, wide):
     lens = [1, 0, 15, 16, 17, 31, 32, 33, 100, 257, 0, 48, 7]
-    _check_attend(_attend_case(lens, hq, hkv, page, False, hq * 100 + page))
+    _check_attend(_attend_case(lens, hq, hkv, page, False, hq * 100 + page, wide=wide))
+
+
+@pytest.mark.parametrize("B,n", [(1, 2000), (3, 700), (20, 513), (150, 60), (300, 33), (2500, 5)])
+def test_attend_short_forms_from_one_to_sixteen_warps_a_head(B, n):
+    g = _gen(B)
+    lens = torch.randint(0, n + 1, (B,), generator=g)
+    lens[0] = n
+    for masked in (False, True):
+        c = _attend_case(lens.tolist(), 4, 1, 16, masked, B + n)
+        if masked:
+            c["slot_pos"][:, 0] = 1
+            _check_attend(c, torch.rand(c["slot_pos"].shape, generator=g) * (torch.rand(c["slot_pos"].shape, generator=g) < 0.3))
+        else:
+            _check_attend(c)
 
 
 @pytest.mark.parametrize("hq,hkv,page,lens", [(28, 4, 16, [1000, 1, 300]), (7, 1, 64, [2500]), (16, 2, 128, [700] * 9),
                                               (32, 8, 16, [64] * 40), (8, 8, 32, [0, 5, 4000])])
-def test_attend_masked_with_score_and_poisoned_free_slots(hq, hkv, page, lens):
-    c = _attend_case(lens, hq, hkv, page, True, 7 + hq)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_masked_with_score_and_poisoned_free_slots(hq, hkv, page, lens, wide):
+    c = _attend_case(lens, hq, hkv, page, True, 7 + hq, wide=wide)
     for b, n in enumerate(lens):
         if n:
             c["slot_pos"][b, n // 2] = 5  # no sequence without a live slot here
@@ -273,12 +292,13 @@ def test_attend_masked_with_score_and_poisoned_free_slots(hq, hkv, page, lens):
     _check_attend(c, score)
     _check_attend(c)
     c["slot_pos"] = None  # a score without a mask needs clean slots
-    c["pool"] = _attend_case(lens, hq, hkv, page, False, 7 + hq)["pool"]
+    c["pool"] = _attend_case(lens, hq, hkv, page, False, 7 + hq, wide=wide)["pool"]
     _check_attend(c, torch.zeros(B, S))
 
 
-def test_attend_sequences_without_a_live_slot_give_zeros():
-    c = _attend_case([40, 40, 0, 700], 8, 2, 16, True, 11)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_sequences_without_a_live_slot_give_zeros(wide):
+    c = _attend_case([40, 40, 0, 700], 8, 2, 16, True, 11, wide=wide)
     c["slot_pos"][0] = -1
     c["slot_pos"][3, :700] = -1
     _poison(c)
@@ -287,8 +307,9 @@ def test_attend_sequences_without_a_live_slot_give_zeros():
     assert (out[[0, 2, 3]] == 0).all() and (out[1] != 0).any()
 
 
-def test_attend_one_live_slot_returns_its_value():
-    c = _attend_case([300, 300], 4, 1, 16, True, 12)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_one_live_slot_returns_its_value(wide):
+    c = _attend_case([300, 300], 4, 1, 16, True, 12, wide=wide)
     c["slot_pos"][:] = -1
     c["slot_pos"][0, 299] = 9
     c["slot_pos"][1, 0] = 0
@@ -297,9 +318,10 @@ def test_attend_one_live_slot_returns_its_value():
 
 
 @pytest.mark.parametrize("loud", [1e-7, 1e-4, 3e4, 2e5])
-def test_attend_value_magnitudes(loud):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_value_magnitudes(loud, wide):
     """V scales from f16's subnormals to its top: the weights keep their precision."""
-    _check_attend(_attend_case([600, 33], 4, 1, 32, False, 13, loud=loud))
+    _check_attend(_attend_case([600, 33], 4, 1, 32, False, 13, loud=loud, wide=wide))
 
 
 def test_attend_mixed_magnitudes_rescale_the_running_sums():
@@ -316,8 +338,9 @@ def test_attend_mixed_magnitudes_rescale_the_running_sums():
     _check_attend(c, torch.zeros(1, 3000))
 
 
-def test_attend_nan_in_a_live_slot_reaches_only_its_sequence():
-    c = _attend_case([200, 200], 4, 2, 16, False, 15)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_nan_in_a_live_slot_reaches_only_its_sequence(wide):
+    c = _attend_case([200, 200], 4, 2, 16, False, 15, wide=wide)
     p = c["pool"].numpy().copy()
     (_, ks), _ = ref.layout()
     p[c["table"][0, 3], 0, 0, ks[5, 2] + 1] = 0x7F  # slot 53 of head 0: a NaN K scale
@@ -328,25 +351,27 @@ def test_attend_nan_in_a_live_slot_reaches_only_its_sequence():
     assert torch.equal(out[0, 2:], clean[0, 2:]) and torch.equal(out[1], clean[1])
 
 
-def test_attend_bad_pages_and_lengths():
-    c = _attend_case([100, 64], 4, 2, 16, False, 16)
+@pytest.mark.parametrize("width", [7, 200])
+def test_attend_bad_pages_and_lengths(width):
+    c = _attend_case([100, 64], 4, 2, 16, False, 16, width=width)
     c["table"][0, 2] = 9999
     c["table"][1, 0] = -1
     _check_attend(c, dev_err_want=4)
-    c = _attend_case([100, 64], 4, 2, 16, False, 17, width=7)
+    c = _attend_case([100, 64], 4, 2, 16, False, 17, width=width)
     d = _on_gpu(c)
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     c["table"][0, :] = c["table"][0, :].clamp(min=0)
     long = torch.tensor([10 ** 6, -3], dtype=torch.int32, device="cuda")
     out = lowbit.kv4_attend(d["pool"], c["table"].cuda(), long, d["q"], dev_err=err)
     assert int(err) == 4
-    c["lens"] = torch.tensor([112, 0], dtype=torch.int32)
+    c["lens"] = torch.tensor([16 * width, 0], dtype=torch.int32)  # as many slots as the table has
     want, _, bound, _ = ref.attend(c["pool"], c["table"], c["lens"], c["q"], None, 1 / math.sqrt(128))
     assert ((out.cpu().double() - want).abs() <= bound).all()
 
 
-def test_attend_scale_and_unusual_queries():
-    c = _attend_case([130, 20], 4, 2, 16, False, 18)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_scale_and_unusual_queries(wide):
+    c = _attend_case([130, 20], 4, 2, 16, False, 18, wide=wide)
     c["q"][0, 0] = 0
     c["q"][0, 1] *= 1e-30
     c["q"][1, 2] = (c["q"][1, 2].float() * 1e-3).to(BF)
@@ -361,7 +386,8 @@ def test_attend_scale_and_unusual_queries():
 def test_attend_many_sequences_and_one_long():
     """More sequences than one launch takes, and one whose parts every CTA shares."""
     lens = [(37 * b) % 90 for b in range(1100)]
-    _check_attend(_attend_case(lens, 2, 1, 16, False, 19))
+    _check_attend(_attend_case(lens, 2, 1, 16, False, 19, wide=True))
+    _check_attend(_attend_case([3, 0, 5] * 30, 8, 8, 16, False, 23, wide=True))
     c = _attend_case([30011], 4, 1, 64, True, 20)
     _check_attend(c, torch.zeros(c["slot_pos"].shape))
 

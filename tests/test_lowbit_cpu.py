@@ -65,19 +65,20 @@ def test_gather_refusals(L, bad):
 
 @pytest.mark.parametrize(
     "bad,status",
-    [(dict(q=None), 1), (dict(lens=None), 1), (dict(out=None), 1), (dict(ws=None), 1), (dict(Hq=5), 1), (dict(Hq=0), 1),
+    [(dict(q=None), 1), (dict(lens=None), 1), (dict(out=None), 1), (dict(ws=None, width=1000), 1), (dict(wsb=100, width=1000), 1), (dict(Hq=5), 1), (dict(Hq=0), 1),
      (dict(Hq=18), 2), (dict(Hq=8192, Hkv=1024), 2), (dict(pos=A), 1), (dict(score=A), 1), (dict(S=-1), 1),
-     (dict(q=A + 8), 1), (dict(out=A + 65544), 1), (dict(out=A), 1), (dict(ws=A + 4), 1)],
+     (dict(q=A + 8), 1), (dict(out=A + 65544), 1), (dict(out=A), 1), (dict(ws=A + 4, width=1000), 1)],
 )
 def test_attention_refusals(L, bad, status):
     assert _attn(L, **bad) == status
 
 
 def test_attention_workspace(L):
-    plain = L.kvbp_kv4_attn_workspace(2, 4, 2, 100, 0)
+    assert L.kvbp_kv4_attn_workspace(2, 4, 2, 2048, 1) == 0  # short sequences: one launch, none needed
+    plain = L.kvbp_kv4_attn_workspace(2, 4, 2, 2049, 0)
     assert plain > 0 and plain == L.kvbp_kv4_attn_workspace(100, 32, 8, 100000, 0)  # no score: whatever the size
-    scored = L.kvbp_kv4_attn_workspace(2, 4, 2, 100, 1)
-    assert scored - plain == 2 * 2 * 64 + 2 * 2 * 112 * 2 * 4  # (ref, sum) and the logits of 112 slots, 2 heads each
+    scored = L.kvbp_kv4_attn_workspace(2, 4, 2, 2050, 1)
+    assert scored - plain == 2 * 2 * 64 + 2 * 2 * 2064 * 2 * 4  # (ref, sum) and the logits of 2064 slots, 2 heads each
     assert L.kvbp_kv4_attn_workspace(0, 4, 2, 100, 1) == 0
 
 
