@@ -1016,11 +1016,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
 // for that, and few blocks a warp).
 constexpr int kShortBlocks = 128;      // blocks of a head at most (2048 slots)
 constexpr int kShortSmem = 168 * 1024;
-constexpr long long kShortTotal = 8192;   // blocks of all heads at most
-constexpr int kShortSpread = 148 * 16;    // warps wanted
+constexpr int kShortAlways = 16;          // blocks of a head up to which this form always wins
+constexpr long long kShortTotal = 16384;  // beyond them: blocks of all heads at most
+constexpr int kShortSpread = 148 * 16;    // warps that are resident at once
 
 template <int W, bool kScore>
-__global__ void __launch_bounds__(W > 8 ? 512 : 256) short_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(W > 8 ? 512 : 256, W > 8 ? 1 : 2) short_kernel(const AttnArgs a) {
   constexpr int kTeam = W > 8 ? 16 : 8, kHeads = kTeam / W;  // warps and heads of a CTA
   extern __shared__ __align__(16) float smem_f[];
   auto part = reinterpret_cast<float(*)[8][kHeadPitch]>(smem_f);  // [kTeam]
@@ -1170,11 +1171,16 @@ static int seqs_per_launch(int B, int Hkv, int limit) {
 }
 
 // Warps per head of the one-launch form, 0 where the streaming form is the faster one.
+// Measured, one launch against streaming, without a score (28 heads over 4): 4.6 against 6.6 us
+// at 64 kv heads of 64 slots, 34.8 against 54.9 at 2048 of 256 (so always up to 16 blocks), 9.6
+// against 10.4 at 64 of 1024, 18.0 against 22.8 at 512 of 512, 14.9 against 18.6 at 128 of 2048;
+// but 33.2 against 31.1 at 512 of 1024 and 32.5 against 27.6 at 256 of 2048.
 static int short_warps(int B, int Hkv, int limit) {
   const long long heads = static_cast<long long>(B) * Hkv, nsb = (limit + 15) / 16;
-  if (nsb > kShortBlocks || heads * nsb > kShortTotal) return 0;
-  int W = 1;  // a lane keeps one block's page, and every SM gets its warps
-  while (W < 16 && (32 * W < nsb || (W < nsb && heads * W < kShortSpread))) W *= 2;
+  if (nsb > kShortAlways && (nsb > kShortBlocks || heads * nsb > kShortTotal)) return 0;
+  if (heads > 0x7fffffffll) return 0;
+  int W = 1;  // a lane keeps one block's page; all warps at once where there are few heads
+  while (W < 16 && (32 * W < nsb || (W < nsb && heads * 2 * W <= kShortSpread))) W *= 2;
   return W;
 }
 
