@@ -109,6 +109,33 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
 // past the matrices arrive as zeros: sizes are free); the accumulator is int32 in TMEM, lane =
 // output channel, column = token, so a warp's stores of one token's 32 channels are contiguous.
 // Integer sums are exact, so K may be split and joined in any order with the same bits.
+// The same for rows of up to 1024: a warp per row, eight rows a CTA, no barrier.
+__global__ void __launch_bounds__(256) quant_short_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int K,
+                                                               int rows, int vec, int8_t* __restrict__ q, long long ldq,
+                                                               float* __restrict__ scale) {
+  pdl_wait();
+  pdl_launch_dependents();  // as above
+  const unsigned r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= static_cast<unsigned>(rows)) return;
+  const int lane = threadIdx.x & 31, nv = vec ? K / 8 : 0;
+  const __nv_bfloat16* row = x + static_cast<size_t>(r) * ldx;
+  int8_t* dst = q + static_cast<size_t>(r) * ldq;
+  uint4 keep[4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    keep[u] = lane + 32 * u < nv ? reinterpret_cast<const uint4*>(row)[lane + 32 * u] : make_uint4(0, 0, 0, 0);
+    m = fold_max(m, keep[u]);
+  }
+  for (int i = nv * 8 + lane; i < K; i += 32) m = max(m, abs_bits(row[i]));
+  const RowQuant rq(__reduce_max_sync(0xffffffffu, m));
+  if (lane == 0) scale[r] = rq.scale();
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + 32 * u < nv) *reinterpret_cast<uint2*>(dst + 8 * (lane + 32 * u)) = rq.eight(keep[u]);
+  for (int i = nv * 8 + lane; i < K; i += 32) dst[i] = static_cast<int8_t>(rq.exact(__bfloat162float(row[i])));
+}
+
 struct Args {
   const float* sw;
   const float* sx;
@@ -422,9 +449,11 @@ constexpr int kPN = 256;
 constexpr int kPStages = 4;
 constexpr int kPStage = kTileW + kPN * kBK;
 constexpr int kPBytes = kPStages * kPStage + 1024 + 256 + 2 * kPN * 4;
+constexpr int kPEpilogue = 16;  // warps: with four, one a scheduler, a tile's 256 tokens took 8 us
+constexpr int kPThreads = (2 + kPEpilogue) * 32;
 constexpr int kBand = 16;  // channel tiles per raster band
 
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPThreads, 1)
     persist_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -454,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accfull[b], 1);
-      mbar_init(&accempty[b], 4);
+      mbar_init(&accempty[b], kPEpilogue);
     }
     *bad = 0;
     fence_barrier_init();
@@ -528,39 +557,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, et = tid - 64;  // 128 epilogue threads
+    // four warps per TMEM lane quarter, a quarter of the tokens each
+    constexpr int kShare = kPN * 4 / kPEpilogue;
+    const int q = warp & 3, et = tid - 64, share = (warp - 2) / 4 * kShare;
     int i = 0;
     for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
       const int buf = i & 1;
       int n0, m0;
       tile_of(t, n0, m0);
       const int n = n0 + q * 32 + lane, cols = min(kPN, a.M - m0);
-      for (int c = et; c < kPN; c += 128) sxs[buf * kPN + c] = c < cols ? a.sx[m0 + c] : 0.f;
-      const float sw = n < a.N ? a.sw[n] : 0.f;
-      const float bias = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+      for (int c = et; c < kPN; c += kPEpilogue * 32) sxs[buf * kPN + c] = c < cols ? a.sx[m0 + c] : 0.f;
       const bool ok = wait_or_fail(&accfull[buf], static_cast<uint32_t>(i >> 1) & 1);
       tc_after();
-      // the tile's scales are in place, and all four warps leave together after a failed wait
-      if (named_bar_or(1, 128, !ok || !healthy())) break;
+      // the tile's scales are in place, and all epilogue warps leave together after a failed wait
+      if (named_bar_or(1, kPEpilogue * 32, !ok || !healthy())) break;
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * kPN);
-      const size_t row = static_cast<size_t>(m0) * a.ldo + n;
+      const float* sx = sxs + buf * kPN;
+      // one channel a lane; the warp reads TMEM as a whole, past the last channel too
+      const bool in = n < a.N;
+      const float sw = in ? a.sw[n] : 0.f, bias = a.bias && in ? __bfloat162float(a.bias[n]) : 0.f;
+      const size_t row = static_cast<size_t>(m0 + share) * a.ldo + n;
+      float* pf = static_cast<float*>(a.out) + row;
+      __nv_bfloat16* ph = static_cast<__nv_bfloat16*>(a.out) + row;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
+      for (int c = share; c < min(cols, share + kShare); c += 32) {
         int v[32];
+        __syncwarp();
         ld_acc<32>(acc + c, v);
-        if (n < a.N) {
-          if (a.f32) {
-            float* dst = static_cast<float*>(a.out) + row + static_cast<size_t>(c) * a.ldo;
+        const int live = in ? cols - c : 0;
+        if (a.f32) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c + k < cols) dst[k * a.ldo] = static_cast<float>(v[k]) * sxs[buf * kPN + c + k] * sw + bias;
-          } else {
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + row + static_cast<size_t>(c) * a.ldo;
+          for (int k = 0; k < 32; ++k, pf += a.ldo)
+            if (k < live) *pf = static_cast<float>(v[k]) * sx[c + k] * sw + bias;
+        } else {
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c + k < cols)
-                dst[k * a.ldo] = __float2bfloat16_rn(static_cast<float>(v[k]) * sxs[buf * kPN + c + k] * sw + bias);
-          }
+          for (int k = 0; k < 32; ++k, ph += a.ldo)
+            if (k < live) *ph = __float2bfloat16_rn(static_cast<float>(v[k]) * sx[c + k] * sw + bias);
         }
       }
       tc_before();
@@ -613,9 +645,16 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
   if (misaligned(q, 16) || ldq % 16) return fail(kStatusArg, "int8_quant_rows: q rows must be 16-byte aligned");
   // 16-byte loads where x's rows allow them, else one value at a time
   const int vec = !misaligned(x, 16) && ldx % 8 == 0;
-  auto kernel = K <= 4096 ? quant_rows_kernel<2> : K <= 10240 ? quant_rows_kernel<5> : quant_rows_kernel<8>;
-  const cudaError_t e = launch_pdl(kernel, dim3(rows), dim3(256), 0, st, dim3(0), static_cast<const __nv_bfloat16*>(x),
-                                   ldx, K, vec, static_cast<int8_t*>(q), ldq, scale);
+  const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
+  int8_t* qb = static_cast<int8_t*>(q);
+  cudaError_t e;
+  if (K <= 1024) {
+    e = launch_pdl(quant_short_rows_kernel, dim3((static_cast<unsigned>(rows) + 7) / 8), dim3(256), 0, st, dim3(0), xb, ldx,
+                   K, rows, vec, qb, ldq, scale);
+  } else {
+    auto kernel = K <= 4096 ? quant_rows_kernel<2> : K <= 10240 ? quant_rows_kernel<5> : quant_rows_kernel<8>;
+    e = launch_pdl(kernel, dim3(rows), dim3(256), 0, st, dim3(0), xb, ldx, K, vec, qb, ldq, scale);
+  }
   if (e != cudaSuccess) return fail(kStatusCuda, "int8_quant_rows launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
@@ -661,7 +700,7 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
   const int S = splits(tn * tm, steps, sms);
   cudaError_t e;
   if (many)
-    e = launch_pdl(persist_kernel, dim3(static_cast<unsigned>(tn * tm < sms ? tn * tm : sms)), dim3(kThreads), kPBytes, st, dim3(0), wm, xm, a);
+    e = launch_pdl(persist_kernel, dim3(static_cast<unsigned>(tn * tm < sms ? tn * tm : sms)), dim3(kPThreads), kPBytes, st, dim3(0), wm, xm, a);
   else if (NT == 16)
     e = launch_split<16, false>(st, wm, xm, a, S);
   else if (NT == 32)
