@@ -659,10 +659,14 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
   return kStatusOk;
 }
 
-// CTAs that share a tile's K range: enough to give every SM two CTAs, each at least four
+// CTAs that share a tile's K range: two per SM but for a seventh of them (larger clusters do not
+// fill the last places: 72 tiles of 200 tokens took 19.2 us in 4 parts, 288 CTAs, and 14.3 us in
+// 3; pairs do: 144 tiles of 512 tokens 17.9 us in 2, 21.1 unsplit), each with at least four
 // stages of K, within a portable cluster.
+static int room(int sms) { return 2 * sms * 6 / 7; }
 static int splits(long long tiles, int steps, int sms) {
-  long long s = 2ll * sms / tiles;
+  long long s = room(sms) / tiles;
+  if (s < 2 && tiles <= sms) s = 2;
   if (s > steps / 4) s = steps / 4;
   return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : static_cast<int>(s);
 }
@@ -689,8 +693,12 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
   const long long tn = (a.N + 127) / 128;
   const int steps = (a.K + kBK - 1) / kBK;
-  const bool many = a.M > 128 && tn * ((a.M + kPN - 1) / kPN) >= sms;
-  const int NT = many ? kPN : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  // The persistent form from half a wave of its tiles on (1024 x 2560 x 2560, 80 tiles: 15.8 us
+  // against 19.0; 512 x 4608 x 3584, 72 tiles: 18.3 against 17.9).  Below, the narrowest tile that
+  // holds the tokens, but 64 twice instead of 128 where that leaves room to split K (128 x 2560 x
+  // 9728: 15.1 us against 16.4; without room, 128 x 37888 x 3584: 60 against 39).
+  const bool many = a.M > 128 && tn * ((a.M + kPN - 1) / kPN) * 2 > sms;
+  const int NT = many ? kPN : a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 || (a.M <= 128 && tn * 4 <= room(sms)) ? 64 : 128;
   const long long tm = (a.M + NT - 1) / NT;
   if (!many && tm > 65535) return fail(kStatusUnsupported, "int8_gemm: too many tiles");
   CUtensorMap wm, xm;
