@@ -469,7 +469,8 @@ int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t K, const vo
 /* Product in 8-bit integers: out[m][n] = (sum_k xq[m][k] * w[n][k]) * x_scale[m] * w_scale[n]
  * (+ bias[n], bf16, may be NULL), exact 32-bit integer sums, K <= 131071; out bf16 [M][ldo],
  * or float when fp32_out (partial sums to be reduced).  xq [M][ldq] and w [N][ldw] int8 with
- * 16-byte aligned rows; M, N and K are free, columns past K are not read into the sums. */
+ * 16-byte aligned rows; M, N and K are free, columns past K are not read into the sums; out
+ * overlaps neither. */
 int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w, int64_t ldw,
                    const float* w_scale, const void* xq, int64_t ldq, const float* x_scale, const void* bias,
                    void* out, int64_t ldo, int32_t* dev_err);

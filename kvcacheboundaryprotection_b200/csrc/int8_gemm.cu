@@ -671,6 +671,12 @@ static int splits(long long tiles, int steps, int sms) {
   return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : static_cast<int>(s);
 }
 
+static bool overlap(const void* p, long long np, const void* q, long long nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
+static long long out_bytes(const Args& a) { return ((a.M - 1ll) * a.ldo + a.N) * (a.f32 ? 4 : 2); }
+
 // Checks of all but the tokens.
 static int check(const Args& a, const void* w, long long ldw) {
   if (!w || !a.sw || !a.out) return fail(kStatusArg, "int8_gemm: null pointer");
@@ -679,7 +685,8 @@ static int check(const Args& a, const void* w, long long ldw) {
   if (a.K > 131071) return fail(kStatusUnsupported, "int8_gemm: K %d > 131071 could overflow the 32-bit sums", a.K);
   if (misaligned(w, 16) || ldw % 16) return fail(kStatusArg, "int8_gemm: w's rows must be 16-byte aligned");
   if (misaligned(a.out, a.f32 ? 4 : 2)) return fail(kStatusArg, "int8_gemm: misaligned output");
-  if ((a.N + 127) / 128 > 65535) return fail(kStatusUnsupported, "int8_gemm: N %d is too large", a.N);
+  if (a.N > 65535 * 128 || a.M > 0x7ffffe00) return fail(kStatusUnsupported, "int8_gemm: M %d or N %d is too large", a.M, a.N);
+  if (overlap(a.out, out_bytes(a), w, (a.N - 1ll) * ldw + a.K)) return fail(kStatusArg, "int8_gemm: out must not overlap w");
   return kStatusOk;
 }
 
@@ -688,6 +695,7 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
   if (!xq || !a.sx) return fail(kStatusArg, "int8_gemm: null pointer");
   if (ldq < a.K) return fail(kStatusArg, "int8_gemm: bad size");
   if (misaligned(xq, 16) || ldq % 16) return fail(kStatusArg, "int8_gemm: xq's rows must be 16-byte aligned");
+  if (overlap(a.out, out_bytes(a), xq, (a.M - 1ll) * ldq + a.K)) return fail(kStatusArg, "int8_gemm: out must not overlap xq");
   a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
   const int sms = prepare_device(reinterpret_cast<const void*>(persist_kernel), kPBytes);
   if (sms <= 0) return fail(kStatusCuda, "int8_gemm: no usable CUDA device");
@@ -725,9 +733,6 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
 static bool fused(int M, int K) { return M <= kFuseTokens && K <= kFuseSteps * kMaxSplits * kBK; }
 
 static int gemm_fused(cudaStream_t st, Args a, const void* w, long long ldw) {
-  if (int bad = check(a, w, ldw)) return bad;
-  if (!a.x) return fail(kStatusArg, "int8_linear: null pointer");
-  if (a.ldx < a.K) return fail(kStatusArg, "int8_linear: bad size");
   a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
   a.vec_x = !misaligned(a.x, 16) && a.ldx % 8 == 0;
   const int sms = prepare_device(reinterpret_cast<const void*>(split_kernel<16, true>), Ring<16, true>::kBytes);
@@ -771,6 +776,9 @@ extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t 
                    static_cast<const __nv_bfloat16*>(x), ldx, 0, 0, 1, dev_err};
   // the product's arguments first: a refused call leaves the workspace alone
   if (int st = kvbp::i8::check(a, w, ldw)) return st;
+  if (!x || ldx < K) return kvbp::fail(kvbp::kStatusArg, "int8_linear: bad x");
+  if (kvbp::i8::overlap(out, kvbp::i8::out_bytes(a), x, 2 * ((M - 1ll) * ldx + K)))
+    return kvbp::fail(kvbp::kStatusArg, "int8_linear: out must not overlap x");
   if (kvbp::i8::fused(M, K)) return kvbp::i8::gemm_fused(reinterpret_cast<cudaStream_t>(stream), a, w, ldw);
   if (!workspace || kvbp::i8::misaligned(workspace, 16)) return kvbp::fail(kvbp::kStatusArg, "int8_linear: no aligned workspace");
   if (workspace_bytes < kvbp_int8_linear_workspace(M, K))

@@ -150,6 +150,37 @@ def test_append_rows_per_sequence_skips_and_strided_rows():
     assert (k[[1, 4]] == 0).all() and (v[[1, 4]] == 0).all() and (k[0] != 0).any()
 
 
+def test_append_rows_at_any_offset():
+    """qkv, bias and norms off 16-byte boundaries give the bits of aligned ones; eight rows per
+    CTA (many rows) those of one row per CTA."""
+    g = _gen(6)
+    hq, hkv, n = 3, 2, 2100
+    cols = (hq + 2 * hkv) * 128
+    wide = torch.randn(n, cols + 9, generator=g).to(BF).cuda()
+    extra = torch.randn(cols + 300, generator=g).to(BF).cuda()
+    freq = (1e4 ** (-torch.arange(64) / 64.0)).float().cuda()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda") * 191
+    seq = torch.zeros(n, dtype=torch.int32, device="cuda")
+    slots = torch.randperm(n, generator=g).to(torch.int32).cuda()
+    table = torch.randperm(140, generator=g).to(torch.int32)[None].cuda()
+    got = []
+    for off in (0, 1):
+        pool = lowbit.kv4_pool(140, hkv, 16)
+        qkv = wide[:, 1:1 + cols] if off else wide[:, 1:1 + cols].contiguous()
+        bias, qn, kn = (extra[i + 1:i + 1 + m] for i, m in ((0, cols), (7, 128), (100, 128)))
+        if not off:
+            bias, qn, kn = bias.clone(), qn.clone(), kn.clone()
+        kw = dict(n_heads=hq, inv_freq=freq, bias=bias, q_norm=qn, k_norm=kn)
+        q = lowbit.kv4_append(pool, table, qkv, slots, seq=seq, positions=pos, **kw)
+        got.append((q, pool))
+        few = lowbit.kv4_pool(140, hkv, 16)
+        for lo, hi in ((0, 900), (900, n)):
+            part = lowbit.kv4_append(few, table, qkv[lo:hi], slots[lo:hi], seq=seq[lo:hi], positions=pos[lo:hi], **kw)
+            assert torch.equal(part, q[lo:hi])
+        assert torch.equal(few, pool)
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 def test_append_extreme_values():
     """Zero rows, values below and beyond the scale's range, infinities and NaN."""
     hq, hkv = 1, 1
@@ -413,6 +444,22 @@ def test_attend_offsets_past_32_bits():
     assert torch.equal(k[0].cpu(), wk) and torch.equal(v[0].cpu(), wv) and k.any()
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_only_empty_sequences(wide):
+    c = _attend_case([0, 0, 0], 8, 2, 16, True, 24, wide=wide)
+    score = torch.rand(c["slot_pos"].shape, generator=_gen(9))
+    assert not _check_attend(c, score).any()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_sequences_that_share_pages(wide):
+    """A common prefix kept once: the tables of two sequences name the same pages."""
+    c = _attend_case([100, 70, 33], 8, 2, 16, False, 25, wide=wide)
+    c["table"][1, :4] = c["table"][0, :4]
+    c["table"][2, :2] = c["table"][0, :2]
+    _check_attend(c)
+
+
 def test_attend_is_deterministic():
     c = _on_gpu(_attend_case([900, 3, 2000, 0, 77], 28, 4, 16, True, 22))
     s = [torch.zeros(c["slot_pos"].shape, device="cuda") for _ in range(3)]
@@ -545,6 +592,13 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError):
         lowbit.kv4_append(pool, table.long(), q.view(1, -1), lens, n_heads=7)
     x = torch.zeros(2, 17, dtype=BF, device="cuda")
+    w, s = lowbit.int8_quantize_rows(torch.ones(32, 32, dtype=BF, device="cuda"))
+    y = torch.ones(1, 32, dtype=BF, device="cuda")
+    with pytest.raises(capi.KVBPError, match="overlap"):  # CTAs would read what others wrote
+        lowbit.int8_linear(y, w, s, out=y)
+    with pytest.raises(capi.KVBPError, match="overlap"):
+        p = torch.zeros(1, 4, 128, dtype=BF, device="cuda")
+        lowbit.kv4_attend(pool, table, lens, p, out=p)
     with pytest.raises(ValueError):  # weight rows off their 16-byte boundaries
         lowbit.int8_linear(x, torch.zeros(4, 17, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"))
 

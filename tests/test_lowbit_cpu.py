@@ -83,7 +83,7 @@ def test_attention_workspace(L):
 
 
 def _gemm(L, **kw):
-    a = dict(f32=0, M=2, N=64, K=32, w=A, ldw=32, ws=A, xq=A, ldq=32, xs=A, bias=None, out=A, ldo=64, err=None)
+    a = dict(f32=0, M=2, N=64, K=32, w=A, ldw=32, ws=A, xq=A, ldq=32, xs=A, bias=None, out=A + 65536, ldo=64, err=None)
     a.update(kw)
     return L.kvbp_int8_gemm(None, *a.values())
 
@@ -92,8 +92,9 @@ def _gemm(L, **kw):
     "bad,status",
     [(dict(w=None), 1), (dict(ws=None), 1), (dict(xq=None), 1), (dict(xs=None), 1), (dict(out=None), 1), (dict(M=0), 1),
      (dict(N=0), 1), (dict(K=0), 1), (dict(K=33), 1), (dict(ldw=40, K=32), 1), (dict(ldq=40), 1), (dict(ldo=60), 1),
-     (dict(w=A + 8), 1), (dict(xq=A + 8), 1), (dict(out=A + 1), 1), (dict(f32=1, out=A + 2), 1),
-     (dict(K=131072, ldw=131072, ldq=131072), 2)],
+     (dict(w=A + 8), 1), (dict(xq=A + 8), 1), (dict(out=A + 65537), 1), (dict(f32=1, out=A + 65538), 1),
+     (dict(K=131072, ldw=131072, ldq=131072), 2), (dict(M=0x7fffffff), 2), (dict(N=65536 * 128, ldo=65536 * 128), 2),
+     (dict(out=A), 1), (dict(w=A + 65536 + 64, out=A + 65536), 1)],
 )
 def test_product_refusals(L, bad, status):
     assert _gemm(L, **bad) == status
@@ -107,9 +108,13 @@ def test_linear_and_quantisation_refusals(L):
     assert L.kvbp_int8_quant_rows(None, 2, 8, None, 8, A, 16, A) == 1
     need = L.kvbp_int8_linear_workspace(5, 100)
     assert need == 5 * 112 + 20 and L.kvbp_int8_linear_workspace(1, 100) == 0
-    lin = lambda ws, n, M=5, x=A: L.kvbp_int8_linear(None, 0, M, 64, 100, A, 112, A, x, 100, None, A, 64, ws, n, None)  # noqa: E731
+    lin = lambda ws, n, M=5, x=A, out=A + 65536: L.kvbp_int8_linear(  # noqa: E731
+        None, 0, M, 64, 100, A, 112, A, x, 100, None, out, 64, ws, n, None)
     assert lin(None, need) == 1 and lin(A, need - 1) == 1 and lin(A + 8, need) == 1
     assert lin(None, 0, M=1, x=None) == 1
+    for M in (1, 5):
+        assert lin(A + 131072, need, M=M, x=A + 65536) == 1 and b"overlap x" in L.kvbp_last_error()
+        assert lin(A + 131072, need, M=M, out=A + 64) == 1 and b"overlap w" in L.kvbp_last_error()
 
 
 # ---------------------------------------------------------------- the Python entry points
