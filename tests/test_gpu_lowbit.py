@@ -181,6 +181,29 @@ def test_append_rows_at_any_offset():
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
 
 
+def test_append_the_same_row_twice_and_two_calls_on_two_streams():
+    g = _gen(8)
+    qkv = torch.randn(2, 6 * 128, generator=g).to(BF).cuda()
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    want = lowbit.kv4_pool(2, 2, 16)
+    for b in range(2):
+        lowbit.kv4_append(want, table[b:b + 1], qkv[b:b + 1], torch.tensor([5], dtype=torch.int32, device="cuda"), n_heads=2)
+    twice = lowbit.kv4_pool(2, 2, 16)  # equal rows for one slot: that row
+    seq = torch.tensor([0, 0, 1, 1], dtype=torch.int32, device="cuda")
+    lowbit.kv4_append(twice, table, qkv.repeat_interleave(2, 0), torch.full((4,), 5, dtype=torch.int32, device="cuda"),
+                      n_heads=2, seq=seq)
+    assert torch.equal(twice, want)
+    both = lowbit.kv4_pool(2, 2, 16)
+    slot = torch.tensor([5], dtype=torch.int32, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for b in range(2):
+        with torch.cuda.stream(streams[b]):
+            lowbit.kv4_append(both, table[b:b + 1], qkv[b:b + 1], slot, n_heads=2)
+    torch.cuda.synchronize()
+    assert torch.equal(both, want)
+
+
 def test_append_extreme_values():
     """Zero rows, values below and beyond the scale's range, infinities and NaN."""
     hq, hkv = 1, 1
@@ -577,6 +600,72 @@ def test_int8_linear_out_buffer_and_empty_batch():
     out = torch.empty(3, 64, dtype=BF, device="cuda")
     assert lowbit.int8_linear(x.cuda(), wq, ws, out=out) is out
     assert torch.equal(out, lowbit.int8_linear(x.cuda(), wq, ws))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 260, 300), (7, 130, 640), (40, 300, 2048), (130, 1000, 1500), (2000, 5000, 200)])
+@pytest.mark.parametrize("f32", [0, 1])
+def test_product_entry_with_row_strides_leaves_the_gaps_alone(M, N, K, f32):
+    """kvbp_int8_gemm from stored codes: the bits of int8_linear, into a wider output."""
+    x, w, b = _int8_case(M, N, K, M + N, True)
+    wq, ws = lowbit.int8_quantize_rows(w.cuda())
+    xq, xs = lowbit.int8_quantize_rows(x.cuda())
+    dt = torch.float32 if f32 else BF
+    want = lowbit.int8_linear(x.cuda(), wq, ws, b.cuda(), out_dtype=dt)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for pad in (3, 8):
+        out = torch.full((M, N + pad), 7.0, dtype=dt, device="cuda")
+        bias = b.cuda()
+        capi.check(capi.lib().kvbp_int8_gemm(torch.cuda.current_stream().cuda_stream, f32, M, N, K, wq.data_ptr(),
+                                             max(wq.stride(0), (K + 15) // 16 * 16), ws.data_ptr(), xq.data_ptr(),
+                                             max(xq.stride(0), (K + 15) // 16 * 16), xs.data_ptr(), bias.data_ptr(),
+                                             out.data_ptr(), N + pad, err.data_ptr()), "int8_gemm")
+        assert torch.equal(out[:, :N], want) and (out[:, N:] == 7).all() and int(err) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 512, 1024), (20, 512, 1024), (700, 14000, 256)])
+def test_int8_linear_as_a_graph_and_on_two_streams_at_once(M, N, K):
+    x, w, b = _int8_case(M, N, K, 3, True)
+    wq, ws = lowbit.int8_quantize_rows(w.cuda())
+    b = b.cuda()
+    xs = [(x * f).to(BF).cuda() for f in (1.0, -2.5)]
+    want = [lowbit.int8_linear(v, wq, ws, b) for v in xs]
+    cur = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lowbit.int8_linear(cur, wq, ws, b)
+    for v, y in zip(xs * 2, want * 2):
+        cur.copy_(v)
+        graph.replay()
+        assert torch.equal(out, y)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(lowbit.int8_linear(xs[i], wq, ws, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+def test_weight_quantised_right_before_its_product():
+    """The product may fetch weights ahead of the token codes, but not ahead of the kernel that
+    writes them: quantise and multiply back to back, many times, with changing weights."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for M in (1, 16):
+        x = torch.randn(M, 2048, generator=g, device="cuda").to(BF)
+        ws = [torch.randn(4096, 2048, generator=g, device="cuda").to(BF) for _ in range(2)]
+        buf = torch.empty(4096, 2048, dtype=torch.int8, device="cuda")
+        sc = torch.empty(4096, device="cuda")
+        want = [lowbit.int8_linear(x, *lowbit.int8_quantize_rows(w)) for w in ws]
+        torch.cuda.synchronize()
+        L, got = capi.lib(), []
+        for i in range(40):
+            st = torch.cuda.current_stream().cuda_stream
+            capi.check(L.kvbp_int8_quant_rows(st, 4096, 2048, ws[i % 2].data_ptr(), 2048, buf.data_ptr(), 2048,
+                                              sc.data_ptr()), "quant")
+            got.append(lowbit.int8_linear(x, buf, sc))
+        assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
 
 
 # ------------------------------------------------------------------------------ together
