@@ -112,8 +112,9 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, qkv: torch.Tensor, 
 
     ``qkv`` [rows, (n_heads + 2 kv_heads) * 128] bf16 (rows may be strided); row r goes to
     logical slot ``slots[r]`` (negative: not stored) of sequence ``seq[r]`` (default: the
-    rows divide evenly over the page table's sequences).  With ``inv_freq`` [64] float32,
-    q and k are rotated by ``positions[r]``.  Returns q [rows, n_heads, 128] bf16."""
+    rows divide evenly over the page table's sequences).  The slots that one call stores for a
+    sequence must differ: of two rows for one slot either's bytes may stay.  With ``inv_freq``
+    [64] float32, q and k are rotated by ``positions[r]``.  Returns q [rows, n_heads, 128] bf16."""
     n_pages, hkv, page, B, width, dev = _pool(pool, page_table)
     if qkv.dtype is not _BF16 or qkv.device != dev or qkv.dim() != 2:
         raise ValueError("qkv must be a bfloat16 matrix on the pool's device")
