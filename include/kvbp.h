@@ -448,7 +448,10 @@ int kvbp_kv4_gather(kvbp_stream_t stream, int32_t rows, int32_t rows_per_seq, co
  * over the heads, as kvbp_decode_attn_score does.  lens above max_pages * page_size (or S,
  * when slot_pos or step_score is given) is cut there and sets KVBP_DEV_INDEX.  A sequence
  * without a live slot gives zeros (and KVBP_DEV_NO_VALID_SLOT when lens[b] > 0).  Softmax
- * statistics and sums are fp32; values in free slots and past lens never reach the result.
+ * statistics and sums are fp32.  A slot's weight p and p times V's scale are f16 (2^-11 each, and
+ * in each group of 32 dims an absolute 2^-29 of the largest live scale times the largest p, that
+ * head's), far below the 4-bit codes' own step and mostly below out's bf16.  Values in free slots
+ * and past lens never reach the result.
  * workspace: kvbp_kv4_attn_workspace bytes for max_slots = the smaller of max_pages * page_size
  * and (when slot_pos or step_score is given) S, 16-byte aligned, or NULL where that is 0 (short
  * sequences); free to reuse by the next call on the same stream (calls that may overlap need

@@ -340,9 +340,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
 //    code's own, and its sums came out 2^-16 off.)
 //  * scales never touch the codes: K's multiply the four group sums in fp32, V's multiply the
 //    softmax weights (P' = P * scale, f16, rounded at 2^-11: half a bf16 output step is 2^-9).
-// P is 2^(x - ref) with ref = max(x) - e, e chosen from the exponents of the V scales so that
-// P * scale < 2^14, and moved only when the maximum has grown by kSlack bits: P' keeps f16's 11
-// bits far below the largest weight (to 2^-24 of it for scales below 1).
+// P is 2^(x - ref), ref = max(x) - kTop at least and moved only when the maximum has grown by
+// kSlack bits: the largest P is 2^10 to 2^14, so P's smallest step is 2^-34 of the largest weight
+// or finer.  V's scales are brought near 1 by a power of two for each group of 32 dims (taken off
+// O at the end), from the largest scale of the group's live slots: a product's smallest step is
+// 2^-29 of that scale times the largest weight or finer, whatever the other groups hold (2^-48
+// times the weight where all of the group's scales are subnormal).  One exponent for all groups
+// would cost quiet ones beside a loud one their bits.
 // q is brought to [2^14, 2^15) by a power of two for the same reason (exact: q is bf16).
 // A masked slot's logit is -inf and its V scale zero, so nothing it holds (NaN scales of
 // never-written memory included) reaches a sum; codes are finite whatever their bits.
@@ -367,7 +371,8 @@ constexpr int kWarps = 8;
 constexpr int kStages = 2;       // per warp
 constexpr int kStageBlocks = 2;  // 16-slot blocks per stage
 constexpr int kCtas = 2;         // per SM
-constexpr float kSlack = 5.f;    // how far (in bits) the running maximum may grow before a rescale
+constexpr float kTop = 14.f;     // the largest weight is 2^kTop at most, and P' below twice that
+constexpr float kSlack = 4.f;    // how far (in bits) the running maximum may grow before a rescale
 constexpr int kMaxSeqs = 256;    // sequences per launch (their lengths live in shared memory)
 constexpr int kMaxCtas = 320;
 constexpr int kMinBlocks = 2 * kWarps;  // blocks per CTA at least
@@ -397,12 +402,19 @@ struct AttnArgs {
   int s16, gs;  // logit rows per head, floats per row
 };
 
+// The powers of two that a warp takes V's scales by, group by group: scale * 2^-k.
+struct Moves {
+  uint4 shrink;  // 2^-k as f16 pairs
+  int k[4];
+};
+
 struct Smem {
   uint8_t ring[kWarps][kStages][kStageBlocks * kBlock];
   float part[kWarps][8][kHeadPitch];
   float ref[kWarps][8], sum[kWarps][8];
   uint4 q[2][4][32];  // a head's B operands: [parity of the segment][group][lane]
   float xs[2][8];     // and its logits per unit of the MMAs' sums
+  Moves moves[kWarps];
   uint64_t full[kWarps][kStages];
   int first[kMaxSeqs + 1];  // first block of each sequence's first head
   int len[kMaxSeqs];
@@ -453,46 +465,94 @@ __device__ __forceinline__ uint32_t code_pair_hi(uint32_t w) {
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((127 + k) << 23); }
+
 // What a warp has of its slots' softmax: per query head (columns 2 t, 2 t + 1 of the MMAs) the
 // reference exponent and this thread's share of the sum, and O in the MMAs' layout: thread
 // (g, t) holds dims 32 i + 4 g + {0, 1, 2, 3} of the two heads in o[2 i][0, 1], o[2 i][2, 3],
 // o[2 i + 1][0, 1], o[2 i + 1][2, 3].
 struct Sums {
   float o[8][4], l[2], ref[2];
-  float lim[2];     // ref + e: the largest logit that needs no rescale
-  uint32_t fields;  // or of the V scales' exponent fields so far
-  __device__ __forceinline__ void clear() {
+  bool moved;  // some of this warp's k are not 0 (else none is written)
+  Moves* mv;
+  __device__ __forceinline__ void clear(Moves* to) {
+    mv = to;
+    moved = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
     l[0] = l[1] = 0.f;
-    ref[0] = ref[1] = lim[0] = lim[1] = -INFINITY;
-    fields = 0;
+    ref[0] = ref[1] = -INFINITY;
   }
-  // Rescale where a weight would pass 2^e, then with kSlack bits to spare: most stages only
-  // vote.  e keeps P * scale below 2^14 through the V scales' exponent fields or-ed together
-  // (at least the largest; it has to be small enough only, and stays above -4).
-  __device__ __forceinline__ void vote(float (&top)[2], uint32_t bits) {
-    bits &= 0x7c007c00u;
-    if (!__any_sync(0xffffffffu, (bits & ~fields) || top[0] > lim[0] || top[1] > lim[1])) return;
-    fields |= __reduce_or_sync(0xffffffffu, bits);
-    fields |= fields >> 16 | fields << 16;
-    const float e = static_cast<float>(min(15, 28 - static_cast<int>(fields >> 26)));
+  // a slot pair's V scales of all groups, or of groups 2 half and 2 half + 1, times 2^-k
+  __device__ __forceinline__ uint4 scaled(uint4 v) const {
+    const uint4 by = mv->shrink;
+    v.x = half2_bits(__hmul2(bits_half2(v.x), bits_half2(by.x)));
+    v.y = half2_bits(__hmul2(bits_half2(v.y), bits_half2(by.y)));
+    v.z = half2_bits(__hmul2(bits_half2(v.z), bits_half2(by.z)));
+    v.w = half2_bits(__hmul2(bits_half2(v.w), bits_half2(by.w)));
+    return v;
+  }
+  __device__ __forceinline__ uint2 scaled(uint2 v, int half) const {
+    const uint2 by = reinterpret_cast<const uint2*>(&mv->shrink)[half];
+    v.x = half2_bits(__hmul2(bits_half2(v.x), bits_half2(by.x)));
+    v.y = half2_bits(__hmul2(bits_half2(v.y), bits_half2(by.y)));
+    return v;
+  }
+  // Rescale where a weight would pass 2^kTop, then with kSlack bits to spare, or a scale is 2 or
+  // more: most stages only vote.  ``bits``: the warp's live scales as they would enter the
+  // products, or-ed (only those from 2 on have bit 14); most(m) leaves this lane's largest scales
+  // as stored of each group.  True when k is another than before.
+  template <typename Most>
+  __device__ __forceinline__ bool vote(float (&top)[2], uint32_t bits, int lane, Most most) {
+    if (!__any_sync(0xffffffffu, (bits & 0x40004000u) || top[0] > ref[0] + kTop || top[1] > ref[1] + kTop)) return false;
+    const bool fresh = !__any_sync(0xffffffffu, ref[0] > -INFINITY || ref[1] > -INFINITY);  // O is empty
+    // The largest scale of each group, as bits (they order like integers; a NaN makes its own
+    // group NaN whatever k).  Those in [2^-5, 2) stay as they are, so that ordinary values cost no
+    // more than this vote; others go to [1, 2).  k only grows.
+    uint32_t m[4], flags = bits & 0x40004000u ? 16u : 0u;
+    most(m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) flags |= m[i] >= 10u << 10 ? 1u << i : 0u;
+    flags = __reduce_or_sync(0xffffffffu, flags);
+    const bool move = flags >= 16u || (fresh && flags != 15u);
+    if (move) {
+      int now[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = min(30, static_cast<int>(__reduce_max_sync(0xffffffffu, m[i]) >> 10));
+        const int was = moved ? mv->k[i] : 0;
+        now[i] = f >= 10 && f <= 15 ? 0 : f - 15;
+        if (!fresh) now[i] = max(now[i], was);
+        const float g = pow2(was - now[i]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[2 * i][c] *= g, o[2 * i + 1][c] *= g;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane == i) {
+          mv->k[i] = now[i];  // 2^-15 is subnormal
+          reinterpret_cast<uint32_t*>(&mv->shrink)[i] = (now[i] < 15 ? static_cast<uint32_t>(15 - now[i]) << 10 : 0x200u) * 0x10001u;
+        }
+      __syncwarp();
+      moved = true;
+    }
     float f[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-      const float r = top[c] - e > ref[c] ? top[c] - e + kSlack : ref[c];
+      const float r = top[c] > ref[c] + kTop ? top[c] - kTop + kSlack : ref[c];
       f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
       ref[c] = r;
-      lim[c] = r + e;
       l[c] *= f[c];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] *= f[0], o[i][1] *= f[1], o[i][2] *= f[0], o[i][3] *= f[1];
+    return move;
   }
   // O += P V of a block: its logits x, V codes (v0, v1) and V scales (s0, s1) of the slot pairs
   __device__ __forceinline__ void weigh(const float (&x)[4], const uint4 v0, const uint4 v1, const uint4 s0, const uint4 s1) {
@@ -514,6 +574,14 @@ struct Sums {
   }
   // the warp's sums to shared memory: ref and sum [8], O [8][kHeadPitch] of the live heads
   __device__ __forceinline__ void leave(float* to_ref, float* to_sum, float (*to_o)[kHeadPitch], int group, bool any, int g, int t) {
+    if (moved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = pow2(mv->k[i >> 1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] *= u;
+      }
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
@@ -555,18 +623,22 @@ __device__ __forceinline__ void block_logits(const uint4 k0, const uint4 k1, con
   x[2] *= xs[0];
   x[3] *= xs[1];
 }
+__device__ __forceinline__ uint32_t or4(const uint4 v) { return v.x | v.y | v.z | v.w; }
+__device__ __forceinline__ uint32_t max_half(uint32_t pair) { return max(pair & 0x7fffu, pair >> 16 & 0x7fffu); }
 // -inf for the masked ones of slots sg and sg + 2 (bits 0 and 2 of m)
 __device__ __forceinline__ void mask_logits(float (&x)[4], uint32_t m) {
   if (!(m & 1u)) x[0] = x[1] = -INFINITY;
   if (!(m & 4u)) x[2] = x[3] = -INFINITY;
 }
 // the V scales of a slot pair, zero where masked (the memory may hold anything)
+__device__ __forceinline__ uint32_t pair_mask(uint32_t two) {
+  return (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+}
 __device__ __forceinline__ uint4 mask_scales(uint4 v, uint32_t two) {
-  const uint32_t keep = (two & 1u ? 0x0000ffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+  const uint32_t keep = pair_mask(two);
   v.x &= keep, v.y &= keep, v.z &= keep, v.w &= keep;
   return v;
 }
-__device__ __forceinline__ uint32_t or4(const uint4 v) { return v.x | v.y | v.z | v.w; }
 // q of head g (zeros where not live) as the MMA's B operands, group j in qf[j], brought to
 // [2^14, 2^15) by 2^up; returns the head's logits in units of ln 2 per unit of the MMAs' sums:
 // scale log2(e) / 2^up, in two factors (2^-up alone can overflow).
@@ -778,7 +850,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
     }
     const float xs[2] = {sm.xs[buf][2 * t], sm.xs[buf][2 * t + 1]};
     Sums sums;
-    sums.clear();
+    sums.clear(&sm.moves[warp]);
     auto q_of = [&](int j) { return sm.q[buf][j][lane]; };
 
     const int per = cs.per();
@@ -798,7 +870,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
 #pragma unroll
       for (int s = 1; s < kStages; ++s) mask = s == st ? masks[s] : mask;
       if (dead) mask = 0;
-      const uint8_t* base = sm.ring[warp][st];
+      uint8_t* base = sm.ring[warp][st];
       auto process = [&](auto full_stage) {
         constexpr bool kFull = decltype(full_stage)::value;  // no mask, no missing block
         auto v_scales = [&](int bl, int h) {  // of this thread's slot pair 4 t + 2 h
@@ -806,7 +878,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
           return kFull ? v : mask_scales(v, mask >> (16 * bl + 4 * t + 2 * h));
         };
         float x[kStageBlocks][4], top[2] = {-INFINITY, -INFINITY};
-        uint32_t bits = 0;
 #pragma unroll
         for (int bl = 0; bl < kStageBlocks; ++bl) {
           if (!kFull && bl >= nb) break;
@@ -823,9 +894,24 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) attend_kernel(const AttnAr
           }
           top[0] = fmaxf(top[0], fmaxf(x[bl][0], x[bl][2]));
           top[1] = fmaxf(top[1], fmaxf(x[bl][1], x[bl][3]));
-          bits |= or4(v_scales(bl, 0)) | or4(v_scales(bl, 1));
         }
-        sums.vote(top, bits);
+        // lane 16 bl + 4 t + 2 h + p has the stage's V scales of slots 4 t + 2 h and the next of
+        // block bl, groups 2 p and 2 p + 1
+        static_assert(kStageBlocks == 2, "a lane's two words");
+        uint2* two = reinterpret_cast<uint2*>(base + (lane >> 4) * kBlock + kVScale) + (lane & 15);
+        const uint32_t keep = kFull ? 0xffffffffu : pair_mask(mask >> (lane & 30));
+        uint2 w = *two;
+        if (sums.moved) w = sums.scaled(w, lane & 1);
+        sums.vote(top, (w.x | w.y) & keep, lane, [&](uint32_t (&m)[4]) {
+          const uint2 v = *two;
+          const uint32_t a = max_half(v.x & keep), b = max_half(v.y & keep);
+          m[0] = lane & 1 ? 0u : a, m[1] = lane & 1 ? 0u : b, m[2] = lane & 1 ? a : 0u, m[3] = lane & 1 ? b : 0u;
+        });
+        if (sums.moved) {  // the products below find them scaled
+          *two = sums.scaled(*two, lane & 1);
+          fence_proxy_async_smem();  // the next copy into the stage comes after these writes
+          __syncwarp();
+        }
 #pragma unroll
         for (int bl = 0; bl < kStageBlocks; ++bl) {
           if (!kFull && bl >= nb) break;
@@ -1036,6 +1122,7 @@ __global__ void __launch_bounds__(W > 8 ? 512 : 256, W > 8 ? 1 : 2) short_kernel
   float* logits = smem_f + kTeam * 8 * kHeadPitch;               // [kHeads][s16][gs]
   __shared__ float ref[kTeam][8], sum[kTeam][8];
   __shared__ float2 fin[kHeads][8];
+  __shared__ Moves moves[kTeam];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -1051,7 +1138,7 @@ __global__ void __launch_bounds__(W > 8 ? 512 : 256, W > 8 ? 1 : 2) short_kernel
   const int nsb = (n + 15) >> 4, ppb = a.pool.page >> 4;
   float* lg = logits + static_cast<size_t>(slot) * a.s16 * a.gs;
   Sums sums;
-  sums.clear();
+  sums.clear(&moves[warp]);
   if (wi < nsb) {
     // pages of this warp's blocks wi, wi + W, ...: lane i the i-th
     const int my_blk = wi + W * lane;
@@ -1101,8 +1188,14 @@ __global__ void __launch_bounds__(W > 8 ? 512 : 256, W > 8 ? 1 : 2) short_kernel
       }
       const uint4 s0 = mask_scales(r.s0, mask >> (4 * t)), s1 = mask_scales(r.s1, mask >> (4 * t + 2));
       float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      sums.vote(top, or4(s0) | or4(s1));
-      sums.weigh(x, r.v0, r.v1, s0, s1);
+      uint4 u0 = s0, u1 = s1;
+      if (sums.moved) u0 = sums.scaled(s0), u1 = sums.scaled(s1);
+      if (sums.vote(top, or4(u0) | or4(u1), lane, [&](uint32_t (&m)[4]) {
+            m[0] = max(max_half(s0.x), max_half(s1.x)), m[1] = max(max_half(s0.y), max_half(s1.y));
+            m[2] = max(max_half(s0.z), max_half(s1.z)), m[3] = max(max_half(s0.w), max_half(s1.w));
+          }))
+        u0 = sums.scaled(s0), u1 = sums.scaled(s1);
+      sums.weigh(x, r.v0, r.v1, u0, u1);
     };
     const int count = (nsb - wi + W - 1) / W;
     Raw cur;

@@ -1,0 +1,190 @@
+"""The low-bit serving operators over the whole range of their values: attention where some
+groups of V are far louder than others or one slot outweighs the rest, stored codes beside NaN.
+
+Bounds count roundings of the formulas, group by group, and are small against the values
+themselves (asserted), whatever exponents a kernel chooses."""
+
+import math
+
+import pytest
+import torch
+
+import lowbit_ref as ref
+from kvcacheboundaryprotection_b200 import build, capi, lowbit
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    build.build()
+
+
+# ------------------------------------------------------------------------------- attend
+def _bound(pool, table, lens, q, slot_pos, scale):
+    """(out, each slot's largest probability, bound on out's error, that of a probability) in
+    float64.
+
+    The output is rounded to bf16 (2^-8).  A slot's weight, and that times V's scale, are rounded
+    to f16 (2^-11 each).  Where these are below f16's normals they are rounded to a fixed step
+    instead: with weights held at 2^10 or more for the largest p of the slots and scales at 2^-5
+    or more for the largest scale S of a group (its exponent's field 10 to 15 after a power of two of the group's
+    own), the steps' halves, 2^-25, are 2^-30 S p_max at most, or 2^-49 p_max where S itself is
+    subnormal (a scale moved up by 2^14 only), times a code of at most 7, and once more 2^-35 of p_max s for the
+    weight alone.  Moving a scale down may round it too, by 2^-25 where S is moved below 1, so
+    2^-24 S of a weight's code.  fp32 sums: n / 128 + 16 additions, cut at 2^-23 of sum p |v|.
+    Logits: 2^-21 of the sum of their products' absolute values, an absolute error dl that is a
+    relative one of 2 dl in every probability."""
+    kv = ref.values(pool)
+    (_, sk), (_, sv) = ref.decode(pool)
+    B, hq, _ = q.shape
+    hkv, page = pool.shape[1], pool.shape[2] * 16
+    qd = q.cpu().double().reshape(B, hkv, hq // hkv, 128)
+    out = torch.zeros_like(qd)
+    bound, mass = torch.zeros_like(qd), torch.zeros_like(qd)
+    score = torch.zeros(B, table.shape[1] * page, dtype=torch.float64)
+    drel = torch.zeros(B, dtype=torch.float64)
+    tb = table.cpu().long()
+    for b, n in enumerate(lens.cpu().tolist()):
+        at = torch.arange(n)
+        if slot_pos is not None:
+            at = at[slot_pos[b, :n].cpu() >= 0]
+        if not len(at):
+            continue
+        pg = tb[b][at // page]
+        k, v = (x[pg, :, at % page] for x in kv)
+        s = sv[pg, :, at % page]                                       # [n, hkv, 4]
+        p = torch.softmax(torch.einsum("hgd,nhd->hgn", qd[b], k) * scale, -1)
+        out[b] = torch.einsum("hgn,nhd->hgd", p, v)
+        mass[b] = torch.einsum("hgn,nhd->hgd", p, v.abs())
+        big = 7 * torch.einsum("hgjd,nhj->hgn", qd[b].abs().reshape(hkv, -1, 4, 32), sk[pg, :, at % page])
+        drel[b] = 2 * 2.0 ** -21 * abs(scale) * big.amax() + 2.0 ** -20
+        top = p.amax(-1)[..., None]                                    # [hkv, heads of it, 1]
+        most = s.amax(0).repeat_interleave(32, -1)[:, None]            # [hkv, 1, 128]
+        step = 7 * (len(at) * top * ((2.0 ** -30 + 2.0 ** -35) * most + 2.0 ** -49) + 2.0 ** -24 * most)
+        bound[b] = (2.0 ** -8 * out[b].abs() + step +
+                    (2.0 ** -10 + 2.0 ** -21 + (len(at) / 128 + 16) * 2.0 ** -23 + 2 * drel[b]) * mass[b])
+        score[b, at] = p.amax((0, 1))
+        # all of it is small against the largest outputs of its own group of dims
+        assert (bound[b] <= 2.0 ** -6 * mass[b].reshape(hkv, -1, 4, 32).amax(-1).repeat_interleave(32, -1)).all()
+    return out.reshape(B, hq, 128), score, bound.reshape(B, hq, 128), drel, mass.reshape(B, hq, 128)
+
+
+def _check(c, scored=False):
+    d = {k: v.cuda() if torch.is_tensor(v) else v for k, v in c.items()}
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    S = c["table"].shape[1] * c["pool"].shape[2] * 16
+    got = torch.zeros(c["q"].shape[0], S, device="cuda") if scored else None
+    out = lowbit.kv4_attend(d["pool"], d["table"], d["lens"], d["q"], step_score=got, dev_err=err)
+    assert int(err) == 0, capi.decode_dev_errors(int(err))
+    want, score, bound, drel, mass = _bound(c["pool"], c["table"], c["lens"], c["q"], None, 1 / math.sqrt(128))
+    off = (out.cpu().double() - want).abs()
+    assert (off <= bound).all(), ((off / bound).max(), off.max())
+    if scored:
+        assert ((got.cpu().double() - score).abs() <= (drel[:, None] + 2.0 ** -20) * score + 2.0 ** -60).all()
+    return out, want, mass
+
+
+# half-width of V's values, of each group of 32 dims
+LOUD = {"one channel": (20.0, 0.3, 0.3, 0.3), "around 14": (5.0, 7.0, 0.4, 0.4), "far apart": (1e5, 0.3, 1e-3, 30.0),
+        "all loud": (1e5, 9e4, 1.2e5, 1e5), "all quiet": (1e-3, 2e-3, 1e-4, 1e-3), "ordinary": (1.0, 1.0, 1.0, 1.0)}
+
+
+def _pool(g, n, page, hkv, amps, gap, q0, one_channel):
+    """n slots (whole pages) of hkv heads; a slot in the middle with almost no value whose logit
+    lies ``gap`` nats above the others' (they are within a nat of each other)."""
+    pages = (n + page - 1) // page
+    k = 0.2 * torch.randn(pages * page, hkv, 128, generator=g).double()
+    v = torch.randn(pages * page, hkv, 128, generator=g).double()
+    amp = torch.tensor(amps, dtype=torch.float64).repeat_interleave(32)
+    if one_channel:  # a single value of group 0 is loud, always to the same side
+        amp[:32] = 0.3
+    v *= amp
+    if one_channel:
+        v[..., 5] = amps[0] + 0.1 * v[..., 5]
+    if gap:
+        at = n // 2
+        k[at] = q0 * (gap * math.sqrt(128) / q0.square().sum(-1, keepdim=True))
+        v[at] *= 1e-4
+    shape = (pages, page, hkv, 128)
+    return ref.encode(k.view(shape).transpose(1, 2), v.view(shape).transpose(1, 2), pages)
+
+
+def _case(n, hq, hkv, page, amps, gap, seed, width=None, seqs=1, one_channel=False):
+    """``seqs`` sequences over the same pages (a page may be shared by readers), each its queries."""
+    g = torch.Generator().manual_seed(seed)
+    q0 = 2 * torch.randn(hkv, 128, generator=g).double()
+    q = q0.repeat_interleave(hq // hkv, 0) + 0.1 * torch.randn(seqs, hq, 128, generator=g).double()
+    pool = _pool(g, n, page, hkv, amps, gap, q0, one_channel)
+    pages = pool.shape[0]
+    table = torch.full((seqs, pages if width is None else max(pages, width)), -1, dtype=torch.int32)
+    table[:, :pages] = torch.arange(pages - 1, -1, -1)
+    pool = pool.flip(0).contiguous()
+    return {"pool": pool, "table": table, "lens": torch.full((seqs,), n, dtype=torch.int32), "q": q.to(BF)}
+
+
+@pytest.mark.parametrize("amps", LOUD)
+@pytest.mark.parametrize("gap", [0.0, 9.0, 12.0])
+@pytest.mark.parametrize("n,hq,hkv,page,width", [(512, 4, 1, 16, None), (1999, 7, 1, 64, None), (130, 4, 2, 16, 140),
+                                                 (3001, 8, 2, 64, None), (20011, 4, 1, 64, None)])
+def test_attend_loud_and_quiet_groups_of_values(amps, gap, n, hq, hkv, page, width):
+    """Each group of 32 dims keeps its precision, whatever the other groups hold and however far
+    one slot's weight lies above the rest: short and streaming forms."""
+    c = _case(n, hq, hkv, page, LOUD[amps], gap, n + len(amps), width, one_channel=amps == "one channel")
+    _check(c, scored=True)
+
+
+@pytest.mark.parametrize("gap", [0.0, 9.0, 12.0])
+def test_attend_loud_values_one_warp_a_head(gap):
+    """Many sequences: one warp has all of a head's slots."""
+    out, want, mass = _check(_case(512, 2, 1, 16, LOUD["around 14"], gap, 3, seqs=1200))
+    # and without a lean to either side (the numerator and the sum of weights agree): bf16's
+    # roundings of 128 dims, each off by 2^-9.3 on average squared, add up to 2^-12.8 of the whole
+    lean = ((out.cpu().double() - want) * want.sign()).sum() / want.abs().sum()
+    assert abs(lean) <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("width", [None, 200])
+def test_attend_one_slot_with_far_scales_returns_its_row(width):
+    """One live slot: its row comes back, each group within f16's and bf16's roundings."""
+    amp = torch.tensor([3.8e-4, 2.86, 60000.0, 6e-6], dtype=torch.float64).repeat_interleave(32) * 7
+    v = (amp * torch.linspace(-1, 1, 32).double().repeat(4)).view(1, 1, 1, 128).expand(1, 1, 16, 128)
+    pool = ref.encode(torch.zeros_like(v), v, 1)
+    table = torch.zeros(1, 1 if width is None else width, dtype=torch.int32)
+    c = {"pool": pool, "table": table, "lens": torch.tensor([1], dtype=torch.int32), "q": torch.ones(1, 3, 128, dtype=BF)}
+    out, want, _ = _check(c)
+    row = ref.values(pool)[1][0, 0, 0]
+    assert ((out.cpu().double()[0] - row).abs() <= (2.0 ** -8 + 2.0 ** -10) * row.abs()).all()
+
+
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("n,width", [(1900, None), (6000, None), (500, 200)])
+def test_attend_values_that_grow_or_fall_along_the_sequence(up, n, width):
+    """V from 1e-3 to 1e5, group by group at other places, and logits that grow: the running sums
+    are rescaled again and again."""
+    g = torch.Generator().manual_seed(n)
+    c = _case(n, 8, 1, 16, LOUD["ordinary"], 0.0, n, width)
+    pages = (n + 15) // 16
+    v = torch.randn(pages, 1, 16, 128, generator=g).double()
+    k = torch.randn(pages, 1, 16, 128, generator=g).double() * (torch.arange(pages) / pages).view(-1, 1, 1, 1)
+    for j in range(4):
+        v[..., 32 * j:32 * j + 32] *= 10.0 ** (8 * torch.arange(pages) / pages - 3 - j).view(-1, 1, 1, 1)
+    if not up:
+        k, v = k.flip(0), v.flip(0)
+    c["pool"] = ref.encode(k, v, pages).flip(0).contiguous()
+    _check(c, scored=True)
+
+
+@pytest.mark.parametrize("width", [None, 200])
+def test_attend_nan_in_one_group_of_values_leaves_the_others(width):
+    c = _case(300, 4, 1, 16, LOUD["around 14"], 9.0, 8, width)
+    clean = lowbit.kv4_attend(c["pool"].cuda(), c["table"].cuda(), c["lens"].cuda(), c["q"].cuda()).cpu()
+    p = c["pool"].numpy().copy()
+    _, (_, vs) = ref.layout()
+    p[c["table"][0, 5], 0, 0, vs[3, 1]:vs[3, 1] + 2] = (0xFF, 0x7F)  # slot 83, group 1: a NaN scale
+    out = lowbit.kv4_attend(torch.from_numpy(p).cuda(), c["table"].cuda(), c["lens"].cuda(), c["q"].cuda()).cpu()
+    assert torch.isnan(out[..., 32:64]).all()
+    keep = torch.ones(128, dtype=torch.bool)
+    keep[32:64] = False
+    assert torch.equal(out[..., keep], clean[..., keep])
