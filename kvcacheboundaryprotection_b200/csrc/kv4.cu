@@ -506,7 +506,7 @@ struct Sums {
   // as stored of each group.  True when k is another than before.
   template <typename Most>
   __device__ __forceinline__ bool vote(float (&top)[2], uint32_t bits, int lane, Most most) {
-    if (!__any_sync(0xffffffffu, (bits & 0x40004000u) || top[0] > ref[0] + kTop || top[1] > ref[1] + kTop)) return false;
+    if (!__any_sync(0xffffffffu, (bits & 0x40004000u) || top[0] - ref[0] > kTop || top[1] - ref[1] > kTop)) return false;
     const bool fresh = !__any_sync(0xffffffffu, ref[0] > -INFINITY || ref[1] > -INFINITY);  // O is empty
     // The largest scale of each group, as bits (they order like integers; a NaN makes its own
     // group NaN whatever k).  Those in [2^-5, 2) stay as they are, so that ordinary values cost no
@@ -545,7 +545,10 @@ struct Sums {
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
       top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-      const float r = top[c] > ref[c] + kTop ? top[c] - kTop + kSlack : ref[c];
+      // differences are exact where they are small, sums round: from 2^26 on, top - 10 may lie
+      // 16 below top (there the next smaller weight is 2^-8 of this one at most)
+      float r = top[c] - ref[c] > kTop ? top[c] - (kTop - kSlack) : ref[c];
+      if (top[c] - r > kTop) r = top[c];
       f[c] = r == ref[c] ? 1.0f : ex2(ref[c] - r);  // also where both are -inf
       ref[c] = r;
       l[c] *= f[c];

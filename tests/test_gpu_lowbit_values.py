@@ -188,3 +188,29 @@ def test_attend_nan_in_one_group_of_values_leaves_the_others(width):
     keep = torch.ones(128, dtype=torch.bool)
     keep[32:64] = False
     assert torch.equal(out[..., keep], clean[..., keep])
+
+
+@pytest.mark.parametrize("width", [None, 200])
+@pytest.mark.parametrize("e", range(20, 33))
+def test_attend_logits_beyond_float32s_whole_numbers(e, width):
+    """Equal logits of 2^e: the mean of the slots that have them, where their neighbours in
+    float32 lie 2^(e - 23) apart."""
+    n, page, hkv, hq = 150, 16, 1, 5
+    g = torch.Generator().manual_seed(e)
+    v = torch.randn(10, hkv, page, 128, generator=g).double()
+    for mantissa in (1.0, 1.37, 1.9):
+        k = torch.full((10, hkv, page, 128), 7.0, dtype=torch.float64)
+        k[:, :, 1::2] = -7.0
+        k[:4] *= 0.5  # the largest logit comes after some stages
+        q = torch.full((1, hq, 128), 2.0 ** (e - 10), dtype=torch.float64).to(BF)
+        c = {"pool": ref.encode(k, v, 10), "table": torch.arange(10, dtype=torch.int32)[None], "q": q,
+             "lens": torch.tensor([n], dtype=torch.int32)}
+        if width:
+            c["table"] = torch.nn.functional.pad(c["table"], (0, width - 10), value=-1)
+        d = {a: b.cuda() for a, b in c.items()}
+        scale = mantissa * 2.0 ** 10 / (7 * 128) / math.log2(math.e)  # q . k scale log2(e) = mantissa 2^e
+        out = lowbit.kv4_attend(d["pool"], d["table"], d["lens"], d["q"], scale=scale).cpu().double()[0]
+        rows = ref.values(c["pool"])[1][:, 0].reshape(-1, 128)[64:n:2]
+        want, mass = rows.mean(0), rows.abs().mean(0)
+        # bf16's rounding of the output, f16's of the weights and their products with the scales
+        assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -16) * mass).all(), (e, mantissa)
