@@ -76,7 +76,7 @@ __device__ __forceinline__ __half group_scale(uint32_t amax_bits) {
 // 1e-4 of half-way can round wrongly (bf16 values over an f16 scale often are half-way), and is
 // divided.  Scale 0 (all values below the smallest f16 step) and NaN: code 8.
 __device__ __forceinline__ uint32_t eight_codes(const float (&x)[8], float scale) {
-  const float inv = scale > 0.f ? 1.0f / scale : 0.f;
+  const float inv = 1.0f / scale;
   uint32_t w = 0;
   float worst = 0.f;
 #pragma unroll
@@ -89,11 +89,11 @@ __device__ __forceinline__ uint32_t eight_codes(const float (&x)[8], float scale
     w = 0;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const float q = scale > 0.f ? fminf(fmaxf(rintf(x[n] / scale), -7.f), 7.f) : 0.f;
+      const float q = fminf(fmaxf(rintf(x[n] / scale), -7.f), 7.f);
       w |= static_cast<uint32_t>(static_cast<int>(q) + 8) << (4 * n);
     }
   }
-  return w;
+  return scale > 0.f ? w : 0x88888888u;
 }
 __device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};

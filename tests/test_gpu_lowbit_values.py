@@ -214,3 +214,31 @@ def test_attend_logits_beyond_float32s_whole_numbers(e, width):
         want, mass = rows.mean(0), rows.abs().mean(0)
         # bf16's rounding of the output, f16's of the weights and their products with the scales
         assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -16) * mass).all(), (e, mantissa)
+
+
+# ------------------------------------------------------------------------------- append
+def test_append_groups_without_a_scale_get_code_eight():
+    """Groups whose scale is NaN or rounds to 0 hold code 8 throughout, infinities and ordinary
+    values beside the NaN among them; their neighbours hold their own codes."""
+    x = torch.zeros(6, 3 * 128)
+    x[:, 128:] = torch.linspace(-7, 7, 32).repeat(8)
+    for row, (at, value) in enumerate([(128 + 40, math.nan), (256 + 99, math.nan), (128 + 5, -math.nan)]):
+        x[row, at] = value
+    x[1, 256 + 98], x[1, 256 + 97] = math.inf, -math.inf
+    x[3, 128:160] = 1e-9
+    x[3, 384 - 32:] = -1e-30
+    x[4, 256 + 33] = math.inf
+    pool = torch.full((1, 1, 1, ref.BLOCK), 0xA5, dtype=torch.uint8, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    d = x.to(BF)
+    lowbit.kv4_append(pool, table, d.cuda(), torch.arange(6, dtype=torch.int32, device="cuda"), n_heads=1)
+    for part, ((codes, scales), first) in enumerate(zip(ref.decode(pool), (128, 256))):
+        c, s = codes[0, 0, :6].reshape(6, 4, 32), scales[0, 0, :6]
+        v = d[:, first:first + 128].double().reshape(6, 4, 32)
+        empty = s.isnan() | (s == 0)
+        want_empty = torch.zeros(6, 4, dtype=torch.bool)
+        for row, group in {0: [(0, 1), (2, 0), (3, 0)], 1: [(1, 3), (3, 3)]}[part]:
+            want_empty[row, group] = True
+        assert torch.equal(empty, want_empty) and (c[empty] == 8).all()
+        plain = torch.round(v / s[..., None]).clamp(-7, 7) + 8
+        assert torch.equal(c[~empty].double(), plain[~empty])
