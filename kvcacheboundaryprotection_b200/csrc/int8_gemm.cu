@@ -7,19 +7,24 @@
 namespace kvbp {
 namespace i8 {
 
-// A row's codes from the bits m of its max|x|: rint(127 x / max|x|) (127 x is exact in fp32, so
-// half-way values are half-way in any precision).
+// A row's codes from the bits m of its max|x|: rint(127 x / max|x|), every finite row.  The
+// division works on x and max|x| times the power of two that brings max|x| to [1, 4) (a subnormal
+// one to [2^-7, 1)): 127 x then neither overflows nor loses a bit, so half-way values are half-way
+// (a value that the power of two makes subnormal is far below half a code).
 struct RowQuant {
-  float top, factor;
-  bool fine;  // not zero, infinite or NaN: else every code is 0
+  float top, factor, up;
+  bool fine;   // not zero, infinite or NaN: else every code is 0
+  bool quick;  // 127 / top is finite
   __device__ __forceinline__ explicit RowQuant(uint32_t m) {
     top = __uint_as_float(m);
     fine = m > 0 && m < 0x7f800000u;
-    factor = fine ? 127.0f / top : 0.f;
+    quick = m >= 0x04000000u && m < 0x7f800000u;  // from 2^-119 on
+    factor = quick ? 127.0f / top : 0.f;
+    up = __uint_as_float((254u - min(max(m >> 23, 1u), 253u)) << 23);
   }
   __device__ __forceinline__ float scale() const { return top / 127.0f; }
   __device__ __forceinline__ uint32_t exact(float v) const {
-    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * v / top))) : 0u;
+    return fine ? static_cast<uint32_t>(static_cast<int>(rintf(127.0f * (v * up) / (top * up)))) : 0u;
   }
   // x times the rounded factor plus 1.5 * 2^23 leaves the integer in the low mantissa bits.  The
   // factor is off by 2^-24 of it, so a quotient (at most 127) by 8e-6: only what lies within
@@ -34,7 +39,7 @@ struct RowQuant {
       worst = fmaxf(worst, fabsf(fmaf(x[k], factor, 12582912.0f - s)));
       c[k] = __float_as_uint(s);
     }
-    if (!fine || worst > 0.4999f) {
+    if (!quick || worst > 0.4999f) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) c[k] = exact(x[k]);
     }

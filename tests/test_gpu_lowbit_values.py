@@ -242,3 +242,53 @@ def test_append_groups_without_a_scale_get_code_eight():
         assert torch.equal(empty, want_empty) and (c[empty] == 8).all()
         plain = torch.round(v / s[..., None]).clamp(-7, 7) + 8
         assert torch.equal(c[~empty].double(), plain[~empty])
+
+
+# --------------------------------------------------------------------------------- int8
+TOPS = [9.2e-41, 1e-38, 1.3e-37, 3.5e-37, 4e-37, 1e-30, 1.0, 2.6e36, 2.8e36, 1e37, 1e38, 3.3e38]
+
+
+def _rows(K, seed):
+    """A bf16 row of each largest value in TOPS, half-way values (top / 2 and so on) among them."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.rand(len(TOPS), K, generator=g).double() * 2 - 1
+    x[:, :: 7] = 0.5
+    x[:, 3 % K] = -1.0
+    x = (x * torch.tensor(TOPS, dtype=torch.float64)[:, None]).to(BF)
+    assert torch.isfinite(x).all()
+    return x
+
+
+def _codes64(x):
+    """Codes and scales of the definition; bf16 values and 127 times them are exact in float64."""
+    x = x.double()
+    top = x.abs().amax(1, keepdim=True)
+    return torch.round(127 * x / top), (top / 127)[:, 0]
+
+
+@pytest.mark.parametrize("K", [5, 300, 1000, 1003, 2500, 4096, 4099, 9000, 9007, 17000, 17001])
+@pytest.mark.parametrize("first", [0, 1])
+def test_quantize_rows_at_the_ends_of_the_range(K, first):
+    """Vector loads, tails, misaligned rows, short and long rows."""
+    x = _rows(K, K)
+    wide = torch.zeros(len(TOPS), K + 16, dtype=BF)
+    wide[:, first:first + K] = x
+    q, s = lowbit.int8_quantize_rows(wide.cuda()[:, first:first + K])
+    want_q, want_s = _codes64(x)
+    assert torch.equal(q.cpu().double(), want_q)
+    # the quotient's rounding: 2^-24, or half of the smallest subnormal
+    assert ((s.cpu().double() - want_s).abs() <= 2.0 ** -24 * want_s + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("K", [300, 1003, 2048])
+def test_int8_linear_codes_at_the_ends_of_the_range(K):
+    """An identity weight gives the codes back, in the one-token kernel and the others."""
+    x = _rows(K, K + 1).cuda()
+    w = torch.zeros(K, (K + 15) // 16 * 16, dtype=torch.int8, device="cuda")[:, :K]
+    w.fill_diagonal_(1)
+    want, scale = _codes64(x.cpu())
+    sw = torch.ones(K, device="cuda")
+    for y in (lowbit.int8_linear(x, w, sw, out_dtype=torch.float32),
+              torch.cat([lowbit.int8_linear(x[r:r + 1], w, sw, out_dtype=torch.float32) for r in range(len(TOPS))])):
+        v = want * scale[:, None]
+        assert ((y.cpu().double() - v).abs() <= 2.0 ** -23 * v.abs() + 2.0 ** -149 * want.abs()).all()
