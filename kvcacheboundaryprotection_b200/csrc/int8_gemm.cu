@@ -178,6 +178,12 @@ __device__ __forceinline__ int4 ld_dsmem_v4(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
+// sum * sx * sw + bias in fp32.  A token's scale beyond 2^64 comes last: sum * sx could overflow
+// where the product with a small sw does not (sum * sw then overflows only where all of it does).
+__device__ __forceinline__ float scaled_sum(int sum, float sx, float sw, float bias) {
+  const bool last = fabsf(sx) > 0x1p64f;
+  return static_cast<float>(sum) * (last ? sw : sx) * (last ? sx : sw) + bias;
+}
 // scales and biases of channels n .. n + 3 (those below N)
 struct Four {
   float sw[4], b[4];
@@ -189,8 +195,8 @@ struct Four {
     }
   }
   __device__ __forceinline__ void store(const Args& a, int m, int n, int4 acc, float sx) const {
-    const float y[4] = {static_cast<float>(acc.x) * sx * sw[0] + b[0], static_cast<float>(acc.y) * sx * sw[1] + b[1],
-                        static_cast<float>(acc.z) * sx * sw[2] + b[2], static_cast<float>(acc.w) * sx * sw[3] + b[3]};
+    const float y[4] = {scaled_sum(acc.x, sx, sw[0], b[0]), scaled_sum(acc.y, sx, sw[1], b[1]),
+                        scaled_sum(acc.z, sx, sw[2], b[2]), scaled_sum(acc.w, sx, sw[3], b[3])};
     const size_t at = static_cast<size_t>(m) * a.ldo + n;
     float* f = static_cast<float*>(a.out) + at;
     __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a.out) + at;
@@ -599,11 +605,11 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (a.f32) {
 #pragma unroll
           for (int k = 0; k < 32; ++k, pf += a.ldo)
-            if (k < live) *pf = static_cast<float>(v[k]) * sx[c + k] * sw + bias;
+            if (k < live) *pf = scaled_sum(v[k], sx[c + k], sw, bias);
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k, ph += a.ldo)
-            if (k < live) *ph = __float2bfloat16_rn(static_cast<float>(v[k]) * sx[c + k] * sw + bias);
+            if (k < live) *ph = __float2bfloat16_rn(scaled_sum(v[k], sx[c + k], sw, bias));
         }
       }
       tc_before();

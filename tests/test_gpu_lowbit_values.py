@@ -292,3 +292,23 @@ def test_int8_linear_codes_at_the_ends_of_the_range(K):
               torch.cat([lowbit.int8_linear(x[r:r + 1], w, sw, out_dtype=torch.float32) for r in range(len(TOPS))])):
         v = want * scale[:, None]
         assert ((y.cpu().double() - v).abs() <= 2.0 ** -23 * v.abs() + 2.0 ** -149 * want.abs()).all()
+
+
+@pytest.mark.parametrize("M", [1, 12, 40, 100, 300, 5000])
+@pytest.mark.parametrize("dt", [BF, torch.float32])
+def test_int8_linear_outputs_at_the_ends_of_the_range(M, dt):
+    """Finite outputs of tokens near bf16's largest value, and of its smallest: sum * x_scale alone
+    would overflow.  One token, split tiles of every width, and the persistent form (5000)."""
+    K, N = 640, 1100
+    g = torch.Generator().manual_seed(M)
+    tops = torch.tensor([3e38, 1.0, 2e37, 1e-30, 1e36, 1e-36, 3e22])[torch.arange(M) % 7].double()
+    x = ((torch.rand(M, K, generator=g).double() * 2 - 1) * tops[:, None]).to(BF)
+    w = (1e-3 * torch.randn(N, K, generator=g)).to(BF)
+    wq, ws = lowbit.int8_quantize_rows(w.cuda())
+    y = lowbit.int8_linear(x.cuda(), wq, ws, out_dtype=dt).cpu().double()
+    xq, xs = _codes64(x)
+    want = (xq @ wq.cpu().double().t()) * xs[:, None] * ws.cpu().double()
+    assert (want.abs().amax(1) / tops).amin() > 1e-4 and want.abs().max() < 3e38
+    # the token's scale, the sum's conversion, two products, and bf16's rounding
+    tol = (5 * 2.0 ** -24 + (2.0 ** -8 if dt is BF else 0)) * want.abs()
+    assert ((y - want).abs() <= tol * (1 + 2.0 ** -8) + 2.0 ** -132).all()
