@@ -27,6 +27,7 @@ from .capi import check, lib
 BLOCK = 2304  # bytes of 16 slots of one kv head (KVBP_KV4_BLOCK)
 HEAD_DIM = 128
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_INT_MAX = 0x7FFFFFFF  # the library's sizes are 32-bit, and ctypes would drop the bits above
 _U8, _I8, _I32, _F32, _BF16 = torch.uint8, torch.int8, torch.int32, torch.float32, torch.bfloat16
 # the current stream's handle of a device index (torch.cuda.current_stream makes an object)
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -45,6 +46,11 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, sha
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     raise ValueError(f"{name} must be contiguous")
+
+
+def _fits(a: int, b: int = 0) -> None:
+    if a > _INT_MAX or b > _INT_MAX:
+        raise ValueError(f"a size or stride of {max(a, b)} does not fit the library's 32-bit sizes")
 
 
 def _launch(fn, what: str, dev: torch.device, *args) -> None:
@@ -90,6 +96,7 @@ def _pool(pool: torch.Tensor, table: torch.Tensor) -> tuple:
     n_pages, hkv, per, _ = shape
     _need(pool, "pool", _U8, dev, (n_pages, hkv, per, BLOCK))
     _need(table, "page_table", _I32, dev, tshape)
+    _fits(tshape[0], tshape[1] * (per * 16 or 1) + 64)  # slot numbers (the pool's sizes fit if its bytes do)
     return n_pages, hkv, per * 16, tshape[0], tshape[1], dev
 
 
@@ -127,6 +134,7 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, qkv: torch.Tensor, 
         ldq = cols
     if rows and cols and (step != 1 or ldq < cols):
         raise ValueError("qkv's columns must be contiguous and its rows must not overlap")
+    _fits(rows, ldq)
     _need(slots, "slots", _I32, dev, (rows,))
     per = _rows(rows, B, seq, dev)
     if (inv_freq is None) != (positions is None):
@@ -168,6 +176,7 @@ def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor
     n_pages, hkv, page, B, width, dev = _pool(pool, page_table)
     rows = slots.numel()
     _need(slots, "slots", _I32, dev, (rows,))
+    _fits(rows)
     per = _rows(rows, B, seq, dev)
     if dev_err is not None:
         _need(dev_err, "dev_err", _I32, dev, (1,))
@@ -217,6 +226,7 @@ def kv4_attend(pool: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
         _need(dev_err, "dev_err", _I32, dev, (1,))
     if B == 0:
         return out
+    _fits(S, hq)
     if n_pages == 0 or width == 0 or page == 0 or ((slot_pos is not None or step_score is not None) and S == 0):
         raise ValueError("the pool, the page table, slot_pos and step_score must not be empty")
     limit = min(width * page, S) if S else width * page
@@ -235,6 +245,7 @@ def _matrix(x: torch.Tensor, name: str, dtype: torch.dtype) -> tuple:
     if x.dtype is not dtype or x.dim() != 2:
         raise ValueError(f"{name} must be a {dtype} matrix")
     rows, cols = x.shape
+    _fits(rows, cols)
     ld, step = x.stride()
     if rows <= 1:
         ld = cols

@@ -229,3 +229,32 @@ def test_reference_encoding_round_trips():
         s = scales.repeat_interleave(32, -1)
         assert torch.equal(scales, ref.group_scales(x)) and codes.min() >= 1 and codes.max() <= 15
         assert ((got - x).abs() <= 0.5 * s).all()
+
+
+def test_python_refuses_sizes_past_32_bits():
+    """Sizes that the library's 32-bit arguments cannot hold are refused, not cut (tensors without
+    memory: nothing is read)."""
+    big = (1 << 32) + 3  # would pass as 3
+    i32, meta = torch.int32, "meta"
+    pool = torch.empty(4, 2, 1, 2304, dtype=torch.uint8, device=meta)
+    table = torch.empty(2, 2, dtype=i32, device=meta)
+    two = torch.empty(2, dtype=i32, device=meta)
+    q = torch.empty(2, 4, 128, dtype=BF, device=meta)
+    rows = torch.empty(big, 1, dtype=BF, device=meta)
+    w, s = torch.empty(3, 16, dtype=torch.int8, device=meta), torch.empty(3, device=meta)
+    calls = [
+        lambda: lowbit.kv4_attend(pool, table, two, q, slot_pos=torch.empty(2, big, dtype=i32, device=meta)),
+        lambda: lowbit.kv4_attend(pool, table, two, q, step_score=torch.empty(2, big, device=meta)),
+        lambda: lowbit.kv4_attend(pool, torch.empty(2, big, dtype=i32, device=meta), two, q),
+        lambda: lowbit.kv4_attend(pool, torch.empty(2, 1 << 28, dtype=i32, device=meta), two, q),  # 2^32 slots
+        lambda: lowbit.kv4_gather(pool, table, torch.empty(2 * big, dtype=i32, device=meta)),
+        lambda: lowbit.kv4_append(pool, table, torch.empty(2, big, dtype=BF, device=meta)[:, :1024], two, n_heads=4),
+        lambda: lowbit.kv4_append(pool, table, torch.empty(big, 1024, dtype=BF, device=meta), two, n_heads=4),
+        lambda: lowbit.int8_quantize_rows(rows),
+        lambda: lowbit.int8_linear(rows, w[:, :1], s),
+        lambda: lowbit.int8_linear(torch.empty(2, 16, dtype=BF, device=meta), torch.empty(big, 16, dtype=torch.int8, device=meta), s),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="32-bit"):
+            call()
+            pytest.fail(f"call {i}")
