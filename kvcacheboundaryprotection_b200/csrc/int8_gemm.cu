@@ -108,12 +108,6 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __
   for (int i = nv * 8 + tid; i < K; i += 256) dst[i] = static_cast<int8_t>(rq.exact(__bfloat162float(row[i])));
 }
 
-// ---- the product on the 5th-generation tensor cores (tcgen05.mma kind::i8) -------------
-// The weight block is the M = 128 operand and the tokens the N = NT one, both K-major int8
-// tiles of 128 bytes of K fetched by 2-D TMA with the 128-byte swizzle (rows and columns
-// past the matrices arrive as zeros: sizes are free); the accumulator is int32 in TMEM, lane =
-// output channel, column = token, so a warp's stores of one token's 32 channels are contiguous.
-// Integer sums are exact, so K may be split and joined in any order with the same bits.
 // The same for rows of up to 1024: a warp per row, eight rows a CTA, no barrier.
 __global__ void __launch_bounds__(256) quant_short_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int K,
                                                                int rows, int vec, int8_t* __restrict__ q, long long ldq,
@@ -141,6 +135,12 @@ __global__ void __launch_bounds__(256) quant_short_rows_kernel(const __nv_bfloat
   for (int i = nv * 8 + lane; i < K; i += 32) dst[i] = static_cast<int8_t>(rq.exact(__bfloat162float(row[i])));
 }
 
+// ---- the product on the 5th-generation tensor cores (tcgen05.mma kind::i8) -------------
+// The weight block is the M = 128 operand and the tokens the N = NT one, both K-major int8
+// tiles of 128 bytes of K fetched by 2-D TMA with the 128-byte swizzle (rows and columns
+// past the matrices arrive as zeros: sizes are free); the accumulator is int32 in TMEM, lane =
+// output channel, column = token, so a warp's stores of one token's 32 channels are contiguous.
+// Integer sums are exact, so K may be split and joined in any order with the same bits.
 struct Args {
   const float* sw;
   const float* sx;
@@ -148,9 +148,8 @@ struct Args {
   void* out;
   long long ldo;
   int M, N, K, f32;
-  const __nv_bfloat16* x;  // fused quantisation: the tokens themselves
-  long long ldx;
-  int vec_x;  // its rows are 16-byte aligned
+  const __nv_bfloat16* x;  // fused quantisation: the token itself
+  int vec_x;  // it is 16-byte aligned
   int vec;    // four channels at a time are aligned
   int early;  // the weight is known to be complete before the kernel before this one ends
   int* err;
@@ -242,18 +241,19 @@ __device__ __forceinline__ void ld_acc(uint32_t taddr, int (&v)[C]) {
 // 6.9 us with its quantisation, 2.3 TB/s, latency.
 // With kFuse (one token) the epilogue warps quantise the token themselves while the first
 // weights are under way: each CTA reads all of x for its maximum (a few KB from L2) and puts its
-// own K range's codes into shared memory as the MMA's operand.  That saves a launch: the GPU
+// own K range's codes into shared memory as row 0 of the MMA's operand.  The other 15 rows hold
+// anything: their columns of the accumulator are never stored.  That saves a launch: the GPU
 // time is the same (6.9 against 7.4 us at 6144 x 2560, 27.7 against 26.5 at 37888 x 3584), the
-// host's a third less.  With four tokens the CTAs' repeated work costs more than the
-// launch (8.9 and 33.4 us).
-constexpr int kFuseTokens = 1;
+// host's a third less.  (For four tokens the CTAs' repeated work cost more than the launch: 8.9
+// against 7.5 us.)  The first weights wait for the kernel before this one, which may be the one
+// that writes them; with more tokens the quantisation stands in between.
 constexpr int kFuseSteps = 30;  // stages of K per CTA whose codes fit beside three of weights
 template <int NT, bool kFuse>
 struct Ring {
   static constexpr int kStage = kTileW + (kFuse ? 0 : NT * kBK);
   static constexpr int kStages = kFuse ? 3 : NT <= 32 ? 5 : NT == 64 ? 4 : 3;
   static constexpr int kTokens = kFuse ? kFuseSteps * NT * kBK : 0;
-  static constexpr int kBytes = kStages * kStage + kTokens + 1024 + 256 + NT * 4 + 16 * kFuseTokens;
+  static constexpr int kBytes = kStages * kStage + kTokens + 1024 + 256 + NT * 4 + 16;
   static_assert(kStages * kStage >= NT * 128 * 4, "the partial tile reuses the ring");
   static_assert(kBytes <= 115712, "two CTAs per SM");
 };
@@ -265,11 +265,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kCols = NT < 32 ? 32 : NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* tokens = base + R::kStages * R::kStage;  // kFuse: [step][16 tokens][128], swizzled
+  uint8_t* tokens = base + R::kStages * R::kStage;  // kFuse: [step][16 rows][128], the token in row 0
   uint64_t* full = reinterpret_cast<uint64_t*>(tokens + R::kTokens);
   uint64_t* empty = full + R::kStages;
   uint64_t* done = empty + R::kStages;
-  uint64_t* ready = done + 1;  // kFuse: the tokens' codes are in place
+  uint64_t* ready = done + 1;  // kFuse: the token's codes are in place
   uint32_t* tslot = reinterpret_cast<uint32_t*>(ready + 1);
   int* bad = reinterpret_cast<int*>(tslot + 1);
   float* sxs = reinterpret_cast<float*>(bad + 1);  // the tokens' scales
@@ -362,43 +362,28 @@ __global__ void __launch_bounds__(kThreads, 2)
     pdl_wait();
     uint32_t* red = reinterpret_cast<uint32_t*>(sxs + NT);  // the four warps' maxima
     const int et = tid - 64, nv = a.vec_x ? a.K / 8 : 0;
-    uint32_t m[kFuseTokens] = {};
-    for (int i = et; i < nv; i += 128)
-#pragma unroll
-      for (int r = 0; r < kFuseTokens; ++r)
-        if (r < a.M) m[r] = fold_max(m[r], reinterpret_cast<const uint4*>(a.x + r * a.ldx)[i]);
-    for (int i = nv * 8 + et; i < a.K; i += 128)
-#pragma unroll
-      for (int r = 0; r < kFuseTokens; ++r)
-        if (r < a.M) m[r] = max(m[r], abs_bits(a.x[r * a.ldx + i]));
-#pragma unroll
-    for (int r = 0; r < kFuseTokens; ++r) {
-      m[r] = __reduce_max_sync(0xffffffffu, m[r]);
-      if (lane == 0) red[(warp - 2) * kFuseTokens + r] = m[r];
-    }
+    const uint4* xv = reinterpret_cast<const uint4*>(a.x);
+    uint32_t m = 0;
+    for (int i = et; i < nv; i += 128) m = fold_max(m, xv[i]);
+    for (int i = nv * 8 + et; i < a.K; i += 128) m = max(m, abs_bits(a.x[i]));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) red[warp - 2] = m;
     __syncwarp();
     named_bar(1, 128);
-    for (int r = 0; r < a.M; ++r) {
-      uint32_t top = 0;
+    const RowQuant rq(max(max(red[0], red[1]), max(red[2], red[3])));
+    if (et == 0) sxs[0] = rq.scale();
+    for (int c = et; c < nk * 16; c += 128) {  // eight codes at a time of this CTA's K range
+      const int k = k0 * kBK + 8 * c;          // columns past K meet zero weights
+      uint2 codes = make_uint2(0, 0);
+      if (k / 8 < nv) {
+        codes = rq.eight(xv[k / 8]);
+      } else if (k < a.K) {
+        uint32_t b[8];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = max(top, red[w * kFuseTokens + r]);
-      const RowQuant rq(top);
-      if (et == 0) sxs[r] = rq.scale();
-      const __nv_bfloat16* row = a.x + r * a.ldx;
-      for (int c = et; c < nk * 16; c += 128) {  // eight codes at a time of this CTA's K range
-        const int k = k0 * kBK + 8 * c;          // columns past K meet zero weights
-        uint2 codes = make_uint2(0, 0);
-        if (8 * (k / 8 + 1) <= nv * 8) {
-          codes = rq.eight(reinterpret_cast<const uint4*>(row)[k / 8]);
-        } else if (k < a.K) {
-          uint32_t b[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) b[i] = k + i < a.K ? rq.exact(__bfloat162float(row[k + i])) & 255u : 0u;
-          codes = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
-        }
-        const int chunk = (c & 15) >> 1;  // 16-byte chunk of the row's 128, swizzled by row
-        *reinterpret_cast<uint2*>(tokens + (c >> 4) * (NT * kBK) + r * kBK + ((chunk ^ (r & 7)) << 4) + (c & 1) * 8) = codes;
+        for (int i = 0; i < 8; ++i) b[i] = k + i < a.K ? rq.exact(__bfloat162float(a.x[k + i])) & 255u : 0u;
+        codes = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
       }
+      *reinterpret_cast<uint2*>(tokens + (c >> 4) * (NT * kBK) + (c & 15) * 8) = codes;  // row 0 has no swizzle
     }
     fence_proxy_async_smem();
     mbar_arrive(ready);
@@ -747,11 +732,11 @@ static int gemm(cudaStream_t st, Args a, const void* w, long long ldw, const voi
 }
 
 // One token straight from bf16: quantisation and product in one kernel.
-static bool fused(int M, int K) { return M <= kFuseTokens && K <= kFuseSteps * kMaxSplits * kBK; }
+static bool fused(int M, int K) { return M == 1 && K <= kFuseSteps * kMaxSplits * kBK; }
 
 static int gemm_fused(cudaStream_t st, Args a, const void* w, long long ldw) {
   a.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && !misaligned(a.out, a.f32 ? 16 : 8);
-  a.vec_x = !misaligned(a.x, 16) && a.ldx % 8 == 0;
+  a.vec_x = !misaligned(a.x, 16);
   const int sms = prepare_device(reinterpret_cast<const void*>(split_kernel<16, true>), Ring<16, true>::kBytes);
   if (sms <= 0) return fail(kStatusCuda, "int8_linear: no usable CUDA device");
   CUtensorMap wm;
@@ -777,7 +762,7 @@ extern "C" int kvbp_int8_quant_rows(kvbp_stream_t stream, int32_t rows, int32_t 
 extern "C" int kvbp_int8_gemm(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t N, int32_t K, const void* w,
                               int64_t ldw, const float* w_scale, const void* xq, int64_t ldq, const float* x_scale,
                               const void* bias, void* out, int64_t ldo, int32_t* dev_err) {
-  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, nullptr, 0, 0, 0, 0, dev_err};
+  const kvbp::i8::Args a{w_scale, x_scale, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0, nullptr, 0, 0, 0, dev_err};
   return kvbp::i8::gemm(reinterpret_cast<cudaStream_t>(stream), a, w, ldw, xq, ldq);
 }
 
@@ -790,7 +775,7 @@ extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t 
                                 int64_t ldw, const float* w_scale, const void* x, int64_t ldx, const void* bias,
                                 void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, int32_t* dev_err) {
   kvbp::i8::Args a{w_scale, nullptr, static_cast<const __nv_bfloat16*>(bias), out, ldo, M, N, K, fp32_out ? 1 : 0,
-                   static_cast<const __nv_bfloat16*>(x), ldx, 0, 0, 1, dev_err};
+                   static_cast<const __nv_bfloat16*>(x), 0, 0, 1, dev_err};
   // the product's arguments first: a refused call leaves the workspace alone
   if (int st = kvbp::i8::check(a, w, ldw)) return st;
   if (!x || ldx < K) return kvbp::fail(kvbp::kStatusArg, "int8_linear: bad x");
