@@ -1,6 +1,8 @@
 // Matrix product in 8-bit integers with a scale for each token and each output channel:
 //   y[m][n] = (sum_k xq[m][k] wq[n][k]) * sx[m] * sw[n] (+ bias[n])
 // with exact 32-bit integer sums, and the per-token quantisation that feeds it.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kvbp_internal.h"
 
@@ -179,8 +181,8 @@ __device__ __forceinline__ int4 ld_dsmem_v4(uint32_t cluster_addr) {
 }
 // sum * sx * sw + bias in fp32.  A token's scale beyond 2^64 comes last: sum * sx could overflow
 // where the product with a small sw does not (sum * sw then overflows only where all of it does).
-__device__ __forceinline__ float scaled_sum(int sum, float sx, float sw, float bias) {
-  const bool last = fabsf(sx) > 0x1p64f;
+__device__ __forceinline__ bool far_scale(float sx) { return fabsf(sx) > 0x1p64f; }
+__device__ __forceinline__ float scaled_sum(int sum, float sx, float sw, float bias, bool last) {
   return static_cast<float>(sum) * (last ? sw : sx) * (last ? sx : sw) + bias;
 }
 // scales and biases of channels n .. n + 3 (those below N)
@@ -194,8 +196,9 @@ struct Four {
     }
   }
   __device__ __forceinline__ void store(const Args& a, int m, int n, int4 acc, float sx) const {
-    const float y[4] = {scaled_sum(acc.x, sx, sw[0], b[0]), scaled_sum(acc.y, sx, sw[1], b[1]),
-                        scaled_sum(acc.z, sx, sw[2], b[2]), scaled_sum(acc.w, sx, sw[3], b[3])};
+    const bool far = far_scale(sx);
+    const float y[4] = {scaled_sum(acc.x, sx, sw[0], b[0], far), scaled_sum(acc.y, sx, sw[1], b[1], far),
+                        scaled_sum(acc.z, sx, sw[2], b[2], far), scaled_sum(acc.w, sx, sw[3], b[3], far)};
     const size_t at = static_cast<size_t>(m) * a.ldo + n;
     float* f = static_cast<float*>(a.out) + at;
     __nv_bfloat16* h = static_cast<__nv_bfloat16*>(a.out) + at;
@@ -587,15 +590,23 @@ __global__ void __launch_bounds__(kPThreads, 1)
         __syncwarp();
         ld_acc<32>(acc + c, v);
         const int live = in ? cols - c : 0;
-        if (a.f32) {
+        auto put = [&](auto some_far) {
+          auto y = [&](int k) {
+            return scaled_sum(v[k], sx[c + k], sw, bias, decltype(some_far)::value && far_scale(sx[c + k]));
+          };
+          if (a.f32) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k, pf += a.ldo)
-            if (k < live) *pf = scaled_sum(v[k], sx[c + k], sw, bias);
-        } else {
+            for (int k = 0; k < 32; ++k, pf += a.ldo)
+              if (k < live) *pf = y(k);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k, ph += a.ldo)
-            if (k < live) *ph = __float2bfloat16_rn(scaled_sum(v[k], sx[c + k], sw, bias));
-        }
+            for (int k = 0; k < 32; ++k, ph += a.ldo)
+              if (k < live) *ph = __float2bfloat16_rn(y(k));
+          }
+        };
+        // asked once for the 32 tokens: the comparison for each sum cost 1.2 % of the large product
+        if (__any_sync(0xffffffffu, far_scale(sx[c + lane]))) put(std::true_type{});
+        else put(std::false_type{});
       }
       tc_before();
       __syncwarp();
