@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t abs_bits(const __nv_bfloat16 x) {
 // Per-token quantisation: sx = max|x| / 127 and the codes above (a zero row gives zeros and
 // scale 0).  A row with a NaN or an infinity gets a scale that is not finite, and codes 0:
 // every output of that token is then NaN.  One CTA per row, the row kept in registers between the
-// maximum and the codes (kVec 16-byte vectors per thread: K <= 2048 kVec; longer rows are read
+// maximum and the codes (kVec 16-byte vectors per thread: 2048 kVec values; what is beyond is read
 // again, from L2).  Latency-bound: few registers let many rows share an SM.
 template <int kVec>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int K,
@@ -456,7 +456,7 @@ constexpr int kPStage = kTileW + kPN * kBK;
 constexpr int kPBytes = kPStages * kPStage + 1024 + 256 + 2 * kPN * 4;
 constexpr int kPEpilogue = 16;  // warps: with four, one a scheduler, a tile's 256 tokens took 8 us
 constexpr int kPThreads = (2 + kPEpilogue) * 32;
-constexpr int kBand = 16;  // channel tiles per raster band
+constexpr int kBand = 16;  // channel tiles per raster band (4 to 64 within 2 % of it at 8192 x 37888 x 3584)
 
 __global__ void __launch_bounds__(kPThreads, 1)
     persist_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a) {
@@ -661,11 +661,17 @@ static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
   int8_t* qb = static_cast<int8_t*>(q);
   cudaError_t e;
+  // Short rows a warp each, for many rows (8192 of 128: 4.4 us against 12.3, of 1024: 7.9 against
+  // 14.4; few rows lose up to a microsecond: 300 of 1024 3.1 against 2.0).  Longer ones a CTA each
+  // with as few vectors in registers as pays, since many rows then share an SM (8192 rows, two
+  // vectors against five: K = 4096 26 us and 35, 6144 40 and 42, 8192 52 and 48, 10240 64 and 55);
+  // past 10240 reading most of the row twice is faster than eight vectors (12288 64 us against 75,
+  // 18944 100 against 125).
   if (K <= 1024) {
     e = launch_pdl(quant_short_rows_kernel, dim3((static_cast<unsigned>(rows) + 7) / 8), dim3(256), 0, st, dim3(0), xb, ldx,
                    K, rows, vec, qb, ldq, scale);
   } else {
-    auto kernel = K <= 4096 ? quant_rows_kernel<2> : K <= 10240 ? quant_rows_kernel<5> : quant_rows_kernel<8>;
+    auto kernel = K > 6144 && K <= 10240 ? quant_rows_kernel<5> : quant_rows_kernel<2>;
     e = launch_pdl(kernel, dim3(rows), dim3(256), 0, st, dim3(0), xb, ldx, K, vec, qb, ldq, scale);
   }
   if (e != cudaSuccess) return fail(kStatusCuda, "int8_quant_rows launch: %s", cudaGetErrorString(e));
