@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 // Many tokens: persistent, one CTA per SM over 128 x 256 tiles in a grouped raster, a ring of
 // four 48 KiB stages that runs on across tiles, and two accumulators in TMEM so that the MMAs
 // of one tile run while the epilogue warps drain the other.  8192 x 37888 x 3584 with its
-// quantisation: 836 us, 2.66 POP/s, at the power limit; per stage and SM 48 KiB from L2.
+// quantisation: 830 us, 2.7 POP/s, a dozen at a time; 925 us held up at the power limit; per stage
+// and SM 48 KiB from L2.
 constexpr int kPN = 256;
 constexpr int kPStages = 4;
 constexpr int kPStage = kTileW + kPN * kBK;

@@ -332,12 +332,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
 //
 // What bounds it: HBM, 144 bytes per slot and kv head -- 46 codes per clock and SM at the
 // copy bandwidth, so unpacking has to cost about one instruction per code:
-//  * (word & 0x000f000f) | 0x64006400 is the f16 pair 1024 + n, (word & 0x00f000f0) |
-//    0x64006400 the pair 1024 + 16 n; one packed add or multiply-add makes either the exact
-//    code n - 8: 9 instructions per 8 codes.  (Feeding the MMA the biased pairs, or the bare
-//    bits as f16 subnormals, and taking the bias off the sums saves 4 of the 9 but not the
-//    precision: the MMA aligns products by their operands' exponent fields, 10 bits above the
-//    code's own, and its sums came out 2^-16 off.)
+//  * integers become floats by the published method of or-ing them into the mantissa of a fixed
+//    exponent, which 4-bit weight products use too: (word & 0x000f000f) | 0x64006400 is the f16
+//    pair 1024 + n, (word & 0x00f000f0) | 0x64006400 the pair 1024 + 16 n; one packed add or
+//    multiply-add makes either the exact code n - 8: 9 instructions per 8 codes.  (Feeding the MMA
+//    the biased pairs, or the bare bits as f16 subnormals, and taking the bias off the sums saves
+//    4 of the 9 but not the precision: the MMA aligns products by their operands' exponent fields,
+//    10 bits above the code's own, and its sums came out 2^-16 off.)
 //  * scales never touch the codes: K's multiply the four group sums in fp32, V's multiply the
 //    softmax weights (P' = P * scale, f16, rounded at 2^-11: half a bf16 output step is 2^-9).
 // P is 2^(x - ref), ref = max(x) - kTop at least and moved only when the maximum has grown by
@@ -360,11 +361,12 @@ __global__ void __launch_bounds__(256) gather_kernel(const int* __restrict__ slo
 // CTA) for the combine kernel.  Logits for the eviction score go to the workspace too: the
 // probabilities need the final (ref, sum).
 //
-// Measured: 8 kv heads of one sequence of 131071 slots 46.4 us (3.3 TB/s, 23.1 at the copy
-// bandwidth), 64 sequences x 8 heads of 4104 slots with masks and score 103 us (47).  The copies
-// alone, with the arithmetic skipped, take 36 and 64 us; the rest is issue: 365 instructions per
-// block and warp against 250 that the arithmetic needs, 60 % of the issue slots used (16 warps at
-// 128 registers).  Slower: four-block stages and 8 warps (289 instructions, but 50 % of the
+// Measured: 8 kv heads of one sequence of 131071 slots 46.8 us (3.2 TB/s, 23.1 at the copy
+// bandwidth), 64 sequences x 8 heads of 4104 slots with masks and score 103 us (47); 7 % more where
+// V's scales lie outside [2^-5, 2) (20 % in the one-launch form below).  The copies alone, with the
+// arithmetic skipped, take 36 and 64 us; the rest is issue: 365 instructions per block and warp
+// against 250 that the arithmetic needs, 61 % of the issue slots used (16 warps at 128 registers).
+// Slower: four-block stages and 8 warps (289 instructions, but 50 % of the
 // slots: 46 and 112 us), 12 or 16 warps in one CTA (49 / 109, 49 / 110), one CTA of 8 warps with
 // two-block stages (53 / 125).
 constexpr int kWarps = 8;
@@ -1275,10 +1277,10 @@ static int seqs_per_launch(int B, int Hkv, int limit) {
 }
 
 // Warps per head of the one-launch form, 0 where the streaming form is the faster one.
-// Measured, one launch against streaming, without a score (28 heads over 4): 4.6 against 6.6 us
-// at 64 kv heads of 64 slots, 34.8 against 54.9 at 2048 of 256 (so always up to 16 blocks), 9.6
-// against 10.4 at 64 of 1024, 18.0 against 22.8 at 512 of 512, 14.9 against 18.6 at 128 of 2048;
-// but 33.2 against 31.1 at 512 of 1024 and 32.5 against 27.6 at 256 of 2048.
+// Measured, one launch against streaming, without a score (28 heads over 4): 4.6 against 6.8 us
+// at 64 kv heads of 64 slots, 35.2 against 57 at 2048 of 256 (so always up to 16 blocks), 10.3
+// against 10.4 at 64 of 1024, 18.3 against 23.2 at 512 of 512, 16.0 against 18.9 at 128 of 2048;
+// but 33.6 against 31.8 at 512 of 1024 and 32.9 against 27.8 at 256 of 2048.
 static int short_warps(int B, int Hkv, int limit) {
   const long long heads = static_cast<long long>(B) * Hkv, nsb = (limit + 15) / 16;
   if (nsb > kShortAlways && (nsb > kShortBlocks || heads * nsb > kShortTotal)) return 0;
@@ -1391,7 +1393,11 @@ static int attend(cudaStream_t stream, int B, int Hq, const Pool& pool, const vo
   return kStatusOk;
 }
 
-constexpr int kManyRows = 2048;  // from here on eight rows per CTA
+// From here on eight rows per CTA, below one.  One against eight, 28 + 2 * 4 heads: 6.5 us and 9.3
+// at 512 rows, 11.3 and 14.3 at 1024, 19.3 and 15.9 at 2048, 40 and 17 at 4096; 32 + 2 * 8 heads
+// with norms: 20 and 33 at 1024, 35 and 36 at 2048, 53 and 37 at 3000.  (Two rows per CTA would be
+// the fastest from 768 to 2048: 6.9 us at 1024 rows, 10.9 at 2047.)
+constexpr int kManyRows = 2048;
 
 // Checks shared by the three entry points; fills ``p``.
 static int make_pool(const char* what, int B, int Hkv, int D, int page, int n_pages, int max_pages, const void* pool,

@@ -9,7 +9,8 @@ integers.  ``include/kvbp.h`` states the formats and the arithmetic.
 
 Every call enqueues on the current stream of its tensors' device, allocates what it returns
 (and its workspace) from torch's caching allocator, and can be captured in a CUDA graph.
-Arguments that do not fit raise ``ValueError``; problems found on the device (a slot or page
+Arguments that do not fit raise ``ValueError``, those that the library itself refuses (outputs that
+overlap inputs, a misaligned pool, sizes it does not support) ``capi.KVBPError``; problems found on the device (a slot or page
 out of range) set bits of ``dev_err``, an int32 tensor of one element, when one is given.
 """
 
