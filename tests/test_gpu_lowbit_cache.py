@@ -115,3 +115,51 @@ def test_prefill_attention_over_rows_read_back(P, hq, hkv, page):
     assert d.max().item() <= 1.6e-2 and (out.float() == want).float().mean().item() >= 0.97
     rel = (colmax - want_col).abs() / want_col.clamp_min(1e-30)
     assert (rel <= 1e-5).float().mean().item() >= 0.97 and rel.max().item() <= 2e-2
+
+
+@pytest.mark.parametrize("pages", [0, 150])
+def test_decode_steps_with_eviction_as_a_graph(pages):
+    """One captured step (bookkeeping, append, attention with the score, score update), replayed:
+    the eager run's outputs, slots, scores and cache, in the short and the streaming form."""
+    B, P, cap, steps, page = 4, 40, 32, 20, 16
+    cfg = capi.EvictCfg(cap, 2, capi.policy_id("h2o_faithful"), 0, 0, 0, 1)
+    width = (cap + 5 + page - 1) // page
+    S = cap + 5 if not pages else pages * page  # more slots than the one-launch form takes
+    g = torch.Generator().manual_seed(9)
+    table = torch.full((B, max(width, pages)), -1, dtype=torch.int32)
+    table[:, :width] = torch.randperm(B * width, generator=g).view(B, width)
+    table = table.cuda()
+    qkv = torch.randn(P + steps, B, (HQ + 2 * HKV) * 128, generator=g).to(BF).cuda()
+    freq = (1e6 ** (-torch.arange(64) / 64.0)).float().cuda()
+    scores = torch.rand(B, P, generator=g)
+    lens = torch.full((B,), cap + 5, dtype=torch.int32).cuda()
+
+    def start():
+        D = Driver(B, S, (P + steps + 2 + 31) // 32, P + steps + 2, steps, cfg)
+        pool = lowbit.kv4_pool(B * width, HKV, page)
+        slots = _slots_of(D.prefill(P, scores), P)
+        pos = torch.arange(P, dtype=torch.int32).repeat(B).cuda()
+        lowbit.kv4_append(pool, table, qkv[:P].transpose(0, 1).reshape(B * P, -1), slots.view(-1), n_heads=HQ,
+                          positions=pos, inv_freq=freq, dev_err=D.err)
+        return D, pool
+
+    def step(D, pool, row):
+        D.append_evict()
+        q = lowbit.kv4_append(pool, table, row, D.write_slot, n_heads=HQ, positions=D.cur_pos, inv_freq=freq, dev_err=D.err)
+        out = lowbit.kv4_attend(pool, table, lens, q, slot_pos=D.slot_pos, step_score=D.step_score, dev_err=D.err)
+        D.score_update()
+        return out
+
+    D, pool = start()
+    outs = [step(D, pool, qkv[P + t]) for t in range(steps)]
+    G, gpool = start()
+    row = qkv[P].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(G, gpool, row)
+    for t in range(steps):
+        row.copy_(qkv[P + t])
+        graph.replay()
+        assert torch.equal(out, outs[t]), t
+    assert torch.equal(pool, gpool) and int(D.err) == 0 and int(G.err) == 0
+    assert all(torch.equal(a, b) for a, b in zip(D.metadata(), G.metadata()))
