@@ -651,8 +651,6 @@ static cudaError_t launch_split(cudaStream_t st, const CUtensorMap& wm, const CU
   return launch_pdl(split_kernel<NT, kFuse>, grid, dim3(kThreads), smem, st, S > 1 ? dim3(S, 1, 1) : dim3(0), wm, xm, a);
 }
 
-static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
-
 static int quant_rows(cudaStream_t st, int rows, int K, const void* x, long long ldx, void* q, long long ldq, float* scale) {
   if (!x || !q || !scale) return fail(kStatusArg, "int8_quant_rows: null pointer");
   if (rows <= 0 || K <= 0 || ldx < K || ldq < K) return fail(kStatusArg, "int8_quant_rows: bad size");
@@ -691,10 +689,6 @@ static int splits(long long tiles, int steps, int sms) {
   return s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : static_cast<int>(s);
 }
 
-static bool overlap(const void* p, long long np, const void* q, long long nq) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a < b + nq && b < a + np;
-}
 static long long out_bytes(const Args& a) { return ((a.M - 1ll) * a.ldo + a.N) * (a.f32 ? 4 : 2); }
 
 // Checks of all but the tokens.
@@ -797,10 +791,10 @@ extern "C" int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t 
   // the product's arguments first: a refused call leaves the workspace alone
   if (int st = kvbp::i8::check(a, w, ldw)) return st;
   if (!x || ldx < K) return kvbp::fail(kvbp::kStatusArg, "int8_linear: bad x");
-  if (kvbp::i8::overlap(out, kvbp::i8::out_bytes(a), x, 2 * ((M - 1ll) * ldx + K)))
+  if (kvbp::overlap(out, kvbp::i8::out_bytes(a), x, 2 * ((M - 1ll) * ldx + K)))
     return kvbp::fail(kvbp::kStatusArg, "int8_linear: out must not overlap x");
   if (kvbp::i8::fused(M, K)) return kvbp::i8::gemm_fused(reinterpret_cast<cudaStream_t>(stream), a, w, ldw);
-  if (!workspace || kvbp::i8::misaligned(workspace, 16)) return kvbp::fail(kvbp::kStatusArg, "int8_linear: no aligned workspace");
+  if (!workspace || kvbp::misaligned(workspace, 16)) return kvbp::fail(kvbp::kStatusArg, "int8_linear: no aligned workspace");
   if (workspace_bytes < kvbp_int8_linear_workspace(M, K))
     return kvbp::fail(kvbp::kStatusArg, "int8_linear: workspace of %lld bytes is too small", static_cast<long long>(workspace_bytes));
   const int64_t ldq = (static_cast<int64_t>(K) + 15) / 16 * 16;

@@ -1260,11 +1260,7 @@ __global__ void __launch_bounds__(W > 8 ? 512 : 256, W > 8 ? 1 : 2) short_kernel
   }
 }
 
-static bool overlap(const void* p, long long np, const void* q, long long nq) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a < b + nq && b < a + np;
-}
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool aligned16(const void* p) { return !misaligned(p, 16); }
 
 static int floats_per_row(int group) { return group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 
@@ -1436,7 +1432,7 @@ extern "C" int kvbp_kv4_append(kvbp_stream_t stream, int32_t rows, int32_t rows_
       ldq < (static_cast<long long>(Hq) + 2 * Hkv) * 128)
     return fail(kvbp::kStatusArg, "kv4_append: bad size");
   if (!kv4::aligned16(q_out)) return fail(kvbp::kStatusArg, "kv4_append: q_out must be 16-byte aligned");
-  if (Hq > 0 && kv4::overlap(qkv, 2ll * ((rows - 1ll) * ldq + (Hq + 2ll * Hkv) * 128), q_out, 256ll * rows * Hq))
+  if (Hq > 0 && kvbp::overlap(qkv, 2ll * ((rows - 1ll) * ldq + (Hq + 2ll * Hkv) * 128), q_out, 256ll * rows * Hq))
     return fail(kvbp::kStatusArg, "kv4_append: q_out must not overlap qkv");
   const kv4::AppendArgs a{static_cast<const __nv_bfloat16*>(qkv), static_cast<const __nv_bfloat16*>(bias),
                           static_cast<const __nv_bfloat16*>(q_norm_w), static_cast<const __nv_bfloat16*>(k_norm_w),
@@ -1492,7 +1488,7 @@ extern "C" int kvbp_kv4_attn(kvbp_stream_t stream, int32_t B, int32_t Hq, int32_
   if (S < 0 || ((slot_pos || step_score) && S == 0)) return fail(kvbp::kStatusArg, "kv4_attn: bad slot stride");
   if (!kv4::aligned16(q) || !kv4::aligned16(out))
     return fail(kvbp::kStatusArg, "kv4_attn: q and out must be 16-byte aligned");
-  if (kv4::overlap(q, 256ll * B * Hq, out, 256ll * B * Hq))
+  if (kvbp::overlap(q, 256ll * B * Hq, out, 256ll * B * Hq))
     return fail(kvbp::kStatusArg, "kv4_attn: out must not overlap q");
   return kv4::attend(reinterpret_cast<cudaStream_t>(stream), B, Hq, p, q, lens, slot_pos, S, scale, out, step_score,
                      workspace, workspace_bytes, dev_err);

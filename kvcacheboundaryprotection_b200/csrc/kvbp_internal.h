@@ -48,6 +48,13 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Whether np bytes at p and nq bytes at q share any.
+inline bool overlap(const void* p, long long np, const void* q, long long nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
+inline bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
 // SMs of the current device (0: none usable), after letting ``kernel`` use ``smem`` bytes of
 // dynamic shared memory there.  Asked once per kernel and device.
 int prepare_device(const void* kernel, int smem);
