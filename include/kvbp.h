@@ -487,6 +487,76 @@ int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t 
                      int64_t ldw, const float* w_scale, const void* x, int64_t ldx, const void* bias, void* out,
                      int64_t ldo, void* workspace, int64_t workspace_bytes, int32_t* dev_err);
 
+/* ---- Speculative decoding over the slot cache ---------------------------------------------
+ * (No counterpart in the reference, which decodes one token per step.)
+ *
+ * A tree of up to 128 nodes per sequence is parents [B][T] int32: node 0 is the root (-1: the
+ * token that the last step chose, not yet in the cache), parents[b][t] < t names a node's parent.
+ * A parent below -1 marks an unused node, and so does an unused ancestor; a parent >= t sets
+ * KVBP_DEV_INDEX and counts as unused.  The draft's rows come from kvbp_qkv_rope_scatter with
+ * rows_per_seq = S = T and write_slot[r] = r % T. */
+
+/* Attention of the tree over the cache: node t of sequence b sees the live slots of its cache --
+ * s < lens[b] (lens [B] or NULL: all S) with slot_pos[b][s] >= 0 (slot_pos [B][S] or NULL: all) --
+ * and, of the drafted keys, its ancestors and itself: out = softmax(scale * q . k) v.
+ * q, out [B][T][Hq][128] bf16; kcache / vcache [B][Hkv][S][128] bf16 (S may be 0), k_draft / v_draft
+ * [B][Hkv][T][128] bf16; all 16-byte aligned, out apart from what is read.  Hq / Hkv <= 128.
+ * node_score [B][T][S + T] float (may be NULL, non-negative on entry) is max-accumulated with each
+ * (node, key)'s largest probability over the heads: column s is slot s, S + j is node j.  (Pass the
+ * same buffer for every layer; zero it before a step's first.)  Unused nodes: out is 0, scores stay.
+ * K and V of slots and nodes that a row does not see never reach it.  lens outside [0, S] is cut
+ * there and sets KVBP_DEV_INDEX.  Softmax statistics and sums are fp32.
+ * workspace: kvbp_tree_attn_workspace bytes, 16-byte aligned (NULL where that is 0); free to reuse by
+ * the next call on the same stream (calls that may overlap need one each); nothing is kept in it. */
+int64_t kvbp_tree_attn_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t S, int32_t with_score);
+int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t S,
+                   const void* q, const void* kcache, const void* vcache, const void* k_draft, const void* v_draft,
+                   const int32_t* parents, const int32_t* slot_pos, const int32_t* lens, float scale, void* out,
+                   float* node_score, void* workspace, int64_t workspace_bytes, int32_t* dev_err);
+
+/* Verification of the drafted tokens.  target: logits of row (b, t) at (b * T + t) * ldt, bf16 or
+ * float (fp32_target); the target's distribution there is softmax(logits / temperature[b])
+ * (temperature NULL: 1).  The nodes are walked in order; node j whose parent is the last accepted
+ * node is tested: with r the target's distribution at that parent, x = tokens[b][j] and
+ * u = accept_u[b][j] in [0, 1), it is accepted when u * q(x) * sum(r) < r(x); otherwise
+ * r <- max(r / sum(r) - q, 0).  q is the distribution that the parent's children were drawn from:
+ * draft_probs [.. (b * T + parent) * ldd ..] float, or, where draft_probs is NULL (a draft that is
+ * not random), 1 at x.  next_token[b] is the first x whose running sum of the last r exceeds
+ * sample_u[b] * sum(r).  This keeps the target's distribution whatever the draft.  Where no weight is
+ * left the token is drawn from the node's whole distribution; -1 (and KVBP_DEV_NAN_SCORE) where that
+ * has none.  temperature <= 0: a token is accepted when it is the row's first maximum, and that is
+ * next_token (draft_probs is not read).  NaN logits count as -inf and set KVBP_DEV_NAN_SCORE; a token
+ * outside [0, vocab) is rejected, leaves r as it is and sets KVBP_DEV_INDEX.
+ * path [B][T] int32: the accepted nodes, root first, then -1; n_path[b] their number (1: the root
+ * alone; 0 with next_token -1 for a sequence whose root is unused).  Weights and sums are double.
+ * workspace as for kvbp_tree_attn. */
+int64_t kvbp_tree_verify_workspace(int32_t B, int32_t T, int32_t vocab);
+int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int32_t vocab, int32_t fp32_target,
+                     const void* target, int64_t ldt, const float* temperature, const int32_t* tokens,
+                     const int32_t* parents, const float* draft_probs, int64_t ldd, const float* accept_u,
+                     const float* sample_u, int32_t* path, int32_t* n_path, int32_t* next_token, void* workspace,
+                     int64_t workspace_bytes, int32_t* dev_err);
+
+/* Commit of the accepted path: for i < n_path[b], node path[b][i] becomes position next_pos_in[b] + i,
+ * in the lowest slot that is free then, at step seq_step_in[b] + i + 1, with the metadata that
+ * kvbp_append_evict gives a new position and, when node_score [B][T][S + T] is given, the update that
+ * kvbp_score_update makes of that step's scores (row path[b][i]: the slots, and the path's nodes so
+ * far).  Then, where the step counter has passed a multiple of cfg->evict_every (cfg may be NULL: no
+ * eviction), one eviction at the last step as kvbp_append_evict makes it; its victims are appended to
+ * evlog.  write_slot [B][T] int32 receives each path entry's slot (-1: none, or evicted), and K and V
+ * of those nodes are copied from the drafts [layers][B][Hkv][T][128] to the caches
+ * [layers][B][Hkv][S][128] (bf16, 16-byte aligned; layers may be 0).
+ * State is read from st_in, seq_step_in, next_pos_in, evcount_in and written to st_out, seq_step,
+ * next_pos, evcount: the same arrays, or others that overlap nothing (the old state stays, so that
+ * a step can be taken back).  S <= 16384 with cfg.  A path longer than T, or with an entry that is no
+ * node, ends there (KVBP_DEV_INDEX); entries without a free slot get none (KVBP_DEV_NO_FREE_SLOT). */
+int kvbp_tree_commit(kvbp_stream_t stream, const kvbp_state* st_in, const kvbp_state* st_out,
+                     const kvbp_evict_cfg* cfg, int32_t T, const int32_t* path, const int32_t* n_path,
+                     const float* node_score, int32_t layers, int32_t Hkv, int32_t head_dim, const void* k_draft,
+                     const void* v_draft, void* kcache, void* vcache, const int32_t* seq_step_in,
+                     const int32_t* next_pos_in, const int32_t* evcount_in, int32_t* seq_step, int32_t* next_pos,
+                     int32_t* evcount, int32_t* evlog, int32_t evcap, int32_t* write_slot, int32_t* dev_err);
+
 #ifdef __cplusplus
 }
 #endif

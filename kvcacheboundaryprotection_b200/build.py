@@ -22,7 +22,7 @@ LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libkvbp.so"
 INCLUDE = PKG.parent / "include"
 SOURCES = ["capi.cu", "attn_decode.cu", "dense.cu", "evict.cu", "gemm_decode.cu", "int8_gemm.cu", "kv4.cu",
-           "prefill_attn.cu", "prefill_gemm.cu"]
+           "prefill_attn.cu", "prefill_gemm.cu", "tree_attn.cu", "tree_verify.cu"]
 HEADERS = ["common.cuh", "kvbp_internal.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

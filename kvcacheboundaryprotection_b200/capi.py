@@ -146,6 +146,21 @@ SIGNATURES = {
     "kvbp_int8_gemm": (C.c_int, [P, I32, I32, I32, I32, P, I64, P, P, I64, P, P, P, I64, P]),
     "kvbp_int8_linear_workspace": (I64, [I32, I32]),
     "kvbp_int8_linear": (C.c_int, [P, I32, I32, I32, I32, P, I64, P, P, I64, P, P, I64, P, I64, P]),
+    "kvbp_tree_attn_workspace": (I64, [I32, I32, I32, I32, I32, I32]),
+    "kvbp_tree_attn": (
+        C.c_int,
+        [P, I32, I32, I32, I32, I32, I32, P, P, P, P, P, P, P, P, F32, P, P, P, I64, P],
+    ),
+    "kvbp_tree_verify_workspace": (I64, [I32, I32, I32]),
+    "kvbp_tree_verify": (
+        C.c_int,
+        [P, I32, I32, I32, I32, P, I64, P, P, P, P, I64, P, P, P, P, P, P, I64, P],
+    ),
+    "kvbp_tree_commit": (
+        C.c_int,
+        [P, C.POINTER(State), C.POINTER(State), C.POINTER(EvictCfg), I32, P, P, P, I32, I32, I32, P, P, P, P, P, P, P,
+         P, P, P, P, I32, P, P],
+    ),
 }
 EXTRA_SIGNATURES = {
     "kvbp_decode_attn_score_cs": (C.c_int, [P, I32, I32, I32, I32, I32, P, P, P, P, P, P, P, P, I32]),

@@ -347,6 +347,237 @@ __device__ void log_victim(const AppendArgs& a, int b, int pos) {
   a.evcount[b] = n + 1;
 }
 
+// One cadence eviction of sequence b by the whole block: the policy's victims under the
+// structural protection, then the hard-capacity guardrail.  s_vict: dynamic shared memory
+// (victim list, then the staged position bitmap and keys where they fit); sh: 8 words of
+// which 2..7 are used.  Returns the retained count.
+__device__ __forceinline__ int evict_at_cadence(const AppendArgs& a, const SeqState& s, int b, int step, int* s_vict,
+                                                int* red_i, KeySlot* red_k, int* sh) {
+  const int tid = threadIdx.x, S = a.st.S;
+  int n_vict = 0;
+  // ---- retained count and evict_count -----------------------------------------
+  int cnt = 0;
+  for (int i = tid; i < S; i += kEvictThreads) cnt += s.slot_pos[i] >= 0;
+  const int R = block_sum_int(cnt, red_i);
+  const int k_req = R - a.C > 0 ? R - a.C : 0;
+  // ---- structural protection (ProtectedPolicyWrapper) ---------------------------
+  int thr_lo = -1, thr_hi = 0x7fffffff;  // eligible <=> thr_lo <= pos < thr_hi
+  bool none = false;
+  if (a.protect) {
+    if (k_req <= 0 || a.n_suffix == 0 || a.n_suffix >= R || a.n_prefix >= R) {
+      none = true;  // wrapper returns [] (n_suffix == 0 slices the whole list)
+    } else {
+      // the position bitmap staged in shared memory first (all threads, loads in flight
+      // together): the two selecting warps walk it 32 words per step, which from global
+      // memory was one dependent round trip per step
+      const uint32_t* pm = s.posmap;
+      if (a.pm_smem) {
+        uint32_t* spm = reinterpret_cast<uint32_t*>(s_vict + S);
+        for (int w0 = tid; w0 < a.st.W; w0 += 4 * kEvictThreads) {
+          uint32_t v4[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int w = w0 + q * kEvictThreads;
+            v4[q] = w < a.st.W ? s.posmap[w] : 0u;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int w = w0 + q * kEvictThreads;
+            if (w < a.st.W) spm[w] = v4[q];
+          }
+        }
+        __syncthreads();
+        pm = spm;
+      }
+      const int warp = tid >> 5;
+      if (warp == 0) {
+        const int v = select_bit_warp(pm, a.st.W, a.n_prefix);
+        if ((tid & 31) == 0) sh[2] = v;
+      } else if (warp == 1) {
+        const int v = select_bit_warp(pm, a.st.W, R - a.n_suffix);
+        if ((tid & 31) == 0) sh[3] = v;
+      }
+      __syncthreads();
+      thr_lo = sh[2];
+      thr_hi = sh[3];
+    }
+  }
+  __syncthreads();
+  int k = 0;
+  if (a.ext_pos) {
+    // victims listed by the host, in its order: look up each position's slot
+    int nl = a.ext_n[b];
+    nl = nl < a.ext_stride ? nl : a.ext_stride;
+    for (int j = 0; j < nl; ++j) {
+      const int p = a.ext_pos[static_cast<size_t>(b) * a.ext_stride + j];
+      int hit = 0x7fffffff;
+      for (int i = tid; i < S; i += kEvictThreads)
+        if (s.slot_pos[i] == p && p >= 0) {
+          hit = i;
+          break;
+        }
+      const int sl = block_min_int(hit, red_i);
+      if (tid == 0) {
+        bool dup = false;
+        for (int q = 0; q < n_vict; ++q) dup |= s_vict[q] == sl;
+        if (sl == 0x7fffffff)
+          set_err(a.err, kErrIndex);
+        else if (!dup)
+          s_vict[n_vict] = sl;
+        sh[5] = (sl != 0x7fffffff && !dup) ? 1 : 0;
+      }
+      __syncthreads();
+      n_vict += sh[5];
+      __syncthreads();
+    }
+  } else if (!none && k_req > 0) {
+    auto elig = [&](int i) {
+      const int p = s.slot_pos[i];
+      return p >= 0 && p >= thr_lo && p < thr_hi;
+    };
+    int ne = 0;
+    for (int i = tid; i < S; i += kEvictThreads) ne += elig(i);
+    const int n_elig = block_sum_int(ne, red_i);
+    k = k_req < n_elig ? k_req : n_elig;
+    if (a.policy == kPolicyStreamingLLM && k > 0) {
+      // sink: the 4 smallest by (insert_step, str(pos)); recent: the C-4 largest by
+      // (last, insert, str(pos)); candidates = the rest, or everything if empty.
+      auto skey = [&](int i) { return sink_key(s.slot_pos[i], s.insert_step[i]); };
+      auto okey = [&](int i) {
+        return policy_key(kPolicyLRU, step, s.slot_pos[i], s.insert_step[i], s.last_access[i], 0.f, 0.f, 0.0, 0.f,
+                          a.err);
+      };
+      uint32_t taken = 0;
+      const int n_sink = n_elig < 4 ? n_elig : 4;
+      for (int r = 0; r < n_sink; ++r) {
+        const KeySlot w = take_min(S, taken, skey, elig, red_k);
+        if (tid == 0) sh[4 + r] = w.slot;
+      }
+      __syncthreads();
+      const int recent_n = a.C - 4 > 0 ? a.C - 4 : 0;
+      const int n_notrecent = n_elig - recent_n > 0 ? n_elig - recent_n : 0;
+      taken = 0;
+      for (int r = 0; r < n_notrecent && n_vict < k; ++r) {
+        const KeySlot w = take_min(S, taken, okey, elig, red_k);
+        bool is_sink = false;
+        for (int j = 0; j < n_sink; ++j) is_sink |= (sh[4 + j] == w.slot);
+        if (!is_sink) {
+          if (tid == 0) s_vict[n_vict] = w.slot;
+          ++n_vict;
+        }
+      }
+      if (n_vict == 0) {  // no candidates outside sink/recent: rank all eligible
+        taken = 0;
+        for (int r = 0; r < k; ++r) {
+          const KeySlot w = take_min(S, taken, okey, elig, red_k);
+          if (tid == 0) s_vict[n_vict] = w.slot;
+          ++n_vict;
+        }
+      }
+    } else if (k > 0) {
+      // k rounds of block argmin.  Each thread forms the keys of its slots once (the loads
+      // of kQ slots in flight together) and keeps them -- in shared memory when they fit
+      // (a local array of 512 threads does not stay in L1); a thread's minimum changes only
+      // when it owned a round's winner, and then it rescans its cached keys (a rescan from
+      // global memory put every round's latency on the critical path: 4.7 us per round at
+      // 4104 slots).  A warp-first top-k (each warp its k smallest, then one warp over the
+      // 16 x k candidates) measured slower than these block rounds.
+      Key3* kcs = a.key_smem ? reinterpret_cast<Key3*>(reinterpret_cast<uint8_t*>(s_vict) + a.key_smem) : nullptr;
+      Key3 kc_local[kMaxPerThread];
+      auto kc = [&](int j) -> Key3& { return kcs ? kcs[tid + j * kEvictThreads] : kc_local[j]; };
+      uint32_t skip = 0;  // bit j: slot tid + j * kEvictThreads ineligible or already taken
+      const int nj = tid < S ? (S - tid + kEvictThreads - 1) / kEvictThreads : 0;
+      // only the fields the policy's key reads are loaded
+      const int pol = a.policy;
+      const bool need_cu = pol == kPolicyH2OFaithful || pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyAdaKV;
+      const bool need_at = pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyQuest;
+      const bool need_ma = pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyAdaKV;
+      const bool need_pr = pol == kPolicySnapKVFaithful;
+      constexpr int kQ = 4;  // slots per batch of loads
+      for (int j0 = 0; j0 < nj; j0 += kQ) {
+        int pp[kQ], ins[kQ], lst[kQ];
+        float at[kQ], ma[kQ], pr[kQ];
+        double cu[kQ];
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+          const int j = j0 + q, i = tid + j * kEvictThreads;
+          const bool in = j < nj;
+          pp[q] = in ? s.slot_pos[i] : -1;
+          ins[q] = in ? s.insert_step[i] : 0;
+          lst[q] = in ? s.last_access[i] : 0;
+          at[q] = (in && need_at) ? s.attn[i] : 0.f;
+          ma[q] = (in && need_ma) ? s.max_attn[i] : 0.f;
+          pr[q] = (in && need_pr) ? s.prefill[i] : 0.f;
+          cu[q] = (in && need_cu) ? s.cumul[i] : 0.0;
+        }
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+          const int j = j0 + q;
+          if (j >= nj) break;
+          const bool e = pp[q] >= 0 && pp[q] >= thr_lo && pp[q] < thr_hi;
+          if (e)
+            kc(j) = policy_key(a.policy, step, pp[q], ins[q], lst[q], at[q], ma[q], cu[q], pr[q], a.err);
+          else
+            skip |= 1u << j;
+        }
+      }
+      auto cached_min = [&]() {
+        KeySlot best{key_max(), 0x7fffffff};
+        for (int j = 0; j < nj; ++j) {
+          if ((skip >> j) & 1u) continue;
+          const KeySlot c{kc(j), tid + j * kEvictThreads};
+          if (ks_less(c, best)) best = c;
+        }
+        return best;
+      };
+      KeySlot mine = cached_min();
+      for (int r = 0; r < k; ++r) {
+        const KeySlot w = block_argmin(mine, red_k);
+        if (w.slot != 0x7fffffff && (w.slot % kEvictThreads) == tid) {
+          skip |= 1u << (w.slot / kEvictThreads);
+          mine = cached_min();
+        }
+        if (tid == 0) s_vict[n_vict] = w.slot;
+        ++n_vict;
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int j = 0; j < n_vict; ++j) {
+      const int sl = s_vict[j];
+      const int p = s.slot_pos[sl];
+      log_victim(a, b, p);
+      if ((p >> 5) < a.st.W) s.posmap[p >> 5] &= ~(1u << (p & 31));
+      s.slot_pos[sl] = -1;
+    }
+  }
+  __syncthreads();
+  // ---- hard-capacity guardrail ------------------------------------------------
+  const int overflow = a.no_hardcap ? 0 : (R - n_vict) - a.C;
+  if (overflow > 0) {
+    auto live = [&](int i) { return s.slot_pos[i] >= 0; };
+    auto hkey = [&](int i) { return hardcap_key(s.slot_pos[i], s.insert_step[i], s.last_access[i]); };
+    uint32_t taken = 0;
+    for (int r = 0; r < overflow; ++r) {
+      const KeySlot w = take_min(S, taken, hkey, live, red_k);
+      if (tid == 0) s_vict[r] = w.slot;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      for (int j = 0; j < overflow; ++j) {
+        const int sl = s_vict[j];
+        const int p = s.slot_pos[sl];
+        log_victim(a, b, p);
+        if ((p >> 5) < a.st.W) s.posmap[p >> 5] &= ~(1u << (p & 31));
+        s.slot_pos[sl] = -1;
+      }
+    }
+    n_vict += overflow;
+  }
+  return R - n_vict;
+}
+
 __global__ void __launch_bounds__(kEvictThreads) append_evict_kernel(AppendArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -490,231 +721,11 @@ __global__ void __launch_bounds__(kEvictThreads) append_evict_kernel(AppendArgs 
   }
   __syncthreads();
 
-  int n_vict = 0;
   if (a.decode_regime && step % a.E == 0) {
-    // ---- retained count and evict_count -----------------------------------------
-    int cnt = 0;
-    for (int i = tid; i < S; i += kEvictThreads) cnt += s.slot_pos[i] >= 0;
-    const int R = block_sum_int(cnt, red_i);
-    const int k_req = R - a.C > 0 ? R - a.C : 0;
-    // ---- structural protection (ProtectedPolicyWrapper) ---------------------------
-    int thr_lo = -1, thr_hi = 0x7fffffff;  // eligible <=> thr_lo <= pos < thr_hi
-    bool none = false;
-    if (a.protect) {
-      if (k_req <= 0 || a.n_suffix == 0 || a.n_suffix >= R || a.n_prefix >= R) {
-        none = true;  // wrapper returns [] (n_suffix == 0 slices the whole list)
-      } else {
-        // the position bitmap staged in shared memory first (all threads, loads in flight
-        // together): the two selecting warps walk it 32 words per step, which from global
-        // memory was one dependent round trip per step
-        const uint32_t* pm = s.posmap;
-        if (a.pm_smem) {
-          uint32_t* spm = reinterpret_cast<uint32_t*>(s_vict + S);
-          for (int w0 = tid; w0 < a.st.W; w0 += 4 * kEvictThreads) {
-            uint32_t v4[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int w = w0 + q * kEvictThreads;
-              v4[q] = w < a.st.W ? s.posmap[w] : 0u;
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int w = w0 + q * kEvictThreads;
-              if (w < a.st.W) spm[w] = v4[q];
-            }
-          }
-          __syncthreads();
-          pm = spm;
-        }
-        const int warp = tid >> 5;
-        if (warp == 0) {
-          const int v = select_bit_warp(pm, a.st.W, a.n_prefix);
-          if ((tid & 31) == 0) sh[2] = v;
-        } else if (warp == 1) {
-          const int v = select_bit_warp(pm, a.st.W, R - a.n_suffix);
-          if ((tid & 31) == 0) sh[3] = v;
-        }
-        __syncthreads();
-        thr_lo = sh[2];
-        thr_hi = sh[3];
-      }
-    }
-    __syncthreads();
-    int k = 0;
-    if (a.ext_pos) {
-      // victims listed by the host, in its order: look up each position's slot
-      int nl = a.ext_n[b];
-      nl = nl < a.ext_stride ? nl : a.ext_stride;
-      for (int j = 0; j < nl; ++j) {
-        const int p = a.ext_pos[static_cast<size_t>(b) * a.ext_stride + j];
-        int hit = 0x7fffffff;
-        for (int i = tid; i < S; i += kEvictThreads)
-          if (s.slot_pos[i] == p && p >= 0) {
-            hit = i;
-            break;
-          }
-        const int sl = block_min_int(hit, red_i);
-        if (tid == 0) {
-          bool dup = false;
-          for (int q = 0; q < n_vict; ++q) dup |= s_vict[q] == sl;
-          if (sl == 0x7fffffff)
-            set_err(a.err, kErrIndex);
-          else if (!dup)
-            s_vict[n_vict] = sl;
-          sh[5] = (sl != 0x7fffffff && !dup) ? 1 : 0;
-        }
-        __syncthreads();
-        n_vict += sh[5];
-        __syncthreads();
-      }
-    } else if (!none && k_req > 0) {
-      auto elig = [&](int i) {
-        const int p = s.slot_pos[i];
-        return p >= 0 && p >= thr_lo && p < thr_hi;
-      };
-      int ne = 0;
-      for (int i = tid; i < S; i += kEvictThreads) ne += elig(i);
-      const int n_elig = block_sum_int(ne, red_i);
-      k = k_req < n_elig ? k_req : n_elig;
-      if (a.policy == kPolicyStreamingLLM && k > 0) {
-        // sink: the 4 smallest by (insert_step, str(pos)); recent: the C-4 largest by
-        // (last, insert, str(pos)); candidates = the rest, or everything if empty.
-        auto skey = [&](int i) { return sink_key(s.slot_pos[i], s.insert_step[i]); };
-        auto okey = [&](int i) {
-          return policy_key(kPolicyLRU, step, s.slot_pos[i], s.insert_step[i], s.last_access[i], 0.f, 0.f, 0.0, 0.f,
-                            a.err);
-        };
-        uint32_t taken = 0;
-        const int n_sink = n_elig < 4 ? n_elig : 4;
-        for (int r = 0; r < n_sink; ++r) {
-          const KeySlot w = take_min(S, taken, skey, elig, red_k);
-          if (tid == 0) sh[4 + r] = w.slot;
-        }
-        __syncthreads();
-        const int recent_n = a.C - 4 > 0 ? a.C - 4 : 0;
-        const int n_notrecent = n_elig - recent_n > 0 ? n_elig - recent_n : 0;
-        taken = 0;
-        for (int r = 0; r < n_notrecent && n_vict < k; ++r) {
-          const KeySlot w = take_min(S, taken, okey, elig, red_k);
-          bool is_sink = false;
-          for (int j = 0; j < n_sink; ++j) is_sink |= (sh[4 + j] == w.slot);
-          if (!is_sink) {
-            if (tid == 0) s_vict[n_vict] = w.slot;
-            ++n_vict;
-          }
-        }
-        if (n_vict == 0) {  // no candidates outside sink/recent: rank all eligible
-          taken = 0;
-          for (int r = 0; r < k; ++r) {
-            const KeySlot w = take_min(S, taken, okey, elig, red_k);
-            if (tid == 0) s_vict[n_vict] = w.slot;
-            ++n_vict;
-          }
-        }
-      } else if (k > 0) {
-        // k rounds of block argmin.  Each thread forms the keys of its slots once (the loads
-        // of kQ slots in flight together) and keeps them -- in shared memory when they fit
-        // (a local array of 512 threads does not stay in L1); a thread's minimum changes only
-        // when it owned a round's winner, and then it rescans its cached keys (a rescan from
-        // global memory put every round's latency on the critical path: 4.7 us per round at
-        // 4104 slots).  A warp-first top-k (each warp its k smallest, then one warp over the
-        // 16 x k candidates) measured slower than these block rounds.
-        Key3* kcs = a.key_smem ? reinterpret_cast<Key3*>(reinterpret_cast<uint8_t*>(s_vict) + a.key_smem) : nullptr;
-        Key3 kc_local[kMaxPerThread];
-        auto kc = [&](int j) -> Key3& { return kcs ? kcs[tid + j * kEvictThreads] : kc_local[j]; };
-        uint32_t skip = 0;  // bit j: slot tid + j * kEvictThreads ineligible or already taken
-        const int nj = tid < S ? (S - tid + kEvictThreads - 1) / kEvictThreads : 0;
-        // only the fields the policy's key reads are loaded
-        const int pol = a.policy;
-        const bool need_cu = pol == kPolicyH2OFaithful || pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyAdaKV;
-        const bool need_at = pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyQuest;
-        const bool need_ma = pol == kPolicyH2O || pol == kPolicySnapKV || pol == kPolicyAdaKV;
-        const bool need_pr = pol == kPolicySnapKVFaithful;
-        constexpr int kQ = 4;  // slots per batch of loads
-        for (int j0 = 0; j0 < nj; j0 += kQ) {
-          int pp[kQ], ins[kQ], lst[kQ];
-          float at[kQ], ma[kQ], pr[kQ];
-          double cu[kQ];
-#pragma unroll
-          for (int q = 0; q < kQ; ++q) {
-            const int j = j0 + q, i = tid + j * kEvictThreads;
-            const bool in = j < nj;
-            pp[q] = in ? s.slot_pos[i] : -1;
-            ins[q] = in ? s.insert_step[i] : 0;
-            lst[q] = in ? s.last_access[i] : 0;
-            at[q] = (in && need_at) ? s.attn[i] : 0.f;
-            ma[q] = (in && need_ma) ? s.max_attn[i] : 0.f;
-            pr[q] = (in && need_pr) ? s.prefill[i] : 0.f;
-            cu[q] = (in && need_cu) ? s.cumul[i] : 0.0;
-          }
-#pragma unroll
-          for (int q = 0; q < kQ; ++q) {
-            const int j = j0 + q;
-            if (j >= nj) break;
-            const bool e = pp[q] >= 0 && pp[q] >= thr_lo && pp[q] < thr_hi;
-            if (e)
-              kc(j) = policy_key(a.policy, step, pp[q], ins[q], lst[q], at[q], ma[q], cu[q], pr[q], a.err);
-            else
-              skip |= 1u << j;
-          }
-        }
-        auto cached_min = [&]() {
-          KeySlot best{key_max(), 0x7fffffff};
-          for (int j = 0; j < nj; ++j) {
-            if ((skip >> j) & 1u) continue;
-            const KeySlot c{kc(j), tid + j * kEvictThreads};
-            if (ks_less(c, best)) best = c;
-          }
-          return best;
-        };
-        KeySlot mine = cached_min();
-        for (int r = 0; r < k; ++r) {
-          const KeySlot w = block_argmin(mine, red_k);
-          if (w.slot != 0x7fffffff && (w.slot % kEvictThreads) == tid) {
-            skip |= 1u << (w.slot / kEvictThreads);
-            mine = cached_min();
-          }
-          if (tid == 0) s_vict[n_vict] = w.slot;
-          ++n_vict;
-        }
-      }
-    }
-    __syncthreads();
-    if (tid == 0) {
-      for (int j = 0; j < n_vict; ++j) {
-        const int sl = s_vict[j];
-        const int p = s.slot_pos[sl];
-        log_victim(a, b, p);
-        s.posmap[p >> 5] &= ~(1u << (p & 31));
-        s.slot_pos[sl] = -1;
-      }
-    }
-    __syncthreads();
-    // ---- hard-capacity guardrail ------------------------------------------------
-    const int overflow = a.no_hardcap ? 0 : (R - n_vict) - a.C;
-    if (overflow > 0) {
-      auto live = [&](int i) { return s.slot_pos[i] >= 0; };
-      auto hkey = [&](int i) { return hardcap_key(s.slot_pos[i], s.insert_step[i], s.last_access[i]); };
-      uint32_t taken = 0;
-      for (int r = 0; r < overflow; ++r) {
-        const KeySlot w = take_min(S, taken, hkey, live, red_k);
-        if (tid == 0) s_vict[r] = w.slot;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        for (int j = 0; j < overflow; ++j) {
-          const int sl = s_vict[j];
-          const int p = s.slot_pos[sl];
-          log_victim(a, b, p);
-          s.posmap[p >> 5] &= ~(1u << (p & 31));
-          s.slot_pos[sl] = -1;
-        }
-      }
-      n_vict += overflow;
-    }
+    const int left = evict_at_cadence(a, s, b, step, s_vict, red_i, red_k, sh);
     __syncthreads();
     if (tid == 0 && a.retained_log && step <= a.log_steps)
-      a.retained_log[static_cast<size_t>(b) * (a.log_steps + 1) + step] = R - n_vict;
+      a.retained_log[static_cast<size_t>(b) * (a.log_steps + 1) + step] = left;
   } else if (tid == 0 && a.retained_log && step <= a.log_steps) {
     // retained count = previous count + 1 (no eviction this step)
     const size_t o = static_cast<size_t>(b) * (a.log_steps + 1);
@@ -723,6 +734,176 @@ __global__ void __launch_bounds__(kEvictThreads) append_evict_kernel(AppendArgs 
   __syncthreads();
   if (tid == 0) a.write_slot[b] = (s.slot_pos[slot] == pos) ? slot : -1;
   if (tid == 0 && a.upd_score) a.upd_pending[b] = 1;  // this step's scores are applied by the next call
+}
+
+// ------------------------------------------------------------------------------------
+// commit of the accepted path of a tree of drafted tokens (speculative decoding): the m
+// positions of the path are appended in order, each with its own step's score update, then
+// at most one cadence eviction, from the state ``in`` to the state ``a.st`` (which may be the
+// same arrays).  Node i's step: kv_coupled_generator.py:350-364 (append), :504-516 (score
+// update), with the same arithmetic as append_evict_kernel and score_update_kernel.
+// ------------------------------------------------------------------------------------
+constexpr int kMaxNodes = 128;
+
+struct CommitArgs {
+  AppendArgs a;  // eviction configuration (C == 0: none), state written, log, error word
+  StateArgs in;
+  int T;
+  const int* path;    // [B][T] accepted nodes, root first
+  const int* n_path;  // [B]
+  const float* score; // [B][T][S + T] (may be null)
+  const int* seq_step;
+  const int* next_pos;
+  const int* evcount;
+  int* write_slot;  // [B][T] out
+};
+
+__global__ void __launch_bounds__(kEvictThreads) tree_commit_kernel(CommitArgs c) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ int s_vict[];
+  __shared__ int red_i[32];
+  __shared__ float red_f[32];
+  __shared__ KeySlot red_k[32];
+  __shared__ int sh[8];
+  __shared__ int s_node[kMaxNodes], s_slot[kMaxNodes];
+  __shared__ float s_thr[kMaxNodes];
+  const AppendArgs& a = c.a;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int S = a.st.S, T = c.T, W = a.st.W;
+  const SeqState in = c.in.seq(b), s = a.st.seq(b);
+  const int step0 = c.seq_step[b], pos0 = c.next_pos[b], ev0 = c.evcount[b];
+  int m = c.n_path[b];
+  if (m < 0 || m > T) {
+    if (tid == 0) set_err(a.err, kErrIndex);
+    m = m < 0 ? 0 : T;
+  }
+  // the path's nodes; it ends before one that is no node
+  const int node = tid < m ? c.path[static_cast<size_t>(b) * T + tid] : 0;
+  const int bad = block_min_int(tid < m && (node < 0 || node >= T) ? tid : 0x7fffffff, red_i);
+  if (bad < m) {
+    if (tid == 0) set_err(a.err, kErrIndex);
+    m = bad;
+  }
+  if (tid < m) {
+    s_node[tid] = node;
+    s_slot[tid] = -1;
+  }
+  // the m lowest free slots, in ascending order
+  int found = 0;
+  for (int i0 = 0; i0 < S && found < m; i0 += kEvictThreads) {
+    const int i = i0 + tid;
+    const bool fr = i < S && in.slot_pos[i] < 0;
+    const uint32_t vote = __ballot_sync(0xffffffffu, fr);
+    __syncthreads();
+    if (lane == 0) red_i[warp] = __popc(vote);
+    __syncthreads();
+    int before = found, all = 0;
+    for (int w = 0; w < (kEvictThreads >> 5); ++w) {
+      const int n = red_i[w];
+      before += w < warp ? n : 0;
+      all += n;
+    }
+    const int rank = before + __popc(vote & ((1u << lane) - 1u));
+    if (fr && rank < m) s_slot[rank] = i;
+    found += all;
+  }
+  __syncthreads();
+  if (found < m && tid == 0) set_err(a.err, kErrNoFreeSlot);
+  const int placed = found < m ? found : m;  // nodes that have a slot
+  // each step's access threshold: 5 % of the largest score over what that step attended
+  const size_t pitch = static_cast<size_t>(S) + T;
+  const float* sc = c.score ? c.score + static_cast<size_t>(b) * T * pitch : nullptr;
+  if (sc) {
+    for (int i = 0; i < m; ++i) {
+      const float* row = sc + s_node[i] * pitch;
+      float mx = 0.f;
+      for (int j = tid; j < S; j += kEvictThreads)
+        if (in.slot_pos[j] >= 0) mx = fmaxf(mx, row[j]);
+      if (tid <= i && tid < placed) mx = fmaxf(mx, row[S + s_node[tid]]);
+      mx = block_max_float(mx, red_f);
+      if (tid == 0) s_thr[i] = static_cast<float>(0.05 * static_cast<double>(mx));
+    }
+  }
+  __syncthreads();
+  // one slot's updates over the steps from first on
+  auto update = [&](int j, int col, int first, int pos, int ins, int last, int cnt, float at, float mxa, double cu,
+                    float pre) {
+    if (sc) {
+      for (int i = first; i < m; ++i) {
+        const float ks = sc[s_node[i] * pitch + col];
+        if (ks != ks) set_err(a.err, kErrNanScore);
+        at = ks;
+        mxa = fmaxf(mxa, ks);
+        cu = __dadd_rn(cu, static_cast<double>(ks));
+        if (ks > s_thr[i]) {
+          last = step0 + i + 1;
+          cnt += 1;
+        }
+      }
+    }
+    s.slot_pos[j] = pos;
+    s.insert_step[j] = ins;
+    s.last_access[j] = last;
+    s.access_count[j] = cnt;
+    s.attn[j] = at;
+    s.max_attn[j] = mxa;
+    s.cumul[j] = cu;
+    s.prefill[j] = pre;
+  };
+  for (int j = tid; j < S; j += kEvictThreads) {
+    const int p = in.slot_pos[j];
+    update(j, j, p >= 0 ? 0 : m, p, in.insert_step[j], in.last_access[j], in.access_count[j], in.attn[j],
+           in.max_attn[j], in.cumul[j], in.prefill[j]);
+  }
+  for (int w = tid; w < W; w += kEvictThreads) s.posmap[w] = in.posmap[w];
+  __syncthreads();
+  if (tid < placed) {
+    update(s_slot[tid], S + s_node[tid], tid, pos0 + tid, step0 + tid + 1, step0 + tid + 1, 1, 0.f, 0.f, 0.0, 0.f);
+    const int p = pos0 + tid;
+    if ((p >> 5) < W)
+      atomicOr(&s.posmap[p >> 5], 1u << (p & 31));
+    else
+      set_err(a.err, kErrIndex);
+  }
+  const int step = step0 + m;
+  if (tid == 0) {
+    a.seq_step[b] = step;
+    a.next_pos[b] = pos0 + m;
+    a.evcount[b] = ev0;
+  }
+  __syncthreads();
+  if (a.C > 0 && a.decode_regime && step / a.E != step0 / a.E)
+    evict_at_cadence(a, s, b, step, s_vict, red_i, red_k, sh);
+  __syncthreads();
+  if (tid < T) {
+    const int at = tid < m ? s_slot[tid] : -1;
+    c.write_slot[static_cast<size_t>(b) * T + tid] = (at >= 0 && s.slot_pos[at] == pos0 + tid) ? at : -1;
+  }
+}
+
+// K and V rows of the committed nodes, every layer and kv head: [layers][B][Hkv][T][128] ->
+// [layers][B][Hkv][S][128].  A warp copies one (layer, kv head)'s rows of one sequence.
+__global__ void __launch_bounds__(256) tree_rows_kernel(const __nv_bfloat16* __restrict__ kd,
+                                                        const __nv_bfloat16* __restrict__ vd,
+                                                        __nv_bfloat16* __restrict__ kc, __nv_bfloat16* __restrict__ vc,
+                                                        const int* __restrict__ path, const int* __restrict__ write_slot,
+                                                        int layers, int B, int Hkv, int T, int S) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  const int n = layers * Hkv;
+  for (int i = 0; i < T; ++i) {
+    const int slot = write_slot[static_cast<size_t>(b) * T + i];
+    if (slot < 0) continue;
+    const int node = path[static_cast<size_t>(b) * T + i];
+    for (int u = blockIdx.x * 8 + (threadIdx.x >> 5); u < n; u += gridDim.x * 8) {
+      const size_t head = (static_cast<size_t>(u / Hkv) * B + b) * Hkv + u % Hkv;
+      const size_t src = (head * T + node) * 128, dst = (head * S + slot) * 128;
+      reinterpret_cast<uint2*>(kc + dst)[lane] = reinterpret_cast<const uint2*>(kd + src)[lane];
+      reinterpret_cast<uint2*>(vc + dst)[lane] = reinterpret_cast<const uint2*>(vd + src)[lane];
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------
@@ -990,6 +1171,35 @@ int append_evict(cudaStream_t stream, const AppendArgs& a) {
   return check_launch("append_evict");
 }
 
+int tree_commit(cudaStream_t stream, CommitArgs c, int layers, int Hkv, const void* kd, const void* vd, void* kc,
+                void* vc) {
+  AppendArgs& a = c.a;
+  int smem = 0;
+  if (a.C > 0) {
+    smem = a.st.S * 4;
+    a.pm_smem = (a.st.S + a.st.W) * 4LL <= 160 * 1024;
+    if (a.pm_smem) smem = (a.st.S + a.st.W) * 4;
+    const int key_off = (smem + 15) / 16 * 16;
+    if (key_off + a.st.S * static_cast<int>(sizeof(Key3)) <= 200 * 1024) {
+      a.key_smem = key_off;
+      smem = key_off + a.st.S * static_cast<int>(sizeof(Key3));
+    }
+  }
+  if (!prepare_device(reinterpret_cast<const void*>(tree_commit_kernel), 200 * 1024))
+    return fail(kStatusCuda, "tree_commit: no usable device");
+  cudaError_t e = launch_pdl(tree_commit_kernel, dim3(a.st.B), dim3(kEvictThreads), smem, stream, dim3(0), c);
+  if (e != cudaSuccess) return fail(kStatusCuda, "tree_commit launch: %s", cudaGetErrorString(e));
+  if (layers > 0) {
+    const int per = (layers * Hkv + 7) / 8;
+    e = launch_pdl(tree_rows_kernel, dim3(per < 64 ? per : 64, a.st.B), dim3(256), 0, stream, dim3(0),
+                   static_cast<const __nv_bfloat16*>(kd), static_cast<const __nv_bfloat16*>(vd),
+                   static_cast<__nv_bfloat16*>(kc), static_cast<__nv_bfloat16*>(vc), c.path,
+                   static_cast<const int*>(c.write_slot), layers, a.st.B, Hkv, c.T, a.st.S);
+    if (e != cudaSuccess) return fail(kStatusCuda, "tree_commit rows launch: %s", cudaGetErrorString(e));
+  }
+  return check_launch("tree_commit");
+}
+
 int prefill_select(cudaStream_t stream, const PrefillSelArgs& a) {
   if (!a.victim || !a.evlog || a.B <= 0 || a.P <= 0) return fail(kStatusArg, "prefill_select: bad argument");
   if (a.policy < 0 || a.policy >= kPolicyCount) return fail(kStatusArg, "prefill_select: unknown policy");
@@ -1130,6 +1340,98 @@ int kvbp_head_signal_update(kvbp_stream_t stream, int32_t B, int32_t Hkv, int32_
   if (B <= 0 || Hkv <= 0 || S <= 0 || B > 65535) return kvbp::fail(kvbp::kStatusArg, "head_signal_update: bad size");
   return kvbp::head_signal_update(reinterpret_cast<cudaStream_t>(stream), B, Hkv, S, write_slot, head_score,
                                   head_cumul, head_current, dev_err);
+}
+
+int kvbp_tree_commit(kvbp_stream_t stream, const kvbp_state* st_in, const kvbp_state* st_out,
+                     const kvbp_evict_cfg* cfg, int32_t T, const int32_t* path, const int32_t* n_path,
+                     const float* node_score, int32_t layers, int32_t Hkv, int32_t head_dim, const void* k_draft,
+                     const void* v_draft, void* kcache, void* vcache, const int32_t* seq_step_in,
+                     const int32_t* next_pos_in, const int32_t* evcount_in, int32_t* seq_step, int32_t* next_pos,
+                     int32_t* evcount, int32_t* evlog, int32_t evcap, int32_t* write_slot, int32_t* dev_err) {
+  using kvbp::fail;
+  using kvbp::kStatusArg;
+  using kvbp::kStatusUnsupported;
+  if (!st_in || !st_out) return fail(kStatusArg, "tree_commit: null state");
+  if (!path || !n_path || !seq_step_in || !next_pos_in || !evcount_in || !seq_step || !next_pos || !evcount ||
+      !evlog || !write_slot)
+    return fail(kStatusArg, "tree_commit: null pointer");
+  kvbp::CommitArgs c{};
+  c.a.st = to_state(st_out);
+  c.in = to_state(st_in);
+  const kvbp::StateArgs &o = c.a.st, &i = c.in;
+  if (!kvbp::state_ok(o) || !kvbp::state_ok(i)) return fail(kStatusArg, "tree_commit: bad state");
+  if (i.B != o.B || i.S != o.S || i.W != o.W) return fail(kStatusArg, "tree_commit: the two states differ in size");
+  const long long B = o.B, S = o.S;
+  if (T <= 0 || T > kvbp::kMaxNodes) return fail(kStatusUnsupported, "tree_commit: %d nodes (1 to %d)", T, kvbp::kMaxNodes);
+  if (B > 65535 || S > 0x7fffffff - 1024 || evcap < 0) return fail(kStatusArg, "tree_commit: bad size");
+  if (cfg) {
+    if (cfg->capacity <= 0 || cfg->evict_every <= 0)
+      return fail(kStatusArg, "tree_commit: capacity and evict_every must be > 0");
+    if (cfg->policy < 0 || cfg->policy >= kvbp::kPolicyCount)
+      return fail(kStatusArg, "tree_commit: unknown policy %d", cfg->policy);
+    if (cfg->policy == kvbp::kPolicyRandom)
+      return fail(kStatusUnsupported, "tree_commit: the random policy's victims come from the host");
+    if (cfg->n_prefix < 0 || cfg->n_suffix < 0) return fail(kStatusArg, "tree_commit: negative protection size");
+    if (S > kvbp::kEvictThreads * kvbp::kMaxPerThread)
+      return fail(kStatusUnsupported, "tree_commit: %lld slots exceed %d", S, kvbp::kEvictThreads * kvbp::kMaxPerThread);
+    c.a.C = cfg->capacity;
+    c.a.E = cfg->evict_every;
+    c.a.policy = cfg->policy;
+    c.a.protect = cfg->protect;
+    c.a.n_prefix = cfg->n_prefix;
+    c.a.n_suffix = cfg->n_suffix;
+    c.a.decode_regime = cfg->decode_regime;
+  }
+  if (layers < 0) return fail(kStatusArg, "tree_commit: bad size");
+  if (layers > 0) {
+    if (!k_draft || !v_draft || !kcache || !vcache) return fail(kStatusArg, "tree_commit: null cache");
+    if (head_dim != 128) return fail(kStatusUnsupported, "tree_commit: head_dim %d unsupported (only 128)", head_dim);
+    if (Hkv <= 0 || static_cast<long long>(layers) * Hkv > 0x7fffffff / 8) return fail(kStatusArg, "tree_commit: bad size");
+    if (kvbp::misaligned(k_draft, 16) || kvbp::misaligned(v_draft, 16) || kvbp::misaligned(kcache, 16) ||
+        kvbp::misaligned(vcache, 16))
+      return fail(kStatusArg, "tree_commit: caches must be 16-byte aligned");
+    const long long nd = B * layers * Hkv * T * 256, nc = B * layers * Hkv * S * 256;
+    if (kvbp::overlap(k_draft, nd, kcache, nc) || kvbp::overlap(k_draft, nd, vcache, nc) ||
+        kvbp::overlap(v_draft, nd, kcache, nc) || kvbp::overlap(v_draft, nd, vcache, nc) ||
+        kvbp::overlap(kcache, nc, vcache, nc))
+      return fail(kStatusArg, "tree_commit: drafts and caches overlap");
+  }
+  // an array written is the one it follows from, or apart from everything read
+  struct Array {
+    const void *in, *out;
+    long long bytes;
+  } arrays[] = {{i.slot_pos, o.slot_pos, B * S * 4},         {i.insert_step, o.insert_step, B * S * 4},
+                {i.last_access, o.last_access, B * S * 4},   {i.access_count, o.access_count, B * S * 4},
+                {i.attn, o.attn, B * S * 4},                 {i.max_attn, o.max_attn, B * S * 4},
+                {i.cumul, o.cumul, B * S * 8},               {i.prefill, o.prefill, B * S * 4},
+                {i.posmap, o.posmap, B * static_cast<long long>(o.W) * 4},
+                {seq_step_in, seq_step, B * 4},              {next_pos_in, next_pos, B * 4},
+                {evcount_in, evcount, B * 4},                {nullptr, evlog, B * evcap * 4},
+                {nullptr, write_slot, B * T * 4},            {path, nullptr, B * T * 4},
+                {n_path, nullptr, B * 4},                    {node_score, nullptr, B * T * (S + T) * 4}};
+  for (const Array& x : arrays)
+    for (const Array& y : arrays) {
+      if (!x.out) break;
+      if (y.in && !(&x == &y && x.in == x.out) && kvbp::overlap(x.out, x.bytes, y.in, y.bytes))
+        return fail(kStatusArg, "tree_commit: an output overlaps an input that is not its own");
+      if (y.out && &x != &y && kvbp::overlap(x.out, x.bytes, y.out, y.bytes))
+        return fail(kStatusArg, "tree_commit: two outputs overlap");
+    }
+  c.a.seq_step = seq_step;
+  c.a.next_pos = next_pos;
+  c.a.evcount = evcount;
+  c.a.evlog = evlog;
+  c.a.evcap = evcap;
+  c.a.err = dev_err;
+  c.T = T;
+  c.path = path;
+  c.n_path = n_path;
+  c.score = node_score;
+  c.seq_step = seq_step_in;
+  c.next_pos = next_pos_in;
+  c.evcount = evcount_in;
+  c.write_slot = write_slot;
+  return kvbp::tree_commit(reinterpret_cast<cudaStream_t>(stream), c, layers, Hkv, k_draft, v_draft, kcache, vcache);
 }
 
 int kvbp_prefill_select(kvbp_stream_t stream, int32_t B, int32_t P, const kvbp_evict_cfg* cfg, const float* scores,

@@ -58,7 +58,7 @@ def _launch(fn, what: str, dev: torch.device, *args) -> None:
     """``fn(stream, *args)`` on the current stream of ``dev``, with ``dev`` as the current
     device."""
     if dev.type != "cuda":
-        raise ValueError("the low-bit operators run on CUDA devices only")
+        raise ValueError("these operators run on CUDA devices only")
     idx = dev.index
     if torch.cuda.current_device() == idx:
         status = fn(_raw_stream(idx), *args)
