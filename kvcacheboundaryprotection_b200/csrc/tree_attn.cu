@@ -1,7 +1,37 @@
-// Attention of a tree of drafted tokens over the slot cache, with the eviction score of every
-// (node, key): out = softmax(scale * q . k) v over the live slots and the node's ancestors.
-// One warp per (sequence, node, query head), one pass with the running maximum and sum, a
-// second one over the keys where the score is wanted.
+// Attention of a tree of drafted tokens over the slot cache on the 5th-generation tensor cores
+// (tcgen05 + TMEM), with the eviction score of every (node, key).
+//
+//   out[b, t, h] = sum_s p_s v_s,  p = softmax(scale * q . k) over the live slots of sequence b and
+//   the node's ancestors (itself among them);  score[b, t, key] = max over the heads of p.
+//
+// A kv head's rows are its G = Hq / Hkv query heads of every node: T * G rows read the same keys, so
+// a cache tile is fetched once for all of them, and with more than a few rows the products belong on
+// the tensor cores.  Rows are cut into row tiles of whole nodes (at most 128 rows = TMEM lanes).
+// A unit is (sequence, kv head) with one row tile (form A), or with a pair of row tiles that share
+// each key tile (form B, T * G > 128); its key tiles are the cache's and, last, the drafted nodes'.
+// All units' key tiles stand in one line that is cut into equal ranges, one per CTA, whatever the
+// lengths; a unit cut by a border leaves partial results (sum, running maximum, accumulator) that
+// combine_kernel joins.
+//
+// attend_kernel, one CTA per SM, 11 warps:
+//   * producer: K and V tiles (128 keys, 32 KiB each) by 3-D TMA through one ring in the order the
+//     products need them; Q once per unit;
+//   * MMA warp (one thread): item i = S_w = Q . K^T into TMEM (w = i & 1), then O_w += P . V with P
+//     read from TMEM; form A: the items are the unit's key tiles in turn, two accumulators;
+//     form B: the two row tiles of each key tile;
+//   * 2 x 4 softmax warps, a thread per row: the tile's maximum, weights 2^(c s - c m) in bf16 packed
+//     over S's columns, their sum.  The reference maximum m moves only when a row's maximum passes it
+//     by more than 2^8 in weight (exact in fp32, and bf16 weights keep their 8 bits wherever they lie),
+//     so that O is rescaled rarely;
+//   * mask warp: the live bits of each key tile from slot_pos / lens; V rows of dead slots and
+//     unused nodes are zeroed in shared memory before the product reads them (0 * NaN is NaN), and
+//     drafted V elements that are not finite, which rows off their branch must not meet, are taken out
+//     and added by the rows that see them.
+// Rounding: S, sums and O are fp32; a weight is rounded once to bf16 and the sum that divides is that
+// of the rounded weights (an error common to all weights cancels); out is rounded once.
+//
+// score_kernel forms p again from the final row statistics: S^T = K . Q^T with a slot per thread, so
+// that the maximum over heads stays in the thread and the score rows are written along the slots.
 #include "common.cuh"
 #include "kvbp_internal.h"
 
@@ -10,99 +40,985 @@ namespace ta {
 
 constexpr int kD = 128;
 constexpr int kMaxNodes = 128;
+constexpr int kKeys = 128;
+constexpr int kHalf = 128 * 128;  // a 64-column half of a [128][128] bf16 tile: 16 KiB
+constexpr int kTile = 2 * kHalf;
+constexpr int kProducer = 8, kMma = 9, kMask = 10;  // warps 0-7: softmax; 11 fills the warpgroup
+constexpr int kThreads = 12 * 32;
+constexpr int kAhead = 8;  // barriers in turn over the key tiles: more than the ring holds of either kind
+constexpr int kNf = 8;  // units' records of non-finite drafted values kept at a time
+constexpr float kLog2e = 1.4426950408889634f;
+
+// shared memory (from a 1024-aligned base): Q (32 KiB a row tile), the ring, then
+constexpr int slots_of(int form_b) { return form_b ? 5 : 6; }
+constexpr int kOffStat = 7 * kTile;                  // float2 [2][128]
+constexpr int kOffBars = kOffStat + 2 * 128 * 8;     // mbarriers
+constexpr int kOffMask = kOffBars + 384;             // uint4 [kAhead] live bits
+constexpr int kOffNf = kOffMask + kAhead * 16;            // uint4 [kNf]
+constexpr int kOffMisc = kOffNf + kNf * 16;          // TMEM address, flag, start of the range
+constexpr int kSmem = kOffMisc + 64;
+static_assert(kSmem <= 232448, "shared memory");
 
 struct Args {
-  int B, T, Hq, Hkv, S;
-  float scale;
-  const __nv_bfloat16 *q, *kc, *vc, *kd, *vd;
-  const int *parents, *slot_pos, *lens;
+  int B, T, Hq, Hkv, S, G;
+  int npt;    // nodes of a row tile
+  int pairs;  // units per (sequence, kv head)
+  float c;    // |scale| * log2(e), > 0
+  int neg;    // scale < 0
+  int grid;
   __nv_bfloat16* out;
-  float* score;  // [B][T][S + T] or null
+  const __nv_bfloat16* vd;
+  const int *parents, *slot_pos, *lens;
+  float* part;     // [grid][2][rows][128] partial accumulators, rows = 128 (form A) or 256
+  float2* pstat;   // [grid][2][rows] their maximum and sum(s)
+  float* lse;      // [B][T][Hq] log2 of the sum of weights, for the score (or null)
+  int* base;       // [B + 1] first key tile of each sequence (with lens)
   int* err;
 };
 
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&v)[4]) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  v[0] = bf16lo(w.x), v[1] = bf16hi(w.x), v[2] = bf16lo(w.y), v[3] = bf16hi(w.y);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-__global__ void __launch_bounds__(128) simple_kernel(Args a) {
+// Key tiles of sequence b: its cache's, and the drafted one.
+__device__ __forceinline__ int len_of(const Args& a, int b) {
+  if (!a.lens) return a.S;
+  const int n = a.lens[b];
+  return n < 0 ? 0 : n > a.S ? a.S : n;
+}
+__device__ __forceinline__ int tiles_of(int len) { return (len + kKeys - 1) / kKeys + 1; }
+
+// The nodes that node t sees (bits), none where it is unused.
+__device__ __forceinline__ bool node_sees(const int* par, int t, uint32_t (&sees)[4], int* err) {
+  sees[0] = sees[1] = sees[2] = sees[3] = 0;
+  for (;;) {
+    const int p = par[t];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((t >> 5) == i) sees[i] |= 1u << (t & 31);
+    if (p >= t || p < -1) {
+      if (p >= t) set_err(err, kErrIndex);
+      sees[0] = sees[1] = sees[2] = sees[3] = 0;
+      return false;
+    }
+    if (p < 0) return true;
+    t = p;
+  }
+}
+
+// A walk over the CTA's range of key tiles, unit by unit.
+struct Walk {
+  int t, end;        // global key tiles left: [t, end)
+  int b, base, len;  // sequence, its first tile, its length
+  int h, pair, tile0, n, nt;  // unit, first key tile of the segment, their number, tiles of the unit
+  int seg;
+  __device__ __forceinline__ void start(int t0, int t1, int b0, int base0) {
+    t = t0, end = t1, b = b0, base = base0, n = 0, seg = -1;
+  }
+  __device__ __forceinline__ bool next(const Args& a) {
+    t += n;
+    if (t >= end) return false;
+    const int per_head = a.pairs;
+    len = len_of(a, b);
+    nt = tiles_of(len);
+    while (t - base >= nt * a.Hkv * per_head) {
+      base += nt * a.Hkv * per_head;
+      ++b;
+      len = len_of(a, b);
+      nt = tiles_of(len);
+    }
+    const int rel = t - base, u = rel / nt;
+    tile0 = rel - u * nt;
+    h = u / per_head;
+    pair = u - h * per_head;
+    n = min(nt - tile0, end - t);
+    ++seg;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return n == nt; }
+};
+
+template <bool FormB, bool Score>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kdmap,
+                  const __grid_constant__ CUtensorMap vdmap, const Args a) {
+  extern __shared__ __align__(1024) uint8_t base[];
+  constexpr int NS = slots_of(FormB);
+  constexpr int NQ = FormB ? 2 : 1;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kOffBars);
+  uint64_t* kfull = bars;          // [kAhead] K landed
+  uint64_t* vfull = bars + 8;      // [kAhead] V landed
+  uint64_t* vok = bars + 16;       // [kAhead] the mask warp has cleaned the V tile
+  uint64_t* empty = bars + 24;     // [NS] ring slot: its product is done
+  uint64_t* sfull = bars + 30;     // [2] S written
+  uint64_t* pready = bars + 32;    // [2] P written (4 warps)
+  uint64_t* pvdone = bars + 34;    // [2] O += P V done
+  uint64_t* qfull = bars + 36;
+  uint64_t* qfree = bars + 37;
+  uint64_t* drain = bars + 38;     // after a wait that gave up
+  float2* stat = reinterpret_cast<float2*>(base + kOffStat);
+  uint4* masks = reinterpret_cast<uint4*>(base + kOffMask);
+  uint4* nfs = reinterpret_cast<uint4*>(base + kOffNf);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(base + kOffMisc);
+  volatile int* bad = reinterpret_cast<volatile int*>(misc + 1);
+  uint8_t* ring = base + NQ * kTile;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < 39; ++i) mbar_init(bars + i, (i == 32 || i == 33) ? 4 : 1);
+    *bad = 0;
+    if (smem_u32(base) & 1023) {  // the swizzle needs the base aligned
+      *bad = 1;
+      set_err(a.err, kErrWaitTimeout);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  // the range of key tiles, and the sequence that it starts in
+  if (warp == kProducer) {
+    const int per = a.Hkv * a.pairs;
+    int total, b0, base0;
+    // CTAs that share the tiles: no more than there are tiles
+    auto border = [&](int c) {
+      const int g = min(a.grid, total);
+      return c < g ? static_cast<int>(static_cast<long long>(total) * c / g) : total;
+    };
+    if (!a.lens) {
+      const int nt = tiles_of(a.S) * per;
+      total = nt * a.B;
+      const int t0 = border(blockIdx.x);
+      b0 = t0 / nt;
+      base0 = b0 * nt;
+    } else {
+      total = 0;
+      for (int i = 0; i < a.B; i += 32) {
+        int v = i + lane < a.B ? tiles_of(len_of(a, i + lane)) * per : 0;
+        if (i + lane < a.B && blockIdx.x == 0 && (a.lens[i + lane] < 0 || a.lens[i + lane] > a.S))
+          set_err(a.err, kErrIndex);
+        int incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        if (blockIdx.x == 0 && i + lane < a.B) a.base[i + lane] = total + incl - v;
+        total += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (blockIdx.x == 0 && lane == 0) a.base[a.B] = total;
+      const int t0 = border(blockIdx.x);
+      b0 = base0 = 0;
+      int run = 0;
+      for (int i = 0; i < a.B; i += 32) {
+        int v = i + lane < a.B ? tiles_of(len_of(a, i + lane)) * per : 0;
+        int incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, i + lane < a.B && run + incl - v <= t0);
+        if (hit) {
+          const int l = 31 - __clz(hit);
+          b0 = i + l;
+          base0 = run + __shfl_sync(0xffffffffu, incl - v, l);
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+        if (run > t0) break;
+      }
+    }
+    if (lane == 0) {
+      misc[2] = border(blockIdx.x);
+      misc[3] = border(blockIdx.x + 1);
+      misc[4] = b0;
+      misc[5] = base0;
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = misc[0];
+  Walk w;
+  w.start(misc[2], misc[3], misc[4], misc[5]);
+  const int n_tiles = w.end - w.t;
+  const int R = a.npt * a.G;
+
+  // A wait gives up after a while (or at once when another one has): the walk then runs to its end
+  // without touching data, so that every barrier of threads is still met.
+  auto wait = [&](uint64_t* bar, uint32_t ph) {
+    if (mbar_try_wait(bar, ph)) return;
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+      if (mbar_try_wait(bar, ph)) return;
+      if (*bad) return;
+      if (i > 1024) __nanosleep(32);
+    }
+    set_err(a.err, kErrWaitTimeout);
+    *bad = 1;
+  };
+  // ring position of the K / V tile of the CTA's j-th key tile
+  auto k_pos = [&](int j) { return FormB ? 2 * j : j ? 2 * j - 1 : 0; };
+  auto v_pos = [&](int j) { return FormB ? 2 * j + 1 : j + 1 < n_tiles ? 2 * j + 2 : 2 * j + 1; };
+
+  // the softmax threads hold a row of S each: registers move to them from the other warps
+  // (384 threads at 168 = 256 at 192 + 128 at 120)
+  if (warp >= kProducer) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+  if (warp == kProducer) {
+    // ================================ TMA ==============================================
+    if (lane == 0) {
+      prefetch_tmap(&qmap);
+      prefetch_tmap(&kmap);
+      prefetch_tmap(&vmap);
+      int k_issued = 0, v_issued = 0, q_issued = 0;
+      auto load = [&](const Walk& x, int tile, bool value, int j) {
+        const int pos = value ? v_pos(j) : k_pos(j), s = pos % NS;
+        if (pos >= NS) wait(&empty[s], (pos / NS - 1) & 1);
+        if (*bad) return;
+        (value ? v_issued : k_issued) = j + 1;
+        const bool drafted = tile == x.nt - 1;
+        const CUtensorMap* m = drafted ? (value ? &vdmap : &kdmap) : (value ? &vmap : &kmap);
+        const int y = drafted ? 0 : tile * kKeys, z = x.b * a.Hkv + x.h;
+        uint64_t* bar = (value ? vfull : kfull) + j % kAhead;
+        mbar_expect_tx(bar, kTile);
+        tma_load_3d(ring + s * kTile, m, bar, 0, y, z);
+        tma_load_3d(ring + s * kTile + kHalf, m, bar, 64, y, z);
+      };
+      Walk last = w;  // the unit and tile whose V is still to be loaded
+      int last_tile = -1, j = 0;
+      while (w.next(a)) {
+        if (w.seg > 0) wait(qfree, (w.seg - 1) & 1);
+        if (!*bad) {
+          q_issued = w.seg + 1;
+          mbar_expect_tx(qfull, NQ * 2 * R * 128);
+          for (int r = 0; r < NQ; ++r)
+            for (int hf = 0; hf < 2; ++hf)
+              tma_load_3d(base + r * kTile + hf * kHalf, &qmap, qfull, 64 * hf, w.h * a.G,
+                          w.b * a.T + (w.pair * NQ + r) * a.npt);
+        }
+        for (int i = 0; i < w.n; ++i, ++j) {
+          load(w, w.tile0 + i, false, j);
+          if (FormB) {
+            load(w, w.tile0 + i, true, j);
+          } else {
+            if (j > 0) load(last, last_tile, true, j - 1);
+            last = w;
+            last_tile = w.tile0 + i;
+          }
+        }
+      }
+      if (!FormB && j > 0) load(last, last_tile, true, j - 1);
+      if (*bad) {  // a wait has given up: the copies in flight land before the shared memory goes
+        for (int k = max(0, k_issued - NS); k < k_issued; ++k)
+          mbar_wait_bounded(&kfull[k % kAhead], (k / kAhead) & 1, 1u << 16);
+        for (int k = max(0, v_issued - NS); k < v_issued; ++k)
+          mbar_wait_bounded(&vfull[k % kAhead], (k / kAhead) & 1, 1u << 16);
+        if (q_issued) mbar_wait_bounded(qfull, (q_issued - 1) & 1, 1u << 16);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMma) {
+    // ================================ tensor cores =====================================
+    if (lane == 0) {
+      const uint32_t idS = tc_idesc(128, 128, 0), idO = tc_idesc(128, 128, 1);
+      // S of item i (key tile j of the CTA) into S_w; ``last_q``: the unit's last use of Q,
+      // ``last_k``: the last use of this K tile
+      auto issue_s = [&](int i, int j, bool last_q, bool last_k) {
+        const int x = i & 1, s = k_pos(j) % NS;
+        wait(&kfull[j % kAhead], (j / kAhead) & 1);
+        if (*bad) return;
+        tc_after();
+        const uint32_t q = smem_u32(base) + (FormB ? x * kTile : 0), k = smem_u32(ring + s * kTile);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          tc_mma(tmem + x * 128, tc_sdesc(q + off), tc_sdesc(k + off), idS, ks > 0);
+        }
+        tc_commit(&sfull[x]);
+        if (last_k) tc_commit(&empty[s]);
+        if (last_q) tc_commit(qfree);
+      };
+      auto issue_pv = [&](int i, int j, bool first, bool last_v) {
+        const int x = i & 1, s = v_pos(j) % NS;
+        wait(&vok[j % kAhead], (j / kAhead) & 1);
+        wait(&pready[x], (i >> 1) & 1);
+        if (*bad) return;
+        tc_after();
+        const uint32_t v = smem_u32(ring + s * kTile);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+          tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, tc_sdesc(v + ks * 16 * 128, kHalf, 1024), idO,
+                    !first || ks > 0);
+        tc_commit(&pvdone[x]);
+        if (last_v) tc_commit(&empty[s]);
+      };
+      // the S products run two items ahead of the P V products, over unit borders too
+      Walk ahead = w;
+      int ai = 0, aj = 0, left = 0, aw = 0;  // next S item, its key tile, tiles left in its unit, row tile
+      auto s_next = [&]() {
+        if (left == 0) {
+          if (!ahead.next(a)) return;
+          left = ahead.n;
+          aw = 0;
+          wait(qfull, ahead.seg & 1);
+        }
+        if (FormB) {
+          issue_s(ai, aj, left == 1 && aw == 1, aw == 1);
+          if (aw == 1) ++aj, --left;
+          aw ^= 1;
+        } else {
+          issue_s(ai, aj, left == 1, true);
+          ++aj, --left;
+        }
+        ++ai;
+      };
+      s_next();
+      s_next();
+      int i = 0, j = 0;
+      while (w.next(a)) {
+        const int items = FormB ? 2 * w.n : w.n;
+        for (int k = 0; k < items; ++k, ++i) {
+          issue_pv(i, j, k < 2, FormB ? (k & 1) == 1 : true);
+          if (!FormB || (k & 1)) ++j;
+          s_next();
+        }
+      }
+      if (*bad) {  // products in flight end before TMEM goes
+        tc_commit(drain);
+        mbar_wait_bounded(drain, 0, 1u << 16);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMask) {
+    // ================================ masks ============================================
+    int j = 0;
+    auto value = [&](const Walk& x, int tile, int j) {
+      const int s = v_pos(j) % NS;
+      const bool drafted = tile == x.nt - 1;
+      uint32_t m[4];
+      if (drafted) {
+        const int* par = a.parents + static_cast<size_t>(x.b) * a.T;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t sees[4];
+          const int t = i * 32 + lane;
+          m[i] = __ballot_sync(0xffffffffu, t < a.T && node_sees(par, t, sees, a.err));
+        }
+      } else {
+        int p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int sl = tile * kKeys + i * 32 + lane;
+          p[i] = sl < x.len ? (a.slot_pos ? a.slot_pos[static_cast<size_t>(x.b) * a.S + sl] : 0) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = __ballot_sync(0xffffffffu, p[i] >= 0);
+      }
+      wait(&vfull[j % kAhead], (j / kAhead) & 1);
+      uint8_t* v = ring + s * kTile;
+      if ((m[0] & m[1] & m[2] & m[3]) != 0xffffffffu) {
+        // 16 lanes a row: its two 128-byte halves
+        const int off = ((lane >> 3) & 1) * kHalf + (lane & 7) * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t dead = ~m[i];
+          if (lane >= 16) dead >>= 16;
+          for (int r = 0; r < 16; ++r)
+            if ((dead >> r) & 1u)
+              *reinterpret_cast<uint4*>(v + (i * 32 + (lane & 16) + r) * 128 + off) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (drafted) {
+        // elements that are not finite (exponent all ones) leave the product; nf: their nodes
+        uint32_t nf[4] = {0, 0, 0, 0};
+        __syncwarp();
+        const int off = ((lane >> 3) & 1) * kHalf + (lane & 7) * 16;
+        for (int r = 0; r < a.T; r += 2) {
+          const int row = r + (lane >> 4);
+          uint32_t hit = 0;
+          if (row < a.T) {
+            uint4* at = reinterpret_cast<uint4*>(v + row * 128 + off);
+            uint4 x4 = *at;
+            uint32_t* wd = reinterpret_cast<uint32_t*>(&x4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((wd[i] & 0x7F80u) == 0x7F80u) wd[i] &= 0xFFFF0000u, hit = 1;
+              if ((wd[i] & 0x7F800000u) == 0x7F800000u) wd[i] &= 0xFFFFu, hit = 1;
+            }
+            if (hit) *at = x4;
+          }
+          const uint32_t vote = __ballot_sync(0xffffffffu, hit);
+          if (vote & 0xffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((r >> 5) == i) nf[i] |= 1u << (r & 31);
+          }
+          if (vote >> 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (((r + 1) >> 5) == i) nf[i] |= 1u << ((r + 1) & 31);
+          }
+        }
+        if (lane == 0) nfs[x.seg % kNf] = make_uint4(nf[0], nf[1], nf[2], nf[3]);
+      }
+      if (lane == 0) masks[j % kAhead] = make_uint4(m[0], m[1], m[2], m[3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vok[j % kAhead]);
+    };
+    while (w.next(a))
+      for (int i = 0; i < w.n; ++i, ++j) value(w, w.tile0 + i, j);
+  }
+  } else {
+    // ================================ softmax ==========================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int x = warp >> 2;                 // accumulator: items i with i & 1 == x
+    const int row = (warp & 3) * 32 + lane;  // TMEM lane = row of the row tile
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + x * 128 + lanes;
+    const bool mine = row < R;
+    const bool idle = (warp & 3) * 32 >= R;  // no row of this warp is in use
+    const float NEG_INF = -__int_as_float(0x7f800000);
+    const float c = a.c;
+    int i = 0, j = 0;  // the CTA's items and key tiles so far
+    int done = 0;      // items of this accumulator so far
+    while (w.next(a)) {
+      const int rt = FormB ? w.pair * 2 + x : 0;      // row tile
+      const int node = rt * a.npt + row / a.G;
+      const bool in = mine && node < a.T;
+      uint32_t sees[4] = {0, 0, 0, 0};
+      const bool has_draft = w.tile0 + w.n == w.nt;
+      bool used = false;
+      if (in) used = node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
+      float m = NEG_INF, l = 0.f, lx = 0.f;
+      int mine_n = 0;  // items of this accumulator in this unit
+      const int items = FormB ? 2 * w.n : w.n;
+      for (int k = 0; k < items; ++k, ++i) {
+        const int jt = j;
+        if (!FormB || (k & 1)) ++j;
+        if ((i & 1) != x) continue;
+        const bool drafted = has_draft && (FormB ? k >> 1 : k) == w.n - 1;
+        wait(&sfull[x], done & 1);
+        wait(&vok[jt % kAhead], (jt / kAhead) & 1);
+        tc_after();
+        uint32_t s[4][32];
+        if (!idle && !*bad) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tc_ld32_raw(tS + q * 32, s[q]);
+          tc_wait_ld();
+          uint4 mk = masks[jt % kAhead];
+          if (drafted) mk = make_uint4(sees[0], sees[1], sees[2], sees[3]);
+          const uint32_t mw[4] = {mk.x, mk.y, mk.z, mk.w};
+          if (a.neg) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[q][e] ^= 0x80000000u;
+          }
+          if (!__all_sync(0xffffffffu, (mw[0] & mw[1] & mw[2] & mw[3]) == 0xffffffffu)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[q][e] = ((mw[q] >> e) & 1u) ? s[q][e] : 0xff800000u;
+          }
+          float top[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float t0 = __uint_as_float(s[q][0]), t1 = __uint_as_float(s[q][1]);
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) {
+              t0 = fmaxf(t0, __uint_as_float(s[q][e]));
+              t1 = fmaxf(t1, __uint_as_float(s[q][e + 1]));
+            }
+            top[q] = fmaxf(t0, t1);
+          }
+          const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          const bool move = in && tm > m && !((tm - m) * c <= 8.f);
+          if (__any_sync(0xffffffffu, move)) {
+            const float f = move ? (m == NEG_INF ? 0.f : ex2((m - tm) * c)) : 1.f;
+            if (move) m = tm;
+            l *= f;
+            if (Score) lx *= f;
+            if (mine_n > 0) {
+              wait(&pvdone[x], (done - 1) & 1);
+              tc_after();
+              if (!*bad) {
+#pragma unroll 1
+                for (int q = 0; q < 8; ++q) {
+                  uint32_t o[16];
+                  tc_ld16_raw(tmem + 256 + x * 128 + lanes + q * 16, o);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tc_st16(tmem + 256 + x * 128 + lanes + q * 16, o);
+                }
+                tc_wait_st();
+              }
+            }
+          }
+          const float mc = (m == NEG_INF ? 0.f : m) * c;
+          float add[4] = {0.f, 0.f, 0.f, 0.f}, addx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(s[q][e]), c, -mc));
+              const float p1 = ex2(fmaf(__uint_as_float(s[q][e + 1]), c, -mc));
+              uint32_t pk;
+              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk) : "f"(p1), "f"(p0));
+              add[q] += __uint_as_float(pk << 16) + __uint_as_float(pk & 0xFFFF0000u);
+              if (Score) addx[q] += p0 + p1;
+              s[q >> 1][(q & 1) * 16 + e / 2] = pk;
+            }
+          l += (add[0] + add[1]) + (add[2] + add[3]);
+          if (Score) lx += (addx[0] + addx[1]) + (addx[2] + addx[3]);
+          tc_st32(tS, s[0]);
+          tc_st32(tS + 32, s[1]);
+          tc_wait_st();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[x]);
+        ++done;
+        ++mine_n;
+      }
+      // ---- the unit's rows: accumulators in TMEM, statistics in the threads
+      if (mine_n > 0) wait(&pvdone[x], (done - 1) & 1);
+      float f0 = 1.f, f1 = 0.f, M = m, L = l, Lx = lx;
+      if (!FormB) {
+        // the two accumulators of a row lie in the same TMEM lane: both warpgroups join them, each
+        // for half the dims
+        if (x == 1) stat[row] = make_float2(m, l), stat[128 + row].x = lx;
+        named_bar(1, 256);
+        if (x == 0) {
+          const float2 o = stat[row];
+          const float ox = stat[128 + row].x;
+          M = fmaxf(m, o.x);
+          f0 = m == NEG_INF ? 0.f : ex2((m - M) * c);
+          f1 = o.x == NEG_INF ? 0.f : ex2((o.x - M) * c);
+          L = f0 * l + f1 * o.y;
+          Lx = f0 * lx + f1 * ox;
+          if (M != M || L != L) f0 = f1 = 1.f;  // a NaN logit: the accumulators hold NaN too
+          stat[row] = make_float2(f0, f1);
+          stat[128 + row] = make_float2(M, L);
+        }
+        named_bar(2, 256);
+        if (x == 1) {
+          const float2 o = stat[row], p = stat[128 + row];
+          f0 = o.x, f1 = o.y, M = p.x, L = p.y;
+        }
+      }
+      tc_after();
+      if (!idle && !*bad) {
+        const size_t orow = (static_cast<size_t>(w.b) * a.T + node) * a.Hq + static_cast<size_t>(w.h) * a.G + row % a.G;
+        const bool whole = w.whole();
+        const int rows = FormB ? 256 : 128;
+        const int prow = FormB ? x * 128 + row : row;
+        const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
+        float* part = a.part + (slot * rows + prow) * kD;
+        if (in && (FormB || x == 0)) {
+          if (!whole) {
+            a.pstat[slot * rows + prow] = make_float2(M, L);
+            if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
+          } else if (Score) {
+            a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
+          }
+        }
+        const float inv = whole ? 1.f / L : 1.f;
+        uint4 nf4 = has_draft ? nfs[w.seg % kNf] : make_uint4(0, 0, 0, 0);
+        const bool odd = in && ((nf4.x & sees[0]) | (nf4.y & sees[1]) | (nf4.z & sees[2]) | (nf4.w & sees[3]));
+        constexpr int kChunks = FormB ? 4 : 2;
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q) {
+          const int d0 = (FormB ? 0 : x * 64) + q * 32;
+          float o[32];
+          if (FormB) {
+            uint32_t r0[32];
+            tc_ld32_raw(tmem + 256 + x * 128 + lanes + d0, r0);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r0[e]) * inv;
+          } else {
+            uint32_t r0[32], r1[32];
+            tc_ld32_raw(tmem + 256 + lanes + d0, r0);
+            tc_ld32_raw(tmem + 384 + lanes + d0, r1);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float v0 = f0 > 0.f ? __uint_as_float(r0[e]) * f0 : 0.f;
+              const float v1 = f1 > 0.f ? __uint_as_float(r1[e]) * f1 : 0.f;
+              o[e] = (v0 + v1) * inv;
+            }
+          }
+          if (odd) {
+            for (int t = 0; t < a.T; ++t) {
+              const uint32_t nw = t < 32 ? nf4.x & sees[0] : t < 64 ? nf4.y & sees[1] : t < 96 ? nf4.z & sees[2] : nf4.w & sees[3];
+              if (!((nw >> (t & 31)) & 1u)) continue;
+              const __nv_bfloat16* v = a.vd + ((static_cast<size_t>(w.b) * a.Hkv + w.h) * a.T + t) * kD + d0;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float y = __bfloat162float(v[e]);
+                if (!(fabsf(y) <= 3.4e38f)) o[e] += y;
+              }
+            }
+          }
+          if (in) {
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(a.out + orow * kD + d0);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t pk[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  pk[z] = used ? pack_bf16(o[e * 8 + 2 * z], o[e * 8 + 2 * z + 1]) : 0u;
+                dst[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              }
+            } else {
+              float4* dst = reinterpret_cast<float4*>(part + d0);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+          }
+        }
+      }
+      tc_before();
+      // both halves of a row are read before either accumulator is written again
+      if (!FormB) named_bar(3, 256);
+    }
+  }
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// Joins the parts of units that a border cut: a warp per output row.
+template <bool FormB, bool Score>
+__global__ void __launch_bounds__(256) combine_kernel(const Args a) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), t = blockIdx.y, b = blockIdx.z;
-  if (h >= a.Hq) return;
-  const int g = h / (a.Hq / a.Hkv);
-  const int* par = a.parents + static_cast<size_t>(b) * a.T;
-  const size_t row = ((static_cast<size_t>(b) * a.T + t) * a.Hq + h) * kD + lane * 4;
-  // the node and its ancestors
-  uint32_t sees[kMaxNodes / 32] = {};
-  bool used = true;
-  for (int j = t, n = 0;; ++n) {
-    const int p = par[j];
-    sees[j >> 5] |= 1u << (j & 31);
-    if (p >= j || p < -1) {
-      used = false;
-      if (p >= j && lane == 0) set_err(a.err, kErrIndex);
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= static_cast<long long>(a.B) * a.T * a.Hq) return;
+  const int h = static_cast<int>(row % a.Hq);
+  const int t = static_cast<int>(row / a.Hq % a.T), b = static_cast<int>(row / a.Hq / a.T);
+  const int rt = t / a.npt, pair = FormB ? rt >> 1 : 0, u = h / a.G * a.pairs + pair;
+  const int nt = tiles_of(len_of(a, b)), per = a.Hkv * a.pairs;
+  const long long total = a.lens ? a.base[a.B] : static_cast<long long>(nt) * per * a.B;
+  const long long t0 = (a.lens ? a.base[b] : static_cast<long long>(nt) * per * b) + static_cast<long long>(u) * nt;
+  const long long g = total < a.grid ? total : a.grid;
+  const int c0 = static_cast<int>(((t0 + 1) * g - 1) / total);
+  const int c1 = static_cast<int>(((t0 + nt) * g - 1) / total);
+  if (c0 == c1) return;  // written by the CTA that had it all
+  const int rows = FormB ? 256 : 128;
+  const int prow = (FormB ? (rt & 1) * 128 : 0) + (t - rt * a.npt) * a.G + h % a.G;
+  auto slot_of = [&](int c) {
+    const bool later = c == c0 && total * c0 / g < t0;  // the unit is not the CTA's first
+    return (static_cast<size_t>(c) * 2 + (later ? 1 : 0)) * rows + prow;
+  };
+  const float NEG_INF = -__int_as_float(0x7f800000);
+  float M = NEG_INF;
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.pstat[slot_of(c)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float* exact = reinterpret_cast<const float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows);
+  float L = 0.f, Lx = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const size_t s = slot_of(c);
+    const float2 st = a.pstat[s];
+    const float f = st.x == NEG_INF ? 0.f : ex2((st.x - M) * a.c);
+    const float4 v = reinterpret_cast<const float4*>(a.part + s * kD)[lane];
+    if (st.x != NEG_INF) {
+      L = fmaf(f, st.y, L);
+      if (Score) Lx = fmaf(f, exact[s], Lx);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
     }
-    if (!used || p < 0) break;
-    j = p;
   }
-  int len = a.lens ? a.lens[b] : a.S;
-  if (len < 0 || len > a.S) {
-    if (lane == 0) set_err(a.err, kErrIndex);
-    len = len < 0 ? 0 : a.S;
-  }
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-  if (used) {
-    float q[4];
-    load4(a.q + row, q);
-    float m = -__int_as_float(0x7f800000), l = 0.f;
-    const size_t head = static_cast<size_t>(b) * a.Hkv + g;
-    auto live = [&](int s) {
-      return s < a.S ? s < len && (!a.slot_pos || a.slot_pos[static_cast<size_t>(b) * a.S + s] >= 0)
-                     : ((sees[(s - a.S) >> 5] >> ((s - a.S) & 31)) & 1u) != 0;
-    };
-    auto dot = [&](int s) {
-      float k[4];
-      load4((s < a.S ? a.kc + (head * a.S + s) * kD : a.kd + (head * a.T + (s - a.S)) * kD) + lane * 4, k);
-      float d = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-      for (int x = 16; x; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-      return d * a.scale;
-    };
-    for (int s = 0; s < a.S + a.T; ++s) {
-      if (!live(s)) continue;
-      const float d = dot(s);
-      const float mn = fmaxf(m, d), c = expf(m - mn), p = expf(d - mn);
-      float v[4];
-      load4((s < a.S ? a.vc + (head * a.S + s) * kD : a.vd + (head * a.T + (s - a.S)) * kD) + lane * 4, v);
-      l = l * c + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * c + p * v[i];
-      m = mn;
+  uint32_t sees[4];
+  const bool used = node_sees(a.parents + static_cast<size_t>(b) * a.T, t, sees, nullptr);
+  const float inv = 1.f / L;
+  reinterpret_cast<uint2*>(a.out + row * kD)[lane] =
+      used ? make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv)) : make_uint2(0, 0);
+  if (Score && lane == 0) a.lse[row] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
+}
+
+// ------------------------------------------------------------------------------------
+// score: S^T = K . Q^T, a slot per TMEM lane; every thread keeps its slot's largest weight of each
+// node over the heads in shared memory, and the CTA max-accumulates it into the score at the end.
+// ------------------------------------------------------------------------------------
+constexpr int kScoreThreads = 9 * 32;  // 8 warps over the columns, one for TMA and MMA
+constexpr int kScoreBuf = 2 * kTile;   // K and Q of one head
+constexpr int kScOffMax = 2 * kScoreBuf;                    // float [128 nodes][128 slots]
+constexpr int kScOffLse = kScOffMax + kMaxNodes * 128 * 4;  // float [2][128]
+constexpr int kScOffSee = kScOffLse + 2 * 128 * 4;          // uint4 [128]
+constexpr int kScOffBars = kScOffSee + kMaxNodes * 16;
+constexpr int kScSmem = kScOffBars + 128;
+static_assert(kScSmem <= 232448, "shared memory");
+
+struct ScoreArgs {
+  Args a;
+  float* score;  // [B][T][S + T]
+  int tiles;     // key tiles of a sequence: ceil(S / 128) + 1
+  int hsplit;    // groups of kv heads
+  int npt;       // nodes of a column tile (their rows: at most 128)
+};
+
+__global__ void __launch_bounds__(kScoreThreads, 1)
+    score_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap kdmap, const ScoreArgs p) {
+  extern __shared__ __align__(1024) uint8_t base[];
+  const Args& a = p.a;
+  float* best = reinterpret_cast<float*>(base + kScOffMax);
+  float* slse = reinterpret_cast<float*>(base + kScOffLse);
+  uint4* see = reinterpret_cast<uint4*>(base + kScOffSee);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kScOffBars);
+  uint64_t* full = bars;       // [2] K and Q landed
+  uint64_t* sfull = bars + 2;  // [2] S^T written
+  uint64_t* sfree = bars + 4;  // [2] S^T read by the 8 warps
+  uint64_t* drain = bars + 6;  // after a wait that gave up
+  uint32_t* misc = reinterpret_cast<uint32_t*>(bars + 8);
+  volatile int* bad = reinterpret_cast<volatile int*>(misc + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = blockIdx.x, hg = blockIdx.y, b = blockIdx.z;
+  const bool drafted = tile == p.tiles - 1;
+  const int h0 = hg * a.Hkv / p.hsplit, h1 = (hg + 1) * a.Hkv / p.hsplit;
+  if (tid == 0) {
+    for (int i = 0; i < 7; ++i) mbar_init(bars + i, i == 4 || i == 5 ? 8 : 1);
+    *bad = 0;
+    if (smem_u32(base) & 1023) {
+      *bad = 1;
+      set_err(a.err, kErrWaitTimeout);
     }
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  if (drafted)
+    for (int t = tid; t < a.T; t += kScoreThreads) {
+      uint32_t s[4];
+      node_sees(a.parents + static_cast<size_t>(b) * a.T, t, s, nullptr);
+      see[t] = make_uint4(s[0], s[1], s[2], s[3]);
+    }
+  for (int i = tid; i < a.T * 128; i += kScoreThreads) best[i] = 0.f;
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = misc[0];
+  const int len = len_of(a, b);
+  const bool any = drafted || tile * kKeys < len;
+  const int chunks = (a.T + p.npt - 1) / p.npt;
+  const int items = any ? chunks * (h1 - h0) : 0;
+  auto wait = [&](uint64_t* bar, uint32_t ph) {
+    if (mbar_try_wait(bar, ph)) return;
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+      if (mbar_try_wait(bar, ph)) return;
+      if (*bad) return;
+      if (i > 1024) __nanosleep(32);
+    }
+    set_err(a.err, kErrWaitTimeout);
+    *bad = 1;
+  };
+  if (warp == 8) {
+    if (lane == 0) {
+      const int R = p.npt * a.G;
+      const uint32_t id = tc_idesc(128, (R + 15) / 16 * 16, 0);
+      int loaded = 0;
+      auto load = [&](int i) {
+        loaded = i + 1;
+        const int x = i & 1, h = h0 + i % (h1 - h0), n0 = i / (h1 - h0) * p.npt;
+        uint8_t* k = base + x * kScoreBuf;
+        const CUtensorMap* m = drafted ? &kdmap : &kmap;
+        const int y = drafted ? 0 : tile * kKeys, z = b * a.Hkv + h;
+        mbar_expect_tx(&full[x], kTile + 2 * R * 128);
+        for (int hf = 0; hf < 2; ++hf) {
+          tma_load_3d(k + hf * kHalf, m, &full[x], 64 * hf, y, z);
+          tma_load_3d(k + kTile + hf * kHalf, &qmap, &full[x], 64 * hf, h * a.G, b * a.T + n0);
+        }
+      };
+      if (items > 0 && !*bad) load(0);
+      if (items > 1 && !*bad) load(1);
+      for (int i = 0; i < items; ++i) {
+        const int x = i & 1;
+        wait(&full[x], (i >> 1) & 1);
+        if (i >= 2) wait(&sfree[x], ((i >> 1) - 1) & 1);
+        if (*bad) break;
+        tc_after();
+        const uint32_t k = smem_u32(base + x * kScoreBuf);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] /= l;
-    if (a.score) {
-      float* sc = a.score + (static_cast<size_t>(b) * a.T + t) * (static_cast<size_t>(a.S) + a.T);
-      for (int s = 0; s < a.S + a.T; ++s) {
-        if (!live(s)) continue;
-        const float p = expf(dot(s) - m) / l;
-        if (lane == 0) atomicMax(reinterpret_cast<int*>(sc + s), __float_as_int(p));
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          tc_mma(tmem + x * 128, tc_sdesc(k + off), tc_sdesc(k + kTile + off), id, ks > 0);
+        }
+        tc_commit(&sfull[x]);
+        if (i + 2 < items) {
+          wait(&sfull[x], (i >> 1) & 1);  // the product has read the buffers
+          if (!*bad) load(i + 2);
+        }
+      }
+      if (*bad) {  // copies and products in flight end before their memory goes
+        tc_commit(drain);
+        mbar_wait_bounded(drain, 0, 1u << 16);
+        for (int i = loaded > 2 ? loaded - 2 : 0; i < loaded; ++i) mbar_wait_bounded(&full[i & 1], (i >> 1) & 1, 1u << 16);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int sl = (warp & 3) * 32 + lane, part = warp >> 2;  // slot; half of the nodes
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int key = tile * kKeys + sl;
+    const bool live = drafted ? sl < a.T
+                              : key < len && (!a.slot_pos || a.slot_pos[static_cast<size_t>(b) * a.S + key] >= 0);
+    for (int i = 0; i < items; ++i) {
+      const int x = i & 1, h = h0 + i % (h1 - h0), n0 = i / (h1 - h0) * p.npt;
+      const int nodes = min(p.npt, a.T - n0), cols = nodes * a.G;
+      named_bar(1, 256);  // the previous item's statistics have been read
+      for (int r = tid; r < cols; r += 256)
+        slse[r] = a.lse[(static_cast<size_t>(b) * a.T + n0 + r / a.G) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G];
+      wait(&sfull[x], (i >> 1) & 1);
+      named_bar(2, 256);
+      tc_after();
+      if (!*bad) {
+        // this warp's nodes [lo, hi), their columns in chunks of 16
+        const int lo = part * ((nodes + 1) / 2), hi = min(nodes, lo + (nodes + 1) / 2);
+        int node = lo, g = 0;
+        float mx = 0.f;
+        for (int c0 = lo * a.G; c0 < hi * a.G; c0 += 16) {
+          float v[16];
+          tc_ld16(tmem + x * 128 + lanes + c0, v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (c0 + e < hi * a.G) {
+              const float s = a.neg ? -v[e] : v[e];
+              mx = fmaxf(mx, ex2(fmaf(s, a.c, -slse[c0 + e])));
+              if (++g == a.G) {
+                const int t = n0 + node;
+                float* at = best + t * 128 + sl;
+                *at = fmaxf(*at, mx);
+                g = 0, mx = 0.f, ++node;
+              }
+            }
+          }
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sfree[x]);
+    }
+    // (the nodes' halves depend on the column tile: wait for both)
+    named_bar(1, 256);
+    if (live && any && !*bad) {
+      for (int t = part; t < a.T; t += 2) {
+        if (drafted) {
+          const uint4 m = see[t];
+          const uint32_t w = sl < 32 ? m.x : sl < 64 ? m.y : sl < 96 ? m.z : m.w;
+          if (!((w >> (sl & 31)) & 1u)) continue;
+        }
+        const float v = best[t * 128 + sl];
+        if (v > 0.f)
+          atomicMax(reinterpret_cast<int*>(p.score + (static_cast<size_t>(b) * a.T + t) * (static_cast<size_t>(a.S) + a.T) +
+                                           (drafted ? a.S : tile * kKeys) + sl),
+                    __float_as_int(v));
       }
     }
   }
-  *reinterpret_cast<uint2*>(a.out + row) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 }  // namespace ta
+
+// ------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------
+namespace {
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+// [d2][d1][128] bf16 rows, boxes of 64 columns x b1 x b2
+int map_rows(CUtensorMap* m, const void* ptr, long long d1, long long d2, int b1, int b2) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return fail(kStatusCuda, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(d1), static_cast<cuuint64_t>(d2)};
+  cuuint64_t strides[2] = {256, static_cast<cuuint64_t>(d1) * 256};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(b1), static_cast<cuuint32_t>(b2)};
+  cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(kStatusCuda, "tree_attn: tensor map failed (%d)", static_cast<int>(r));
+  return kStatusOk;
+}
+
+struct Plan {
+  int form_b, npt, pairs, rows;
+};
+
+// Row tiles of whole nodes, at most 128 rows each: one (form A), or an even number of equal ones.
+Plan plan_of(int T, int G) {
+  const int cap = 128 / G;
+  Plan p;
+  p.form_b = T > cap;
+  const int tiles = p.form_b ? 2 * ((T + 2 * cap - 1) / (2 * cap)) : 1;
+  p.npt = (T + tiles - 1) / tiles;
+  p.pairs = p.form_b ? tiles / 2 : 1;
+  p.rows = p.form_b ? 256 : 128;
+  return p;
+}
+
+constexpr int kMaxGrid = 148;  // workspace is sized for a whole B200
+
+struct Work {
+  long long part, pstat, lse, base, bytes;
+};
+Work work_of(int B, int T, int Hq, const Plan& p) {
+  auto up = [](long long x) { return (x + 255) / 256 * 256; };
+  Work w;
+  w.part = 0;
+  w.pstat = up(w.part + 2LL * kMaxGrid * p.rows * 512);
+  w.lse = up(w.pstat + 2LL * kMaxGrid * p.rows * 12);
+  w.base = up(w.lse + static_cast<long long>(B) * T * Hq * 4);
+  w.bytes = up(w.base + (static_cast<long long>(B) + 1) * 4);
+  return w;
+}
+
+}  // namespace
 }  // namespace kvbp
 
 #include "../../include/kvbp.h"
 
 extern "C" int64_t kvbp_tree_attn_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t S,
                                             int32_t with_score) {
-  (void)B, (void)T, (void)Hq, (void)Hkv, (void)S, (void)with_score;
-  return 0;
+  (void)S, (void)with_score;
+  if (B <= 0 || T <= 0 || T > kvbp::ta::kMaxNodes || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128) return 0;
+  return kvbp::work_of(B, T, Hq, kvbp::plan_of(T, Hq / Hkv)).bytes;
 }
 
 extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t head_dim,
@@ -111,19 +1027,100 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
                               const int32_t* lens, float scale, void* out, float* node_score, void* workspace,
                               int64_t workspace_bytes, int32_t* dev_err) {
   using namespace kvbp;
-  (void)workspace, (void)workspace_bytes;
+  using namespace kvbp::ta;
   if (!q || !k_draft || !v_draft || !parents || !out || (S > 0 && (!kcache || !vcache)))
     return fail(kStatusArg, "tree_attn: null pointer");
-  if (head_dim != ta::kD) return fail(kStatusUnsupported, "tree_attn: head_dim %d unsupported (only 128)", head_dim);
+  if (head_dim != kD) return fail(kStatusUnsupported, "tree_attn: head_dim %d unsupported (only 128)", head_dim);
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || S < 0 || B > 65535) return fail(kStatusArg, "tree_attn: bad size");
-  if (T <= 0 || T > ta::kMaxNodes) return fail(kStatusUnsupported, "tree_attn: %d nodes (1 to %d)", T, ta::kMaxNodes);
-  ta::Args a{B, T, Hq, Hkv, S, scale,
-             static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(kcache),
-             static_cast<const __nv_bfloat16*>(vcache), static_cast<const __nv_bfloat16*>(k_draft),
-             static_cast<const __nv_bfloat16*>(v_draft), parents, slot_pos, lens, static_cast<__nv_bfloat16*>(out),
-             node_score, dev_err};
-  ta::simple_kernel<<<dim3((Hq + 3) / 4, T, B), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  cudaError_t e = cudaGetLastError();
+  if (T <= 0 || T > kMaxNodes) return fail(kStatusUnsupported, "tree_attn: %d nodes (1 to %d)", T, kMaxNodes);
+  const int G = Hq / Hkv;
+  if (G > 128) return fail(kStatusUnsupported, "tree_attn: %d query heads per kv head (at most 128)", G);
+  if (!(scale == scale) || scale - scale != 0.f) return fail(kStatusArg, "tree_attn: scale is not finite");
+  if (misaligned(q, 16) || misaligned(kcache, 16) || misaligned(vcache, 16) || misaligned(k_draft, 16) ||
+      misaligned(v_draft, 16) || misaligned(out, 16) || misaligned(workspace, 16))
+    return fail(kStatusArg, "tree_attn: q, caches, drafts, out and workspace must be 16-byte aligned");
+  const Plan p = plan_of(T, G);
+  const long long tiles = (static_cast<long long>(S) + kKeys - 1) / kKeys + 1;
+  const long long total = tiles * B * Hkv * p.pairs;
+  if (total > 0x7fffffffLL || static_cast<long long>(B) * Hkv > 0x7fffffffLL ||
+      static_cast<long long>(B) * T * Hq > 0x7fffffffLL || S > 0x7fffffff - 1024)
+    return fail(kStatusArg, "tree_attn: too many keys or rows for one call");
+  const Work wk = work_of(B, T, Hq, p);
+  if (!workspace || workspace_bytes < wk.bytes)
+    return fail(kStatusArg, "tree_attn: a workspace of %lld bytes is needed", wk.bytes);
+  const long long nq = static_cast<long long>(B) * T * Hq * 256, nc = static_cast<long long>(B) * Hkv * S * 256,
+                  nd = static_cast<long long>(B) * Hkv * T * 256,
+                  ns = node_score ? static_cast<long long>(B) * T * (static_cast<long long>(S) + T) * 4 : 0;
+  const struct {
+    const void* p;
+    long long n;
+  } in[] = {{q, nq}, {kcache, nc}, {vcache, nc}, {k_draft, nd}, {v_draft, nd}, {parents, 4LL * B * T},
+            {slot_pos, slot_pos ? 4LL * B * S : 0}, {lens, lens ? 4LL * B : 0}},
+    written[] = {{out, nq}, {node_score, ns}, {workspace, wk.bytes}};
+  for (int i = 0; i < 3; ++i) {
+    for (const auto& r : in)
+      if (r.n && written[i].n && overlap(written[i].p, written[i].n, r.p, r.n))
+        return fail(kStatusArg, "tree_attn: an output or the workspace overlaps an input");
+    for (int k = 0; k < i; ++k)
+      if (written[i].n && written[k].n && overlap(written[i].p, written[i].n, written[k].p, written[k].n))
+        return fail(kStatusArg, "tree_attn: out, node_score and workspace overlap");
+  }
+  CUtensorMap qm, km, vm, kdm, vdm;
+  int st;
+  if ((st = map_rows(&qm, q, Hq, static_cast<long long>(B) * T, G, p.npt))) return st;
+  if ((st = map_rows(&kdm, k_draft, T, static_cast<long long>(B) * Hkv, kKeys, 1))) return st;
+  if ((st = map_rows(&vdm, v_draft, T, static_cast<long long>(B) * Hkv, kKeys, 1))) return st;
+  km = kdm, vm = vdm;  // never read without a cache
+  if (S > 0) {
+    if ((st = map_rows(&km, kcache, S, static_cast<long long>(B) * Hkv, kKeys, 1))) return st;
+    if ((st = map_rows(&vm, vcache, S, static_cast<long long>(B) * Hkv, kKeys, 1))) return st;
+  }
+  const bool score = node_score != nullptr;
+  auto kernel = p.form_b ? (score ? attend_kernel<true, true> : attend_kernel<true, false>)
+                         : (score ? attend_kernel<false, true> : attend_kernel<false, false>);
+  const int sms = prepare_device(reinterpret_cast<const void*>(kernel), kSmem);
+  if (!sms) return fail(kStatusCuda, "tree_attn: no usable device");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Args a{};
+  a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.S = S, a.G = G;
+  a.npt = p.npt, a.pairs = p.pairs;
+  a.neg = scale < 0.f;
+  a.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  const int most = sms < kMaxGrid ? sms : kMaxGrid;
+  a.grid = static_cast<int>(total < most ? total : most);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.vd = static_cast<const __nv_bfloat16*>(v_draft);
+  a.parents = parents, a.slot_pos = S > 0 ? slot_pos : nullptr, a.lens = lens;
+  a.part = reinterpret_cast<float*>(ws + wk.part);
+  a.pstat = reinterpret_cast<float2*>(ws + wk.pstat);
+  a.lse = reinterpret_cast<float*>(ws + wk.lse);
+  a.base = reinterpret_cast<int*>(ws + wk.base);
+  a.err = dev_err;
+  cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(kThreads), kSmem, cs, dim3(0), qm, km, vm, kdm, vdm, a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn launch: %s", cudaGetErrorString(e));
+  const long long rows = static_cast<long long>(B) * T * Hq;
+  auto join = p.form_b ? (score ? combine_kernel<true, true> : combine_kernel<true, false>)
+                       : (score ? combine_kernel<false, true> : combine_kernel<false, false>);
+  e = launch_pdl(join, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, cs, dim3(0), a);
+  if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn join launch: %s", cudaGetErrorString(e));
+  if (score) {
+    ScoreArgs sa{};
+    sa.a = a;
+    sa.score = node_score;
+    sa.tiles = static_cast<int>(tiles);
+    const long long units = tiles * B;
+    long long hs = (2LL * sms + units - 1) / units;
+    sa.hsplit = static_cast<int>(hs < 1 ? 1 : hs > Hkv ? Hkv : hs);
+    if (sa.hsplit > 65535) sa.hsplit = 65535;
+    sa.npt = T < 128 / G ? T : 128 / G;
+    CUtensorMap sqm;
+    if ((st = map_rows(&sqm, q, Hq, static_cast<long long>(B) * T, G, sa.npt))) return st;
+    if (!prepare_device(reinterpret_cast<const void*>(score_kernel), kScSmem))
+      return fail(kStatusCuda, "tree_attn: no usable device");
+    e = launch_pdl(score_kernel, dim3(static_cast<unsigned>(tiles), sa.hsplit, B), dim3(kScoreThreads), kScSmem, cs,
+                   dim3(0), sqm, km, kdm, sa);
+    if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn score launch: %s", cudaGetErrorString(e));
+  }
   return kStatusOk;
 }
