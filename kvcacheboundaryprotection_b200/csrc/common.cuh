@@ -295,6 +295,18 @@ __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t da, uint64_t db
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
       "l"(da), "l"(db), "r"(id), "r"(acc));
 }
+// True in one thread of the (converged) warp.  Code under it is known to run in a single thread, so
+// that the operands of tcgen05 and TMA instructions go to uniform registers without a search for
+// differing lanes, which ``lane == 0`` costs at every instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
 // D (TMEM) = A (TMEM: lane = row, 16-bit pairs along the columns) . B (+ D when acc != 0)
 __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t id, uint32_t acc) {
   asm volatile(

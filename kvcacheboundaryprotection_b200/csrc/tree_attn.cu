@@ -50,9 +50,9 @@ constexpr int kNf = 8;  // units' records of non-finite drafted values kept at a
 constexpr float kLog2e = 1.4426950408889634f;
 
 // shared memory (from a 1024-aligned base): Q (32 KiB a row tile), the ring, then
-constexpr int slots_of(int form_b) { return form_b ? 5 : 6; }
-constexpr int kOffStat = 7 * kTile;                  // float2 [2][128]
-constexpr int kOffBars = kOffStat + 2 * 128 * 8;     // mbarriers
+constexpr int slots_of(int copies, bool form_b) { return form_b || copies > 1 ? 5 : 6; }
+constexpr int kOffStat = 7 * kTile;                  // float4 [128]
+constexpr int kOffBars = kOffStat + 128 * 16;        // mbarriers
 constexpr int kOffMask = kOffBars + 384;             // uint4 [kAhead] live bits
 constexpr int kOffNf = kOffMask + kAhead * 16;            // uint4 [kNf]
 constexpr int kOffMisc = kOffNf + kNf * 16;          // TMEM address, flag, start of the range
@@ -80,6 +80,53 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// ---- pairs of fp32 in one register pair (two results per issue slot)
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// maximum of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of a pair on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the
+// least relative error on that range (2.6e-6: a Remez fit), n into the exponent.  x below -126 gives
+// 2^-126; NaN too.
+__device__ __forceinline__ void poly_ex2(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpack2(x, x0, x1);
+  x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+  const uint64_t t = add2(x, pack2(kRound, kRound));
+  const uint64_t f = fma2(add2(t, pack2(-kRound, -kRound)), pack2(-1.f, -1.f), x);
+  uint64_t p = pack2(0.009570101911169622f, 0.009570101911169622f);
+  p = fma2(p, f, pack2(0.055917860319387246f, 0.055917860319387246f));
+  p = fma2(p, f, pack2(0.24024744827863667f, 0.24024744827863667f));
+  p = fma2(p, f, pack2(0.6931218147366893f, 0.6931218147366893f));
+  p = fma2(p, f, pack2(0.9999992614457123f, 0.9999992614457123f));
+  float t0, t1;
+  unpack2(t, t0, t1);
+  unpack2(p, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 // Key tiles of sequence b: its cache's, and the drafted one.
@@ -140,13 +187,14 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return n == nt; }
 };
 
-template <bool FormB, bool Score>
+template <int F, bool FormB, bool Score>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kdmap,
                   const __grid_constant__ CUtensorMap vdmap, const Args a) {
   extern __shared__ __align__(1024) uint8_t base[];
-  constexpr int NS = slots_of(FormB);
+  constexpr int NS = slots_of(F, FormB);
+  constexpr int kRowsF = 128 / F;  // TMEM lanes of one copy of the rows
   constexpr int NQ = FormB ? 2 : 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + kOffBars);
   uint64_t* kfull = bars;          // [kAhead] K landed
@@ -154,21 +202,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* vok = bars + 16;       // [kAhead] the mask warp has cleaned the V tile
   uint64_t* empty = bars + 24;     // [NS] ring slot: its product is done
   uint64_t* sfull = bars + 30;     // [2] S written
-  uint64_t* pready = bars + 32;    // [2] P written (4 warps)
-  uint64_t* pvdone = bars + 34;    // [2] O += P V done
-  uint64_t* qfull = bars + 36;
-  uint64_t* qfree = bars + 37;
-  uint64_t* drain = bars + 38;     // after a wait that gave up
-  float2* stat = reinterpret_cast<float2*>(base + kOffStat);
+  uint64_t* pready = bars + 32;    // [2][2] the first / second half of P's columns written (4 warps)
+  uint64_t* pvdone = bars + 36;    // [2] O += P V done
+  uint64_t* qfull = bars + 38;
+  uint64_t* qfree = bars + 39;
+  uint64_t* drain = bars + 40;     // after a wait that gave up
+  float4* stat = reinterpret_cast<float4*>(base + kOffStat);
   uint4* masks = reinterpret_cast<uint4*>(base + kOffMask);
   uint4* nfs = reinterpret_cast<uint4*>(base + kOffNf);
   uint32_t* misc = reinterpret_cast<uint32_t*>(base + kOffMisc);
   volatile int* bad = reinterpret_cast<volatile int*>(misc + 1);
   uint8_t* ring = base + NQ * kTile;
+  float* joint = reinterpret_cast<float*>(ring + NS * kTile);  // F > 1: [2][128 lanes][32 dims]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < 39; ++i) mbar_init(bars + i, (i == 32 || i == 33) ? 4 : 1);
+    for (int i = 0; i < 41; ++i) mbar_init(bars + i, i >= 32 && i < 36 ? 4 : 1);
     *bad = 0;
     if (smem_u32(base) & 1023) {  // the swizzle needs the base aligned
       *bad = 1;
@@ -272,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
   if (warp == kProducer) {
     // ================================ TMA ==============================================
-    if (lane == 0) {
+    if (elect_one()) {
       prefetch_tmap(&qmap);
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
@@ -296,11 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.seg > 0) wait(qfree, (w.seg - 1) & 1);
         if (!*bad) {
           q_issued = w.seg + 1;
-          mbar_expect_tx(qfull, NQ * 2 * R * 128);
-          for (int r = 0; r < NQ; ++r)
+          mbar_expect_tx(qfull, NQ * F * 2 * R * 128);
+          for (int r = 0; r < NQ * F; ++r)
             for (int hf = 0; hf < 2; ++hf)
-              tma_load_3d(base + r * kTile + hf * kHalf, &qmap, qfull, 64 * hf, w.h * a.G,
-                          w.b * a.T + (w.pair * NQ + r) * a.npt);
+              tma_load_3d(base + (FormB ? r * kTile : r * kRowsF * 128) + hf * kHalf, &qmap, qfull, 64 * hf, w.h * a.G,
+                          w.b * a.T + (FormB ? w.pair * 2 + r : 0) * a.npt);
         }
         for (int i = 0; i < w.n; ++i, ++j) {
           load(w, w.tile0 + i, false, j);
@@ -325,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kMma) {
     // ================================ tensor cores =====================================
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idS = tc_idesc(128, 128, 0), idO = tc_idesc(128, 128, 1);
       // S of item i (key tile j of the CTA) into S_w; ``last_q``: the unit's last use of Q,
       // ``last_k``: the last use of this K tile
@@ -347,14 +396,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_pv = [&](int i, int j, bool first, bool last_v) {
         const int x = i & 1, s = v_pos(j) % NS;
         wait(&vok[j % kAhead], (j / kAhead) & 1);
-        wait(&pready[x], (i >> 1) & 1);
-        if (*bad) return;
-        tc_after();
         const uint32_t v = smem_u32(ring + s * kTile);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, tc_sdesc(v + ks * 16 * 128, kHalf, 1024), idO,
-                    !first || ks > 0);
+        for (int half = 0; half < 2; ++half) {
+          if (half == 0 || F == 1) wait(&pready[half * 2 + x], (i >> 1) & 1);
+          if (*bad) return;
+          tc_after();
+#pragma unroll
+          for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+            tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, tc_sdesc(v + ks * 16 * 128, kHalf, 1024), idO,
+                      !first || ks > 0);
+        }
         tc_commit(&pvdone[x]);
         if (last_v) tc_commit(&empty[s]);
       };
@@ -478,213 +530,331 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ================================ softmax ==========================================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    const int x = warp >> 2;                 // accumulator: items i with i & 1 == x
-    const int row = (warp & 3) * 32 + lane;  // TMEM lane = row of the row tile
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + x * 128 + lanes;
-    const bool mine = row < R;
-    const bool idle = (warp & 3) * 32 >= R;  // no row of this warp is in use
+    constexpr int NC = kRowsF;  // columns of a tile that a thread takes: all, or those of its row's copy
+    const int x = warp >> 2, quarter = warp & 3;  // accumulator: items i with i & 1 == x; TMEM lanes
+    const int row = F == 4 ? lane : F == 2 ? (quarter & 1) * 32 + lane : quarter * 32 + lane;
+    const int copy = F == 4 ? quarter : F == 2 ? quarter >> 1 : 0;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS = tmem + x * 128 + lanes, tO = tmem + 256 + x * 128 + lanes;
+    const bool idle = F == 1 && quarter * 32 >= R;  // no row of this warp is in use
     const float NEG_INF = -__int_as_float(0x7f800000);
     const float c = a.c;
-    int i = 0, j = 0;  // the CTA's items and key tiles so far
-    int done = 0;      // items of this accumulator so far
+    const uint64_t c2 = pack2(c, c);
+    int i0 = 0, j0 = 0;  // the CTA's items and key tiles before this unit
+    int done = 0;        // items of this accumulator so far
     while (w.next(a)) {
-      const int rt = FormB ? w.pair * 2 + x : 0;      // row tile
+      const int rt = FormB ? w.pair * 2 + x : 0;  // row tile
       const int node = rt * a.npt + row / a.G;
-      const bool in = mine && node < a.T;
+      const bool in = row < R && node < a.T;
       uint32_t sees[4] = {0, 0, 0, 0};
       const bool has_draft = w.tile0 + w.n == w.nt;
       bool used = false;
       if (in) used = node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
       float m = NEG_INF, l = 0.f, lx = 0.f;
-      int mine_n = 0;  // items of this accumulator in this unit
       const int items = FormB ? 2 * w.n : w.n;
-      for (int k = 0; k < items; ++k, ++i) {
-        const int jt = j;
-        if (!FormB || (k & 1)) ++j;
-        if ((i & 1) != x) continue;
-        const bool drafted = has_draft && (FormB ? k >> 1 : k) == w.n - 1;
+      const int first = (i0 & 1) == x ? 0 : 1;
+      for (int k = first; k < items; k += 2) {
+        const int kt = FormB ? k >> 1 : k, j = j0 + kt;
         wait(&sfull[x], done & 1);
-        wait(&vok[jt % kAhead], (jt / kAhead) & 1);
+        wait(&vok[j % kAhead], (j / kAhead) & 1);
         tc_after();
-        uint32_t s[4][32];
         if (!idle && !*bad) {
+          uint32_t s[NC];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) tc_ld32_raw(tS + q * 32, s[q]);
+          for (int q = 0; q < NC / 32; ++q)
+            tc_ld32_raw(tS + copy * NC + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
           tc_wait_ld();
-          uint4 mk = masks[jt % kAhead];
-          if (drafted) mk = make_uint4(sees[0], sees[1], sees[2], sees[3]);
-          const uint32_t mw[4] = {mk.x, mk.y, mk.z, mk.w};
+          uint4 mk = masks[j % kAhead];
+          if (has_draft && kt == w.n - 1) mk = make_uint4(sees[0], sees[1], sees[2], sees[3]);
+          uint32_t mw[NC / 32];
+          if constexpr (F == 4) {
+            mw[0] = copy == 0 ? mk.x : copy == 1 ? mk.y : copy == 2 ? mk.z : mk.w;
+          } else if constexpr (F == 2) {
+            mw[0] = copy ? mk.z : mk.x, mw[1] = copy ? mk.w : mk.y;
+          } else {
+            mw[0] = mk.x, mw[1] = mk.y, mw[2] = mk.z, mw[3] = mk.w;
+          }
           if (a.neg) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) s[q][e] ^= 0x80000000u;
+            for (int e = 0; e < NC; ++e) s[e] ^= 0x80000000u;
           }
-          if (!__all_sync(0xffffffffu, (mw[0] & mw[1] & mw[2] & mw[3]) == 0xffffffffu)) {
+          uint32_t all = mw[0];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+          for (int q = 1; q < NC / 32; ++q) all &= mw[q];
+          if (!__all_sync(0xffffffffu, all == 0xffffffffu)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) s[q][e] = ((mw[q] >> e) & 1u) ? s[q][e] : 0xff800000u;
+            for (int e = 0; e < NC; ++e) s[e] = ((mw[e / 32] >> (e % 32)) & 1u) ? s[e] : 0xff800000u;
           }
-          float top[4];
+          float top[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float t0 = __uint_as_float(s[q][0]), t1 = __uint_as_float(s[q][1]);
+          for (int e = 4; e < NC - 4; e += 8)
 #pragma unroll
-            for (int e = 2; e < 32; e += 2) {
-              t0 = fmaxf(t0, __uint_as_float(s[q][e]));
-              t1 = fmaxf(t1, __uint_as_float(s[q][e + 1]));
-            }
-            top[q] = fmaxf(t0, t1);
-          }
-          const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          const bool move = in && tm > m && !((tm - m) * c <= 8.f);
+            for (int q = 0; q < 4; ++q) top[q] = max3(top[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + 4 + q]));
+          top[0] = max3(top[0], __uint_as_float(s[NC - 4]), __uint_as_float(s[NC - 3]));
+          top[1] = max3(top[1], __uint_as_float(s[NC - 2]), __uint_as_float(s[NC - 1]));
+          const float tm = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+          // (a NaN moves the reference to NaN: the row ends as NaN)
+          const bool move = in && !(tm <= m) && !((tm - m) * c <= 8.f);
           if (__any_sync(0xffffffffu, move)) {
             const float f = move ? (m == NEG_INF ? 0.f : ex2((m - tm) * c)) : 1.f;
             if (move) m = tm;
             l *= f;
             if (Score) lx *= f;
-            if (mine_n > 0) {
+            if (k >= 2) {
               wait(&pvdone[x], (done - 1) & 1);
               tc_after();
               if (!*bad) {
 #pragma unroll 1
                 for (int q = 0; q < 8; ++q) {
                   uint32_t o[16];
-                  tc_ld16_raw(tmem + 256 + x * 128 + lanes + q * 16, o);
+                  tc_ld16_raw(tO + q * 16, o);
                   tc_wait_ld();
 #pragma unroll
                   for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tc_st16(tmem + 256 + x * 128 + lanes + q * 16, o);
+                  tc_st16(tO + q * 16, o);
                 }
                 tc_wait_st();
               }
             }
           }
           const float mc = (m == NEG_INF ? 0.f : m) * c;
-          float add[4] = {0.f, 0.f, 0.f, 0.f}, addx[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t nmc2 = pack2(-mc, -mc);
+          uint64_t add[2] = {0, 0}, addx[2] = {0, 0};
+          // weights of 64 columns at a time, packed over the same registers; the first half goes to the
+          // tensor cores while the second is formed
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int half = 0; half < (NC + 63) / 64; ++half) {
+            constexpr int kHalfCols = NC < 64 ? NC : 64;
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(s[q][e]), c, -mc));
-              const float p1 = ex2(fmaf(__uint_as_float(s[q][e + 1]), c, -mc));
+            for (int e = half * 64; e < half * 64 + kHalfCols; e += 2) {
+              const uint64_t y = fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nmc2);
+              float p0, p1;
+              if (FormB && !Score && (e / 2) % 4 == 3) {  // see kPolyShare
+                poly_ex2(y, p0, p1);
+              } else {
+                unpack2(y, p0, p1);
+                p0 = ex2(p0), p1 = ex2(p1);
+              }
               uint32_t pk;
               asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk) : "f"(p1), "f"(p0));
-              add[q] += __uint_as_float(pk << 16) + __uint_as_float(pk & 0xFFFF0000u);
-              if (Score) addx[q] += p0 + p1;
-              s[q >> 1][(q & 1) * 16 + e / 2] = pk;
+              if (FormB || Score) addx[e / 2 % 2] = add2(addx[e / 2 % 2], pack2(p0, p1));
+              if (!FormB)
+                add[e / 2 % 2] =
+                    add2(add[e / 2 % 2], pack2(__uint_as_float(pk << 16), __uint_as_float(pk & 0xFFFF0000u)));
+              s[e / 2] = pk;
             }
-          l += (add[0] + add[1]) + (add[2] + add[3]);
-          if (Score) lx += (addx[0] + addx[1]) + (addx[2] + addx[3]);
-          tc_st32(tS, s[0]);
-          tc_st32(tS + 32, s[1]);
-          tc_wait_st();
+            if constexpr (F == 1) {
+              tc_st32(tS + half * 32, *reinterpret_cast<uint32_t(*)[32]>(s + half * 32));
+              tc_wait_st();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&pready[half * 2 + x]);
+            }
+          }
+          if constexpr (F > 1) {
+            // this copy's columns, zeros in the others'
+            uint32_t zero[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero[e] = 0;
+#pragma unroll
+            for (int q = 0; q < F; ++q) {
+              if (q == copy) {
+                if constexpr (F == 4)
+                  tc_st16(tS + q * 16, *reinterpret_cast<uint32_t(*)[16]>(s));
+                else
+                  tc_st32(tS + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s));
+              } else {
+                tc_st16(tS + q * (64 / F), zero);
+                if constexpr (F == 2) tc_st16(tS + q * 32 + 16, zero);
+              }
+            }
+            tc_wait_st();
+          }
+          float a0, a1, b0, b1;
+          if (FormB || Score) {
+            unpack2(addx[0], a0, a1);
+            unpack2(addx[1], b0, b1);
+            lx += (a0 + a1) + (b0 + b1);
+          }
+          if (!FormB) {
+            unpack2(add[0], a0, a1);
+            unpack2(add[1], b0, b1);
+            l += (a0 + a1) + (b0 + b1);
+          }
+        } else if (F == 1) {
+          if (lane == 0) mbar_arrive(&pready[x]), mbar_arrive(&pready[2 + x]);
         }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pready[x]);
+        if (F > 1) {
+          tc_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[x]);
+        }
         ++done;
-        ++mine_n;
       }
+      i0 += items;
+      j0 += w.n;
+      if (FormB) l = lx;
       // ---- the unit's rows: accumulators in TMEM, statistics in the threads
-      if (mine_n > 0) wait(&pvdone[x], (done - 1) & 1);
+      if (first < items) wait(&pvdone[x], (done - 1) & 1);
       float f0 = 1.f, f1 = 0.f, M = m, L = l, Lx = lx;
       if (!FormB) {
         // the two accumulators of a row lie in the same TMEM lane: both warpgroups join them, each
         // for half the dims
-        if (x == 1) stat[row] = make_float2(m, l), stat[128 + row].x = lx;
+        const int at = quarter * 32 + lane;
+        if (x == 1) stat[at] = make_float4(m, l, lx, 0.f);
         named_bar(1, 256);
+        float m0 = m, m1 = m;
         if (x == 0) {
-          const float2 o = stat[row];
-          const float ox = stat[128 + row].x;
-          M = fmaxf(m, o.x);
-          f0 = m == NEG_INF ? 0.f : ex2((m - M) * c);
-          f1 = o.x == NEG_INF ? 0.f : ex2((o.x - M) * c);
-          L = f0 * l + f1 * o.y;
-          Lx = f0 * lx + f1 * ox;
-          if (M != M || L != L) f0 = f1 = 1.f;  // a NaN logit: the accumulators hold NaN too
-          stat[row] = make_float2(f0, f1);
-          stat[128 + row] = make_float2(M, L);
+          const float4 o = stat[at];
+          m1 = o.x;
+          M = fmaxf(m, m1);
+          const float e0 = m == NEG_INF ? 0.f : ex2((m - M) * c), e1 = m1 == NEG_INF ? 0.f : ex2((m1 - M) * c);
+          L = e0 * l + e1 * o.y;
+          Lx = e0 * lx + e1 * o.z;
+          stat[at] = make_float4(m, M, L, Lx);
         }
         named_bar(2, 256);
         if (x == 1) {
-          const float2 o = stat[row], p = stat[128 + row];
-          f0 = o.x, f1 = o.y, M = p.x, L = p.y;
+          const float4 o = stat[at];
+          m0 = o.x, M = o.y, L = o.z, Lx = o.w;
+        }
+        f0 = m0 == NEG_INF ? 0.f : ex2((m0 - M) * c);
+        f1 = m1 == NEG_INF ? 0.f : ex2((m1 - M) * c);
+        if (M != M || L != L) f0 = f1 = 1.f;  // a NaN logit: L is NaN, the row will be
+        if (F > 1) {
+          // and the copies of the row, each with the sums of its own columns
+          const float own = M;
+          float Mf = NEG_INF, Lf = 0.f, Lxf = 0.f;
+#pragma unroll
+          for (int q = 0; q < F; ++q) Mf = fmaxf(Mf, stat[q * kRowsF + row].y);
+#pragma unroll
+          for (int q = 0; q < F; ++q) {
+            const float4 o = stat[q * kRowsF + row];
+            const float e = o.y == NEG_INF ? 0.f : ex2((o.y - Mf) * c);
+            Lf = fmaf(e, o.z, Lf);
+            Lxf = fmaf(e, o.w, Lxf);
+          }
+          const float e = own == NEG_INF ? 0.f : ex2((own - Mf) * c);
+          f0 *= e, f1 *= e;
+          M = Mf, L = Lf, Lx = Lxf;
         }
       }
       tc_after();
-      if (!idle && !*bad) {
-        const size_t orow = (static_cast<size_t>(w.b) * a.T + node) * a.Hq + static_cast<size_t>(w.h) * a.G + row % a.G;
-        const bool whole = w.whole();
-        const int rows = FormB ? 256 : 128;
-        const int prow = FormB ? x * 128 + row : row;
-        const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
-        float* part = a.part + (slot * rows + prow) * kD;
-        if (in && (FormB || x == 0)) {
-          if (!whole) {
-            a.pstat[slot * rows + prow] = make_float2(M, L);
-            if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
-          } else if (Score) {
-            a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
+      const size_t orow = (static_cast<size_t>(w.b) * a.T + node) * a.Hq + static_cast<size_t>(w.h) * a.G + row % a.G;
+      const bool whole = w.whole();
+      const int rows = FormB ? 256 : 128;
+      const int prow = FormB ? x * 128 + row : row;
+      const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
+      float* part = a.part + (slot * rows + prow) * kD;
+      const bool ok = !*bad;
+      if (in && ok && (FormB || x == 0) && copy == 0) {
+        if (!whole) {
+          a.pstat[slot * rows + prow] = make_float2(M, L);
+          if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
+        } else if (Score) {
+          a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
+        }
+      }
+      const float inv = whole ? 1.f / L : 1.f;
+      const uint4 nf4 = has_draft ? nfs[w.seg % kNf] : make_uint4(0, 0, 0, 0);
+      const bool odd = in && ((nf4.x & sees[0]) | (nf4.y & sees[1]) | (nf4.z & sees[2]) | (nf4.w & sees[3]));
+      // N finished sums of dims d0 .. of this thread's row go out
+      auto put = [&](auto& o, int d0) {
+        constexpr int N = sizeof(o) / 4;
+        if (odd) {
+          for (int t = 0; t < a.T; ++t) {
+            const uint32_t nw = t < 32 ? nf4.x & sees[0] : t < 64 ? nf4.y & sees[1] : t < 96 ? nf4.z & sees[2] : nf4.w & sees[3];
+            if (!((nw >> (t & 31)) & 1u)) continue;
+            const __nv_bfloat16* v = a.vd + ((static_cast<size_t>(w.b) * a.Hkv + w.h) * a.T + t) * kD + d0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float y = __bfloat162float(v[e]);
+              if (!(fabsf(y) <= 3.4e38f)) o[e] += y;
+            }
           }
         }
-        const float inv = whole ? 1.f / L : 1.f;
-        uint4 nf4 = has_draft ? nfs[w.seg % kNf] : make_uint4(0, 0, 0, 0);
-        const bool odd = in && ((nf4.x & sees[0]) | (nf4.y & sees[1]) | (nf4.z & sees[2]) | (nf4.w & sees[3]));
-        constexpr int kChunks = FormB ? 4 : 2;
+        if (!in || !ok) return;
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + orow * kD + d0);
 #pragma unroll
-        for (int q = 0; q < kChunks; ++q) {
-          const int d0 = (FormB ? 0 : x * 64) + q * 32;
-          float o[32];
-          if (FormB) {
+          for (int e = 0; e < N / 8; ++e) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) pk[z] = used ? pack_bf16(o[e * 8 + 2 * z], o[e * 8 + 2 * z + 1]) : 0u;
+            dst[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(part + d0);
+#pragma unroll
+          for (int e = 0; e < N / 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      };
+      // 32 dims of the joined accumulators of this lane
+      auto get = [&](float (&o)[32], int d0) {
+        uint32_t r0[32], r1[32];
+        tc_ld32_raw(tmem + 256 + lanes + d0, r0);
+        tc_ld32_raw(tmem + 384 + lanes + d0, r1);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float v0 = f0 > 0.f ? __uint_as_float(r0[e]) * f0 : 0.f;
+          const float v1 = f1 > 0.f ? __uint_as_float(r1[e]) * f1 : 0.f;
+          o[e] = (v0 + v1) * inv;
+        }
+      };
+      if constexpr (FormB) {
+        if (!idle && ok) {
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
             uint32_t r0[32];
-            tc_ld32_raw(tmem + 256 + x * 128 + lanes + d0, r0);
+            float o[32];
+            tc_ld32_raw(tO + q * 32, r0);
             tc_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r0[e]) * inv;
-          } else {
-            uint32_t r0[32], r1[32];
-            tc_ld32_raw(tmem + 256 + lanes + d0, r0);
-            tc_ld32_raw(tmem + 384 + lanes + d0, r1);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float v0 = f0 > 0.f ? __uint_as_float(r0[e]) * f0 : 0.f;
-              const float v1 = f1 > 0.f ? __uint_as_float(r1[e]) * f1 : 0.f;
-              o[e] = (v0 + v1) * inv;
-            }
+            put(o, q * 32);
           }
-          if (odd) {
-            for (int t = 0; t < a.T; ++t) {
-              const uint32_t nw = t < 32 ? nf4.x & sees[0] : t < 64 ? nf4.y & sees[1] : t < 96 ? nf4.z & sees[2] : nf4.w & sees[3];
-              if (!((nw >> (t & 31)) & 1u)) continue;
-              const __nv_bfloat16* v = a.vd + ((static_cast<size_t>(w.b) * a.Hkv + w.h) * a.T + t) * kD + d0;
+        }
+      } else if constexpr (F == 1) {
+        if (!idle && ok) {
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {
+            float o[32];
+            get(o, x * 64 + q * 32);
+            put(o, x * 64 + q * 32);
+          }
+        }
+      } else {
+        // the copies' sums meet in shared memory, 32 dims of each warpgroup's half at a time
+        float* mine = joint + x * 128 * 32;
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {
+          if (ok) {
+            float o[32];
+            get(o, x * 64 + q * 32);
+            const int at = quarter * 32 + lane;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float y = __bfloat162float(v[e]);
-                if (!(fabsf(y) <= 3.4e38f)) o[e] += y;
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(mine + at * 32 + ((e ^ (at & 7)) << 2)) =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          named_bar(4 + x, 128);
+          if (ok) {
+            float o[32 / F];
+#pragma unroll
+            for (int e = 0; e < 8 / F; ++e) {
+              float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int g = 0; g < F; ++g) {
+                const int at = g * kRowsF + row;
+                const float4 v = *reinterpret_cast<float4*>(mine + at * 32 + (((copy * (8 / F) + e) ^ (at & 7)) << 2));
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
               }
+              o[4 * e] = sum.x, o[4 * e + 1] = sum.y, o[4 * e + 2] = sum.z, o[4 * e + 3] = sum.w;
             }
+            put(o, x * 64 + q * 32 + copy * (32 / F));
           }
-          if (in) {
-            if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(a.out + orow * kD + d0);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t pk[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  pk[z] = used ? pack_bf16(o[e * 8 + 2 * z], o[e * 8 + 2 * z + 1]) : 0u;
-                dst[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-              }
-            } else {
-              float4* dst = reinterpret_cast<float4*>(part + d0);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
-          }
+          named_bar(4 + x, 128);
         }
       }
       tc_before();
@@ -831,7 +1001,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
     *bad = 1;
   };
   if (warp == 8) {
-    if (lane == 0) {
+    if (elect_one()) {
       const int R = p.npt * a.G;
       const uint32_t id = tc_idesc(128, (R + 15) / 16 * 16, 0);
       int loaded = 0;
@@ -1076,8 +1246,11 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
     if ((st = map_rows(&vm, vcache, S, static_cast<long long>(B) * Hkv, kKeys, 1))) return st;
   }
   const bool score = node_score != nullptr;
-  auto kernel = p.form_b ? (score ? attend_kernel<true, true> : attend_kernel<true, false>)
-                         : (score ? attend_kernel<false, true> : attend_kernel<false, false>);
+  const int copies = p.form_b ? 1 : p.npt * G <= 32 ? 4 : p.npt * G <= 64 ? 2 : 1;
+  auto kernel = p.form_b      ? (score ? attend_kernel<1, true, true> : attend_kernel<1, true, false>)
+                : copies == 4 ? (score ? attend_kernel<4, false, true> : attend_kernel<4, false, false>)
+                : copies == 2 ? (score ? attend_kernel<2, false, true> : attend_kernel<2, false, false>)
+                              : (score ? attend_kernel<1, false, true> : attend_kernel<1, false, false>);
   const int sms = prepare_device(reinterpret_cast<const void*>(kernel), kSmem);
   if (!sms) return fail(kStatusCuda, "tree_attn: no usable device");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
