@@ -155,7 +155,11 @@ __device__ __forceinline__ bool node_sees(const int* par, int t, uint32_t (&sees
   }
 }
 
-// A walk over the CTA's range of key tiles, unit by unit.
+// A value that is the same in every lane, so that the compiler knows it and keeps what follows from it
+// in uniform registers (the operands of tcgen05 and TMA instructions).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// A walk over the CTA's range of key tiles, unit by unit, by whole warps.
 struct Walk {
   int t, end;        // global key tiles left: [t, end)
   int b, base, len;  // sequence, its first tile, its length
@@ -168,12 +172,12 @@ struct Walk {
     t += n;
     if (t >= end) return false;
     const int per_head = a.pairs;
-    len = len_of(a, b);
+    len = uniform(len_of(a, b));
     nt = tiles_of(len);
     while (t - base >= nt * a.Hkv * per_head) {
       base += nt * a.Hkv * per_head;
       ++b;
-      len = len_of(a, b);
+      len = uniform(len_of(a, b));
       nt = tiles_of(len);
     }
     const int rel = t - base, u = rel / nt;
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* bad = reinterpret_cast<volatile int*>(misc + 1);
   uint8_t* ring = base + NQ * kTile;
   float* joint = reinterpret_cast<float*>(ring + NS * kTile);  // F > 1: [2][128 lanes][32 dims]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < 41; ++i) mbar_init(bars + i, i >= 32 && i < 36 ? 4 : 1);
@@ -293,9 +297,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = misc[0];
+  constexpr uint32_t tmem = 0;  // all 512 columns: they begin at 0
+  if (tid == 0 && misc[0] != tmem) {
+    *bad = 1;
+    set_err(a.err, kErrWaitTimeout);
+  }
   Walk w;
-  w.start(misc[2], misc[3], misc[4], misc[5]);
+  w.start(uniform(misc[2]), uniform(misc[3]), uniform(misc[4]), uniform(misc[5]));
   const int n_tiles = w.end - w.t;
   const int R = a.npt * a.G;
 
@@ -321,130 +329,139 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
   if (warp == kProducer) {
     // ================================ TMA ==============================================
-    if (elect_one()) {
+    const bool leader = elect_one();
+    if (leader) {
       prefetch_tmap(&qmap);
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
-      int k_issued = 0, v_issued = 0, q_issued = 0;
-      auto load = [&](const Walk& x, int tile, bool value, int j) {
-        const int pos = value ? v_pos(j) : k_pos(j), s = pos % NS;
-        if (pos >= NS) wait(&empty[s], (pos / NS - 1) & 1);
-        if (*bad) return;
-        (value ? v_issued : k_issued) = j + 1;
-        const bool drafted = tile == x.nt - 1;
-        const CUtensorMap* m = drafted ? (value ? &vdmap : &kdmap) : (value ? &vmap : &kmap);
-        const int y = drafted ? 0 : tile * kKeys, z = x.b * a.Hkv + x.h;
-        uint64_t* bar = (value ? vfull : kfull) + j % kAhead;
+    }
+    int k_issued = 0, v_issued = 0, q_issued = 0;
+    auto load = [&](const Walk& x, int tile, bool value, int j) {
+      const int pos = value ? v_pos(j) : k_pos(j), s = pos % NS;
+      if (pos >= NS) wait(&empty[s], (pos / NS - 1) & 1);
+      (value ? v_issued : k_issued) = j + 1;
+      const bool drafted = tile == x.nt - 1;
+      const CUtensorMap* m = drafted ? (value ? &vdmap : &kdmap) : (value ? &vmap : &kmap);
+      const int y = drafted ? 0 : tile * kKeys, z = x.b * a.Hkv + x.h;
+      uint64_t* bar = (value ? vfull : kfull) + j % kAhead;
+      if (leader && !*bad) {
         mbar_expect_tx(bar, kTile);
         tma_load_3d(ring + s * kTile, m, bar, 0, y, z);
         tma_load_3d(ring + s * kTile + kHalf, m, bar, 64, y, z);
-      };
-      Walk last = w;  // the unit and tile whose V is still to be loaded
-      int last_tile = -1, j = 0;
-      while (w.next(a)) {
-        if (w.seg > 0) wait(qfree, (w.seg - 1) & 1);
-        if (!*bad) {
-          q_issued = w.seg + 1;
-          mbar_expect_tx(qfull, NQ * F * 2 * R * 128);
-          for (int r = 0; r < NQ * F; ++r)
-            for (int hf = 0; hf < 2; ++hf)
-              tma_load_3d(base + (FormB ? r * kTile : r * kRowsF * 128) + hf * kHalf, &qmap, qfull, 64 * hf, w.h * a.G,
-                          w.b * a.T + (FormB ? w.pair * 2 + r : 0) * a.npt);
-        }
-        for (int i = 0; i < w.n; ++i, ++j) {
-          load(w, w.tile0 + i, false, j);
-          if (FormB) {
-            load(w, w.tile0 + i, true, j);
-          } else {
-            if (j > 0) load(last, last_tile, true, j - 1);
-            last = w;
-            last_tile = w.tile0 + i;
-          }
+      }
+    };
+    Walk last = w;  // the unit and tile whose V is still to be loaded
+    int last_tile = -1, j = 0;
+    while (w.next(a)) {
+      if (w.seg > 0) wait(qfree, (w.seg - 1) & 1);
+      q_issued = w.seg + 1;
+      if (leader && !*bad) {
+        mbar_expect_tx(qfull, NQ * F * 2 * R * 128);
+        for (int r = 0; r < NQ * F; ++r)
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_3d(base + (FormB ? r * kTile : r * kRowsF * 128) + hf * kHalf, &qmap, qfull, 64 * hf, w.h * a.G,
+                        w.b * a.T + (FormB ? w.pair * 2 + r : 0) * a.npt);
+      }
+      for (int i = 0; i < w.n; ++i, ++j) {
+        load(w, w.tile0 + i, false, j);
+        if (FormB) {
+          load(w, w.tile0 + i, true, j);
+        } else {
+          if (j > 0) load(last, last_tile, true, j - 1);
+          last = w;
+          last_tile = w.tile0 + i;
         }
       }
-      if (!FormB && j > 0) load(last, last_tile, true, j - 1);
-      if (*bad) {  // a wait has given up: the copies in flight land before the shared memory goes
-        for (int k = max(0, k_issued - NS); k < k_issued; ++k)
-          mbar_wait_bounded(&kfull[k % kAhead], (k / kAhead) & 1, 1u << 16);
-        for (int k = max(0, v_issued - NS); k < v_issued; ++k)
-          mbar_wait_bounded(&vfull[k % kAhead], (k / kAhead) & 1, 1u << 16);
-        if (q_issued) mbar_wait_bounded(qfull, (q_issued - 1) & 1, 1u << 16);
-      }
+    }
+    if (!FormB && j > 0) load(last, last_tile, true, j - 1);
+    if (leader && *bad) {  // a wait has given up: the copies in flight land before the shared memory goes
+      for (int k = max(0, k_issued - NS); k < k_issued; ++k)
+        mbar_wait_bounded(&kfull[k % kAhead], (k / kAhead) & 1, 1u << 14);
+      for (int k = max(0, v_issued - NS); k < v_issued; ++k)
+        mbar_wait_bounded(&vfull[k % kAhead], (k / kAhead) & 1, 1u << 14);
+      if (q_issued) mbar_wait_bounded(qfull, (q_issued - 1) & 1, 1u << 14);
     }
     __syncwarp();
   } else if (warp == kMma) {
     // ================================ tensor cores =====================================
-    if (elect_one()) {
-      const uint32_t idS = tc_idesc(128, 128, 0), idO = tc_idesc(128, 128, 1);
-      // S of item i (key tile j of the CTA) into S_w; ``last_q``: the unit's last use of Q,
-      // ``last_k``: the last use of this K tile
-      auto issue_s = [&](int i, int j, bool last_q, bool last_k) {
-        const int x = i & 1, s = k_pos(j) % NS;
-        wait(&kfull[j % kAhead], (j / kAhead) & 1);
-        if (*bad) return;
-        tc_after();
-        const uint32_t q = smem_u32(base) + (FormB ? x * kTile : 0), k = smem_u32(ring + s * kTile);
+    // (the warp walks together, so that everything but the issue itself is in uniform registers: one
+    // lane walking alone spent 2200 cycles on an item's 16 products, 1000 of them useful)
+    const bool leader = elect_one();
+    constexpr uint32_t idS = tc_idesc(128, 128, 0), idO = tc_idesc(128, 128, 1);
+    const uint64_t dq = tc_sdesc(smem_u32(base)), dk = tc_sdesc(smem_u32(ring)), dv = tc_sdesc(smem_u32(ring), kHalf, 1024);
+    // S of item i (key tile j of the CTA) into S_w; ``last_q``: the unit's last use of Q,
+    // ``last_k``: the last use of this K tile
+    auto issue_s = [&](int i, int j, bool last_q, bool last_k) {
+      const int x = i & 1, s = k_pos(j) % NS;
+      wait(&kfull[j % kAhead], (j / kAhead) & 1);
+      tc_after();
+      const uint64_t q = dq + (FormB ? x * (kTile >> 4) : 0), k = dk + s * (kTile >> 4);
+      if (leader && !*bad) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-          tc_mma(tmem + x * 128, tc_sdesc(q + off), tc_sdesc(k + off), idS, ks > 0);
+          const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+          tc_mma(tmem + x * 128, q + off, k + off, idS, ks > 0);
         }
         tc_commit(&sfull[x]);
         if (last_k) tc_commit(&empty[s]);
         if (last_q) tc_commit(qfree);
-      };
-      auto issue_pv = [&](int i, int j, bool first, bool last_v) {
-        const int x = i & 1, s = v_pos(j) % NS;
-        wait(&vok[j % kAhead], (j / kAhead) & 1);
-        const uint32_t v = smem_u32(ring + s * kTile);
+      }
+      __syncwarp();
+    };
+    auto issue_pv = [&](int i, int j, bool first, bool last_v) {
+      const int x = i & 1, s = v_pos(j) % NS;
+      wait(&vok[j % kAhead], (j / kAhead) & 1);
+      const uint64_t v = dv + s * (kTile >> 4);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half == 0 || F == 1) wait(&pready[half * 2 + x], (i >> 1) & 1);
-          if (*bad) return;
-          tc_after();
+      for (int half = 0; half < 2; ++half) {
+        if (half == 0 || F == 1) wait(&pready[half * 2 + x], (i >> 1) & 1);
+        tc_after();
+        if (leader && !*bad) {
 #pragma unroll
           for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-            tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, tc_sdesc(v + ks * 16 * 128, kHalf, 1024), idO,
-                      !first || ks > 0);
+            tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, v + ks * (16 * 128 >> 4), idO, !first || ks > 0);
+          if (half == 1) {
+            tc_commit(&pvdone[x]);
+            if (last_v) tc_commit(&empty[s]);
+          }
         }
-        tc_commit(&pvdone[x]);
-        if (last_v) tc_commit(&empty[s]);
-      };
-      // the S products run two items ahead of the P V products, over unit borders too
-      Walk ahead = w;
-      int ai = 0, aj = 0, left = 0, aw = 0;  // next S item, its key tile, tiles left in its unit, row tile
-      auto s_next = [&]() {
-        if (left == 0) {
-          if (!ahead.next(a)) return;
-          left = ahead.n;
-          aw = 0;
-          wait(qfull, ahead.seg & 1);
-        }
-        if (FormB) {
-          issue_s(ai, aj, left == 1 && aw == 1, aw == 1);
-          if (aw == 1) ++aj, --left;
-          aw ^= 1;
-        } else {
-          issue_s(ai, aj, left == 1, true);
-          ++aj, --left;
-        }
-        ++ai;
-      };
-      s_next();
-      s_next();
-      int i = 0, j = 0;
-      while (w.next(a)) {
-        const int items = FormB ? 2 * w.n : w.n;
-        for (int k = 0; k < items; ++k, ++i) {
-          issue_pv(i, j, k < 2, FormB ? (k & 1) == 1 : true);
-          if (!FormB || (k & 1)) ++j;
-          s_next();
-        }
+        __syncwarp();
       }
-      if (*bad) {  // products in flight end before TMEM goes
-        tc_commit(drain);
-        mbar_wait_bounded(drain, 0, 1u << 16);
+    };
+    // the S products run two items ahead of the P V products, over unit borders too
+    Walk ahead = w;
+    int ai = 0, aj = 0, left = 0, aw = 0;  // next S item, its key tile, tiles left in its unit, row tile
+    auto s_next = [&]() {
+      if (left == 0) {
+        if (!ahead.next(a)) return;
+        left = ahead.n;
+        aw = 0;
+        wait(qfull, ahead.seg & 1);
       }
+      if (FormB) {
+        issue_s(ai, aj, left == 1 && aw == 1, aw == 1);
+        if (aw == 1) ++aj, --left;
+        aw ^= 1;
+      } else {
+        issue_s(ai, aj, left == 1, true);
+        ++aj, --left;
+      }
+      ++ai;
+    };
+    s_next();
+    s_next();
+    int i = 0, j = 0;
+    while (w.next(a)) {
+      const int items = FormB ? 2 * w.n : w.n;
+      for (int k = 0; k < items; ++k, ++i) {
+        issue_pv(i, j, k < 2, FormB ? (k & 1) == 1 : true);
+        if (!FormB || (k & 1)) ++j;
+        s_next();
+      }
+    }
+    if (leader && *bad) {  // products in flight end before TMEM goes
+      tc_commit(drain);
+      mbar_wait_bounded(drain, 0, 1u << 14);
     }
     __syncwarp();
   } else if (warp == kMask) {
@@ -865,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_before();
   __syncthreads();
-  if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(misc[0]), "r"(512));
 }
 
 // Joins the parts of units that a border cut: a warp per output row.
