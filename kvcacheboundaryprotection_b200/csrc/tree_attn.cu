@@ -43,8 +43,9 @@ constexpr int kMaxNodes = 128;
 constexpr int kKeys = 128;
 constexpr int kHalf = 128 * 128;  // a 64-column half of a [128][128] bf16 tile: 16 KiB
 constexpr int kTile = 2 * kHalf;
-constexpr int kProducer = 8, kMma = 9, kMask = 10;  // warps 0-7: softmax; 11 fills the warpgroup
-constexpr int kThreads = 12 * 32;
+// softmax warps: 8, or 16 where a row's columns are not already shared by its copies
+constexpr int halves_of(int copies) { return copies == 1 ? 2 : 1; }
+constexpr int threads_of(int copies) { return halves_of(copies) * 256 + 128; }
 constexpr int kAhead = 8;  // barriers in turn over the key tiles: more than the ring holds of either kind
 constexpr int kNf = 8;  // units' records of non-finite drafted values kept at a time
 constexpr float kLog2e = 1.4426950408889634f;
@@ -107,26 +108,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of a pair on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with the
-// least relative error on that range (2.6e-6: a Remez fit), n into the exponent.  x below -126 gives
-// 2^-126; NaN too.
-__device__ __forceinline__ void poly_ex2(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  unpack2(x, x0, x1);
-  x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
-  const uint64_t t = add2(x, pack2(kRound, kRound));
-  const uint64_t f = fma2(add2(t, pack2(-kRound, -kRound)), pack2(-1.f, -1.f), x);
-  uint64_t p = pack2(0.009570101911169622f, 0.009570101911169622f);
-  p = fma2(p, f, pack2(0.055917860319387246f, 0.055917860319387246f));
-  p = fma2(p, f, pack2(0.24024744827863667f, 0.24024744827863667f));
-  p = fma2(p, f, pack2(0.6931218147366893f, 0.6931218147366893f));
-  p = fma2(p, f, pack2(0.9999992614457123f, 0.9999992614457123f));
-  float t0, t1;
-  unpack2(t, t0, t1);
-  unpack2(p, p0, p1);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+// Barrier of 64 threads; true in all where it is in one.
+__device__ __forceinline__ bool any_of_pair(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, %2, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v)), "r"(id)
+      : "memory");
+  return r != 0;
 }
 
 // Key tiles of sequence b: its cache's, and the drafted one.
@@ -192,13 +184,15 @@ struct Walk {
 };
 
 template <int F, bool FormB, bool Score>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(F), 1)
     attend_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kdmap,
                   const __grid_constant__ CUtensorMap vdmap, const Args a) {
   extern __shared__ __align__(1024) uint8_t base[];
   constexpr int NS = slots_of(F, FormB);
   constexpr int kRowsF = 128 / F;  // TMEM lanes of one copy of the rows
+  constexpr int H = halves_of(F);  // warps that share a row's columns
+  constexpr int kProducer = 8 * H, kMma = kProducer + 1, kMask = kProducer + 2;  // one more fills the warpgroup
   constexpr int NQ = FormB ? 2 : 1;
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + kOffBars);
   uint64_t* kfull = bars;          // [kAhead] K landed
@@ -206,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* vok = bars + 16;       // [kAhead] the mask warp has cleaned the V tile
   uint64_t* empty = bars + 24;     // [NS] ring slot: its product is done
   uint64_t* sfull = bars + 30;     // [2] S written
-  uint64_t* pready = bars + 32;    // [2][2] the first / second half of P's columns written (4 warps)
-  uint64_t* pvdone = bars + 36;    // [2] O += P V done
+  uint64_t* pready = bars + 32;    // [2] P written (4 H warps)
+  uint64_t* odone = bars + 36;     // the unit's last products are done
   uint64_t* qfull = bars + 38;
   uint64_t* qfree = bars + 39;
   uint64_t* drain = bars + 40;     // after a wait that gave up
@@ -221,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < 41; ++i) mbar_init(bars + i, i >= 32 && i < 36 ? 4 : 1);
+    for (int i = 0; i < 41; ++i) mbar_init(bars + i, i == 32 || i == 33 ? 4 * H : 1);
     *bad = 0;
     if (smem_u32(base) & 1023) {  // the swizzle needs the base aligned
       *bad = 1;
@@ -323,10 +317,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto k_pos = [&](int j) { return FormB ? 2 * j : j ? 2 * j - 1 : 0; };
   auto v_pos = [&](int j) { return FormB ? 2 * j + 1 : j + 1 < n_tiles ? 2 * j + 2 : 2 * j + 1; };
 
-  // the softmax threads hold a row of S each: registers move to them from the other warps
-  // (384 threads at 168 = 256 at 192 + 128 at 120)
+  // the softmax threads hold their part of a row of S: registers move to them from the other warps
+  // (640 threads at 96 = 512 at 104 + 128 at 64)
   if (warp >= kProducer) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    if constexpr (H == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == kProducer) {
     // ================================ TMA ==============================================
     const bool leader = elect_one();
@@ -389,44 +383,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = elect_one();
     constexpr uint32_t idS = tc_idesc(128, 128, 0), idO = tc_idesc(128, 128, 1);
     const uint64_t dq = tc_sdesc(smem_u32(base)), dk = tc_sdesc(smem_u32(ring)), dv = tc_sdesc(smem_u32(ring), kHalf, 1024);
-    // S of item i (key tile j of the CTA) into S_w; ``last_q``: the unit's last use of Q,
-    // ``last_k``: the last use of this K tile
-    auto issue_s = [&](int i, int j, bool last_q, bool last_k) {
+    // One commit an item: S(i + 2) is issued after P V(i), so that its completion says that both are done,
+    // and the softmax warps that wait for it anyway hand Q, K and V back.  (A commit costs 115 cycles of
+    // this warp, a wait that is over 100: at five waits and three commits an item they were half its time.)
+    auto issue_s = [&](int i, int j) {  // S of item i (key tile j of the CTA) into S_w
       const int x = i & 1, s = k_pos(j) % NS;
-      wait(&kfull[j % kAhead], (j / kAhead) & 1);
+      if (!FormB || x == 0) wait(&kfull[j % kAhead], (j / kAhead) & 1);
       tc_after();
       const uint64_t q = dq + (FormB ? x * (kTile >> 4) : 0), k = dk + s * (kTile >> 4);
-      if (leader && !*bad) {
+      if (leader) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
           tc_mma(tmem + x * 128, q + off, k + off, idS, ks > 0);
         }
         tc_commit(&sfull[x]);
-        if (last_k) tc_commit(&empty[s]);
-        if (last_q) tc_commit(qfree);
       }
       __syncwarp();
     };
-    auto issue_pv = [&](int i, int j, bool first, bool last_v) {
+    auto issue_pv = [&](int i, int j, bool first, bool last) {
       const int x = i & 1, s = v_pos(j) % NS;
-      wait(&vok[j % kAhead], (j / kAhead) & 1);
+      wait(&pready[x], (i >> 1) & 1);  // (its warps have waited for the cleaned V)
+      tc_after();
       const uint64_t v = dv + s * (kTile >> 4);
+      if (leader) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half == 0 || F == 1) wait(&pready[half * 2 + x], (i >> 1) & 1);
-        tc_after();
-        if (leader && !*bad) {
-#pragma unroll
-          for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-            tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, v + ks * (16 * 128 >> 4), idO, !first || ks > 0);
-          if (half == 1) {
-            tc_commit(&pvdone[x]);
-            if (last_v) tc_commit(&empty[s]);
-          }
-        }
-        __syncwarp();
+        for (int ks = 0; ks < 8; ++ks)
+          tc_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, v + ks * (16 * 128 >> 4), idO, !first || ks > 0);
+        if (last) tc_commit(odone);
       }
+      __syncwarp();
     };
     // the S products run two items ahead of the P V products, over unit borders too
     Walk ahead = w;
@@ -439,11 +425,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(qfull, ahead.seg & 1);
       }
       if (FormB) {
-        issue_s(ai, aj, left == 1 && aw == 1, aw == 1);
+        issue_s(ai, aj);
         if (aw == 1) ++aj, --left;
         aw ^= 1;
       } else {
-        issue_s(ai, aj, left == 1, true);
+        issue_s(ai, aj);
         ++aj, --left;
       }
       ++ai;
@@ -454,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (w.next(a)) {
       const int items = FormB ? 2 * w.n : w.n;
       for (int k = 0; k < items; ++k, ++i) {
-        issue_pv(i, j, k < 2, FormB ? (k & 1) == 1 : true);
+        issue_pv(i, j, k < 2, k == items - 1);
         if (!FormB || (k & 1)) ++j;
         s_next();
       }
@@ -546,50 +532,72 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     // ================================ softmax ==========================================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    constexpr int NC = kRowsF;  // columns of a tile that a thread takes: all, or those of its row's copy
-    const int x = warp >> 2, quarter = warp & 3;  // accumulator: items i with i & 1 == x; TMEM lanes
+    if constexpr (H == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    constexpr int NC = kRowsF / H;  // columns of a tile that a thread takes
+    // accumulator (items i with i & 1 == x), part of the columns, TMEM lanes
+    const int x = warp / (4 * H), hc = H == 2 ? (warp >> 2) & 1 : 0, quarter = warp & 3;
     const int row = F == 4 ? lane : F == 2 ? (quarter & 1) * 32 + lane : quarter * 32 + lane;
     const int copy = F == 4 ? quarter : F == 2 ? quarter >> 1 : 0;
+    const int pair_bar = 6 + x * 4 + quarter;  // (H == 2) the two warps of the same rows
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + x * 128 + lanes, tO = tmem + 256 + x * 128 + lanes;
     const bool idle = F == 1 && quarter * 32 >= R;  // no row of this warp is in use
     const float NEG_INF = -__int_as_float(0x7f800000);
     const float c = a.c;
     const uint64_t c2 = pack2(c, c);
+    float* xchg = reinterpret_cast<float*>(stat) + x * 256;  // [2][128]
+    const bool releases = quarter == 0 && hc == 0 && (!FormB || x == 1);  // hands tiles back
     int i0 = 0, j0 = 0;  // the CTA's items and key tiles before this unit
     int done = 0;        // items of this accumulator so far
     while (w.next(a)) {
       const int rt = FormB ? w.pair * 2 + x : 0;  // row tile
       const int node = rt * a.npt + row / a.G;
       const bool in = row < R && node < a.T;
-      uint32_t sees[4] = {0, 0, 0, 0};
       const bool has_draft = w.tile0 + w.n == w.nt;
+      uint32_t own[NC / 32];  // the drafted nodes of this thread's columns that the row sees
+#pragma unroll
+      for (int q = 0; q < NC / 32; ++q) own[q] = 0;
       bool used = false;
-      if (in) used = node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
+      if (in) {
+        uint32_t sees[4];
+        used = node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
+        if constexpr (F == 4) {
+          own[0] = copy == 0 ? sees[0] : copy == 1 ? sees[1] : copy == 2 ? sees[2] : sees[3];
+        } else {
+          const bool upper = F == 2 ? copy == 1 : hc == 1;
+          own[0] = upper ? sees[2] : sees[0], own[1] = upper ? sees[3] : sees[1];
+        }
+      }
       float m = NEG_INF, l = 0.f, lx = 0.f;
       const int items = FormB ? 2 * w.n : w.n;
       const int first = (i0 & 1) == x ? 0 : 1;
       for (int k = first; k < items; k += 2) {
         const int kt = FormB ? k >> 1 : k, j = j0 + kt;
         wait(&sfull[x], done & 1);
+        if (releases) {  // products up to this S are done
+          if (lane == 0) {
+            mbar_arrive(&empty[k_pos(j) % NS]);
+            if (k >= 2) mbar_arrive(&empty[v_pos(FormB ? j - 1 : j - 2) % NS]);
+            if (k == items - 1) mbar_arrive(qfree);
+          }
+          __syncwarp();
+        }
         wait(&vok[j % kAhead], (j / kAhead) & 1);
         tc_after();
-        if (!idle && !*bad) {
+        if (!idle) {
           uint32_t s[NC];
 #pragma unroll
           for (int q = 0; q < NC / 32; ++q)
-            tc_ld32_raw(tS + copy * NC + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
+            tc_ld32_raw(tS + (copy * H + hc) * NC + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
           tc_wait_ld();
-          uint4 mk = masks[j % kAhead];
-          if (has_draft && kt == w.n - 1) mk = make_uint4(sees[0], sees[1], sees[2], sees[3]);
           uint32_t mw[NC / 32];
-          if constexpr (F == 4) {
-            mw[0] = copy == 0 ? mk.x : copy == 1 ? mk.y : copy == 2 ? mk.z : mk.w;
-          } else if constexpr (F == 2) {
-            mw[0] = copy ? mk.z : mk.x, mw[1] = copy ? mk.w : mk.y;
+          if (has_draft && kt == w.n - 1) {
+#pragma unroll
+            for (int q = 0; q < NC / 32; ++q) mw[q] = own[q];
           } else {
-            mw[0] = mk.x, mw[1] = mk.y, mw[2] = mk.z, mw[3] = mk.w;
+            const uint32_t* mk = reinterpret_cast<const uint32_t*>(masks + j % kAhead) + (copy * H + hc) * (NC / 32);
+#pragma unroll
+            for (int q = 0; q < NC / 32; ++q) mw[q] = mk[q];
           }
           if (a.neg) {
 #pragma unroll
@@ -609,66 +617,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 4; ++q) top[q] = max3(top[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + 4 + q]));
           top[0] = max3(top[0], __uint_as_float(s[NC - 4]), __uint_as_float(s[NC - 3]));
           top[1] = max3(top[1], __uint_as_float(s[NC - 2]), __uint_as_float(s[NC - 1]));
-          const float tm = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+          float tm = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
           // (a NaN moves the reference to NaN: the row ends as NaN)
-          const bool move = in && !(tm <= m) && !((tm - m) * c <= 8.f);
-          if (__any_sync(0xffffffffu, move)) {
+          auto moves = [&]() { return in && !(tm <= m) && !((tm - m) * c <= 8.f); };
+          // the two warps of a row move together.  Past this barrier both have read S, whose columns
+          // P will take.
+          const bool any = H == 2 ? any_of_pair(pair_bar, moves()) : __any_sync(0xffffffffu, moves());
+          if (any) {
+            if (H == 2) {
+              xchg[hc * 128 + quarter * 32 + lane] = tm;
+              named_bar(pair_bar, 64);
+              tm = max3(tm, xchg[(hc ^ 1) * 128 + quarter * 32 + lane], tm);
+            }
+            const bool move = moves();
             const float f = move ? (m == NEG_INF ? 0.f : ex2((m - tm) * c)) : 1.f;
             if (move) m = tm;
             l *= f;
             if (Score) lx *= f;
-            if (k >= 2) {
-              wait(&pvdone[x], (done - 1) & 1);
-              tc_after();
-              if (!*bad) {
+            if (k >= 2) {  // (S of this item was issued after the previous P V product: that is done)
 #pragma unroll 1
-                for (int q = 0; q < 8; ++q) {
-                  uint32_t o[16];
-                  tc_ld16_raw(tO + q * 16, o);
-                  tc_wait_ld();
+              for (int q = hc * (8 / H); q < (hc + 1) * (8 / H); ++q) {
+                uint32_t o[16];
+                tc_ld16_raw(tO + q * 16, o);
+                tc_wait_ld();
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tc_st16(tO + q * 16, o);
-                }
-                tc_wait_st();
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st16(tO + q * 16, o);
               }
+              tc_wait_st();
+            }
+            if (H == 2) {  // either half of P lets a product begin: O is whole before that
+              tc_before();
+              named_bar(pair_bar, 64);
             }
           }
           const float mc = (m == NEG_INF ? 0.f : m) * c;
           const uint64_t nmc2 = pack2(-mc, -mc);
           uint64_t add[2] = {0, 0}, addx[2] = {0, 0};
-          // weights of 64 columns at a time, packed over the same registers; the first half goes to the
-          // tensor cores while the second is formed
+          // the weights, packed over the same registers
 #pragma unroll
-          for (int half = 0; half < (NC + 63) / 64; ++half) {
-            constexpr int kHalfCols = NC < 64 ? NC : 64;
-#pragma unroll
-            for (int e = half * 64; e < half * 64 + kHalfCols; e += 2) {
-              const uint64_t y = fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nmc2);
-              float p0, p1;
-              if (FormB && !Score && (e / 2) % 4 == 3) {  // see kPolyShare
-                poly_ex2(y, p0, p1);
-              } else {
-                unpack2(y, p0, p1);
-                p0 = ex2(p0), p1 = ex2(p1);
-              }
-              uint32_t pk;
-              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk) : "f"(p1), "f"(p0));
-              if (FormB || Score) addx[e / 2 % 2] = add2(addx[e / 2 % 2], pack2(p0, p1));
-              if (!FormB)
-                add[e / 2 % 2] =
-                    add2(add[e / 2 % 2], pack2(__uint_as_float(pk << 16), __uint_as_float(pk & 0xFFFF0000u)));
-              s[e / 2] = pk;
-            }
-            if constexpr (F == 1) {
-              tc_st32(tS + half * 32, *reinterpret_cast<uint32_t(*)[32]>(s + half * 32));
-              tc_wait_st();
-              tc_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&pready[half * 2 + x]);
-            }
+          for (int e = 0; e < NC; e += 2) {
+            float p0, p1;
+            unpack2(fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nmc2), p0, p1);
+            p0 = ex2(p0), p1 = ex2(p1);
+            uint32_t pk;
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(pk) : "f"(p1), "f"(p0));
+            if (FormB || Score) addx[e / 2 % 2] = add2(addx[e / 2 % 2], pack2(p0, p1));
+            if (!FormB)
+              add[e / 2 % 2] =
+                  add2(add[e / 2 % 2], pack2(__uint_as_float(pk << 16), __uint_as_float(pk & 0xFFFF0000u)));
+            s[e / 2] = pk;
           }
-          if constexpr (F > 1) {
+          if constexpr (F == 1) {
+            tc_st32(tS + hc * 32, *reinterpret_cast<uint32_t(*)[32]>(s));
+          } else {
             // this copy's columns, zeros in the others'
             uint32_t zero[16];
 #pragma unroll
@@ -685,8 +687,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (F == 2) tc_st16(tS + q * 32 + 16, zero);
               }
             }
-            tc_wait_st();
           }
+          tc_wait_st();
           float a0, a1, b0, b1;
           if (FormB || Score) {
             unpack2(addx[0], a0, a1);
@@ -698,49 +700,67 @@ __global__ void __launch_bounds__(kThreads, 1)
             unpack2(add[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
           }
-        } else if (F == 1) {
-          if (lane == 0) mbar_arrive(&pready[x]), mbar_arrive(&pready[2 + x]);
         }
-        if (F > 1) {
-          tc_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pready[x]);
-        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[x]);
         ++done;
       }
       i0 += items;
       j0 += w.n;
       if (FormB) l = lx;
       // ---- the unit's rows: accumulators in TMEM, statistics in the threads
-      if (first < items) wait(&pvdone[x], (done - 1) & 1);
+      wait(odone, w.seg & 1);
+      if (releases && lane == 0 && first < items) mbar_arrive(&empty[v_pos(j0 - (FormB || ((items - 1 - first) & 1) == 0 ? 1 : 2)) % NS]);
       float f0 = 1.f, f1 = 0.f, M = m, L = l, Lx = lx;
+      const int at = quarter * 32 + lane;
+      if (H == 2) {  // the sums of the two warps of a row
+        float2* sums = reinterpret_cast<float2*>(xchg);
+        if (hc == 1) sums[at] = make_float2(l, lx);
+        named_bar(pair_bar, 64);
+        if (hc == 0) {
+          const float2 o = sums[at];
+          L = l = l + o.x;
+          Lx = lx = lx + o.y;
+          if (FormB) sums[at] = make_float2(l, lx);
+        }
+        if (FormB) {
+          named_bar(pair_bar, 64);
+          if (hc == 1) L = sums[at].x, Lx = sums[at].y;
+          named_bar(pair_bar, 64);  // read before the next unit writes
+        } else {
+          named_bar(3, 256 * H);
+        }
+      }
       if (!FormB) {
         // the two accumulators of a row lie in the same TMEM lane: both warpgroups join them, each
         // for half the dims
-        const int at = quarter * 32 + lane;
-        if (x == 1) stat[at] = make_float4(m, l, lx, 0.f);
-        named_bar(1, 256);
+        if (x == 1 && hc == 0) stat[at] = make_float4(m, l, lx, 0.f);
+        named_bar(1, 256 * H);
         float m0 = m, m1 = m;
-        if (x == 0) {
+        if (x == 0 && hc == 0) {
           const float4 o = stat[at];
           m1 = o.x;
           M = fmaxf(m, m1);
           const float e0 = m == NEG_INF ? 0.f : ex2((m - M) * c), e1 = m1 == NEG_INF ? 0.f : ex2((m1 - M) * c);
           L = e0 * l + e1 * o.y;
           Lx = e0 * lx + e1 * o.z;
-          stat[at] = make_float4(m, M, L, Lx);
+          // (the threads that know one of m0, m1 need the other: it is not the larger, M, or both are)
+          stat[at] = make_float4(fminf(m, m1), M, L, Lx);
         }
-        named_bar(2, 256);
-        if (x == 1) {
+        named_bar(2, 256 * H);
+        if (x == 1 || hc == 1) {
           const float4 o = stat[at];
-          m0 = o.x, M = o.y, L = o.z, Lx = o.w;
+          M = o.y, L = o.z, Lx = o.w;
+          const float other = m == M ? o.x : M;
+          (x == 0 ? m1 : m0) = other;
         }
         f0 = m0 == NEG_INF ? 0.f : ex2((m0 - M) * c);
         f1 = m1 == NEG_INF ? 0.f : ex2((m1 - M) * c);
         if (M != M || L != L) f0 = f1 = 1.f;  // a NaN logit: L is NaN, the row will be
         if (F > 1) {
           // and the copies of the row, each with the sums of its own columns
-          const float own = M;
+          const float mine = M;
           float Mf = NEG_INF, Lf = 0.f, Lxf = 0.f;
 #pragma unroll
           for (int q = 0; q < F; ++q) Mf = fmaxf(Mf, stat[q * kRowsF + row].y);
@@ -751,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Lf = fmaf(e, o.z, Lf);
             Lxf = fmaf(e, o.w, Lxf);
           }
-          const float e = own == NEG_INF ? 0.f : ex2((own - Mf) * c);
+          const float e = mine == NEG_INF ? 0.f : ex2((mine - Mf) * c);
           f0 *= e, f1 *= e;
           M = Mf, L = Lf, Lx = Lxf;
         }
@@ -764,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
       float* part = a.part + (slot * rows + prow) * kD;
       const bool ok = !*bad;
-      if (in && ok && (FormB || x == 0) && copy == 0) {
+      if (in && ok && (FormB || x == 0) && copy == 0 && hc == 0) {
         if (!whole) {
           a.pstat[slot * rows + prow] = make_float2(M, L);
           if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
@@ -774,7 +794,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float inv = whole ? 1.f / L : 1.f;
       const uint4 nf4 = has_draft ? nfs[w.seg % kNf] : make_uint4(0, 0, 0, 0);
-      const bool odd = in && ((nf4.x & sees[0]) | (nf4.y & sees[1]) | (nf4.z & sees[2]) | (nf4.w & sees[3]));
+      bool odd = false;
+      uint32_t sees[4] = {0, 0, 0, 0};
+      if (nf4.x | nf4.y | nf4.z | nf4.w) {
+        if (in) node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
+        odd = ((nf4.x & sees[0]) | (nf4.y & sees[1]) | (nf4.z & sees[2]) | (nf4.w & sees[3])) != 0;
+      }
       // N finished sums of dims d0 .. of this thread's row go out
       auto put = [&](auto& o, int d0) {
         constexpr int N = sizeof(o) / 4;
@@ -808,21 +833,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // 32 dims of the joined accumulators of this lane
       auto get = [&](float (&o)[32], int d0) {
-        uint32_t r0[32], r1[32];
-        tc_ld32_raw(tmem + 256 + lanes + d0, r0);
-        tc_ld32_raw(tmem + 384 + lanes + d0, r1);
-        tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float v0 = f0 > 0.f ? __uint_as_float(r0[e]) * f0 : 0.f;
-          const float v1 = f1 > 0.f ? __uint_as_float(r1[e]) * f1 : 0.f;
-          o[e] = (v0 + v1) * inv;
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r0[16], r1[16];
+          tc_ld16_raw(tmem + 256 + lanes + d0 + q * 16, r0);
+          tc_ld16_raw(tmem + 384 + lanes + d0 + q * 16, r1);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float v0 = f0 > 0.f ? __uint_as_float(r0[e]) * f0 : 0.f;
+            const float v1 = f1 > 0.f ? __uint_as_float(r1[e]) * f1 : 0.f;
+            o[q * 16 + e] = (v0 + v1) * inv;
+          }
         }
       };
       if constexpr (FormB) {
         if (!idle && ok) {
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = hc * 2; q < hc * 2 + 2; ++q) {
             uint32_t r0[32];
             float o[32];
             tc_ld32_raw(tO + q * 32, r0);
@@ -834,12 +862,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else if constexpr (F == 1) {
         if (!idle && ok) {
-#pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
-            float o[32];
-            get(o, x * 64 + q * 32);
-            put(o, x * 64 + q * 32);
-          }
+          float o[32];
+          get(o, x * 64 + hc * 32);
+          put(o, x * 64 + hc * 32);
         }
       } else {
         // the copies' sums meet in shared memory, 32 dims of each warpgroup's half at a time
@@ -849,7 +874,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok) {
             float o[32];
             get(o, x * 64 + q * 32);
-            const int at = quarter * 32 + lane;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               *reinterpret_cast<float4*>(mine + at * 32 + ((e ^ (at & 7)) << 2)) =
@@ -875,8 +899,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_before();
-      // both halves of a row are read before either accumulator is written again
-      if (!FormB) named_bar(3, 256);
+      // both halves of a row are read before either accumulator is written again (and the statistics)
+      if (!FormB) named_bar(3, 256 * H);
     }
   }
   __syncwarp();
@@ -1287,7 +1311,7 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   a.base = reinterpret_cast<int*>(ws + wk.base);
   a.err = dev_err;
   cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(kThreads), kSmem, cs, dim3(0), qm, km, vm, kdm, vdm, a);
+  cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(threads_of(copies)), kSmem, cs, dim3(0), qm, km, vm, kdm, vdm, a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn launch: %s", cudaGetErrorString(e));
   const long long rows = static_cast<long long>(B) * T * Hq;
   auto join = p.form_b ? (score ? combine_kernel<true, true> : combine_kernel<true, false>)
