@@ -70,7 +70,7 @@ struct Args {
   __nv_bfloat16* out;
   const __nv_bfloat16* vd;
   const int *parents, *slot_pos, *lens;
-  float* part;     // [grid][2][rows][128] partial accumulators, rows = 128 (form A) or 256
+  float* part;     // [grid][2][128][rows] partial accumulators, rows = 128 (form A) or 256
   float2* pstat;   // [grid][2][rows] their maximum and sum(s)
   float* lse;      // [B][T][Hq] log2 of the sum of weights, for the score (or null)
   int* base;       // [B + 1] first key tile of each sequence (with lens)
@@ -782,11 +782,11 @@ __global__ void __launch_bounds__(threads_of(F), 1)
       const int rows = FormB ? 256 : 128;
       const int prow = FormB ? x * 128 + row : row;
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
-      float* part = a.part + (slot * rows + prow) * kD;
+      float* part = a.part + slot * kD * rows + prow;  // (a dim's rows side by side: stores of whole lines)
       const bool ok = !*bad;
       if (in && ok && (FormB || x == 0) && copy == 0 && hc == 0) {
         if (!whole) {
-          a.pstat[slot * rows + prow] = make_float2(M, L);
+          a.pstat[slot * rows + prow] = used ? make_float2(M, L) : make_float2(NEG_INF, 0.f);
           if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
         } else if (Score) {
           a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
@@ -826,9 +826,8 @@ __global__ void __launch_bounds__(threads_of(F), 1)
             dst[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
         } else {
-          float4* dst = reinterpret_cast<float4*>(part + d0);
 #pragma unroll
-          for (int e = 0; e < N / 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < N; ++e) part[static_cast<size_t>(d0 + e) * rows] = o[e];
         }
       };
       // 32 dims of the joined accumulators of this lane
@@ -909,80 +908,81 @@ __global__ void __launch_bounds__(threads_of(F), 1)
   if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(misc[0]), "r"(512));
 }
 
-// Joins the parts of units that a border cut: a warp per output row.
+// Joins the parts of units that a border cut: a block for 32 rows of a row tile (a lane each), a warp
+// for four dims.
 template <bool FormB, bool Score>
-__global__ void __launch_bounds__(256) combine_kernel(const Args a) {
+__global__ void __launch_bounds__(1024) combine_kernel(const Args a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(a.B) * a.T * a.Hq) return;
-  const int h = static_cast<int>(row % a.Hq);
-  const int t = static_cast<int>(row / a.Hq % a.T), b = static_cast<int>(row / a.Hq / a.T);
-  const int rt = t / a.npt, pair = FormB ? rt >> 1 : 0, u = h / a.G * a.pairs + pair;
-  const int nt = tiles_of(len_of(a, b)), per = a.Hkv * a.pairs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // blocks: sequence, kv head, pair, (row tile of the pair, 32 rows of it)
+  const int groups = (a.npt * a.G + 31) / 32, per_unit = (FormB ? 2 : 1) * groups, per = a.Hkv * a.pairs;
+  const int b = blockIdx.x / (per * per_unit), u = blockIdx.x / per_unit % per, part = blockIdx.x % per_unit;
+  const int half = FormB ? part / groups : 0, r = part % groups * 32 + lane;
+  const int h = u / a.pairs, rt = FormB ? u % a.pairs * 2 + half : 0;
+  const int nt = tiles_of(len_of(a, b));
   const long long total = a.lens ? a.base[a.B] : static_cast<long long>(nt) * per * a.B;
   const long long t0 = (a.lens ? a.base[b] : static_cast<long long>(nt) * per * b) + static_cast<long long>(u) * nt;
   const long long g = total < a.grid ? total : a.grid;
   const int c0 = static_cast<int>(((t0 + 1) * g - 1) / total);
   const int c1 = static_cast<int>(((t0 + nt) * g - 1) / total);
   if (c0 == c1) return;  // written by the CTA that had it all
+  const int t = rt * a.npt + r / a.G;
+  if (r >= a.npt * a.G || t >= a.T) return;
   const int rows = FormB ? 256 : 128;
-  const int prow = (FormB ? (rt & 1) * 128 : 0) + (t - rt * a.npt) * a.G + h % a.G;
-  auto slot_of = [&](int c) {
-    const bool later = c == c0 && total * c0 / g < t0;  // the unit is not the CTA's first
-    return (static_cast<size_t>(c) * 2 + (later ? 1 : 0)) * rows + prow;
-  };
+  const int prow = half * 128 + r;
+  // the unit's first part is its CTA's second where it does not begin there
+  const int later = total * c0 / g < t0 ? 1 : 0;
+  auto slot = [&](int c) { return static_cast<size_t>(c) * 2 + (c == c0 ? later : 0); };
   const float NEG_INF = -__int_as_float(0x7f800000);
   float M = NEG_INF;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.pstat[slot_of(c)].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) M = fmaxf(M, a.pstat[slot(c) * rows + prow].x);
   const float* exact = reinterpret_cast<const float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows);
-  float L = 0.f, Lx = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f, Lx = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int c = c0; c <= c1; ++c) {
-    const size_t s = slot_of(c);
-    const float2 st = a.pstat[s];
-    const float f = st.x == NEG_INF ? 0.f : ex2((st.x - M) * a.c);
-    const float4 v = reinterpret_cast<const float4*>(a.part + s * kD)[lane];
-    if (st.x != NEG_INF) {
-      L = fmaf(f, st.y, L);
-      if (Score) Lx = fmaf(f, exact[s], Lx);
-      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-    }
+    const size_t s = slot(c);
+    const float2 st = a.pstat[s * rows + prow];
+    const float* v = a.part + (s * kD + warp * 4) * rows + prow;
+    const float v0 = v[0], v1 = v[rows], v2 = v[2 * rows], v3 = v[3 * rows];
+    const float e = st.x == NEG_INF ? 0.f : ex2((st.x - M) * a.c);
+    L = fmaf(e, st.y, L);
+    if (Score && warp == 0) Lx = fmaf(e, exact[s * rows + prow], Lx);
+    if (e != 0.f) o[0] = fmaf(e, v0, o[0]), o[1] = fmaf(e, v1, o[1]), o[2] = fmaf(e, v2, o[2]), o[3] = fmaf(e, v3, o[3]);
   }
-  uint32_t sees[4];
-  const bool used = node_sees(a.parents + static_cast<size_t>(b) * a.T, t, sees, nullptr);
+  const bool used = L != 0.f;  // (a node in use sees itself; the parts of another say nothing)
   const float inv = 1.f / L;
-  reinterpret_cast<uint2*>(a.out + row * kD)[lane] =
-      used ? make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv)) : make_uint2(0, 0);
-  if (Score && lane == 0) a.lse[row] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
+  const size_t orow = (static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G;
+  *reinterpret_cast<uint2*>(a.out + orow * kD + warp * 4) =
+      used ? make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)) : make_uint2(0, 0);
+  if (Score && warp == 0) a.lse[orow] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
 }
 
 // ------------------------------------------------------------------------------------
-// score: S^T = K . Q^T, a slot per TMEM lane; every thread keeps its slot's largest weight of each
-// node over the heads in shared memory, and the CTA max-accumulates it into the score at the end.
+// score: S^T = K . Q^T, a slot per TMEM lane, the columns query head by query head (nodes side by side),
+// so that the maximum over the heads stays in the thread's registers and, over the kv heads, in its
+// words of shared memory; the CTA max-accumulates it into the score at the end, along the slots.
+// Several small CTAs share an SM: the loads of one hide behind the weights of another.
 // ------------------------------------------------------------------------------------
 constexpr int kScoreThreads = 9 * 32;  // 8 warps over the columns, one for TMA and MMA
-constexpr int kScoreBuf = 2 * kTile;   // K and Q of one head
-constexpr int kScOffMax = 2 * kScoreBuf;                    // float [128 nodes][128 slots]
-constexpr int kScOffLse = kScOffMax + kMaxNodes * 128 * 4;  // float [2][128]
-constexpr int kScOffSee = kScOffLse + 2 * 128 * 4;          // uint4 [128]
+constexpr int kScOffQ = kTile;                      // K, then Q of one item
+constexpr int kScOffLse = 2 * kTile;                // float [128]
+constexpr int kScOffSee = kScOffLse + 128 * 4;      // uint4 [128]
 constexpr int kScOffBars = kScOffSee + kMaxNodes * 16;
-constexpr int kScSmem = kScOffBars + 128;
-static_assert(kScSmem <= 232448, "shared memory");
+constexpr int kScOffMax = kScOffBars + 64;          // float [nodes, a multiple of 8][128 slots]
+constexpr int score_smem(int T) { return kScOffMax + (T + 7) / 8 * 8 * 128 * 4; }
 
 struct ScoreArgs {
   Args a;
   float* score;  // [B][T][S + T]
   int tiles;     // key tiles of a sequence: ceil(S / 128) + 1
   int hsplit;    // groups of kv heads
-  int npt;       // nodes of a column tile (their rows: at most 128)
+  int chunk;     // nodes of an item, a multiple of 8
+  int gb;        // query heads of an item: gb * chunk <= 128
 };
 
-__global__ void __launch_bounds__(kScoreThreads, 1)
+__global__ void __launch_bounds__(kScoreThreads, 3)
     score_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap kdmap, const ScoreArgs p) {
   extern __shared__ __align__(1024) uint8_t base[];
@@ -991,18 +991,18 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
   float* slse = reinterpret_cast<float*>(base + kScOffLse);
   uint4* see = reinterpret_cast<uint4*>(base + kScOffSee);
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + kScOffBars);
-  uint64_t* full = bars;       // [2] K and Q landed
-  uint64_t* sfull = bars + 2;  // [2] S^T written
-  uint64_t* sfree = bars + 4;  // [2] S^T read by the 8 warps
-  uint64_t* drain = bars + 6;  // after a wait that gave up
-  uint32_t* misc = reinterpret_cast<uint32_t*>(bars + 8);
+  uint64_t* full = bars;       // K and Q landed
+  uint64_t* sfull = bars + 1;  // S^T written
+  uint64_t* sfree = bars + 2;  // S^T read by the 8 warps
+  uint64_t* drain = bars + 3;  // after a wait that gave up
+  uint32_t* misc = reinterpret_cast<uint32_t*>(bars + 4);
   volatile int* bad = reinterpret_cast<volatile int*>(misc + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int tile = blockIdx.x, hg = blockIdx.y, b = blockIdx.z;
   const bool drafted = tile == p.tiles - 1;
   const int h0 = hg * a.Hkv / p.hsplit, h1 = (hg + 1) * a.Hkv / p.hsplit;
   if (tid == 0) {
-    for (int i = 0; i < 7; ++i) mbar_init(bars + i, i == 4 || i == 5 ? 8 : 1);
+    for (int i = 0; i < 4; ++i) mbar_init(bars + i, i == 2 ? 8 : 1);
     *bad = 0;
     if (smem_u32(base) & 1023) {
       *bad = 1;
@@ -1011,9 +1011,11 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
     fence_barrier_init();
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "r"(512));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "r"(128));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
+  const int T8 = (a.T + 7) / 8 * 8;
+  for (int i = tid; i < T8 * 128; i += kScoreThreads) best[i] = 0.f;
   pdl_launch_dependents();
   pdl_wait();
   if (drafted)
@@ -1022,15 +1024,18 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
       node_sees(a.parents + static_cast<size_t>(b) * a.T, t, s, nullptr);
       see[t] = make_uint4(s[0], s[1], s[2], s[3]);
     }
-  for (int i = tid; i < a.T * 128; i += kScoreThreads) best[i] = 0.f;
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = misc[0];
   const int len = len_of(a, b);
   const bool any = drafted || tile * kKeys < len;
-  const int chunks = (a.T + p.npt - 1) / p.npt;
-  const int items = any ? chunks * (h1 - h0) : 0;
+  const int gparts = (a.G + p.gb - 1) / p.gb, chunks = (a.T + p.chunk - 1) / p.chunk;
+  const int items = any ? (h1 - h0) * gparts * chunks : 0;
+  // item i: kv head, first query head, first node (the kv head changes last: K is loaded once for it)
+  auto head_of = [&](int i) { return h0 + i / (gparts * chunks); };
+  auto g_of = [&](int i) { return i / chunks % gparts * p.gb; };
+  auto node_of = [&](int i) { return i % chunks * p.chunk; };
   auto wait = [&](uint64_t* bar, uint32_t ph) {
     if (mbar_try_wait(bar, ph)) return;
     for (uint32_t i = 0; i < (1u << 22); ++i) {
@@ -1042,92 +1047,104 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
     *bad = 1;
   };
   if (warp == 8) {
-    if (elect_one()) {
-      const int R = p.npt * a.G;
-      const uint32_t id = tc_idesc(128, (R + 15) / 16 * 16, 0);
-      int loaded = 0;
-      auto load = [&](int i) {
-        loaded = i + 1;
-        const int x = i & 1, h = h0 + i % (h1 - h0), n0 = i / (h1 - h0) * p.npt;
-        uint8_t* k = base + x * kScoreBuf;
-        const CUtensorMap* m = drafted ? &kdmap : &kmap;
-        const int y = drafted ? 0 : tile * kKeys, z = b * a.Hkv + h;
-        mbar_expect_tx(&full[x], kTile + 2 * R * 128);
-        for (int hf = 0; hf < 2; ++hf) {
-          tma_load_3d(k + hf * kHalf, m, &full[x], 64 * hf, y, z);
-          tma_load_3d(k + kTile + hf * kHalf, &qmap, &full[x], 64 * hf, h * a.G, b * a.T + n0);
+    const bool leader = elect_one();
+    int loaded = 0;
+    auto load = [&](int i) {
+      const int h = head_of(i), g0 = g_of(i), gn = min(p.gb, a.G - g0);
+      const bool new_k = i == 0 || head_of(i - 1) != h;
+      loaded = i + 1;
+      if (!leader || *bad) return;
+      mbar_expect_tx(full, (new_k ? kTile : 0) + gn * p.chunk * 256);
+      for (int hf = 0; hf < 2; ++hf) {
+        if (new_k) {
+          if (drafted)
+            tma_load_3d(base + hf * kHalf, &kdmap, full, 64 * hf, 0, b * a.Hkv + h);
+          else
+            tma_load_3d(base + hf * kHalf, &kmap, full, 64 * hf, tile * kKeys, b * a.Hkv + h);
         }
-      };
-      if (items > 0 && !*bad) load(0);
-      if (items > 1 && !*bad) load(1);
-      for (int i = 0; i < items; ++i) {
-        const int x = i & 1;
-        wait(&full[x], (i >> 1) & 1);
-        if (i >= 2) wait(&sfree[x], ((i >> 1) - 1) & 1);
-        if (*bad) break;
-        tc_after();
-        const uint32_t k = smem_u32(base + x * kScoreBuf);
+        for (int g = 0; g < gn; ++g)  // a query head's nodes: whole swizzle atoms of 8 rows
+          tma_load_3d(base + kScOffQ + hf * kHalf + g * p.chunk * 128, &qmap, full, 64 * hf, h * a.G + g0 + g,
+                      b * a.T + node_of(i));
+      }
+    };
+    if (items > 0) load(0);
+    const uint64_t dk = tc_sdesc(smem_u32(base)), dq = tc_sdesc(smem_u32(base + kScOffQ));
+    for (int i = 0; i < items; ++i) {
+      wait(full, i & 1);
+      if (i > 0) wait(sfree, (i - 1) & 1);
+      tc_after();
+      const uint32_t id = tc_idesc(128, (min(p.gb, a.G - g_of(i)) * p.chunk + 15) / 16 * 16, 0);
+      if (leader && !*bad) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-          tc_mma(tmem + x * 128, tc_sdesc(k + off), tc_sdesc(k + kTile + off), id, ks > 0);
+          const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+          tc_mma(tmem, dk + off, dq + off, id, ks > 0);
         }
-        tc_commit(&sfull[x]);
-        if (i + 2 < items) {
-          wait(&sfull[x], (i >> 1) & 1);  // the product has read the buffers
-          if (!*bad) load(i + 2);
-        }
+        tc_commit(sfull);
       }
-      if (*bad) {  // copies and products in flight end before their memory goes
-        tc_commit(drain);
-        mbar_wait_bounded(drain, 0, 1u << 16);
-        for (int i = loaded > 2 ? loaded - 2 : 0; i < loaded; ++i) mbar_wait_bounded(&full[i & 1], (i >> 1) & 1, 1u << 16);
+      __syncwarp();
+      if (i + 1 < items) {
+        wait(sfull, i & 1);  // the product has read the buffers
+        load(i + 1);
       }
+    }
+    if (leader && *bad) {  // copies and products in flight end before their memory goes
+      tc_commit(drain);
+      mbar_wait_bounded(drain, 0, 1u << 14);
+      if (loaded) mbar_wait_bounded(full, (loaded - 1) & 1, 1u << 14);
     }
     __syncwarp();
   } else {
-    const int sl = (warp & 3) * 32 + lane, part = warp >> 2;  // slot; half of the nodes
+    const int sl = (warp & 3) * 32 + lane, part = warp >> 2;  // slot; which of every two blocks of 8 nodes
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int key = tile * kKeys + sl;
     const bool live = drafted ? sl < a.T
                               : key < len && (!a.slot_pos || a.slot_pos[static_cast<size_t>(b) * a.S + key] >= 0);
     for (int i = 0; i < items; ++i) {
-      const int x = i & 1, h = h0 + i % (h1 - h0), n0 = i / (h1 - h0) * p.npt;
-      const int nodes = min(p.npt, a.T - n0), cols = nodes * a.G;
+      const int h = head_of(i), g0 = g_of(i), gn = min(p.gb, a.G - g0), n0 = node_of(i);
       named_bar(1, 256);  // the previous item's statistics have been read
-      for (int r = tid; r < cols; r += 256)
-        slse[r] = a.lse[(static_cast<size_t>(b) * a.T + n0 + r / a.G) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G];
-      wait(&sfull[x], (i >> 1) & 1);
+      for (int r = tid; r < gn * p.chunk; r += 256) {
+        const int t = n0 + r % p.chunk;
+        slse[r] = t < a.T ? a.lse[(static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + g0 + r / p.chunk]
+                          : __int_as_float(0x7f800000);
+      }
+      wait(sfull, i & 1);
       named_bar(2, 256);
       tc_after();
-      if (!*bad) {
-        // this warp's nodes [lo, hi), their columns in chunks of 16
-        const int lo = part * ((nodes + 1) / 2), hi = min(nodes, lo + (nodes + 1) / 2);
-        int node = lo, g = 0;
-        float mx = 0.f;
-        for (int c0 = lo * a.G; c0 < hi * a.G; c0 += 16) {
-          float v[16];
-          tc_ld16(tmem + x * 128 + lanes + c0, v);
+      for (int n = part * 8; n < p.chunk && n0 + n < a.T; n += 16) {
+        float mx[8];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (c0 + e < hi * a.G) {
-              const float s = a.neg ? -v[e] : v[e];
-              mx = fmaxf(mx, ex2(fmaf(s, a.c, -slse[c0 + e])));
-              if (++g == a.G) {
-                const int t = n0 + node;
-                float* at = best + t * 128 + sl;
-                *at = fmaxf(*at, mx);
-                g = 0, mx = 0.f, ++node;
-              }
+        for (int e = 0; e < 8; ++e) mx[e] = 0.f;
+        for (int g = 0; g < gn; g += 4) {
+          uint32_t v[4][8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (g + q < gn) tc_ld8_raw(tmem + lanes + (g + q) * p.chunk + n, v[q]);
+          tc_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (g + q >= gn) break;
+            const float4* ls = reinterpret_cast<const float4*>(slse + (g + q) * p.chunk + n);
+            const float4 l0 = ls[0], l1 = ls[1];
+            const float lse[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float s = __uint_as_float(v[q][e]);
+              mx[e] = fmaxf(mx[e], ex2(fmaf(a.neg ? -s : s, a.c, -lse[e])));
             }
           }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float* at = best + (n0 + n + e) * 128 + sl;
+          *at = fmaxf(*at, mx[e]);
         }
       }
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sfree[x]);
+      if (lane == 0) mbar_arrive(sfree);
     }
-    // (the nodes' halves depend on the column tile: wait for both)
+    // (the blocks of nodes shift between warps from chunk to chunk: wait for all)
     named_bar(1, 256);
     if (live && any && !*bad) {
       for (int t = part; t < a.T; t += 2) {
@@ -1147,7 +1164,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1)
   __syncwarp();
   tc_before();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128));
 }
 
 }  // namespace ta
@@ -1302,6 +1319,14 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   a.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   const int most = sms < kMaxGrid ? sms : kMaxGrid;
   a.grid = static_cast<int>(total < most ? total : most);
+  if (!lens) {
+    // Equal ranges over all SMs cut units anywhere, and each cut costs its CTA another set of partial
+    // results (about two tiles' time).  With few units, the same number of CTAs for each of them cuts
+    // none needlessly: 64 units of 10 tiles, 34 us on 148 CTAs, 26 us on 128.
+    const long long units = total / tiles, each = most / units;
+    if (units <= most && (tiles + each - 1) / each + 2 <= (total + most - 1) / most + 4 && each <= tiles)
+      a.grid = static_cast<int>(units * each);
+  }
   a.out = static_cast<__nv_bfloat16*>(out);
   a.vd = static_cast<const __nv_bfloat16*>(v_draft);
   a.parents = parents, a.slot_pos = S > 0 ? slot_pos : nullptr, a.lens = lens;
@@ -1313,26 +1338,31 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(threads_of(copies)), kSmem, cs, dim3(0), qm, km, vm, kdm, vdm, a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn launch: %s", cudaGetErrorString(e));
-  const long long rows = static_cast<long long>(B) * T * Hq;
+  const long long blocks = static_cast<long long>(B) * Hkv * p.pairs * (p.form_b ? 2 : 1) * ((p.npt * G + 31) / 32);
   auto join = p.form_b ? (score ? combine_kernel<true, true> : combine_kernel<true, false>)
                        : (score ? combine_kernel<false, true> : combine_kernel<false, false>);
-  e = launch_pdl(join, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, cs, dim3(0), a);
+  e = launch_pdl(join, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, cs, dim3(0), a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn join launch: %s", cudaGetErrorString(e));
   if (score) {
     ScoreArgs sa{};
     sa.a = a;
     sa.score = node_score;
     sa.tiles = static_cast<int>(tiles);
-    const long long units = tiles * B;
-    long long hs = (2LL * sms + units - 1) / units;
-    sa.hsplit = static_cast<int>(hs < 1 ? 1 : hs > Hkv ? Hkv : hs);
-    if (sa.hsplit > 65535) sa.hsplit = 65535;
-    sa.npt = T < 128 / G ? T : 128 / G;
-    CUtensorMap sqm;
-    if ((st = map_rows(&sqm, q, Hq, static_cast<long long>(B) * T, G, sa.npt))) return st;
-    if (!prepare_device(reinterpret_cast<const void*>(score_kernel), kScSmem))
+    // nodes in eights, as many as fit beside the query heads; heads in sixteens beyond that
+    sa.gb = G < 16 ? G : 16;
+    const int fit = 128 / sa.gb / 8 * 8, all = (T + 7) / 8 * 8;
+    sa.chunk = all < fit ? all : fit;
+    const int smem = score_smem(T);
+    if (!prepare_device(reinterpret_cast<const void*>(score_kernel), score_smem(kMaxNodes)))
       return fail(kStatusCuda, "tree_attn: no usable device");
-    e = launch_pdl(score_kernel, dim3(static_cast<unsigned>(tiles), sa.hsplit, B), dim3(kScoreThreads), kScSmem, cs,
+    // kv heads of a sequence's tile side by side while there are SMs for them
+    const int resident = smem <= 76800 ? 3 : smem <= 115712 ? 2 : 1;
+    const long long units = tiles * B;
+    const long long hs = (static_cast<long long>(resident) * sms + units - 1) / units;
+    sa.hsplit = static_cast<int>(hs < 1 ? 1 : hs > Hkv ? Hkv : hs);
+    CUtensorMap sqm;
+    if ((st = map_rows(&sqm, q, Hq, static_cast<long long>(B) * T, 1, sa.chunk))) return st;
+    e = launch_pdl(score_kernel, dim3(static_cast<unsigned>(tiles), sa.hsplit, B), dim3(kScoreThreads), smem, cs,
                    dim3(0), sqm, km, kdm, sa);
     if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn score launch: %s", cudaGetErrorString(e));
   }
