@@ -151,6 +151,39 @@ __device__ __forceinline__ bool node_sees(const int* par, int t, uint32_t (&sees
 // in uniform registers (the operands of tcgen05 and TMA instructions).
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
+// The parents of a tree, four to a lane, and the same walk with them: a whole warp, each lane from its
+// node ``t`` (-1: none).  Steps cost a few shuffles; through memory they were 0.3 us each.
+struct Parents {
+  int p[4];
+  __device__ __forceinline__ void load(const int* par, int T, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = i * 32 + lane < T ? par[i * 32 + lane] : -2;
+  }
+  __device__ __forceinline__ bool sees(int t, int T, uint32_t (&bits)[4]) const {
+    bits[0] = bits[1] = bits[2] = bits[3] = 0;
+    bool used = t >= 0;
+    while (__any_sync(0xffffffffu, t >= 0)) {
+      int up = __shfl_sync(0xffffffffu, p[0], t & 31);
+      if (T > 32) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+          const int v = __shfl_sync(0xffffffffu, p[i], t & 31);
+          if ((t >> 5) == i) up = v;
+        }
+      }
+      if (t >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((t >> 5) == i) bits[i] |= 1u << (t & 31);
+        if (up >= t || up < -1) used = false;
+        t = used ? up : -1;
+      }
+    }
+    if (!used) bits[0] = bits[1] = bits[2] = bits[3] = 0;
+    return used;
+  }
+};
+
 // A walk over the CTA's range of key tiles, unit by unit, by whole warps.
 struct Walk {
   int t, end;        // global key tiles left: [t, end)
@@ -233,10 +266,10 @@ __global__ void __launch_bounds__(threads_of(F), 1)
   if (warp == kProducer) {
     const int per = a.Hkv * a.pairs;
     int total, b0, base0;
-    // CTAs that share the tiles: no more than there are tiles
+    // border c of the CTAs' ranges, total * c / g over g CTAs (no more than there are tiles)
     auto border = [&](int c) {
-      const int g = min(a.grid, total);
-      return c < g ? static_cast<int>(static_cast<long long>(total) * c / g) : total;
+      const int g = min(a.grid, total), q = total / g;
+      return c < g ? q * c + (total - q * g) * c / g : total;
     };
     if (!a.lens) {
       const int nt = tiles_of(a.S) * per;
@@ -458,12 +491,17 @@ __global__ void __launch_bounds__(threads_of(F), 1)
       const bool drafted = tile == x.nt - 1;
       uint32_t m[4];
       if (drafted) {
-        const int* par = a.parents + static_cast<size_t>(x.b) * a.T;
+        Parents tree;
+        tree.load(a.parents + static_cast<size_t>(x.b) * a.T, a.T, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t sees[4];
           const int t = i * 32 + lane;
-          m[i] = __ballot_sync(0xffffffffu, t < a.T && node_sees(par, t, sees, a.err));
+          m[i] = 0;
+          if (i * 32 < a.T) {
+            m[i] = __ballot_sync(0xffffffffu, tree.sees(t < a.T ? t : -1, a.T, sees));
+            if (t < a.T && tree.p[i] >= t) set_err(a.err, kErrIndex);
+          }
         }
       } else {
         int p[4];
@@ -549,6 +587,8 @@ __global__ void __launch_bounds__(threads_of(F), 1)
     const bool releases = quarter == 0 && hc == 0 && (!FormB || x == 1);  // hands tiles back
     int i0 = 0, j0 = 0;  // the CTA's items and key tiles before this unit
     int done = 0;        // items of this accumulator so far
+    Parents tree;
+    int tree_of = -1;  // the sequence whose tree it is
     while (w.next(a)) {
       const int rt = FormB ? w.pair * 2 + x : 0;  // row tile
       const int node = rt * a.npt + row / a.G;
@@ -558,9 +598,13 @@ __global__ void __launch_bounds__(threads_of(F), 1)
 #pragma unroll
       for (int q = 0; q < NC / 32; ++q) own[q] = 0;
       bool used = false;
-      if (in) {
+      {
+        if (w.b != tree_of) {
+          tree.load(a.parents + static_cast<size_t>(w.b) * a.T, a.T, lane);
+          tree_of = w.b;
+        }
         uint32_t sees[4];
-        used = node_sees(a.parents + static_cast<size_t>(w.b) * a.T, node, sees, nullptr);
+        used = tree.sees(in ? node : -1, a.T, sees);
         if constexpr (F == 4) {
           own[0] = copy == 0 ? sees[0] : copy == 1 ? sees[1] : copy == 2 ? sees[2] : sees[3];
         } else {
@@ -908,13 +952,13 @@ __global__ void __launch_bounds__(threads_of(F), 1)
   if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(misc[0]), "r"(512));
 }
 
-// Joins the parts of units that a border cut: a block for 32 rows of a row tile (a lane each), a warp
-// for four dims.
+// Joins the parts of units that a border cut: a block for 32 rows of a row tile (a lane each) and 32
+// dims, four to a warp.
 template <bool FormB, bool Score>
-__global__ void __launch_bounds__(1024) combine_kernel(const Args a) {
+__global__ void __launch_bounds__(256) combine_kernel(const Args a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   // blocks: sequence, kv head, pair, (row tile of the pair, 32 rows of it)
   const int groups = (a.npt * a.G + 31) / 32, per_unit = (FormB ? 2 : 1) * groups, per = a.Hkv * a.pairs;
   const int b = blockIdx.x / (per * per_unit), u = blockIdx.x / per_unit % per, part = blockIdx.x % per_unit;
@@ -1341,7 +1385,7 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   const long long blocks = static_cast<long long>(B) * Hkv * p.pairs * (p.form_b ? 2 : 1) * ((p.npt * G + 31) / 32);
   auto join = p.form_b ? (score ? combine_kernel<true, true> : combine_kernel<true, false>)
                        : (score ? combine_kernel<false, true> : combine_kernel<false, false>);
-  e = launch_pdl(join, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, cs, dim3(0), a);
+  e = launch_pdl(join, dim3(static_cast<unsigned>(blocks), 4), dim3(256), 0, cs, dim3(0), a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn join launch: %s", cudaGetErrorString(e));
   if (score) {
     ScoreArgs sa{};
