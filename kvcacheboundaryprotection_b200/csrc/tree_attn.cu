@@ -32,6 +32,8 @@
 //
 // score_kernel forms p again from the final row statistics: S^T = K . Q^T with a slot per thread, so
 // that the maximum over heads stays in the thread and the score rows are written along the slots.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kvbp_internal.h"
 
@@ -67,6 +69,7 @@ struct Args {
   float c;    // |scale| * log2(e), > 0
   int neg;    // scale < 0
   int grid;
+  int join;   // (Join) CTAs of the cluster that works on a unit and joins it itself
   __nv_bfloat16* out;
   const __nv_bfloat16* vd;
   const int *parents, *slot_pos, *lens;
@@ -216,7 +219,7 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return n == nt; }
 };
 
-template <int F, bool FormB, bool Score>
+template <int F, bool FormB, bool Score, bool Join>
 __global__ void __launch_bounds__(threads_of(F), 1)
     attend_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kdmap,
@@ -826,12 +829,17 @@ __global__ void __launch_bounds__(threads_of(F), 1)
       const int rows = FormB ? 256 : 128;
       const int prow = FormB ? x * 128 + row : row;
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (w.seg > 0 ? 1 : 0);
-      float* part = a.part + slot * kD * rows + prow;  // (a dim's rows side by side: stores of whole lines)
+      // (a dim's rows side by side: stores of whole lines.  A cluster's parts stay in shared memory: the
+      // ring is idle once the CTA's one segment is done.)
+      float* part = (Join ? reinterpret_cast<float*>(ring) : a.part + slot * kD * rows) + prow;
+      float2* pstat = Join ? reinterpret_cast<float2*>(ring + kD * rows * 4) : a.pstat + slot * rows;
+      float* pexact = Join ? reinterpret_cast<float*>(ring + kD * rows * 4 + rows * 8)
+                           : reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows) + slot * rows;
       const bool ok = !*bad;
       if (in && ok && (FormB || x == 0) && copy == 0 && hc == 0) {
         if (!whole) {
-          a.pstat[slot * rows + prow] = used ? make_float2(M, L) : make_float2(NEG_INF, 0.f);
-          if (Score) reinterpret_cast<float*>(a.pstat + static_cast<size_t>(a.grid) * 2 * rows)[slot * rows + prow] = Lx;
+          pstat[prow] = used ? make_float2(M, L) : make_float2(NEG_INF, 0.f);
+          if (Score) pexact[prow] = Lx;
         } else if (Score) {
           a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
         }
@@ -950,6 +958,60 @@ __global__ void __launch_bounds__(threads_of(F), 1)
   tc_before();
   __syncthreads();
   if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(misc[0]), "r"(512));
+  if constexpr (Join) {
+    // ---- the cluster's CTAs have the parts of one unit in their shared memory: each joins some of the
+    // dims, eight at a time (a warp for 32 rows)
+    cluster_sync_all();
+    const int p = a.join, rank = blockIdx.x % p, u = blockIdx.x / p;
+    const int b = u / (a.Hkv * a.pairs), h = u / a.pairs % a.Hkv, pair = u % a.pairs;
+    constexpr int rows = FormB ? 256 : 128;
+    const float NEG_INF = -__int_as_float(0x7f800000);
+    const uint32_t mem = smem_u32(ring);
+    const int d_lo = rank * 16 / p, d_hi = (rank + 1) * 16 / p;  // groups of 8 dims
+    const int groups = (R + 31) / 32, units = groups * NQ * (d_hi - d_lo);
+    if (warp < kProducer)
+      for (int i = warp; i < units; i += kProducer) {
+        const int d0 = (d_lo + i / (groups * NQ)) * 8, half = NQ == 2 ? i / groups % NQ : 0;
+        const int r = i % groups * 32 + lane, t = (pair * NQ + half) * a.npt + r / a.G;
+        if (r >= R || t >= a.T) continue;
+        const int prow = half * 128 + r;
+        float M = NEG_INF, L = 0.f, Lx = 0.f, o[8];
+        float2 st[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < p) st[q] = ld_dsmem_f2(mapa_u32(mem + kD * rows * 4 + prow * 8, q));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < p) M = fmaxf(M, st[q].x);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q >= p) break;
+          const uint32_t at = mapa_u32(mem + (d0 * rows + prow) * 4, q);
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = ld_dsmem_f32(at + e * rows * 4);
+          const float f = st[q].x == NEG_INF ? 0.f : ex2((st[q].x - M) * a.c);
+          L = fmaf(f, st[q].y, L);
+          if (Score && d0 == 0) Lx = fmaf(f, ld_dsmem_f32(mapa_u32(mem + kD * rows * 4 + rows * 8 + prow * 4, q)), Lx);
+          if (f != 0.f) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
+          }
+        }
+        const bool used = L != 0.f;
+        const float inv = 1.f / L;
+        const size_t orow = (static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G;
+        uint32_t pk[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pk[e] = used ? pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
+        *reinterpret_cast<uint4*>(a.out + orow * kD + d0) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        if (Score && d0 == 0) a.lse[orow] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
+      }
+    __syncwarp();
+    cluster_sync_all();  // its parts are read before a CTA leaves
+  }
 }
 
 // Joins the parts of units that a border cut: a block for 32 rows of a row tile (a lane each) and 32
@@ -1349,11 +1411,7 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   }
   const bool score = node_score != nullptr;
   const int copies = p.form_b ? 1 : p.npt * G <= 32 ? 4 : p.npt * G <= 64 ? 2 : 1;
-  auto kernel = p.form_b      ? (score ? attend_kernel<1, true, true> : attend_kernel<1, true, false>)
-                : copies == 4 ? (score ? attend_kernel<4, false, true> : attend_kernel<4, false, false>)
-                : copies == 2 ? (score ? attend_kernel<2, false, true> : attend_kernel<2, false, false>)
-                              : (score ? attend_kernel<1, false, true> : attend_kernel<1, false, false>);
-  const int sms = prepare_device(reinterpret_cast<const void*>(kernel), kSmem);
+  const int sms = prepare_device(reinterpret_cast<const void*>(attend_kernel<1, false, false, false>), kSmem);
   if (!sms) return fail(kStatusCuda, "tree_attn: no usable device");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Args a{};
@@ -1363,13 +1421,35 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   a.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   const int most = sms < kMaxGrid ? sms : kMaxGrid;
   a.grid = static_cast<int>(total < most ? total : most);
+  a.join = 0;
+  bool cut = true;  // some unit may lie in two CTAs' ranges
   if (!lens) {
-    // Equal ranges over all SMs cut units anywhere, and each cut costs its CTA another set of partial
-    // results (about two tiles' time).  With few units, the same number of CTAs for each of them cuts
-    // none needlessly: 64 units of 10 tiles, 34 us on 148 CTAs, 26 us on 128.
-    const long long units = total / tiles, each = most / units;
-    if (units <= most && (tiles + each - 1) / each + 2 <= (total + most - 1) / most + 4 && each <= tiles)
-      a.grid = static_cast<int>(units * each);
+    // How the units are shared out, by the time of the slowest CTA in key tiles:
+    //  * equal ranges over all SMs: the best balance, but a CTA begins twice where a border lies inside a
+    //    unit (about two), and a second launch joins the parts (about five);
+    //  * n CTAs for each unit: borders between units;
+    //  * the n a cluster, which joins its parts in shared memory (about one and a half), or n = 1.
+    // Each wave of CTAs begins anew (about three).  clusters[n]: how many clusters of n CTAs with this much
+    // shared memory a B200 holds.  On B200: 64 units of 10 tiles 25 us by ranges over 148 CTAs, 20 us in
+    // clusters of 2; 48 units of 65 (form B) 75 us by ranges, 70 us on 3 CTAs a unit; 512 units of 34
+    // 189 us by ranges, 222 us in clusters of 2.
+    static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    const long long units = total / tiles, n_all = most / units;
+    double best = static_cast<double>(total) / most + 10;
+    if (n_all >= 1 && n_all <= tiles && (tiles + n_all - 1) / n_all + 8 < best) {
+      best = static_cast<double>((tiles + n_all - 1) / n_all + 8);
+      a.grid = static_cast<int>(units * n_all);
+    }
+    for (int n = 1; n <= 8 && n <= tiles; ++n) {
+      const double waves = static_cast<double>((units + clusters[n] - 1) / clusters[n]);
+      const double time = waves * ((tiles + n - 1) / n + 3) + (n > 1 ? 1.5 : 0);
+      if (time < best) {
+        best = time;
+        cut = false;
+        a.join = n;
+        a.grid = static_cast<int>(units * n);
+      }
+    }
   }
   a.out = static_cast<__nv_bfloat16*>(out);
   a.vd = static_cast<const __nv_bfloat16*>(v_draft);
@@ -1380,12 +1460,25 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
   a.base = reinterpret_cast<int*>(ws + wk.base);
   a.err = dev_err;
   cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(threads_of(copies)), kSmem, cs, dim3(0), qm, km, vm, kdm, vdm, a);
+  const bool joined = a.join > 1;
+  auto pick = [&](auto score_c, auto join_c) {
+    constexpr bool sc = decltype(score_c)::value, jn = decltype(join_c)::value;
+    return p.form_b      ? attend_kernel<1, true, sc, jn>
+           : copies == 4 ? attend_kernel<4, false, sc, jn>
+           : copies == 2 ? attend_kernel<2, false, sc, jn>
+                         : attend_kernel<1, false, sc, jn>;
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  auto kernel = score ? (joined ? pick(Yes{}, Yes{}) : pick(Yes{}, No{})) : (joined ? pick(No{}, Yes{}) : pick(No{}, No{}));
+  if (!prepare_device(reinterpret_cast<const void*>(kernel), kSmem)) return fail(kStatusCuda, "tree_attn: no usable device");
+  cudaError_t e = launch_pdl(kernel, dim3(a.grid), dim3(threads_of(copies)), kSmem, cs,
+                             joined ? dim3(a.join, 1, 1) : dim3(0), qm, km, vm, kdm, vdm, a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn launch: %s", cudaGetErrorString(e));
   const long long blocks = static_cast<long long>(B) * Hkv * p.pairs * (p.form_b ? 2 : 1) * ((p.npt * G + 31) / 32);
   auto join = p.form_b ? (score ? combine_kernel<true, true> : combine_kernel<true, false>)
                        : (score ? combine_kernel<false, true> : combine_kernel<false, false>);
-  e = launch_pdl(join, dim3(static_cast<unsigned>(blocks), 4), dim3(256), 0, cs, dim3(0), a);
+  if (cut) e = launch_pdl(join, dim3(static_cast<unsigned>(blocks), 4), dim3(256), 0, cs, dim3(0), a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_attn join launch: %s", cudaGetErrorString(e));
   if (score) {
     ScoreArgs sa{};
