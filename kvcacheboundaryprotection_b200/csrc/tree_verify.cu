@@ -8,8 +8,16 @@
 // Each test keeps the target's law: P(accept x) + the residual's mass add up to r / R.  The
 // last accepted node's r gives one more token: the first x whose running sum exceeds u * R.
 //
-// Weights and sums are double: a token is chosen where a running sum of a hundred thousand
-// terms passes a border, and 32 bits would choose another one every few hundred draws.
+// A token is chosen where a running sum of a hundred thousand terms passes a border; it has to be the
+// token that the definition gives, so sums in 32 bits are trusted only as far as their error goes:
+// every node's row is read once with fp32 weights, whose sums are off by less than ``eps`` of the row's; a
+// test or a draw that comes out the same anywhere within that is decided, another one is made again with
+// double weights (one in some ten thousand tests, and draws that end in a flat tail).  The residuals of a
+// random draft, differences of near values, are double from the start.
+//
+// A cluster of CTAs per sequence, each with a contiguous share of the row, each warp with a contiguous
+// share of that: a warp's sum is both part of the row's and, for the draw, the sum of what lies before the
+// next one's.  The CTAs exchange their sums through shared memory and take every decision alike.
 #include <math.h>
 
 #include "common.cuh"
@@ -18,9 +26,11 @@
 namespace kvbp {
 namespace tv {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxNodes = 128;
+constexpr int kMaxCluster = 8;
+constexpr int kNone = 0x7fffffff;
 
 struct Args {
   int T, V;
@@ -39,214 +49,511 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ float logit(const float* row, int x) { return row[x]; }
-__device__ __forceinline__ float logit(const __nv_bfloat16* row, int x) { return __bfloat162float(row[x]); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <typename L>
-__global__ void __launch_bounds__(kThreads) verify_kernel(Args a) {
-  __shared__ float red_f[kWarps];
-  __shared__ int red_i[kWarps];
-  __shared__ double red_d[kWarps];
-  __shared__ double s_R[kMaxNodes + 1];
+struct Row;
+template <>
+struct Row<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ void many(const uint4& v, float (&x)[8]) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  }
+};
+template <>
+struct Row<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void many(const uint4& v, float (&x)[8]) {
+    x[0] = bf16lo(v.x), x[1] = bf16hi(v.x), x[2] = bf16lo(v.y), x[3] = bf16hi(v.y);
+    x[4] = bf16lo(v.z), x[5] = bf16hi(v.z), x[6] = bf16lo(v.w), x[7] = bf16hi(v.w);
+  }
+};
+
+// What one CTA tells the others: its largest logit and the first index of it, its sum relative to that;
+// or a double sum.
+struct alignas(16) Message {
+  float top;
+  int first;
+  double sum;
+};
+
+// e^y, y <= 0, to about 1e-14: y = n ln2 / 32 + r, e^r by its series, 2^(n / 32) from a table.
+__device__ __forceinline__ double exp_of(double y, const double* table) {
+  if (!(y > -700.0)) return 0.0;
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the nearest integer is left in the low bits
+  const double t = fma(y, 46.166241308446828384, kRound);  // 32 / ln 2
+  const int n = __double2loint(t);
+  const double r = fma(t - kRound, -0.021660849392498290195, y);  // ln 2 / 32
+  double p = fma(r, 1.0 / 120, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  const double v = table[n & 31] * p;
+  return __hiloint2double(__double2hiint(v) + (n >> 5) * (1 << 20), __double2loint(v));
+}
+
+template <typename L>
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
+  using R = Row<L>;
+  constexpr int N = R::N;
+  __shared__ Message box[2];
+  __shared__ float w_top[kWarps];
+  __shared__ int w_first[kWarps];
+  __shared__ double w_sum[kWarps];  // each warp's sum at the current node, relative to ``top``
+  __shared__ double s_R[kMaxNodes + 1], s_inv[kMaxNodes + 1];  // sums after 0, 1, ... rejections
   __shared__ int s_rej[kMaxNodes];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int T = a.T, V = a.V;
+  __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes];
+  __shared__ double table[32];
+  __shared__ __align__(8) int s_token[2];  // the draw: token, and whether it is certain
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float NEG_INF = -__int_as_float(0x7f800000);
-  const int* par = a.parents + static_cast<size_t>(b) * T;
-  const int* tok = a.tokens + static_cast<size_t>(b) * T;
+  uint32_t rank, cs;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cs));
+  const int b = blockIdx.x / cs;
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int T = a.T, V = a.V;
+  for (int i = tid; i < T; i += kThreads) {
+    s_par[i] = a.parents[static_cast<size_t>(b) * T + i];
+    s_tok[i] = a.tokens[static_cast<size_t>(b) * T + i];
+  }
+  __syncthreads();
   int* path = a.path + static_cast<size_t>(b) * T;
   const float heat = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(heat > 0.f);
   const double inv = 1.0 / static_cast<double>(greedy ? 1.f : heat);
-  if (par[0] != -1) {  // no tree
-    for (int i = tid; i < T; i += kThreads) path[i] = -1;
-    if (tid == 0) {
-      a.n_path[b] = 0;
-      a.next_token[b] = -1;
+  const float c = static_cast<float>(1.4426950408889634 * inv);
+  if (s_par[0] != -1) {  // no tree
+    if (rank == 0) {
+      for (int i = tid; i < T; i += kThreads) path[i] = -1;
+      if (tid == 0) {
+        a.n_path[b] = 0;
+        a.next_token[b] = -1;
+      }
     }
-    return;
+    return;  // the whole cluster does
   }
   const bool drawn = a.draft && !greedy;
   const L* row = nullptr;
   const float* q = nullptr;
-  float top = 0.f;
-  int first = 0, n_rej = 0;
-  // weight of token x at the current node before any rejection
-  auto weight = [&](int x) -> double {
-    if (greedy) return x == first ? 1.0 : 0.0;
-    const float l = logit(row, x);
-    if (l == top) return 1.0;
-    return l < top ? exp((static_cast<double>(l) - static_cast<double>(top)) * inv) : 0.0;  // NaN: none
+  // this warp's share of the row: the head up to the first 16-byte boundary (first warp), vectors
+  // [lo, hi), the tail (last warp)
+  int head = 0, tail = 0, lo = 0, hi = 0;
+  int parity = 0, n_rej = 0, first = kNone;
+  float top = NEG_INF;
+  double S = 0.0;      // the row's sum in fp32 weights
+  float eps = 0.f;
+  bool exact = false;  // s_R and w_sum are double sums
+
+  auto share = [&]() {
+    const int ahead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(L));
+    head = min(V, ahead);
+    const int vecs = (V - head) / N;
+    tail = V - head - vecs * N;
+    const int w = rank * kWarps + warp, all = cs * kWarps;
+    lo = static_cast<int>(static_cast<long long>(vecs) * w / all);
+    hi = static_cast<int>(static_cast<long long>(vecs) * (w + 1) / all);
+    if (w != 0) head = 0;
+    if (w != all - 1) tail = 0;
+    // error of the row's fp32 sum: the weights' (2^x of the hardware 2^-22; the exponent's three roundings
+    // 2^-24 of up to 31, beyond which a row's terms do not matter) and the joins': 24 steps of 2^-22;
+    // for each vector of a lane its sums and one change of the reference maximum: 3 steps
+    eps = (24.f + 3.f * static_cast<float>(vecs / (all * 32) + 1)) * 0x1p-22f;
   };
-  auto rest = [&](int x) -> double {  // what the rejections left of it
-    double r = weight(x);
-    for (int j = 0; j < n_rej; ++j) {
-      if (drawn)
-        r = fmax(r / s_R[j] - static_cast<double>(q[x]), 0.0);
-      else if (x == s_rej[j])
-        r = 0.0;
+  auto vec0 = [&]() { return min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(L))); };
+  auto clean = [&](float l) { return l == l ? l : NEG_INF; };
+
+  // ---- double weights
+  auto weight = [&](float l) -> double {
+    if (l == top) return 1.0;
+    return l < top ? exp_of((static_cast<double>(l) - static_cast<double>(top)) * inv, table) : 0.0;
+  };
+  auto rest = [&](int x, float l) -> double {  // what the rejections left of token x
+    if (greedy) return x == first ? 1.0 : 0.0;
+    double r = weight(l);
+    if (drawn) {
+      if (n_rej) {
+        const double qx = static_cast<double>(q[x]);
+        for (int j = 0; j < n_rej; ++j) r = fmax(fma(r, s_inv[j], -qx), 0.0);
+      }
+    } else {
+      for (int j = 0; j < n_rej; ++j)
+        if (x == s_rej[j]) r = 0.0;
     }
     return r;
   };
-  auto block_sum = [&](double v) -> double {
+  // every element of this warp's share in order: f(x, logit) a lane each
+  auto for_share = [&](auto f) {
+    const int v0 = vec0();
+    if (lane < head) f(lane, clean(R::one(row + lane)));
+    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+    for (int i = lo + lane; i < hi; i += 32) {
+      float x[8];
+      R::many(vec[i], x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(v0 + i * N + e, clean(x[e]));
+    }
+    if (lane < tail) f(V - tail + lane, clean(R::one(row + V - tail + lane)));
+  };
+
+  // ---- the messages of all CTAs, one a lane (lanes from cs on: none)
+  auto exchange = [&](const Message& m) {  // m: thread 0's
+    if (tid == 0) box[parity] = m;
+    cluster_sync_all();
+    Message got{NEG_INF, kNone, 0.0};
+    if (lane < static_cast<int>(cs)) {
+      const uint32_t at = mapa_u32(smem_u32(&box[parity]), lane);
+      uint32_t w0, w1, w2, w3;
+      asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3)
+                   : "r"(at)
+                   : "memory");
+      got.top = __uint_as_float(w0);
+      got.first = static_cast<int>(w1);
+      got.sum = __hiloint2double(static_cast<int>(w3), static_cast<int>(w2));
+    }
+    parity ^= 1;  // (the next exchange's barrier comes before this box is written again)
+    return got;
+  };
+  auto better = [](float m2, int i2, float m, int i) { return m2 > m || (m2 == m && i2 < i); };
+  auto scale_to = [&](float from, float to) { return from == to ? 1.f : ex2((from - to) * c); };
+  auto sum_lanes = [&](double v) {
+    for (int o = 1; o < kMaxCluster; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+  };
+
+  // ---- a node's row: its maximum and sum with fp32 weights
+  auto enter = [&](int node) {
+    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
+    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
+    n_rej = 0;
+    exact = false;
+    share();
+    float m = NEG_INF, s = 0.f;
+    int at = kNone;
+    bool nan = false;
+    auto take = [&](float mv, int i) {  // a new maximum of this lane
+      s *= m == NEG_INF ? 0.f : ex2((m - mv) * c);
+      m = mv, at = i;
+    };
+    auto single = [&](int x) {
+      float l = R::one(row + x);
+      nan |= l != l;
+      l = clean(l);
+      if (l > m || at == kNone) take(l, x);
+      if (!greedy) s += l == m ? 1.f : ex2((l - m) * c);
+    };
+    if (lane < head) single(lane);
+    const int v0 = vec0();
+    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+    constexpr int U = 5;  // loads in flight
+    for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * 32 < hi) v[u] = vec[i0 + u * 32];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * 32 >= hi) break;
+        float x[8], mv = NEG_INF;
+        R::many(v[u], x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          nan |= x[e] != x[e];
+          x[e] = clean(x[e]);
+          mv = fmaxf(mv, x[e]);
+        }
+        if (mv > m || at == kNone) {
+          int e0 = 0;
+#pragma unroll
+          for (int e = N - 1; e >= 0; --e)
+            if (x[e] == mv) e0 = e;
+          take(mv, v0 + (i0 + u * 32) * N + e0);
+        }
+        if (!greedy) {
+          float add = 0.f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) add += x[e] == m ? 1.f : ex2((x[e] - m) * c);
+          s += add;
+        }
+      }
+    }
+    if (lane < tail) single(V - tail + lane);
+    if (nan) set_err(a.err, kErrNanScore);
+    if (at == kNone) s = 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+      const float mm = fmaxf(m, m2);
+      s = s * scale_to(m, mm) + s2 * scale_to(m2, mm);
+      if (better(m2, a2, m, at)) at = a2;
+      m = mm;
+    }
+    __syncthreads();  // the previous node's sums have been read
+    if (lane == 0) w_top[warp] = m, w_first[warp] = at, w_sum[warp] = static_cast<double>(s);
+    __syncthreads();
+    // the CTA's, in every warp: lanes are its warps
+    float cm = lane < kWarps ? w_top[lane] : NEG_INF;
+    int ca = lane < kWarps ? w_first[lane] : kNone;
+    const float own_top = cm;
+    const double own_sum = lane < kWarps ? w_sum[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, cm, o);
+      const int a2 = __shfl_xor_sync(0xffffffffu, ca, o);
+      if (better(m2, a2, cm, ca)) cm = m2, ca = a2;
+    }
+    double sum = own_sum * static_cast<double>(scale_to(own_top, cm));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const Message got = exchange(Message{cm, ca, sum});
+    top = got.top, first = got.first;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, top, o);
+      const int a2 = __shfl_xor_sync(0xffffffffu, first, o);
+      if (better(m2, a2, top, first)) top = m2, first = a2;
+    }
+    top = __shfl_sync(0xffffffffu, top, 0);
+    first = __shfl_sync(0xffffffffu, first, 0);
+    S = sum_lanes(got.sum * static_cast<double>(scale_to(got.top, top)));
+    if (warp == 0 && lane < kWarps) w_sum[lane] = own_sum * static_cast<double>(scale_to(own_top, top));
+    if (tid == 0) s_R[0] = greedy ? 1.0 : S;
+    __syncthreads();
+  };
+  // ---- the double sum of what the first ``n`` rejections leave, to s_R[n] (and each warp's to w_sum)
+  auto sum_exact = [&](int n) {
+    const int keep = n_rej;
+    n_rej = n;
+    double v = 0.0;
+    for_share([&](int x, float l) { v += rest(x, l); });
+    n_rej = keep;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
-    if (lane == 0) red_d[warp] = v;
+    if (lane == 0) w_sum[warp] = v;
     __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < kWarps; ++w) t += red_d[w];
-    return t;
-  };
-  auto enter = [&](int node) {  // statistics of a node's row
-    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
-    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
-    float m = NEG_INF;
-    int at = 0x7fffffff;
-    bool nan = false;
-    for (int x = tid; x < V; x += kThreads) {
-      const float l = logit(row, x);
-      nan |= l != l;
-      if (l > m || (l == m && x < at)) {
-        m = l;
-        at = x;
-      }
-    }
-    if (nan) set_err(a.err, kErrNanScore);
+    double sum = lane < kWarps ? w_sum[lane] : 0.0;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-      if (m2 > m || (m2 == m && a2 < at)) {
-        m = m2;
-        at = a2;
-      }
-    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const Message got = exchange(Message{0.f, 0, sum});
+    const double all = sum_lanes(got.sum);
+    if (tid == 0) s_R[n] = all, s_inv[n] = 1.0 / all;
     __syncthreads();
-    if (lane == 0) {
-      red_f[warp] = m;
-      red_i[warp] = at;
-    }
-    __syncthreads();
-    top = red_f[0];
-    first = red_i[0];
-    for (int w = 1; w < kWarps; ++w)
-      if (red_f[w] > top || (red_f[w] == top && red_i[w] < first)) {
-        top = red_f[w];
-        first = red_i[w];
-      }
-    n_rej = 0;
-    double sum = 0.0;
-    if (!greedy)
-      for (int x = tid; x < V; x += kThreads) sum += weight(x);
-    sum = block_sum(sum);
-    if (tid == 0) s_R[0] = greedy ? 1.0 : sum;
-    __syncthreads();
+  };
+  auto make_exact = [&]() {  // every sum of the current node again, in double
+    if (exact) return;
+    exact = true;
+    if (greedy) return;
+    if (drawn)
+      for (int n = 0; n <= n_rej; ++n) sum_exact(n);
+    else
+      sum_exact(n_rej);
   };
 
   enter(0);
   int cur = 0, n = 1;
-  if (tid == 0) path[0] = 0;
+  if (rank == 0 && tid == 0) path[0] = 0;
   for (int j = 1; j < T; ++j) {
-    if (par[j] != cur) continue;
-    const int x = tok[j];
+    if (s_par[j] != cur) continue;
+    const int x = s_tok[j];
     if (x < 0 || x >= V) {
-      if (tid == 0) set_err(a.err, kErrIndex);
+      if (rank == 0 && tid == 0) set_err(a.err, kErrIndex);
       continue;
     }
-    const double u = static_cast<double>(a.accept_u[static_cast<size_t>(b) * T + j]);
-    const double qx = drawn ? static_cast<double>(q[x]) : 1.0;
-    const double rx = rest(x);
-    if (u * qx * s_R[n_rej] < rx) {
-      if (tid == 0) path[n] = j;
+    const double lhs = static_cast<double>(a.accept_u[static_cast<size_t>(b) * T + j]) *
+                       (drawn ? static_cast<double>(q[x]) : 1.0);
+    const double rx = rest(x, clean(R::one(row + x)));
+    bool yes;
+    if (exact || greedy) {
+      yes = lhs * s_R[n_rej] < rx;
+    } else {
+      const double off = S * eps;
+      const double left = s_R[n_rej];
+      yes = lhs * (left + off) < rx;
+      if (!yes && lhs * (left - off) < rx) {  // too near to say
+        make_exact();
+        yes = lhs * s_R[n_rej] < rx;
+      }
+    }
+    if (yes) {
+      if (rank == 0 && tid == 0) path[n] = j;
       ++n;
       cur = j;
-      __syncthreads();
       enter(j);
       continue;
     }
-    // rejected: the sum of what is left
-    double left;
     if (drawn) {
-      left = 0.0;
+      make_exact();
       ++n_rej;
-      for (int y = tid; y < V; y += kThreads) left += rest(y);
-      left = block_sum(left);
+      sum_exact(n_rej);
     } else {
-      left = s_R[n_rej] - rx;
-      if (tid == 0) s_rej[n_rej] = x;
+      __syncthreads();  // s_R[n_rej] has been read
+      if (tid == 0) {
+        s_rej[n_rej] = x;
+        s_R[n_rej + 1] = s_R[n_rej] - rx;
+      }
       ++n_rej;
       __syncthreads();
+      if (exact && !greedy) sum_exact(n_rej);
     }
-    if (tid == 0) s_R[n_rej] = left;
-    __syncthreads();
   }
-  for (int i = n + tid; i < T; i += kThreads) path[i] = -1;
-  // the next token: warps own contiguous ranges, the range where the running sum passes the
-  // border is walked again
-  const int seg = (V + kWarps - 1) / kWarps;
-  const int lo = min(V, warp * seg), hi = min(V, lo + seg);
-  auto range_sum = [&]() {
-    double v = 0.0;
-    for (int x = lo + lane; x < hi; x += 32) v += rest(x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
-  double mine = range_sum(), total = 0.0;
-  for (int round = 0; round < 2; ++round) {
-    __syncthreads();
-    if (lane == 0) red_d[warp] = mine;
-    __syncthreads();
-    total = 0.0;
-    for (int w = 0; w < kWarps; ++w) total += red_d[w];
-    if (total > 0.0 || n_rej == 0) break;
-    n_rej = 0;  // nothing is left: the node's own distribution
-    mine = range_sum();
+  if (rank == 0) {
+    for (int i = n + tid; i < T; i += kThreads) path[i] = -1;
+    if (tid == 0) a.n_path[b] = n;
   }
-  const double want = static_cast<double>(a.sample_u[b]) * total;
-  double before = 0.0;
-  int owner = -1, last = -1;
-  double at_owner = 0.0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (red_d[w] > 0.0) last = w;
-    if (owner < 0 && before + red_d[w] > want) {
-      owner = w;
-      at_owner = before;
+  // ---- the next token
+  if (greedy) {
+    if (rank == 0 && tid == 0) {
+      a.next_token[b] = first == kNone ? -1 : first;
+      if (first == kNone) set_err(a.err, kErrNanScore);
     }
-    before += red_d[w];
+    cluster_sync_all();  // messages are read before a CTA leaves
+    return;
   }
-  if (owner < 0) {  // u >= 1, or no weight at all
-    owner = last;
-    at_owner = before;
-  }
-  if (owner < 0) {
-    if (tid == 0) {
-      a.next_token[b] = -1;
-      set_err(a.err, kErrNanScore);
-    }
-  } else if (warp == owner) {
-    int pick = 0x7fffffff, any = -1;
-    double sum = at_owner;
-    for (int x0 = lo; x0 < hi && pick == 0x7fffffff; x0 += 32) {
-      const int x = x0 + lane;
-      const double r = x < hi ? rest(x) : 0.0;
-      double incl = r;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
+  for (int round = 0;; ++round) {
+    // sums of the warps before this one: the CTAs', then the warps'
+    double mine = lane < kWarps ? w_sum[lane] : 0.0;
+    if (!exact && lane < kWarps && n_rej) {  // rejected tokens leave their warps' fp32 sums
+      const int v0 = vec0(), vecs = (V - v0) / N, all = cs * kWarps, w = rank * kWarps + lane;
+      const int wl = static_cast<int>(static_cast<long long>(vecs) * w / all),
+                wh = static_cast<int>(static_cast<long long>(vecs) * (w + 1) / all);
+      const int from = w == 0 ? 0 : v0 + wl * N, to = w == all - 1 ? V : v0 + wh * N;
+      for (int j = 0; j < n_rej; ++j) {
+        const int x = s_rej[j];
+        bool again = false;
+        for (int k = 0; k < j; ++k) again |= s_rej[k] == x;
+        if (x >= from && x < to && !again) mine -= weight(clean(R::one(row + x)));
       }
-      const uint32_t pos = __ballot_sync(0xffffffffu, r > 0.0);
-      const uint32_t over = __ballot_sync(0xffffffffu, r > 0.0 && sum + incl > want);
-      if (over) pick = x0 + __ffs(over) - 1;
-      if (pos) any = x0 + 31 - __clz(pos);
-      sum += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (pick == 0x7fffffff) pick = any;
-    if (lane == 0) a.next_token[b] = pick;
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const double cta = __shfl_sync(0xffffffffu, incl, 31);
+    const Message got = exchange(Message{0.f, 0, cta});
+    double upto = got.sum;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    const double total = __shfl_sync(0xffffffffu, upto, kMaxCluster - 1);
+    if (exact && !(total > 0.0) && n_rej) {  // nothing is left: the node's own distribution
+      n_rej = 0;
+      sum_exact(0);
+      continue;
+    }
+    const double want = static_cast<double>(a.sample_u[b]) * total;
+    // the CTA and the warp where the sum passes the border (or the last ones with any weight)
+    const uint32_t over = __ballot_sync(0xffffffffu, lane < static_cast<int>(cs) && got.sum > 0.0 && upto > want);
+    const uint32_t some = __ballot_sync(0xffffffffu, lane < static_cast<int>(cs) && got.sum > 0.0);
+    const int owner = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : 0;
+    const double before = __shfl_sync(0xffffffffu, upto - got.sum, owner);
+    if (static_cast<int>(rank) == owner) {
+      const uint32_t wo = __ballot_sync(0xffffffffu, lane < kWarps && mine > 0.0 && before + incl > want);
+      const uint32_t ws = __ballot_sync(0xffffffffu, lane < kWarps && mine > 0.0);
+      const int w = wo ? __ffs(wo) - 1 : ws ? 31 - __clz(ws) : 0;
+      double sum = before + __shfl_sync(0xffffffffu, incl - mine, w);
+      if (warp == w) {
+        int pick = kNone, any = -1;
+        bool sure = exact;
+        const double off = exact ? 0.0 : 2.0 * S * eps;
+        // a chunk of the share: N elements a lane, contiguous
+        auto chunk = [&](const int* xs, const float* ls, int count, bool in) {
+          double r[8], here = 0.0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            r[e] = in && e < count ? rest(xs[e], ls[e]) : 0.0;
+            here += r[e];
+          }
+          double inc = here;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+          }
+          double at = sum + inc - here;
+          int mine_x = kNone, mine_any = -1;
+          bool mine_sure = true;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (r[e] > 0.0) {
+              mine_any = xs[e];
+              if (mine_x == kNone && at + r[e] > want) {
+                mine_x = xs[e];
+                mine_sure = at + off <= want && at + r[e] - off > want;
+              }
+            }
+            at += r[e];
+          }
+          const uint32_t hit = __ballot_sync(0xffffffffu, mine_x != kNone);
+          if (hit) {
+            const int l0 = __ffs(hit) - 1;
+            pick = __shfl_sync(0xffffffffu, mine_x, l0);
+            const bool s0 = __shfl_sync(0xffffffffu, static_cast<int>(mine_sure), l0) != 0;
+            sure = exact || s0;
+          }
+          const uint32_t has = __ballot_sync(0xffffffffu, mine_any >= 0);
+          if (has) any = __shfl_sync(0xffffffffu, mine_any, 31 - __clz(has));
+          sum += __shfl_sync(0xffffffffu, inc, 31);
+        };
+        int xs[8];
+        float ls[8];
+        const int v0 = vec0();
+        if (head) {  // (uniform: the warp's)
+          xs[0] = lane;
+          ls[0] = lane < head ? clean(R::one(row + lane)) : NEG_INF;
+          chunk(xs, ls, 1, lane < head);
+        }
+        const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+        for (int i0 = lo; i0 < hi && pick == kNone; i0 += 32) {
+          const int i = i0 + lane;
+          if (i < hi) {
+            R::many(vec[i], ls);
+#pragma unroll
+            for (int e = 0; e < N; ++e) xs[e] = v0 + i * N + e, ls[e] = clean(ls[e]);
+          }
+          chunk(xs, ls, N, i < hi);
+        }
+        if (tail && pick == kNone) {
+          xs[0] = V - tail + lane;
+          ls[0] = lane < tail ? clean(R::one(row + V - tail + lane)) : NEG_INF;
+          chunk(xs, ls, 1, lane < tail);
+        }
+        if (lane == 0) {
+          s_token[0] = pick != kNone ? pick : any;
+          s_token[1] = sure || (exact && pick == kNone);
+        }
+      }
+    }
+    cluster_sync_all();
+    uint32_t token, certain;
+    const uint32_t from = mapa_u32(smem_u32(s_token), owner);
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(token), "=r"(certain) : "r"(from) : "memory");
+    if (certain) {
+      if (rank == 0 && tid == 0) {
+        a.next_token[b] = static_cast<int>(token);
+        if (static_cast<int>(token) < 0) set_err(a.err, kErrNanScore);
+      }
+      break;
+    }
+    cluster_sync_all();  // the token is read before it is made again
+    make_exact();
   }
-  if (tid == 0) a.n_path[b] = n;
+  cluster_sync_all();  // messages are read before a CTA leaves
 }
 
 }  // namespace tv
@@ -268,7 +575,7 @@ extern "C" int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int3
   (void)workspace, (void)workspace_bytes;
   if (!target || !tokens || !parents || !accept_u || !sample_u || !path || !n_path || !next_token)
     return fail(kStatusArg, "tree_verify: null pointer");
-  if (B <= 0 || vocab <= 0 || B > 65535) return fail(kStatusArg, "tree_verify: bad size");
+  if (B <= 0 || vocab <= 0 || B > 1 << 24 || vocab > 0x7fffffff - 1024) return fail(kStatusArg, "tree_verify: bad size");
   if (T <= 0 || T > tv::kMaxNodes) return fail(kStatusUnsupported, "tree_verify: %d nodes (1 to %d)", T, tv::kMaxNodes);
   if (ldt < vocab || (draft_probs && ldd < vocab)) return fail(kStatusArg, "tree_verify: rows overlap");
   if (misaligned(target, fp32_target ? 4 : 2) || misaligned(draft_probs, 4))
@@ -276,11 +583,11 @@ extern "C" int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int3
   tv::Args a{T, vocab, target, ldt, temperature, tokens, parents, draft_probs, ldd, accept_u, sample_u, path, n_path,
              next_token, dev_err};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (fp32_target)
-    tv::verify_kernel<float><<<B, tv::kThreads, 0, st>>>(a);
-  else
-    tv::verify_kernel<__nv_bfloat16><<<B, tv::kThreads, 0, st>>>(a);
-  cudaError_t e = cudaGetLastError();
+  // CTAs of a sequence: as many as leave two an SM for the whole batch
+  int cs = 8;
+  while (cs > 1 && static_cast<long long>(B) * cs > 2 * 148) cs /= 2;
+  auto kernel = fp32_target ? tv::verify_kernel<float> : tv::verify_kernel<__nv_bfloat16>;
+  cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(B) * cs), dim3(tv::kThreads), 0, st, dim3(cs, 1, 1), a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_verify launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
