@@ -12,8 +12,8 @@
 // token that the definition gives, so sums in 32 bits are trusted only as far as their error goes:
 // every node's row is read once with fp32 weights, whose sums are off by less than ``eps`` of the row's; a
 // test or a draw that comes out the same anywhere within that is decided, another one is made again with
-// double weights (one in some ten thousand tests, and draws that end in a flat tail).  The residuals of a
-// random draft, differences of near values, are double from the start.
+// double weights (one in some ten thousand tests, and draws that end in a flat tail).  A random draft's
+// residuals, differences of near values, carry a bound of their own that grows with every rejection.
 //
 // A cluster of CTAs per sequence, each with a contiguous share of the row, each warp with a contiguous
 // share of that: a warp's sum is both part of the row's and, for the draw, the sum of what lies before the
@@ -26,8 +26,6 @@
 namespace kvbp {
 namespace tv {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxNodes = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kNone = 0x7fffffff;
@@ -84,7 +82,7 @@ struct alignas(16) Message {
 };
 
 // e^y, y <= 0, to about 1e-14: y = n ln2 / 32 + r, e^r by its series, 2^(n / 32) from a table.
-__device__ __forceinline__ double exp_of(double y, const double* table) {
+__device__ __noinline__ double exp_of(double y, const double* table) {
   if (!(y > -700.0)) return 0.0;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the nearest integer is left in the low bits
   const double t = fma(y, 46.166241308446828384, kRound);  // 32 / ln 2
@@ -99,17 +97,23 @@ __device__ __forceinline__ double exp_of(double y, const double* table) {
   return __hiloint2double(__double2hiint(v) + (n >> 5) * (1 << 20), __double2loint(v));
 }
 
-template <typename L>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
+// kThreads: 512, or 256 where two CTAs share an SM.  (128 registers a thread either way: at 64 the spills cost
+// more than the second CTA gains.)
+template <typename L, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a) {
+  constexpr int kWarps = kThreads / 32;
   using R = Row<L>;
   constexpr int N = R::N;
   __shared__ Message box[2];
   __shared__ float w_top[kWarps];
   __shared__ int w_first[kWarps];
+  __shared__ double s_part[kWarps];
   __shared__ double w_sum[kWarps];  // each warp's sum at the current node, relative to ``top``
   __shared__ double s_R[kMaxNodes + 1], s_inv[kMaxNodes + 1];  // sums after 0, 1, ... rejections
+  __shared__ float s_finv[kMaxNodes + 1];
   __shared__ int s_rej[kMaxNodes];
   __shared__ int s_par[kMaxNodes], s_tok[kMaxNodes];
+  __shared__ float s_u[kMaxNodes];
   __shared__ double table[32];
   __shared__ __align__(8) int s_token[2];  // the draw: token, and whether it is certain
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -125,10 +129,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
   for (int i = tid; i < T; i += kThreads) {
     s_par[i] = a.parents[static_cast<size_t>(b) * T + i];
     s_tok[i] = a.tokens[static_cast<size_t>(b) * T + i];
+    s_u[i] = a.accept_u[static_cast<size_t>(b) * T + i];
   }
+  const float heat = a.temperature ? a.temperature[b] : 1.f;
+  const float draw = a.sample_u[b];
   __syncthreads();
   int* path = a.path + static_cast<size_t>(b) * T;
-  const float heat = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(heat > 0.f);
   const double inv = 1.0 / static_cast<double>(greedy ? 1.f : heat);
   const float c = static_cast<float>(1.4426950408889634 * inv);
@@ -152,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
   float top = NEG_INF;
   double S = 0.0;      // the row's sum in fp32 weights
   float eps = 0.f;
+  double E = 0.0;  // how far the weights that the rejections of a random draft left may be off, all together
   bool exact = false;  // s_R and w_sum are double sums
 
   auto share = [&]() {
@@ -191,20 +198,25 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
     }
     return r;
   };
-  // every element of this warp's share in order: f(x, logit) a lane each
-  auto for_share = [&](auto f) {
-    const int v0 = vec0();
-    if (lane < head) f(lane, clean(R::one(row + lane)));
-    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
-    for (int i = lo + lane; i < hi; i += 32) {
-      float x[8];
-      R::many(vec[i], x);
-#pragma unroll
-      for (int e = 0; e < N; ++e) f(v0 + i * N + e, clean(x[e]));
+  auto rest_fast = [&](int x, float l) -> float {  // the same with fp32 weights
+    float r = l == top ? 1.f : ex2((l - top) * c);
+    if (drawn) {
+      if (n_rej) {
+        const float qx = q[x];
+        for (int j = 0; j < n_rej; ++j) r = fmaxf(fmaf(r, s_finv[j], -qx), 0.f);
+      }
+    } else {
+      for (int j = 0; j < n_rej; ++j)
+        if (x == s_rej[j]) r = 0.f;
     }
-    if (lane < tail) f(V - tail + lane, clean(R::one(row + V - tail + lane)));
+    return r;
   };
-
+  // the elements [from, to) of warp w of all the cluster's
+  auto range = [&](int w, int& from, int& to) {
+    const int v0 = vec0(), vecs = (V - v0) / N, all = cs * kWarps;
+    from = w == 0 ? 0 : v0 + static_cast<int>(static_cast<long long>(vecs) * w / all) * N;
+    to = w == all - 1 ? V : v0 + static_cast<int>(static_cast<long long>(vecs) * (w + 1) / all) * N;
+  };
   // ---- the messages of all CTAs, one a lane (lanes from cs on: none)
   auto exchange = [&](const Message& m) {  // m: thread 0's
     if (tid == 0) box[parity] = m;
@@ -224,7 +236,11 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
     parity ^= 1;  // (the next exchange's barrier comes before this box is written again)
     return got;
   };
-  auto better = [](float m2, int i2, float m, int i) { return m2 > m || (m2 == m && i2 < i); };
+  auto max_of = [](float v) {  // over the warp (no NaN), by an integer of the same order
+    const uint32_t u = __float_as_uint(v + 0.f);
+    const uint32_t k = __reduce_max_sync(0xffffffffu, (u >> 31) ? ~u : u | 0x80000000u);
+    return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+  };
   auto scale_to = [&](float from, float to) { return from == to ? 1.f : ex2((from - to) * c); };
   auto sum_lanes = [&](double v) {
     for (int o = 1; o < kMaxCluster; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -290,54 +306,34 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
     if (lane < tail) single(V - tail + lane);
     if (nan) set_err(a.err, kErrNanScore);
     if (at == kNone) s = 0.f;
+    const float wm = max_of(m);
+    const int wa = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(m == wm ? at : kNone)));
+    s *= scale_to(m, wm);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-      const float mm = fmaxf(m, m2);
-      s = s * scale_to(m, mm) + s2 * scale_to(m2, mm);
-      if (better(m2, a2, m, at)) at = a2;
-      m = mm;
-    }
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     __syncthreads();  // the previous node's sums have been read
-    if (lane == 0) w_top[warp] = m, w_first[warp] = at, w_sum[warp] = static_cast<double>(s);
+    if (lane == 0) w_top[warp] = wm, w_first[warp] = wa, w_sum[warp] = static_cast<double>(s);
     __syncthreads();
     // the CTA's, in every warp: lanes are its warps
-    float cm = lane < kWarps ? w_top[lane] : NEG_INF;
-    int ca = lane < kWarps ? w_first[lane] : kNone;
-    const float own_top = cm;
+    const float own_top = lane < kWarps ? w_top[lane] : NEG_INF;
     const double own_sum = lane < kWarps ? w_sum[lane] : 0.0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, cm, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, ca, o);
-      if (better(m2, a2, cm, ca)) cm = m2, ca = a2;
-    }
+    const float cm = max_of(own_top);
+    const int ca = static_cast<int>(
+        __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(lane < kWarps && own_top == cm ? w_first[lane] : kNone)));
     double sum = own_sum * static_cast<double>(scale_to(own_top, cm));
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const Message got = exchange(Message{cm, ca, sum});
-    top = got.top, first = got.first;
-#pragma unroll
-    for (int o = 1; o < kMaxCluster; o <<= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, top, o);
-      const int a2 = __shfl_xor_sync(0xffffffffu, first, o);
-      if (better(m2, a2, top, first)) top = m2, first = a2;
-    }
-    top = __shfl_sync(0xffffffffu, top, 0);
-    first = __shfl_sync(0xffffffffu, first, 0);
+    top = max_of(got.top);
+    first = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(got.top == top ? got.first : kNone)));
     S = sum_lanes(got.sum * static_cast<double>(scale_to(got.top, top)));
     if (warp == 0 && lane < kWarps) w_sum[lane] = own_sum * static_cast<double>(scale_to(own_top, top));
-    if (tid == 0) s_R[0] = greedy ? 1.0 : S;
+    if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
+    E = 0.0;
     __syncthreads();
   };
-  // ---- the double sum of what the first ``n`` rejections leave, to s_R[n] (and each warp's to w_sum)
-  auto sum_exact = [&](int n) {
-    const int keep = n_rej;
-    n_rej = n;
-    double v = 0.0;
-    for_share([&](int x, float l) { v += rest(x, l); });
-    n_rej = keep;
+  // ---- a warp's share ``v`` of the sum of what ``n`` rejections leave, to s_R[n] (and each warp's to w_sum)
+  auto join_sum = [&](int n, double v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
@@ -348,8 +344,65 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const Message got = exchange(Message{0.f, 0, sum});
     const double all = sum_lanes(got.sum);
-    if (tid == 0) s_R[n] = all, s_inv[n] = 1.0 / all;
+    if (tid == 0) s_R[n] = all, s_inv[n] = 1.0 / all, s_finv[n] = static_cast<float>(1.0 / all);
     __syncthreads();
+  };
+  auto sum_exact = [&](int n) {  // in double
+    const int keep = n_rej;
+    n_rej = n;
+    double v = 0.0;
+    int from, to;
+    range(rank * kWarps + warp, from, to);
+#pragma unroll 2
+    for (int x = from + lane; x < to; x += 32) v += rest(x, clean(R::one(row + x)));
+    n_rej = keep;
+    join_sum(n, v);
+  };
+  auto sum_fast = [&](int n) {  // (a random draft) in fp32; E from n - 1 to n
+    float v = 0.f;
+    const float inv0 = s_finv[0];
+    auto left = [&](float l, float qx) {
+      float r = fmaxf(fmaf(l == top ? 1.f : ex2((l - top) * c), inv0, -qx), 0.f);
+      for (int j = 1; j < n; ++j) r = fmaxf(fmaf(r, s_finv[j], -qx), 0.f);
+      return r;
+    };
+    const int v0 = vec0();
+    if (lane < head) v += left(clean(R::one(row + lane)), q[lane]);
+    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+    const float* qv = q + v0;
+    const bool whole = (reinterpret_cast<uintptr_t>(qv) & 15) == 0;
+    constexpr int U = 2;
+    for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
+      uint4 t[U];
+      float4 d[U][N / 4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * 32;
+        if (i >= hi) break;
+        t[u] = vec[i];
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+          const float* at = qv + static_cast<size_t>(i) * N + k * 4;
+          d[u][k] = whole ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * 32 >= hi) break;
+        float x[8], add = 0.f;
+        R::many(t[u], x);
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+          add += left(clean(x[4 * k]), d[u][k].x) + left(clean(x[4 * k + 1]), d[u][k].y);
+          add += left(clean(x[4 * k + 2]), d[u][k].z) + left(clean(x[4 * k + 3]), d[u][k].w);
+        }
+        v += add;
+      }
+    }
+    if (lane < tail) v += left(clean(R::one(row + V - tail + lane)), q[V - tail + lane]);
+    // weights off by E in all (at first by eps of their sum), divided by a sum that is as far off
+    E = (n == 1 ? 2.0 * eps : 2.0 * (E + eps * s_R[n - 1]) * s_inv[n - 1]) + 0x1p-22;
+    join_sum(n, static_cast<double>(v));
   };
   auto make_exact = [&]() {  // every sum of the current node again, in double
     if (exact) return;
@@ -371,19 +424,19 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
       if (rank == 0 && tid == 0) set_err(a.err, kErrIndex);
       continue;
     }
-    const double lhs = static_cast<double>(a.accept_u[static_cast<size_t>(b) * T + j]) *
+    const double lhs = static_cast<double>(s_u[j]) *
                        (drawn ? static_cast<double>(q[x]) : 1.0);
     const double rx = rest(x, clean(R::one(row + x)));
     bool yes;
     if (exact || greedy) {
       yes = lhs * s_R[n_rej] < rx;
     } else {
-      const double off = S * eps;
       const double left = s_R[n_rej];
-      yes = lhs * (left + off) < rx;
-      if (!yes && lhs * (left - off) < rx) {  // too near to say
+      const double off = drawn ? E + eps * left : S * eps;
+      yes = lhs * (left + off) < rx - E;
+      if (!yes && lhs * (left - off) < rx + E) {  // too near to say
         make_exact();
-        yes = lhs * s_R[n_rej] < rx;
+        yes = lhs * s_R[n_rej] < rest(x, clean(R::one(row + x)));
       }
     }
     if (yes) {
@@ -394,9 +447,10 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
       continue;
     }
     if (drawn) {
-      make_exact();
       ++n_rej;
-      sum_exact(n_rej);
+      if (!exact) sum_fast(n_rej);
+      if (!exact && !(E < 0.25 * s_R[n_rej])) make_exact();  // (nothing to go by)
+      else if (exact) sum_exact(n_rej);
     } else {
       __syncthreads();  // s_R[n_rej] has been read
       if (tid == 0) {
@@ -424,11 +478,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
   for (int round = 0;; ++round) {
     // sums of the warps before this one: the CTAs', then the warps'
     double mine = lane < kWarps ? w_sum[lane] : 0.0;
-    if (!exact && lane < kWarps && n_rej) {  // rejected tokens leave their warps' fp32 sums
-      const int v0 = vec0(), vecs = (V - v0) / N, all = cs * kWarps, w = rank * kWarps + lane;
-      const int wl = static_cast<int>(static_cast<long long>(vecs) * w / all),
-                wh = static_cast<int>(static_cast<long long>(vecs) * (w + 1) / all);
-      const int from = w == 0 ? 0 : v0 + wl * N, to = w == all - 1 ? V : v0 + wh * N;
+    if (!exact && !drawn && lane < kWarps && n_rej) {  // rejected tokens leave their warps' fp32 sums
+      int from, to;
+      range(rank * kWarps + lane, from, to);
       for (int j = 0; j < n_rej; ++j) {
         const int x = s_rej[j];
         bool again = false;
@@ -456,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
       sum_exact(0);
       continue;
     }
-    const double want = static_cast<double>(a.sample_u[b]) * total;
+    const double want = static_cast<double>(draw) * total;
     // the CTA and the warp where the sum passes the border (or the last ones with any weight)
     const uint32_t over = __ballot_sync(0xffffffffu, lane < static_cast<int>(cs) && got.sum > 0.0 && upto > want);
     const uint32_t some = __ballot_sync(0xffffffffu, lane < static_cast<int>(cs) && got.sum > 0.0);
@@ -467,71 +519,59 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Args a) {
       const uint32_t ws = __ballot_sync(0xffffffffu, lane < kWarps && mine > 0.0);
       const int w = wo ? __ffs(wo) - 1 : ws ? 31 - __clz(ws) : 0;
       double sum = before + __shfl_sync(0xffffffffu, incl - mine, w);
-      if (warp == w) {
+      // that warp's share again, split over the CTA's warps: their sums, then the one that has the border
+      int from, to;
+      range(rank * kWarps + w, from, to);
+      const int count = to - from;
+      to = from + static_cast<int>(static_cast<long long>(count) * (warp + 1) / kWarps);
+      from += static_cast<int>(static_cast<long long>(count) * warp / kWarps);
+      auto value = [&](int x) {
+        const float l = clean(R::one(row + x));
+        return exact ? rest(x, l) : static_cast<double>(rest_fast(x, l));
+      };
+      double part = 0.0;
+#pragma unroll 1
+      for (int x = from + lane; x < to; x += 32) part += value(x);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      if (lane == 0) s_part[warp] = part;
+      __syncthreads();
+      const double parts = lane < kWarps ? s_part[lane] : 0.0;
+      double pin = parts;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, pin, o);
+        if (lane >= o) pin += t;
+      }
+      const uint32_t po = __ballot_sync(0xffffffffu, lane < kWarps && parts > 0.0 && sum + pin > want);
+      const uint32_t ps = __ballot_sync(0xffffffffu, lane < kWarps && parts > 0.0);
+      const int sub = po ? __ffs(po) - 1 : ps ? 31 - __clz(ps) : 0;
+      sum += __shfl_sync(0xffffffffu, pin - parts, sub);
+      if (warp == sub) {
         int pick = kNone, any = -1;
         bool sure = exact;
-        const double off = exact ? 0.0 : 2.0 * S * eps;
-        // a chunk of the share: N elements a lane, contiguous
-        auto chunk = [&](const int* xs, const float* ls, int count, bool in) {
-          double r[8], here = 0.0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            r[e] = in && e < count ? rest(xs[e], ls[e]) : 0.0;
-            here += r[e];
-          }
-          double inc = here;
+        const double off = exact ? 0.0 : drawn && n_rej ? 2.0 * (E + eps * total) : 2.0 * S * eps;
+#pragma unroll 1
+        for (int x0 = from; x0 < to && pick == kNone; x0 += 32) {
+          const int x = x0 + lane;
+          const double r = x < to ? value(x) : 0.0;
+          double inc = r;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const double t = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += t;
           }
-          double at = sum + inc - here;
-          int mine_x = kNone, mine_any = -1;
-          bool mine_sure = true;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (r[e] > 0.0) {
-              mine_any = xs[e];
-              if (mine_x == kNone && at + r[e] > want) {
-                mine_x = xs[e];
-                mine_sure = at + off <= want && at + r[e] - off > want;
-              }
-            }
-            at += r[e];
-          }
-          const uint32_t hit = __ballot_sync(0xffffffffu, mine_x != kNone);
+          const bool over_here = r > 0.0 && sum + inc > want;
+          const uint32_t hit = __ballot_sync(0xffffffffu, over_here);
+          const uint32_t has = __ballot_sync(0xffffffffu, r > 0.0);
           if (hit) {
             const int l0 = __ffs(hit) - 1;
-            pick = __shfl_sync(0xffffffffu, mine_x, l0);
-            const bool s0 = __shfl_sync(0xffffffffu, static_cast<int>(mine_sure), l0) != 0;
-            sure = exact || s0;
+            pick = x0 + l0;
+            // the border lies inside the token's own stretch by more than the sums are off
+            sure = exact || __shfl_sync(0xffffffffu, sum + inc - r + off <= want && sum + inc - off > want, l0);
           }
-          const uint32_t has = __ballot_sync(0xffffffffu, mine_any >= 0);
-          if (has) any = __shfl_sync(0xffffffffu, mine_any, 31 - __clz(has));
+          if (has) any = x0 + 31 - __clz(has);
           sum += __shfl_sync(0xffffffffu, inc, 31);
-        };
-        int xs[8];
-        float ls[8];
-        const int v0 = vec0();
-        if (head) {  // (uniform: the warp's)
-          xs[0] = lane;
-          ls[0] = lane < head ? clean(R::one(row + lane)) : NEG_INF;
-          chunk(xs, ls, 1, lane < head);
-        }
-        const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
-        for (int i0 = lo; i0 < hi && pick == kNone; i0 += 32) {
-          const int i = i0 + lane;
-          if (i < hi) {
-            R::many(vec[i], ls);
-#pragma unroll
-            for (int e = 0; e < N; ++e) xs[e] = v0 + i * N + e, ls[e] = clean(ls[e]);
-          }
-          chunk(xs, ls, N, i < hi);
-        }
-        if (tail && pick == kNone) {
-          xs[0] = V - tail + lane;
-          ls[0] = lane < tail ? clean(R::one(row + V - tail + lane)) : NEG_INF;
-          chunk(xs, ls, 1, lane < tail);
         }
         if (lane == 0) {
           s_token[0] = pick != kNone ? pick : any;
@@ -583,11 +623,16 @@ extern "C" int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int3
   tv::Args a{T, vocab, target, ldt, temperature, tokens, parents, draft_probs, ldd, accept_u, sample_u, path, n_path,
              next_token, dev_err};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // CTAs of a sequence: as many as leave two an SM for the whole batch
+  // CTAs of a sequence: as many as a portable cluster has, for what takes the time is the longest path's chain
+  // of rows (64 sequences with a draft: 260 us with clusters of 4, 230 with 8); fewer from 75 sequences on,
+  // where the rows' bytes do.  CTAs of 512 threads while all are resident, one an SM; else of 256, two an SM
+  // (24 sequences: 47 us with 512, 30 with 256; one sequence with a draft: 46 and 54).
   int cs = 8;
-  while (cs > 1 && static_cast<long long>(B) * cs > 2 * 148) cs /= 2;
-  auto kernel = fp32_target ? tv::verify_kernel<float> : tv::verify_kernel<__nv_bfloat16>;
-  cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(B) * cs), dim3(tv::kThreads), 0, st, dim3(cs, 1, 1), a);
+  while (cs > 1 && static_cast<long long>(B) * cs > 4 * 148) cs /= 2;
+  const bool wide = static_cast<long long>(B) * cs <= 120;  // (clusters of 8 that fit: 15)
+  auto kernel = fp32_target ? (wide ? tv::verify_kernel<float, 512> : tv::verify_kernel<float, 256>)
+                            : (wide ? tv::verify_kernel<__nv_bfloat16, 512> : tv::verify_kernel<__nv_bfloat16, 256>);
+  cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(B) * cs), dim3(wide ? 512 : 256), 0, st, dim3(cs, 1, 1), a);
   if (e != cudaSuccess) return fail(kStatusCuda, "tree_verify launch: %s", cudaGetErrorString(e));
   return kStatusOk;
 }
