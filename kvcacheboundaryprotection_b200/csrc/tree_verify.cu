@@ -47,6 +47,12 @@ struct Args {
   int* err;
 };
 
+// maximum of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -157,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   int parity = 0, n_rej = 0, first = kNone;
   float top = NEG_INF;
   double S = 0.0;      // the row's sum in fp32 weights
-  float eps = 0.f;
+  float base_eps = 0.f, eps = 0.f;
+  bool odd_row = false;  // NaN or infinities decide: no short cuts
   double E = 0.0;  // how far the weights that the rejections of a random draft left may be off, all together
   bool exact = false;  // s_R and w_sum are double sums
 
@@ -171,13 +178,18 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     hi = static_cast<int>(static_cast<long long>(vecs) * (w + 1) / all);
     if (w != 0) head = 0;
     if (w != all - 1) tail = 0;
-    // error of the row's fp32 sum: the weights' (2^x of the hardware 2^-22; the exponent's three roundings
-    // 2^-24 of up to 31, beyond which a row's terms do not matter) and the joins': 24 steps of 2^-22;
+    // error of the row's fp32 sum: the weights' (2^x of the hardware 2^-22; the exponent's roundings, 2^-24 of
+    // up to 31, beyond which a row's terms do not matter, and of the maximum's, below) and the joins': 24 steps of 2^-22;
     // for each vector of a lane its sums and one change of the reference maximum: 3 steps
-    eps = (24.f + 3.f * static_cast<float>(vecs / (all * 32) + 1)) * 0x1p-22f;
+    base_eps = (24.f + 3.f * static_cast<float>(vecs / (all * 32) + 1)) * 0x1p-22f;
   };
   auto vec0 = [&]() { return min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(L))); };
   auto clean = [&](float l) { return l == l ? l : NEG_INF; };
+
+  auto sync_cluster = []() {
+    __syncwarp();  // (the cluster's barrier wants whole warps)
+    cluster_sync_all();
+  };
 
   // ---- double weights
   auto weight = [&](float l) -> double {
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   // ---- the messages of all CTAs, one a lane (lanes from cs on: none)
   auto exchange = [&](const Message& m) {  // m: thread 0's
     if (tid == 0) box[parity] = m;
-    cluster_sync_all();
+    sync_cluster();
     Message got{NEG_INF, kNone, 0.0};
     if (lane < static_cast<int>(cs)) {
       const uint32_t at = mapa_u32(smem_u32(&box[parity]), lane);
@@ -248,63 +260,70 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   };
 
   // ---- a node's row: its maximum and sum with fp32 weights
-  auto enter = [&](int node) {
-    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
-    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
-    n_rej = 0;
-    exact = false;
-    share();
+  auto read_row = [&](bool odd) {
     float m = NEG_INF, s = 0.f;
     int at = kNone;
-    bool nan = false;
     auto take = [&](float mv, int i) {  // a new maximum of this lane
       s *= m == NEG_INF ? 0.f : ex2((m - mv) * c);
       m = mv, at = i;
     };
-    auto single = [&](int x) {
-      float l = R::one(row + x);
-      nan |= l != l;
-      l = clean(l);
-      if (l > m || at == kNone) take(l, x);
-      if (!greedy) s += l == m ? 1.f : ex2((l - m) * c);
-    };
-    if (lane < head) single(lane);
-    const int v0 = vec0();
-    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
-    constexpr int U = 5;  // loads in flight
-    for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
-      uint4 v[U];
+    if (!odd) {
+      // four instructions an element: NaN logits, or infinities at the top, leave a NaN in the sum (and the
+      // row is read again)
+      auto single = [&](int x) {
+        const float l = R::one(row + x);
+        if (l > m || at == kNone) take(l, x);
+        s += greedy ? (l == l ? 0.f : l) : ex2(fmaf(l, c, m == NEG_INF ? 0.f : -m * c));
+      };
+      if (lane < head) single(lane);
+      const int v0 = vec0();
+      const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+      constexpr int U = 5;  // loads in flight
+      for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
+        uint4 v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i0 + u * 32 < hi) v[u] = vec[i0 + u * 32];
+        for (int u = 0; u < U; ++u)
+          if (i0 + u * 32 < hi) v[u] = vec[i0 + u * 32];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i0 + u * 32 >= hi) break;
-        float x[8], mv = NEG_INF;
-        R::many(v[u], x);
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u * 32 >= hi) break;
+          float x[8], mv;
+          R::many(v[u], x);
+          mv = max3(x[0], x[1], x[2]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          nan |= x[e] != x[e];
-          x[e] = clean(x[e]);
-          mv = fmaxf(mv, x[e]);
-        }
-        if (mv > m || at == kNone) {
-          int e0 = 0;
+          for (int e = 3; e < N; e += 2) mv = max3(mv, x[e], x[e + 1 < N ? e + 1 : e]);
+          if (mv != mv) s = mv;
+          if (mv > m || at == kNone) {
+            int e0 = 0;
 #pragma unroll
-          for (int e = N - 1; e >= 0; --e)
-            if (x[e] == mv) e0 = e;
-          take(mv, v0 + (i0 + u * 32) * N + e0);
-        }
-        if (!greedy) {
-          float add = 0.f;
+            for (int e = N - 1; e >= 0; --e)
+              if (x[e] == mv) e0 = e;
+            take(mv, v0 + (i0 + u * 32) * N + e0);
+          }
+          if (!greedy) {
+            const float mc = m == NEG_INF ? 0.f : m * c;
+            float add = 0.f, add2 = 0.f;
 #pragma unroll
-          for (int e = 0; e < N; ++e) add += x[e] == m ? 1.f : ex2((x[e] - m) * c);
-          s += add;
+            for (int e = 0; e < N; e += 2) add += ex2(fmaf(x[e], c, -mc)), add2 += ex2(fmaf(x[e + 1], c, -mc));
+            s += add + add2;
+          }
         }
       }
+      if (lane < tail) single(V - tail + lane);
+    } else {
+      bool nan = false;
+      int from, to;
+      range(rank * kWarps + warp, from, to);
+#pragma unroll 1
+      for (int x = from + lane; x < to; x += 32) {
+        float l = R::one(row + x);
+        nan |= l != l;
+        l = clean(l);
+        if (l > m || at == kNone) take(l, x);
+        if (!greedy) s += l == m ? 1.f : ex2((l - m) * c);
+      }
+      if (nan) set_err(a.err, kErrNanScore);
     }
-    if (lane < tail) single(V - tail + lane);
-    if (nan) set_err(a.err, kErrNanScore);
     if (at == kNone) s = 0.f;
     const float wm = max_of(m);
     const int wa = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(m == wm ? at : kNone)));
@@ -325,9 +344,20 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const Message got = exchange(Message{cm, ca, sum});
     top = max_of(got.top);
+    eps = base_eps + 0x1.8p-23f * fabsf(top * c);  // (c times the maximum is rounded before the difference)
     first = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(got.top == top ? got.first : kNone)));
     S = sum_lanes(got.sum * static_cast<double>(scale_to(got.top, top)));
     if (warp == 0 && lane < kWarps) w_sum[lane] = own_sum * static_cast<double>(scale_to(own_top, top));
+  };
+  auto enter = [&](int node) {
+    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
+    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
+    n_rej = 0;
+    exact = false;
+    share();
+    read_row(false);
+    odd_row = !(S >= 0.0) || top == NEG_INF || top == -NEG_INF;
+    if (odd_row) read_row(true);
     if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
     E = 0.0;
     __syncthreads();
@@ -360,58 +390,61 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   };
   auto sum_fast = [&](int n) {  // (a random draft) in fp32; E from n - 1 to n
     float v = 0.f;
-    const float inv0 = s_finv[0];
-    auto left = [&](float l, float qx) {
-      float r = fmaxf(fmaf(l == top ? 1.f : ex2((l - top) * c), inv0, -qx), 0.f);
-      for (int j = 1; j < n; ++j) r = fmaxf(fmaf(r, s_finv[j], -qx), 0.f);
-      return r;
-    };
     const int v0 = vec0();
-    if (lane < head) v += left(clean(R::one(row + lane)), q[lane]);
     const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
     const float* qv = q + v0;
     const bool whole = (reinterpret_cast<uintptr_t>(qv) & 15) == 0;
-    constexpr int U = 2;
-    for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
-      uint4 t[U];
-      float4 d[U][N / 4];
+    const float tc = top * c;
+    // (a NaN logit gives 0: its product is no larger than 0)
+    auto pass = [&](auto left) {
+      if (lane < head) v += left(R::one(row + lane), q[lane]);
+      constexpr int U = 2;
+      for (int i0 = lo + lane; i0 < hi; i0 += 32 * U) {
+        uint4 t[U];
+        float4 d[U][N / 4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * 32;
-        if (i >= hi) break;
-        t[u] = vec[i];
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * 32;
+          if (i >= hi) break;
+          t[u] = vec[i];
 #pragma unroll
-        for (int k = 0; k < N / 4; ++k) {
-          const float* at = qv + static_cast<size_t>(i) * N + k * 4;
-          d[u][k] = whole ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+          for (int k = 0; k < N / 4; ++k) {
+            const float* at = qv + static_cast<size_t>(i) * N + k * 4;
+            d[u][k] = whole ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u * 32 >= hi) break;
+          float x[8], add = 0.f;
+          R::many(t[u], x);
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k) {
+            add += left(x[4 * k], d[u][k].x) + left(x[4 * k + 1], d[u][k].y);
+            add += left(x[4 * k + 2], d[u][k].z) + left(x[4 * k + 3], d[u][k].w);
+          }
+          v += add;
         }
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i0 + u * 32 >= hi) break;
-        float x[8], add = 0.f;
-        R::many(t[u], x);
-#pragma unroll
-        for (int k = 0; k < N / 4; ++k) {
-          add += left(clean(x[4 * k]), d[u][k].x) + left(clean(x[4 * k + 1]), d[u][k].y);
-          add += left(clean(x[4 * k + 2]), d[u][k].z) + left(clean(x[4 * k + 3]), d[u][k].w);
-        }
-        v += add;
-      }
-    }
-    if (lane < tail) v += left(clean(R::one(row + V - tail + lane)), q[V - tail + lane]);
+      if (lane < tail) v += left(R::one(row + V - tail + lane), q[V - tail + lane]);
+    };
+    const float f0 = s_finv[0], f1 = s_finv[1];
+    if (n == 1)
+      pass([&](float l, float qx) { return fmaxf(fmaf(ex2(fmaf(l, c, -tc)), f0, -qx), 0.f); });
+    else
+      pass([&](float l, float qx) {
+        float r = fmaxf(fmaf(ex2(fmaf(l, c, -tc)), f0, -qx), 0.f);
+        r = fmaxf(fmaf(r, f1, -qx), 0.f);
+        for (int j = 2; j < n; ++j) r = fmaxf(fmaf(r, s_finv[j], -qx), 0.f);
+        return r;
+      });
     // weights off by E in all (at first by eps of their sum), divided by a sum that is as far off
     E = (n == 1 ? 2.0 * eps : 2.0 * (E + eps * s_R[n - 1]) * s_inv[n - 1]) + 0x1p-22;
     join_sum(n, static_cast<double>(v));
   };
   auto make_exact = [&]() {  // every sum of the current node again, in double
-    if (exact) return;
     exact = true;
-    if (greedy) return;
-    if (drawn)
-      for (int n = 0; n <= n_rej; ++n) sum_exact(n);
-    else
-      sum_exact(n_rej);
+    for (int k = drawn ? 0 : n_rej; k <= n_rej; ++k) sum_exact(k);
   };
 
   enter(0);
@@ -448,9 +481,14 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     }
     if (drawn) {
       ++n_rej;
-      if (!exact) sum_fast(n_rej);
-      if (!exact && !(E < 0.25 * s_R[n_rej])) make_exact();  // (nothing to go by)
-      else if (exact) sum_exact(n_rej);
+      if (exact)
+        sum_exact(n_rej);
+      else if (odd_row)
+        make_exact();
+      else {
+        sum_fast(n_rej);
+        if (!(E < 0.25 * s_R[n_rej])) make_exact();  // nothing to go by
+      }
     } else {
       __syncthreads();  // s_R[n_rej] has been read
       if (tid == 0) {
@@ -472,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
       a.next_token[b] = first == kNone ? -1 : first;
       if (first == kNone) set_err(a.err, kErrNanScore);
     }
-    cluster_sync_all();  // messages are read before a CTA leaves
+    sync_cluster();  // messages are read before a CTA leaves
     return;
   }
   for (int round = 0;; ++round) {
@@ -579,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
         }
       }
     }
-    cluster_sync_all();
+    sync_cluster();
     uint32_t token, certain;
     const uint32_t from = mapa_u32(smem_u32(s_token), owner);
     asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(token), "=r"(certain) : "r"(from) : "memory");
@@ -590,10 +628,10 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
       }
       break;
     }
-    cluster_sync_all();  // the token is read before it is made again
+    sync_cluster();  // the token is read before it is made again
     make_exact();
   }
-  cluster_sync_all();  // messages are read before a CTA leaves
+  sync_cluster();  // messages are read before a CTA leaves
 }
 
 }  // namespace tv

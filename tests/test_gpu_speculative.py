@@ -328,6 +328,17 @@ def test_verification_of_padded_rows(V, pad):
         _check_verify(c, _run_verify(c))
 
 
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("B,T,V", [(3, 9, 1000), (16, 33, 4097), (2, 6, 50257)])
+def test_verification_where_fp32_decides_nothing(B, T, V, draft):
+    """Logits far from zero: the fp32 sums' error bound grows with the maximum, so that every test and
+    draw is made again in double."""
+    for kind, temp in (("star", [1.0]), ("chain", [0.7, 0.0, 1.3])):
+        c = _verify_case(B, T, V, 5 * T + V, kind, True, draft, temp)
+        c["target"] += 2.0 ** 18
+        _check_verify(c, _run_verify(c))
+
+
 def test_verification_of_greedy_ties_and_equal_tokens():
     c = _verify_case(4, 8, 300, 3, "star", temp=[0.0, 1.0])
     c["target"][:, :, 17] = c["target"][:, :, 211] = 50.0  # a tie: the first one
