@@ -88,7 +88,7 @@ struct alignas(16) Message {
 };
 
 // e^y, y <= 0, to about 1e-14: y = n ln2 / 32 + r, e^r by its series, 2^(n / 32) from a table.
-__device__ __noinline__ double exp_of(double y, const double* table) {
+__device__ __forceinline__ double exp_of(double y, const double* table) {
   if (!(y > -700.0)) return 0.0;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the nearest integer is left in the low bits
   const double t = fma(y, 46.166241308446828384, kRound);  // 32 / ln 2
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   int parity = 0, n_rej = 0, first = kNone;
   float top = NEG_INF;
   double S = 0.0;      // the row's sum in fp32 weights
-  float base_eps = 0.f, eps = 0.f;
+  float base_eps = 0.f, eps = 0.f, sum_eps = 0.f;  // (sum_eps: the summation's part)
   bool odd_row = false;  // NaN or infinities decide: no short cuts
   double E = 0.0;  // how far the weights that the rejections of a random draft left may be off, all together
   bool exact = false;  // s_R and w_sum are double sums
@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     // error of the row's fp32 sum: the weights' (2^x of the hardware 2^-22; the exponent's roundings, 2^-24 of
     // up to 31, beyond which a row's terms do not matter, and of the maximum's, below) and the joins': 24 steps of 2^-22;
     // for each vector of a lane its sums and one change of the reference maximum: 3 steps
+    sum_eps = (16.f + static_cast<float>(vecs / (all * 32) + 1)) * 0x1p-24f;
     base_eps = (24.f + 3.f * static_cast<float>(vecs / (all * 32) + 1)) * 0x1p-22f;
   };
   auto vec0 = [&]() { return min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(L))); };
@@ -196,20 +197,18 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     if (l == top) return 1.0;
     return l < top ? exp_of((static_cast<double>(l) - static_cast<double>(top)) * inv, table) : 0.0;
   };
-  auto rest = [&](int x, float l) -> double {  // what the rejections left of token x
+  auto rest_of = [&](int x, float l, float qx) -> double {  // what the rejections left of token x
     if (greedy) return x == first ? 1.0 : 0.0;
     double r = weight(l);
     if (drawn) {
-      if (n_rej) {
-        const double qx = static_cast<double>(q[x]);
-        for (int j = 0; j < n_rej; ++j) r = fmax(fma(r, s_inv[j], -qx), 0.0);
-      }
+      for (int j = 0; j < n_rej; ++j) r = fmax(fma(r, s_inv[j], -static_cast<double>(qx)), 0.0);
     } else {
       for (int j = 0; j < n_rej; ++j)
         if (x == s_rej[j]) r = 0.0;
     }
     return r;
   };
+  auto rest = [&](int x, float l) -> double { return rest_of(x, l, drawn && n_rej ? q[x] : 0.f); };
   auto rest_fast = [&](int x, float l) -> float {  // the same with fp32 weights
     float r = l == top ? 1.f : ex2((l - top) * c);
     if (drawn) {
@@ -383,8 +382,19 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     double v = 0.0;
     int from, to;
     range(rank * kWarps + warp, from, to);
-#pragma unroll 2
-    for (int x = from + lane; x < to; x += 32) v += rest(x, clean(R::one(row + x)));
+    constexpr int U = 4;
+    for (int x = from + lane; x < to; x += 32 * U) {
+      float l[U], qx[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = x + u * 32 < to;
+        l[u] = in ? clean(R::one(row + x + u * 32)) : NEG_INF;
+        qx[u] = in && drawn && n ? q[x + u * 32] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x + u * 32 < to) v += rest_of(x + u * 32, l[u], qx[u]);
+    }
     n_rej = keep;
     join_sum(n, v);
   };
@@ -439,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
         return r;
       });
     // weights off by E in all (at first by eps of their sum), divided by a sum that is as far off
-    E = (n == 1 ? 2.0 * eps : 2.0 * (E + eps * s_R[n - 1]) * s_inv[n - 1]) + 0x1p-22;
+    E = (n == 1 ? 2.0 * eps : (2.0 * E + sum_eps * s_R[n - 1]) * s_inv[n - 1]) + 0x1p-22;
     join_sum(n, static_cast<double>(v));
   };
   auto make_exact = [&]() {  // every sum of the current node again, in double
@@ -465,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
       yes = lhs * s_R[n_rej] < rx;
     } else {
       const double left = s_R[n_rej];
-      const double off = drawn ? E + eps * left : S * eps;
+      const double off = drawn && n_rej ? E + sum_eps * left : S * eps;
       yes = lhs * (left + off) < rx - E;
       if (!yes && lhs * (left - off) < rx + E) {  // too near to say
         make_exact();
@@ -588,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
       if (warp == sub) {
         int pick = kNone, any = -1;
         bool sure = exact;
-        const double off = exact ? 0.0 : drawn && n_rej ? 2.0 * (E + eps * total) : 2.0 * S * eps;
+        const double off = exact ? 0.0 : drawn && n_rej ? 2.0 * (E + sum_eps * total) : 2.0 * S * eps;
 #pragma unroll 1
         for (int x0 = from; x0 < to && pick == kNone; x0 += 32) {
           const int x = x0 + lane;
