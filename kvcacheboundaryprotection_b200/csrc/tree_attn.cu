@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(threads_of(F), 1)
             const float f = move ? (m == NEG_INF ? 0.f : ex2((m - tm) * c)) : 1.f;
             if (move) m = tm;
             l *= f;
-            if (Score) lx *= f;
+            lx *= f;
             if (k >= 2) {  // (S of this item was issued after the previous P V product: that is done)
 #pragma unroll 1
               for (int q = hc * (8 / H); q < (hc + 1) * (8 / H); ++q) {

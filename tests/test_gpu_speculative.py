@@ -185,13 +185,24 @@ def test_extreme_logits_and_scale():
     _check_attn(c, _run(c, score, scale=-0.3), score, scale=-0.3)
 
 
-def test_growing_logits():
-    """The running maximum rises in every tile."""
-    c = _attn_case(1, 9, 8, 2, 1500, 8, mask=None)
+@pytest.mark.parametrize("with_score", [False, True])
+@pytest.mark.parametrize("T,hq,hkv,S", [(9, 8, 2, 1500), (5, 8, 2, 3000), (13, 8, 2, 3000), (29, 8, 2, 3000),
+                                        (40, 8, 2, 2600), (64, 4, 1, 5000)])
+def test_growing_logits(T, hq, hkv, S, with_score):
+    """The running maximum rises in every tile: few and many rows, one and two row tiles, several
+    tiles a CTA (two sequences of which one is empty: ranges over all SMs)."""
+    c = _attn_case(2, T, hq, hkv, S, 8, mask=None, lens=[S, 0])
     c["q"] = c["q"].abs()
-    c["k"] = (c["k"].abs() * torch.linspace(0.01, 6, 1500)[:, None]).to(BF)
-    score = torch.zeros(1, 9, 1509, device="cuda")
+    c["k"] = (c["k"].abs() * torch.linspace(0.01, 6, S)[:, None]).to(BF)
+    score = torch.zeros(2, T, S + T, device="cuda") if with_score else None
     _check_attn(c, _run(c, score), score)
+    c = {k: v[:1] if torch.is_tensor(v) else v for k, v in c.items()}
+    c["lens"] = None
+    many = {k: v.repeat(*([40] + [1] * (v.dim() - 1))) if torch.is_tensor(v) else v for k, v in c.items()}
+    out = _run(many)  # forty copies, cut in different places
+    for i in (0, 7, 18, 39):
+        _check_attn(c, out[i:i + 1])
+    assert torch.equal(_run(many), out)
 
 
 def test_bad_parents_and_lengths_are_flagged():
