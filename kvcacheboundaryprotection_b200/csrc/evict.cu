@@ -763,7 +763,6 @@ __global__ void __launch_bounds__(kEvictThreads) tree_commit_kernel(CommitArgs c
   pdl_wait();
   extern __shared__ int s_vict[];
   __shared__ int red_i[32];
-  __shared__ float red_f[32];
   __shared__ KeySlot red_k[32];
   __shared__ int sh[8];
   __shared__ int s_node[kMaxNodes], s_slot[kMaxNodes];
@@ -815,14 +814,28 @@ __global__ void __launch_bounds__(kEvictThreads) tree_commit_kernel(CommitArgs c
   const size_t pitch = static_cast<size_t>(S) + T;
   const float* sc = c.score ? c.score + static_cast<size_t>(b) * T * pitch : nullptr;
   if (sc) {
-    for (int i = 0; i < m; ++i) {
+    // a warp for each node, eight loads in flight (a block for one node after another was two barriers
+    // and a round of memory latency a node)
+    for (int i = warp; i < m; i += kEvictThreads >> 5) {
       const float* row = sc + s_node[i] * pitch;
       float mx = 0.f;
-      for (int j = tid; j < S; j += kEvictThreads)
-        if (in.slot_pos[j] >= 0) mx = fmaxf(mx, row[j]);
-      if (tid <= i && tid < placed) mx = fmaxf(mx, row[S + s_node[tid]]);
-      mx = block_max_float(mx, red_f);
-      if (tid == 0) s_thr[i] = static_cast<float>(0.05 * static_cast<double>(mx));
+      for (int j0 = lane; j0 < S; j0 += 8 * 32) {
+        int ps[8];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + k * 32;
+          ps[k] = j < S ? in.slot_pos[j] : -1;
+          v[k] = j < S ? row[j] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (ps[k] >= 0) mx = fmaxf(mx, v[k]);
+      }
+      for (int k = lane; k <= i && k < placed; k += 32) mx = fmaxf(mx, row[S + s_node[k]]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (lane == 0) s_thr[i] = static_cast<float>(0.05 * static_cast<double>(mx));
     }
   }
   __syncthreads();

@@ -13,25 +13,35 @@
 // lengths; a unit cut by a border leaves partial results (sum, running maximum, accumulator) that
 // combine_kernel joins.
 //
-// attend_kernel, one CTA per SM, 11 warps:
-//   * producer: K and V tiles (128 keys, 32 KiB each) by 3-D TMA through one ring in the order the
-//     products need them; Q once per unit;
-//   * MMA warp (one thread): item i = S_w = Q . K^T into TMEM (w = i & 1), then O_w += P . V with P
-//     read from TMEM; form A: the items are the unit's key tiles in turn, two accumulators;
-//     form B: the two row tiles of each key tile;
-//   * 2 x 4 softmax warps, a thread per row: the tile's maximum, weights 2^(c s - c m) in bf16 packed
-//     over S's columns, their sum.  The reference maximum m moves only when a row's maximum passes it
-//     by more than 2^8 in weight (exact in fp32, and bf16 weights keep their 8 bits wherever they lie),
-//     so that O is rescaled rarely;
+// attend_kernel, one CTA per SM (ranges over all SMs, or with few units a cluster of CTAs for each that
+// joins its parts in shared memory):
+//   * producer warp: K and V tiles (128 keys, 32 KiB each) by 3-D TMA through one ring in the order the
+//     products need them; Q once per unit, rows of small trees 2 or 4 times over the TMEM lanes;
+//   * MMA warp: item i = S_w = Q . K^T into TMEM (w = i & 1), then O_w += P . V with P read from TMEM;
+//     form A: the items are the unit's key tiles in turn, two accumulators; form B: the two row tiles of
+//     each key tile;
+//   * softmax warps, a thread per row and part of the columns (copies of a row take a part each; a row
+//     without copies has two warps, 16 in all): the tile's maximum, weights 2^(c s - c m) in bf16 packed
+//     over S's columns, their sum.  The reference maximum m moves only when a row's maximum passes it by
+//     more than 2^8 in weight (exact in fp32, and bf16 weights keep their 8 bits wherever they lie), so
+//     that O is rescaled rarely;
 //   * mask warp: the live bits of each key tile from slot_pos / lens; V rows of dead slots and
 //     unused nodes are zeroed in shared memory before the product reads them (0 * NaN is NaN), and
 //     drafted V elements that are not finite, which rows off their branch must not meet, are taken out
 //     and added by the rows that see them.
-// Rounding: S, sums and O are fp32; a weight is rounded once to bf16 and the sum that divides is that
-// of the rounded weights (an error common to all weights cancels); out is rounded once.
+// Rounding: S, sums and O are fp32; a weight is rounded once to bf16 (half a step, 2^-8 of it), in form A
+// the sum that divides is that of the rounded weights (an error common to all cancels), in form B, where
+// the issue slots count, that of the unrounded ones; out is rounded once.
+// Measured on B200 (graph replay): 64 sequences x 5 nodes x 4104 slots, 8 kv heads: 187 us, 5.5 TB/s of the
+// 6.46 of a copy (without the loads the same hand-overs between the warps take 122 us, without the softmax
+// 180: the two overlap but for the start of each unit); 1 x 64 nodes x 131071 slots, 8 kv heads: 143 us, the
+// tensor pipe 45 % busy, bound by the chain S -> weights -> P . V of each row tile (without the weights'
+// arithmetic 128 us); exponentials on the FMA pipe instead of the MUFU for 1/8 to 5/8 of the columns were
+// slower (161 -> 166-180 us at the time).
 //
-// score_kernel forms p again from the final row statistics: S^T = K . Q^T with a slot per thread, so
-// that the maximum over heads stays in the thread and the score rows are written along the slots.
+// combine_kernel joins the parts of units that a border cut.  score_kernel forms p again from the final row
+// statistics: S^T = K . Q^T with a slot per thread, so that the maximum over heads stays in the thread and
+// the score rows are written along the slots (16 x 16 nodes x 1032 slots, 4 kv heads: 16 us of 37).
 #include <type_traits>
 
 #include "common.cuh"
