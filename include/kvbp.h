@@ -528,7 +528,8 @@ int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_t Hq, int32
  * next_token (draft_probs is not read).  NaN logits count as -inf and set KVBP_DEV_NAN_SCORE; a token
  * outside [0, vocab) is rejected, leaves r as it is and sets KVBP_DEV_INDEX.
  * path [B][T] int32: the accepted nodes, root first, then -1; n_path[b] their number (1: the root
- * alone; 0 with next_token -1 for a sequence whose root is unused).  Weights and sums are double.
+ * alone; 0 with next_token -1 for a sequence whose root is unused).  Tests and draws are decided as by
+ * weights and sums in double.
  * workspace as for kvbp_tree_attn. */
 int64_t kvbp_tree_verify_workspace(int32_t B, int32_t T, int32_t vocab);
 int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int32_t vocab, int32_t fp32_target,
