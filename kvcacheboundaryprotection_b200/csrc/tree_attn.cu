@@ -72,6 +72,18 @@ constexpr int kOffMisc = kOffNf + kNf * 16;          // TMEM address, flag, star
 constexpr int kSmem = kOffMisc + 64;
 static_assert(kSmem <= 232448, "shared memory");
 
+// What the two warps of the same 32 rows tell each other lies in two words a TMEM lane, maxima and sums alike.
+// Nothing but their own barriers orders these uses (the pairs of warps drift apart by more than a unit), so
+// each word belongs to one pair for good.
+constexpr int pair_word(int half, int lane128) { return half * 128 + lane128; }
+constexpr bool pair_words_apart() {
+  for (int i = 0; i < 256; ++i)
+    for (int k = 0; k < 256; ++k)
+      if (i % 128 / 32 != k % 128 / 32 && pair_word(i / 128, i % 128) == pair_word(k / 128, k % 128)) return false;
+  return true;
+}
+static_assert(pair_words_apart(), "a word of two pairs of warps");
+
 struct Args {
   int B, T, Hq, Hkv, S, G;
   int npt;    // nodes of a row tile
@@ -596,7 +608,9 @@ __global__ void __launch_bounds__(threads_of(F), 1)
     const float NEG_INF = -__int_as_float(0x7f800000);
     const float c = a.c;
     const uint64_t c2 = pack2(c, c);
-    float* xchg = reinterpret_cast<float*>(stat) + x * 256;  // [2][128]
+    float* xchg = reinterpret_cast<float*>(stat) + x * 256;  // (H == 2) pair_word
+    const int at = quarter * 32 + lane;  // this thread's TMEM lane
+    const int word0 = pair_word(0, at), word1 = pair_word(1, at);
     const bool releases = quarter == 0 && hc == 0 && (!FormB || x == 1);  // hands tiles back
     int i0 = 0, j0 = 0;  // the CTA's items and key tiles before this unit
     int done = 0;        // items of this accumulator so far
@@ -682,9 +696,9 @@ __global__ void __launch_bounds__(threads_of(F), 1)
           const bool any = H == 2 ? any_of_pair(pair_bar, moves()) : __any_sync(0xffffffffu, moves());
           if (any) {
             if (H == 2) {
-              xchg[hc * 128 + quarter * 32 + lane] = tm;
+              xchg[hc ? word1 : word0] = tm;
               named_bar(pair_bar, 64);
-              tm = max3(tm, xchg[(hc ^ 1) * 128 + quarter * 32 + lane], tm);
+              tm = max3(tm, xchg[hc ? word0 : word1], tm);
             }
             const bool move = moves();
             const float f = move ? (m == NEG_INF ? 0.f : ex2((m - tm) * c)) : 1.f;
@@ -770,21 +784,18 @@ __global__ void __launch_bounds__(threads_of(F), 1)
       wait(odone, w.seg & 1);
       if (releases && lane == 0 && first < items) mbar_arrive(&empty[v_pos(j0 - (FormB || ((items - 1 - first) & 1) == 0 ? 1 : 2)) % NS]);
       float f0 = 1.f, f1 = 0.f, M = m, L = l, Lx = lx;
-      const int at = quarter * 32 + lane;
       if (H == 2) {  // the sums of the two warps of a row
-        float2* sums = reinterpret_cast<float2*>(xchg);
-        if (hc == 1) sums[at] = make_float2(l, lx);
+        if (hc == 1) xchg[word0] = l, xchg[word1] = lx;
         named_bar(pair_bar, 64);
         if (hc == 0) {
-          const float2 o = sums[at];
-          L = l = l + o.x;
-          Lx = lx = lx + o.y;
-          if (FormB) sums[at] = make_float2(l, lx);
+          L = l = l + xchg[word0];
+          Lx = lx = lx + xchg[word1];
+          if (FormB) xchg[word0] = l, xchg[word1] = lx;
         }
         if (FormB) {
           named_bar(pair_bar, 64);
-          if (hc == 1) L = sums[at].x, Lx = sums[at].y;
-          named_bar(pair_bar, 64);  // read before the next unit writes
+          if (hc == 1) L = xchg[word0], Lx = xchg[word1];
+          named_bar(pair_bar, 64);  // read before this pair writes them again in the next unit
         } else {
           named_bar(3, 256 * H);
         }
@@ -948,8 +959,8 @@ __global__ void __launch_bounds__(threads_of(F), 1)
               float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
               for (int g = 0; g < F; ++g) {
-                const int at = g * kRowsF + row;
-                const float4 v = *reinterpret_cast<float4*>(mine + at * 32 + (((copy * (8 / F) + e) ^ (at & 7)) << 2));
+                const int lg = g * kRowsF + row;
+                const float4 v = *reinterpret_cast<float4*>(mine + lg * 32 + (((copy * (8 / F) + e) ^ (lg & 7)) << 2));
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
               }
               o[4 * e] = sum.x, o[4 * e + 1] = sum.y, o[4 * e + 2] = sum.z, o[4 * e + 3] = sum.w;

@@ -205,6 +205,26 @@ def test_growing_logits(T, hq, hkv, S, with_score):
     assert torch.equal(_run(many), out)
 
 
+@pytest.mark.parametrize("T,hq,hkv,S", [(40, 8, 2, 140), (33, 28, 4, 70), (128, 8, 1, 300)])
+def test_many_units_of_two_row_tiles_a_cta(T, hq, hkv, S):
+    """Several hundred units over the SMs, so that every CTA goes from unit to unit, maxima that rise and fall
+    with them: the rows' statistics of one unit are not those of the next.  The same bits in every run."""
+    B = 900 // hkv // (2 if T == 128 else 1)
+    c = _attn_case(4, T, hq, hkv, S, 3, mask="slots", kind="chain")
+    c["k"] = (c["k"] * torch.linspace(0.05, 5, S)[:, None]).to(BF)
+    c["k"][1::2] = c["k"][1::2].flip(2)
+    c["q"] = (c["q"] * torch.tensor([0.1, 3.0, 1.0, 6.0])[:, None, None, None]).to(BF)
+    many = {k: v.repeat(*([B // 4 + 1] + [1] * (v.dim() - 1)))[:B].cuda() if torch.is_tensor(v) else v for k, v in c.items()}
+    out = _run(many)
+    for i in (0, 4 * (B // 8), B // 4 * 4 - 4):
+        _check_attn(c, out[i:i + 4])
+    score = torch.zeros(B, T, S + T, device="cuda")
+    assert torch.equal(_run(many, score), out)
+    _check_attn(c, out[:4], score[:4])
+    for _ in range(20):
+        assert torch.equal(_run(many), out)
+
+
 def test_bad_parents_and_lengths_are_flagged():
     c = _attn_case(2, 6, 8, 2, 70, 8, mask=None)
     c["parents"][0] = torch.tensor([-1, 0, 4, 2, 7, 1])  # 2 and 4 name later nodes; 3 hangs on 2
