@@ -196,6 +196,9 @@ class FusedWeights:
 
 
 class CappedKVEngine:
+    """``extra_slots``: slots beyond those that the decode steps need, for commits of several positions at
+    once (``speculative.commit_tree`` evicts after a whole path: the longest path's length - 1)."""
+
     def __init__(
         self,
         cfg: ModelConfig,
@@ -209,6 +212,7 @@ class CappedKVEngine:
         kv_heads: Optional[List[int]] = None,
         gemm: str = "kvbp",
         host_policy=None,
+        extra_slots: int = 0,
     ):
         if cfg.head_dim != 128:
             raise ValueError("only head_dim 128 is supported")
@@ -220,6 +224,9 @@ class CappedKVEngine:
             raise ValueError("evict_every_n_steps must be > 0")
         if evict.regime not in ("decode", "prefill"):
             raise ValueError("eviction_regime must be 'decode' or 'prefill'")
+        extra = int(extra_slots)
+        if extra < 0:
+            raise ValueError("extra_slots must be >= 0")
         lib()  # fail loudly when the CUDA library is missing
         # a policy that draws its victims on the host (the random policy) through the
         # reference's select_evictions protocol; the device applies them
@@ -248,9 +255,9 @@ class CappedKVEngine:
         self.policy_id = capi.policy_id(evict.policy)
         self.n_prefix, self.n_suffix = evict.sizes()
         C = evict.capacity
-        self.S = C + (evict.evict_every if evict.regime == "decode" else max(1, self.max_new))
-        self.W = (self.max_prompt + self.max_new + 2 + 31) // 32
-        self.evcap = self.max_prompt + self.max_new + 2
+        self.S = C + (evict.evict_every if evict.regime == "decode" else max(1, self.max_new)) + extra
+        self.W = (self.max_prompt + self.max_new + extra + 2 + 31) // 32  # (the last path may pass max_new)
+        self.evcap = self.max_prompt + self.max_new + extra + 2
         self.gemm = weights.gemm if isinstance(weights, FusedWeights) else gemm
         if self.gemm == "kvbp" and self.B > 32:
             raise ValueError("the decode GEMM handles up to 32 sequences per GPU")

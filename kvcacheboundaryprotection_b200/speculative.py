@@ -22,7 +22,7 @@ element, when one is given.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass, fields
+from dataclasses import dataclass, field, fields
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -179,18 +179,22 @@ class SlotState:
     next_pos: torch.Tensor
     evlog: torch.Tensor
     evcount: torch.Tensor
+    engine: Optional[object] = field(default=None, repr=False, compare=False)  # whose arrays they are (``of``)
 
     @classmethod
     def of(cls, engine) -> "SlotState":
-        """The state of a ``CappedKVEngine`` (its own arrays)."""
+        """The state of a ``CappedKVEngine`` (its own arrays).  A commit evicts after the whole path, so build
+        the engine with ``extra_slots`` >= the longest path - 1.  What a commit finds on the device (no free
+        slot among it) goes to the engine's error word unless another is given: ``engine.check_device_errors()``.
+        The engine's ``token_log`` and ``retained_log`` hold its own steps only."""
         return cls(engine.slot_pos, engine.insert_step, engine.last_access, engine.access_count, engine.attn_s,
                    engine.max_attn, engine.cumul, engine.prefill_s, engine.posmap, engine.seq_step, engine.next_pos,
-                   engine.evlog, engine.evcount)
+                   engine.evlog, engine.evcount, engine)
 
     def like(self) -> "SlotState":
         """Another state of the same sizes, with the same eviction log."""
         return SlotState(*[self.evlog if f.name == "evlog" else torch.empty_like(getattr(self, f.name))
-                           for f in fields(self)])
+                           for f in fields(self) if f.name != "engine"])
 
     def _struct(self) -> tuple:
         """(kvbp_state, its device, log size) after the checks."""
@@ -254,6 +258,8 @@ def commit_tree(state: SlotState, path: torch.Tensor, n_path: torch.Tensor, k_dr
         _need(t, name, _BF16, dev, (L, B, hkv, rows, HEAD_DIM))
     if node_score is not None:
         _need(node_score, "node_score", _F32, dev, (B, T, S + T))
+    if dev_err is None and state.engine is not None:
+        dev_err = state.engine.dev_err
     if dev_err is not None:
         _need(dev_err, "dev_err", _I32, dev, (1,))
     cfg = _evict_cfg(evict)

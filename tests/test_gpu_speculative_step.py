@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import spec_ref as ref
 from kvcacheboundaryprotection_b200 import build, capi, speculative as sp
 from kvcacheboundaryprotection_b200.config import get_config
 from kvcacheboundaryprotection_b200.engine import CappedKVEngine, EvictionSpec
@@ -173,3 +174,78 @@ def test_speculative_steps_with_eviction_in_a_graph():
         last = path[torch.arange(B), n.long() - 1].long()
         assert torch.equal(nxt.long(), logits[torch.arange(B), last].float().argmax(-1))
     eng.check_device_errors()
+
+
+SLOT = {"slot_pos": "slot_pos", "insert_step": "insert_step", "last_access": "last_access", "access_count": "access_count",
+        "attn": "attn_s", "max_attn": "max_attn", "cumul": "cumul", "prefill": "prefill_s"}
+
+
+def _snapshot(eng, b):
+    """Sequence b of an engine as ``ref.commit`` takes it."""
+    st = {k: getattr(eng, v)[b].cpu().numpy().copy() for k, v in SLOT.items()}
+    st.update(seq_step=int(eng.seq_step[b]), next_pos=int(eng.next_pos[b]), log=[])
+    return st
+
+
+def _equal(eng, b, st, logged):
+    for k, v in SLOT.items():
+        assert np.array_equal(getattr(eng, v)[b].cpu().numpy(), st[k]), (b, k)
+    assert int(eng.seq_step[b]) == st["seq_step"] and int(eng.next_pos[b]) == st["next_pos"]
+    assert eng.evlog[b, logged: int(eng.evcount[b])].tolist() == st["log"]
+
+
+def _commits(eng, state, T, steps, seed, kd, vd, longest):
+    """``steps`` commits of random paths with random scores, each checked against ``ref.commit``."""
+    g, rng = torch.Generator().manual_seed(seed), np.random.default_rng(seed)
+    ev = eng.ev
+    spec = (ev.policy, ev.capacity, ev.evict_every, ev.protect, ev.prefix_frac, ev.suffix_frac)
+    lost = 0
+    for it in range(steps):
+        n = torch.tensor([longest if it % 3 else 1 + int(rng.integers(longest)) for _ in range(eng.B)], dtype=torch.int32)
+        path = torch.full((eng.B, T), -1, dtype=torch.int32)
+        for b in range(eng.B):
+            path[b, : n[b]] = torch.from_numpy(np.sort(np.concatenate([[0], 1 + rng.permutation(T - 1)])[: n[b]]))
+        score = torch.rand(eng.B, T, eng.S + T, generator=g) ** 4
+        before = [_snapshot(eng, b) for b in range(eng.B)]
+        logged = eng.evcount.tolist()
+        write = sp.commit_tree(state, path.cuda(), n.cuda(), kd, vd, eng.kc, eng.vc, node_score=score.cuda(), evict=ev)
+        for b in range(eng.B):
+            slots = ref.commit(before[b], path[b].tolist(), int(n[b]), score[b].numpy(), spec)
+            assert write[b].tolist() == slots + [-1] * (T - int(n[b])), (it, b)
+            _equal(eng, b, before[b], logged[b])
+            for i, s in enumerate(slots):
+                lost += s < 0
+                if s >= 0:
+                    assert torch.equal(eng.kc[:, b, :, s], kd[:, b, :, path[b, i]])
+                    assert torch.equal(eng.vc[:, b, :, s], vd[:, b, :, path[b, i]])
+    return lost
+
+
+@pytest.mark.parametrize("policy,every,longest", [("h2o_faithful", 8, 3), ("lru", 4, 5), ("streamingllm", 1, 2)])
+def test_commits_at_the_engines_own_cadence(policy, every, longest):
+    """Steps of several tokens over many evictions of one cadence: an engine with slots for the longest path
+    loses none (without them the step before an eviction finds no free slot)."""
+    B, T, cap = 3, 6, 48
+    cfg = get_config("parity-qwen2")
+    w = init_weights(cfg, seed=1)
+    kd = torch.randn(cfg.n_layers, B, cfg.n_kv_heads, T, 128, device="cuda").to(BF)
+    vd = torch.randn_like(kd)
+    for extra in (longest - 1, 0):
+        eng = CappedKVEngine(cfg, w, batch=B, evict=EvictionSpec(policy, cap, every, True), max_prompt_len=70,
+                             max_new_tokens=80, extra_slots=extra)
+        assert eng.S == cap + every + extra
+        eng.synthetic_prefill(70, seed=3)
+        lost = _commits(eng, sp.SlotState.of(eng), T, 14, 5, kd, vd, longest)
+        if extra:
+            # a victim may be among the newest, but no entry goes without a slot
+            eng.check_device_errors()
+        else:
+            assert lost
+            with pytest.raises(capi.KVBPError, match="slot"):
+                eng.check_device_errors()
+
+
+def test_an_engine_refuses_a_negative_number_of_slots():
+    cfg = get_config("parity-qwen2")
+    with pytest.raises(ValueError, match="extra_slots"):
+        CappedKVEngine(cfg, {}, batch=1, evict=EvictionSpec("lru", 8, 4), max_prompt_len=8, max_new_tokens=4, extra_slots=-1)
