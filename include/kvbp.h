@@ -182,12 +182,18 @@ int kvbp_append_evict(kvbp_stream_t stream, const kvbp_state* st, const kvbp_evi
  * holds the scores the previous step's layers max-accumulated; the kernel applies them
  * where pending[b] != 0, clears step_score for this step's layers and sets pending[b] = 1.
  * pending [B] int32 is 0 before the first decode step after prefill (no scores yet); after
- * the last step, kvbp_score_update applies the scores still pending. */
+ * the last step, kvbp_score_update applies the scores still pending, and before a
+ * kvbp_tree_commit kvbp_score_update_pending does. */
 int kvbp_update_append_evict(kvbp_stream_t stream, const kvbp_state* st, const kvbp_evict_cfg* cfg,
                              int32_t* seq_step, int32_t* next_pos, int32_t* cur_pos, int32_t* write_slot,
                              const int32_t* tokens, int32_t* token_log, int32_t log_steps, int32_t* evlog,
                              int32_t* evcount, int32_t evcap, int32_t* retained_log, float* step_score,
                              int32_t* pending, int32_t* dev_err);
+
+/* kvbp_score_update for the sequences with pending[b] != 0, which is cleared: what
+ * kvbp_update_append_evict would do first, without an append. */
+int kvbp_score_update_pending(kvbp_stream_t stream, const kvbp_state* st, const int32_t* seq_step, float* step_score,
+                              int32_t* pending, int32_t* dev_err);
 
 /* K3 with the victims chosen on the host -- the random policy's path.
  * RandomEvictionPolicy (src/counterfact_kv_eviction/policies.py:1553-1582) draws its
@@ -549,7 +555,9 @@ int kvbp_tree_verify(kvbp_stream_t stream, int32_t B, int32_t T, int32_t vocab, 
  * [layers][B][Hkv][S][128] (bf16, 16-byte aligned; layers may be 0).
  * State is read from st_in, seq_step_in, next_pos_in, evcount_in and written to st_out, seq_step,
  * next_pos, evcount: the same arrays, or others that overlap nothing (the old state stays, so that
- * a step can be taken back).  S <= 16384 with cfg.  A path longer than T, or with an entry that is no
+ * a step can be taken back).  Scores that kvbp_update_append_evict has left pending are not applied here:
+ * kvbp_score_update_pending does that, before.  As the eviction comes after the whole path, the slots have to
+ * hold capacity + evict_every - 1 + the longest path.  S <= 16384 with cfg.  A path longer than T, or with an entry that is no
  * node, ends there (KVBP_DEV_INDEX); entries without a free slot get none (KVBP_DEV_NO_FREE_SLOT). */
 int kvbp_tree_commit(kvbp_stream_t stream, const kvbp_state* st_in, const kvbp_state* st_out,
                      const kvbp_evict_cfg* cfg, int32_t T, const int32_t* path, const int32_t* n_path,

@@ -87,6 +87,7 @@ SIGNATURES = {
         [P, I32, I32, I32, I32, I32, I32, P, I32, P, P, P, F32, P, P, P, P, P, P, P],
     ),
     "kvbp_score_update": (C.c_int, [P, C.POINTER(State), P, P, P]),
+    "kvbp_score_update_pending": (C.c_int, [P, C.POINTER(State), P, P, P, P]),
     "kvbp_append_evict": (
         C.c_int,
         [P, C.POINTER(State), C.POINTER(EvictCfg), P, P, P, P, P, P, I32, P, P, I32, P, P],

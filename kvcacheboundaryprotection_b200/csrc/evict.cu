@@ -256,13 +256,16 @@ __device__ int select_bit_warp(const uint32_t* words, int W, int k) {
 // ------------------------------------------------------------------------------------
 constexpr int kScoreThreads = 256;
 
+// pending (may be null): only sequences with pending[b] != 0, which is cleared.
 __global__ void __launch_bounds__(kScoreThreads) score_update_kernel(StateArgs st, const int* __restrict__ seq_step,
-                                                                     float* __restrict__ step_score, int* err) {
+                                                                     float* __restrict__ step_score, int* pending,
+                                                                     int* err) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[32];
   __shared__ float cta_max;
   const int b = blockIdx.y, CS = gridDim.x;
+  if (pending && pending[b] == 0) return;  // the whole cluster does: it is cleared after the last barrier
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int lo = (static_cast<int>(rank) * st.S) / CS, hi = ((static_cast<int>(rank) + 1) * st.S) / CS;
@@ -304,6 +307,7 @@ __global__ void __launch_bounds__(kScoreThreads) score_update_kernel(StateArgs s
     sc[i] = 0.f;
   }
   cluster_sync_all();  // peers have read cta_max before this CTA leaves
+  if (pending && rank == 0 && threadIdx.x == 0) pending[b] = 0;
 }
 
 // ------------------------------------------------------------------------------------
@@ -1105,7 +1109,8 @@ static bool state_ok(const StateArgs& s) {
          s.prefill && s.posmap && s.B > 0 && s.S > 0 && s.W > 0;
 }
 
-int score_update(cudaStream_t stream, const StateArgs& st, const int* seq_step, float* step_score, int* err) {
+int score_update(cudaStream_t stream, const StateArgs& st, const int* seq_step, float* step_score, int* pending,
+                 int* err) {
   if (!state_ok(st) || !seq_step || !step_score) return fail(kStatusArg, "score_update: bad argument");
   // a cluster of up to 8 CTAs per sequence, each with at most ~512 slots
   int cs = (st.S + 511) / 512;
@@ -1113,7 +1118,7 @@ int score_update(cudaStream_t stream, const StateArgs& st, const int* seq_step, 
   if (cs < 1) cs = 1;
   if (st.B > 65535) return fail(kStatusArg, "score_update: batch %d too large", st.B);
   cudaError_t le = launch_pdl(score_update_kernel, dim3(cs, st.B), dim3(kScoreThreads), 0, stream, dim3(cs, 1, 1), st,
-                              seq_step, step_score, err);
+                              seq_step, step_score, pending, err);
   if (le != cudaSuccess) return fail(kStatusCuda, "score_update launch: %s", cudaGetErrorString(le));
   return check_launch("score_update");
 }
@@ -1275,7 +1280,13 @@ extern "C" {
 int kvbp_score_update(kvbp_stream_t stream, const kvbp_state* st, const int32_t* seq_step, float* step_score,
                       int32_t* dev_err) {
   if (!st) return kvbp::fail(kvbp::kStatusArg, "score_update: null state");
-  return kvbp::score_update(reinterpret_cast<cudaStream_t>(stream), to_state(st), seq_step, step_score, dev_err);
+  return kvbp::score_update(reinterpret_cast<cudaStream_t>(stream), to_state(st), seq_step, step_score, nullptr, dev_err);
+}
+
+int kvbp_score_update_pending(kvbp_stream_t stream, const kvbp_state* st, const int32_t* seq_step, float* step_score,
+                              int32_t* pending, int32_t* dev_err) {
+  if (!st || !pending) return kvbp::fail(kvbp::kStatusArg, "score_update: null state or pending");
+  return kvbp::score_update(reinterpret_cast<cudaStream_t>(stream), to_state(st), seq_step, step_score, pending, dev_err);
 }
 
 static int append_evict_common(kvbp_stream_t stream, const kvbp_state* st, const kvbp_evict_cfg* cfg,

@@ -863,13 +863,16 @@ class CappedKVEngine:
         return not self.per_head and self.host_policy is None and type(self) is CappedKVEngine
 
     def apply_pending_scores(self) -> None:
-        """Apply a forwarded step's scores that no append has consumed yet (deferred mode)."""
-        if not self.deferred_score_update or not self._forwarded:
+        """Apply a forwarded step's scores that no append has consumed yet (deferred mode).  While a graph is
+        captured the update always goes into it: at each replay the device knows which scores are pending."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        if not self.deferred_score_update or not (self._forwarded or capturing):
             return
-        check(lib().kvbp_score_update(self.stream, capi.C.byref(self._state), _ptr(self.seq_step),
-                                      _ptr(self.step_score), _ptr(self.dev_err)), "score_update")
-        self.upd_pending.zero_()
-        self._forwarded = False
+        check(lib().kvbp_score_update_pending(self.stream, capi.C.byref(self._state), _ptr(self.seq_step),
+                                              _ptr(self.step_score), _ptr(self.upd_pending), _ptr(self.dev_err)),
+              "score_update_pending")
+        if not capturing:
+            self._forwarded = False
 
     def _attention(self, li: int) -> None:
         c, L = self.cfg, lib()

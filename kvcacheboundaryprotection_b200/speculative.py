@@ -186,6 +186,7 @@ class SlotState:
         """The state of a ``CappedKVEngine`` (its own arrays).  A commit evicts after the whole path, so build
         the engine with ``extra_slots`` >= the longest path - 1.  What a commit finds on the device (no free
         slot among it) goes to the engine's error word unless another is given: ``engine.check_device_errors()``.
+        Each commit first applies the scores that the engine's last step has left pending.
         The engine's ``token_log`` and ``retained_log`` hold its own steps only."""
         return cls(engine.slot_pos, engine.insert_step, engine.last_access, engine.access_count, engine.attn_s,
                    engine.max_attn, engine.cumul, engine.prefill_s, engine.posmap, engine.seq_step, engine.next_pos,
@@ -243,6 +244,7 @@ def commit_tree(state: SlotState, path: torch.Tensor, n_path: torch.Tensor, k_dr
     Returns write_slot [B, T] int32: each path entry's slot, -1 where there is none."""
     st_in, dev, cap = state._struct()
     B, S = st_in.B, st_in.S
+    engine = state.engine
     new = state if out is None else out
     st_out, dev_out, cap_out = (st_in, dev, cap) if out is None else out._struct()
     if (st_out.B, st_out.S, st_out.W, dev_out) != (B, S, st_in.W, dev):
@@ -258,8 +260,8 @@ def commit_tree(state: SlotState, path: torch.Tensor, n_path: torch.Tensor, k_dr
         _need(t, name, _BF16, dev, (L, B, hkv, rows, HEAD_DIM))
     if node_score is not None:
         _need(node_score, "node_score", _F32, dev, (B, T, S + T))
-    if dev_err is None and state.engine is not None:
-        dev_err = state.engine.dev_err
+    if dev_err is None and engine is not None:
+        dev_err = engine.dev_err
     if dev_err is not None:
         _need(dev_err, "dev_err", _I32, dev, (1,))
     cfg = _evict_cfg(evict)
@@ -272,6 +274,9 @@ def commit_tree(state: SlotState, path: torch.Tensor, n_path: torch.Tensor, k_dr
     _fits(L * hkv * 8)
     if L * hkv == 0:
         L = 0
+    if engine is not None:  # the old state's last step is part of it
+        with torch.cuda.device(dev):
+            engine.apply_pending_scores()
     _launch(
         lib().kvbp_tree_commit, "tree_commit", dev, C.byref(st_in), C.byref(st_out),
         None if cfg is None else C.byref(cfg), T, path.data_ptr(), n_path.data_ptr(), _ptr(node_score), L, hkv, HEAD_DIM,

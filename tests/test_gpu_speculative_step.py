@@ -245,6 +245,74 @@ def test_commits_at_the_engines_own_cadence(policy, every, longest):
                 eng.check_device_errors()
 
 
+def _arrays(eng):
+    return [getattr(eng, n).clone() for n in (*SLOT.values(), "posmap", "seq_step", "next_pos", "evcount", "evlog",
+                                              "upd_pending", "step_score", "tokens", "kc", "vc")]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("graph_steps", [False, True])
+def test_commits_between_the_engines_own_steps(captured, graph_steps):
+    """run_step leaves its scores pending: a commit (eager, or captured and replayed) applies them first, once,
+    and the next run_step starts from the committed state.  Against the plain sequence with the scores applied
+    by hand and the commit by ``ref.commit``."""
+    B, T, n = 3, 5, 3
+    cfg = get_config("parity-qwen2")
+    w = init_weights(cfg, seed=1)
+    engs = []
+    for _ in range(2):
+        eng = CappedKVEngine(cfg, w, batch=B, evict=EvictionSpec("h2o_faithful", 48, 4, True), max_prompt_len=70,
+                             max_new_tokens=60, extra_slots=n - 1)
+        eng.synthetic_prefill(70, seed=3)
+        if graph_steps:
+            eng.capture()
+        engs.append(eng)
+    one, plain = engs
+    ev = one.ev
+    spec = (ev.policy, ev.capacity, ev.evict_every, ev.protect, ev.prefix_frac, ev.suffix_frac)
+    kd = torch.randn(cfg.n_layers, B, cfg.n_kv_heads, T, 128, device="cuda").to(BF)
+    vd = torch.randn_like(kd)
+    path = torch.tensor([[0, 2, 3, -1, -1]] * B, dtype=torch.int32, device="cuda")
+    count = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    score = torch.zeros(B, T, one.S + T, device="cuda")
+    state = sp.SlotState.of(one)
+    call = lambda: sp.commit_tree(state, path, count, kd, vd, one.kc, one.vc, node_score=score, evict=ev)  # noqa: E731
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            write = call()
+    for it in range(7):
+        for eng in engs:
+            for _ in range(it % 3):  # none, one or two steps between commits
+                eng.run_step(use_graph=graph_steps)
+        score.copy_(torch.rand(B, T, one.S + T, generator=torch.Generator().manual_seed(it)) ** 4)
+        if captured:
+            graph.replay()
+        else:
+            write = call()
+        if it % 3:  # the plain sequence
+            capi.check(capi.lib().kvbp_score_update(plain.stream, capi.C.byref(plain._state), plain.seq_step.data_ptr(),
+                                                    plain.step_score.data_ptr(), plain.dev_err.data_ptr()), "score_update")
+            plain.upd_pending.zero_()
+            plain._forwarded = False
+        for b in range(B):
+            st = _snapshot(plain, b)
+            logged = int(plain.evcount[b])
+            slots = ref.commit(st, path[b].tolist(), n, score[b].cpu().numpy(), spec)
+            assert write[b].tolist() == slots + [-1] * (T - n), (it, b)
+            _equal(one, b, st, logged)
+        sp.commit_tree(sp.SlotState.of(plain), path, count, kd, vd, plain.kc, plain.vc, node_score=score, evict=ev)
+        for x, y in zip(_arrays(one), _arrays(plain)):
+            assert torch.equal(x, y), it
+        assert int(one.upd_pending.sum()) == 0 and float(one.step_score.abs().sum()) == 0
+    for eng in engs:
+        eng.run_step(use_graph=graph_steps)
+        eng.check_device_errors()
+    for x, y in zip(_arrays(one), _arrays(plain)):
+        assert torch.equal(x, y)
+
+
 def test_an_engine_refuses_a_negative_number_of_slots():
     cfg = get_config("parity-qwen2")
     with pytest.raises(ValueError, match="extra_slots"):

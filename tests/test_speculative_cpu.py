@@ -101,6 +101,13 @@ def test_commit_refusals(L, bad, status):
     assert _commit(L, **bad) == status and L.kvbp_last_error().startswith(b"tree_commit")
 
 
+def test_pending_update_refusals(L):
+    st = _state(A)
+    for a in ((None, A, 2 * A, 3 * A), (C.byref(st), None, 2 * A, 3 * A), (C.byref(st), A, None, 3 * A),
+              (C.byref(st), A, 2 * A, None), (C.byref(_state(A, slot_pos=None)), A, 2 * A, 3 * A)):
+        assert L.kvbp_score_update_pending(None, *a, None) == 1 and L.kvbp_last_error().startswith(b"score_update")
+
+
 def _tensors(B=2, T=4, hq=4, hkv=2, S=20):
     z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt)  # noqa: E731
     return dict(q=z(B, T, hq, 128), k_cache=z(B, hkv, S, 128), v_cache=z(B, hkv, S, 128), k_draft=z(B, hkv, T, 128),
