@@ -187,7 +187,13 @@ class SlotState:
         the engine with ``extra_slots`` >= the longest path - 1.  What a commit finds on the device (no free
         slot among it) goes to the engine's error word unless another is given: ``engine.check_device_errors()``.
         Each commit first applies the scores that the engine's last step has left pending.
-        The engine's ``token_log`` and ``retained_log`` hold its own steps only."""
+        The engine's ``token_log`` and ``retained_log`` hold its own steps only.
+
+        Engines with per-head retention are refused: these operators know no head masks and signals.  The ranks
+        of a tensor-parallel engine have the scores of their own heads: reduce ``node_score`` to its maximum over
+        the ranks before the commit, or their states part."""
+        if engine.per_head:
+            raise ValueError("engines with per-KV-head retention have no slot state that commits could change")
         return cls(engine.slot_pos, engine.insert_step, engine.last_access, engine.access_count, engine.attn_s,
                    engine.max_attn, engine.cumul, engine.prefill_s, engine.posmap, engine.seq_step, engine.next_pos,
                    engine.evlog, engine.evcount, engine)

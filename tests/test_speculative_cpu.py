@@ -2,6 +2,8 @@
 argument before their first CUDA call, the Python ones before they launch."""
 
 import ctypes as C
+import dataclasses
+import types
 
 import pytest
 import torch
@@ -11,6 +13,7 @@ from kvcacheboundaryprotection_b200 import build, capi, speculative as sp
 import spec_ref as ref
 
 BF = torch.bfloat16
+_FIELDS = [f.name for f in dataclasses.fields(sp.SlotState) if f.name != "engine"]
 A = 1 << 30  # an aligned address that is never read
 
 
@@ -165,6 +168,16 @@ def _slot_state(B=2, S=20, W=4, cap=30):
     z = lambda *s, dt=i: torch.zeros(*s, dtype=dt)  # noqa: E731
     return sp.SlotState(z(B, S), z(B, S), z(B, S), z(B, S), z(B, S, dt=f), z(B, S, dt=f), z(B, S, dt=torch.float64),
                         z(B, S, dt=f), z(B, W), z(B), z(B), z(B, cap), z(B))
+
+
+def test_engines_with_per_head_retention_are_refused():
+    names = dict(attn="attn_s", prefill="prefill_s")
+    eng = types.SimpleNamespace(per_head=False, **{names.get(k, k): getattr(_slot_state(), k) for k in _FIELDS})
+    state = sp.SlotState.of(eng)
+    assert state.engine is eng and state.like().engine is None and state.attn is eng.attn_s
+    eng.per_head = True
+    with pytest.raises(ValueError, match="per-KV-head"):
+        sp.SlotState.of(eng)
 
 
 def test_python_commit_refusals():
