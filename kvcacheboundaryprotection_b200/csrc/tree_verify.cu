@@ -353,19 +353,6 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     S = sum_lanes(got.sum * static_cast<double>(scale_to(got.top, top)));
     if (warp == 0 && lane < kWarps) w_sum[lane] = own_sum * static_cast<double>(scale_to(own_top, top));
   };
-  auto enter = [&](int node) {
-    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
-    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
-    n_rej = 0;
-    exact = false;
-    share();
-    read_row(false);
-    odd_row = !(S >= 0.0) || top == NEG_INF || top == -NEG_INF;
-    if (odd_row) read_row(true);
-    if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
-    E = 0.0;
-    __syncthreads();
-  };
   // ---- a warp's share ``v`` of the sum of what ``n`` rejections leave, to s_R[n] (and each warp's to w_sum)
   auto join_sum = [&](int n, double v) {
 #pragma unroll
@@ -460,6 +447,24 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   auto make_exact = [&]() {  // every sum of the current node again, in double
     exact = true;
     for (int k = drawn ? 0 : n_rej; k <= n_rej; ++k) sum_exact(k);
+  };
+
+  auto enter = [&](int node) {
+    row = reinterpret_cast<const L*>(a.target) + (static_cast<long long>(b) * T + node) * a.ldt;
+    if (drawn) q = a.draft + (static_cast<long long>(b) * T + node) * a.ldd;
+    n_rej = 0;
+    exact = false;
+    share();
+    read_row(false);
+    odd_row = !(S >= 0.0) || top == NEG_INF || top == -NEG_INF;
+    if (odd_row) read_row(true);
+    if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
+    E = 0.0;
+    __syncthreads();
+    // A bound that is no small number bounds nothing (its terms are first order): at very low temperatures, c times
+    // a logit is rounded by more than the differences that count.  Nor does a sum that is none, as at an infinite
+    // temperature.
+    if (!greedy && !(eps < 0x1p-4f && S > 0.5 && S < 4.0 * V)) make_exact();
   };
 
   enter(0);

@@ -370,6 +370,38 @@ def test_verification_where_fp32_decides_nothing(B, T, V, draft):
         _check_verify(c, _run_verify(c))
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("temp", [1e-3, 1e-5, 1e-6, 1e-7, 1e-9, 1e-20, 1e-30, 1e-38, 1e-42])
+def test_verification_at_very_low_temperatures(temp, draft, f32):
+    """The logit over the temperature is so large that fp32 does not hold the differences between logits: ties of
+    the largest logits share the weight, what lies below has what is left of it."""
+    c = _verify_case(32, 6, 3001, 17, "star", f32, draft, [temp])
+    top = 20 + 44 * torch.rand(32, 6, generator=_gen(4))
+    for i, at in enumerate((40, 41, 1500, 2900)):
+        c["target"][:, :, at] = (top * (1 if i != 2 else 1 + 2.0 ** -20)).to(c["target"].dtype)
+    if draft:
+        c["draft"] = 0.5 * c["draft"]
+        c["draft"][:, :, [40, 41, 1500, 2900]] += 0.125
+    c["tokens"][:, 1:] = torch.tensor([40, 2900, 1500, 41, 7], dtype=torch.int32)
+    for seed in range(4):
+        c["u"], c["s"] = torch.rand(32, 6, generator=_gen(seed)), torch.rand(32, generator=_gen(seed + 9))
+        _check_verify(c, _run_verify(c))
+
+
+def test_verification_at_an_infinite_temperature():
+    """Every finite logit has the same weight, filtered tokens none."""
+    c = _verify_case(4, 4, 1000, 3, "star", True, False, [float("inf")])
+    c["target"][2:, :, ::2] = -float("inf")
+    c["parents"][:] = torch.tensor([-1, 0, 0, 0])
+    c["tokens"][:, 1:] = torch.tensor([11, 12, 13], dtype=torch.int32)
+    c["u"][:] = torch.tensor([0.0, 0.01, 0.0, 0.0])  # 0.01 * 1000 and 0.01 * 500 are above 1
+    c["s"] = torch.tensor([0.25, 0.999, 0.25, 0.999])
+    path, n, token = _run_verify(c)
+    assert path[:, :2].tolist() == [[0, 2], [0, 2], [0, 3], [0, 3]] and n.tolist() == [2] * 4
+    assert token.tolist() == [250, 999, 251, 999]
+
+
 def test_verification_of_greedy_ties_and_equal_tokens():
     c = _verify_case(4, 8, 300, 3, "star", temp=[0.0, 1.0])
     c["target"][:, :, 17] = c["target"][:, :, 211] = 50.0  # a tie: the first one
