@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   const int T = a.T, V = a.V;
   for (int i = tid; i < T; i += kThreads) {
     s_par[i] = a.parents[static_cast<size_t>(b) * T + i];
+    if (rank == 0 && s_par[i] >= i) set_err(a.err, kErrIndex);  // names a later node: matches no accepted one
     s_tok[i] = a.tokens[static_cast<size_t>(b) * T + i];
     s_u[i] = a.accept_u[static_cast<size_t>(b) * T + i];
   }

@@ -440,6 +440,20 @@ def test_verification_of_bad_tokens_and_unused_roots():
     assert err.item() == 4 and got[1][1].item() == 0 and got[2][1].item() == -1 and got[1][0].item() == 1
 
 
+@pytest.mark.parametrize("b,node,parent", [(0, 0, 0), (1, 0, 3), (2, 3, 3), (2, 2, 4), (1, 4, 2 ** 31 - 1)])
+def test_verification_flags_parents_that_are_no_earlier_node(b, node, parent):
+    """Such a node counts as unused, a root of the kind leaves its sequence without a tree."""
+    c = _verify_case(3, 5, 300, 6, "tree")
+    c["parents"][:] = torch.tensor([-1, 0, 0, 1, 2])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _check_verify(c, _run_verify(c, dev_err=err))
+    assert err.item() == 0
+    c["parents"][b, node] = parent
+    got = _run_verify(c, dev_err=err)
+    _check_verify(c, got)
+    assert err.item() == 4 and (got[1][b].item() == 0) == (node == 0)
+
+
 def test_verification_at_the_ends_of_the_random_numbers():
     c = _verify_case(6, 6, 999, 4, "tree", draft=True)
     c["u"][:3] = 0.0  # accepted wherever the target has any weight
