@@ -529,10 +529,11 @@ int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_t Hq, int32
  * draft_probs [.. (b * T + parent) * ldd ..] float, or, where draft_probs is NULL (a draft that is
  * not random), 1 at x.  next_token[b] is the first x whose running sum of the last r exceeds
  * sample_u[b] * sum(r).  This keeps the target's distribution whatever the draft.  Where no weight is
- * left the token is drawn from the node's whole distribution; -1 (and KVBP_DEV_NAN_SCORE) where that
- * has none.  temperature <= 0: a token is accepted when it is the row's first maximum, and that is
- * next_token (draft_probs is not read).  NaN logits count as -inf and set KVBP_DEV_NAN_SCORE; a token
- * outside [0, vocab) is rejected, leaves r as it is and sets KVBP_DEV_INDEX.
+ * left the token is drawn from the node's whole distribution.  temperature <= 0: a token is accepted when
+ * it is the row's first maximum, and that is next_token (draft_probs is not read).  NaN logits count as
+ * -inf and set KVBP_DEV_NAN_SCORE; in a row of nothing but -inf all tokens have the same weight (softmax is
+ * undefined there), which sets KVBP_DEV_NAN_SCORE too.  A token outside [0, vocab) is rejected, leaves r as
+ * it is and sets KVBP_DEV_INDEX.
  * path [B][T] int32: the accepted nodes, root first, then -1; n_path[b] their number (1: the root
  * alone; 0 with next_token -1 for a sequence whose root is unused).  Tests and draws are decided as by
  * weights and sums in double.

@@ -459,6 +459,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     read_row(false);
     odd_row = !(S >= 0.0) || top == NEG_INF || top == -NEG_INF;
     if (odd_row) read_row(true);
+    if (tid == 0 && rank == 0 && top == NEG_INF) set_err(a.err, kErrNanScore);  // (all the same weight then)
     if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
     E = 0.0;
     __syncthreads();
@@ -527,10 +528,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   }
   // ---- the next token
   if (greedy) {
-    if (rank == 0 && tid == 0) {
-      a.next_token[b] = first == kNone ? -1 : first;
-      if (first == kNone) set_err(a.err, kErrNanScore);
-    }
+    if (rank == 0 && tid == 0) a.next_token[b] = first;
     sync_cluster();  // messages are read before a CTA leaves
     return;
   }
@@ -643,10 +641,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     const uint32_t from = mapa_u32(smem_u32(s_token), owner);
     asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(token), "=r"(certain) : "r"(from) : "memory");
     if (certain) {
-      if (rank == 0 && tid == 0) {
-        a.next_token[b] = static_cast<int>(token);
-        if (static_cast<int>(token) < 0) set_err(a.err, kErrNanScore);
-      }
+      if (rank == 0 && tid == 0) a.next_token[b] = static_cast<int>(token);
       break;
     }
     sync_cluster();  // the token is read before it is made again

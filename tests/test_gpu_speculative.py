@@ -430,6 +430,31 @@ def test_verification_of_odd_logits():
     assert token[5].item() in range(-1, 500)
 
 
+@pytest.mark.parametrize("temp", [0.0, 0.7])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("what", [-float("inf"), float("nan")])
+def test_verification_flags_rows_without_any_weight(what, f32, temp):
+    """All tokens of such a row have the same weight (greedy: the first one is its maximum), and the error word
+    says so; only where the walk comes by."""
+    c = _verify_case(2, 3, 700, 4, "chain", f32, temp=[temp])
+    c["parents"][:] = torch.tensor([-1, 0, 1])
+    c["tokens"][:, 1] = torch.argmax(c["target"][:, 0].float(), -1).to(torch.int32)
+    c["u"][:] = torch.tensor([0.0, 0.0, 0.5])
+    c["s"] = torch.tensor([0.5, 0.0])
+    c["target"][:, 2] = what  # never reached: node 2 is rejected
+    c["tokens"][:, 2] = 699
+    c["target"][:, 1, 699] = -float("inf")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _check_verify(c, _run_verify(c, dev_err=err))
+    assert err.item() == 0
+    c["target"][:, 1] = what
+    path, n, token = _run_verify(c, dev_err=err)
+    _check_verify(c, (path, n, token))
+    assert err.item() == 2 and n.tolist() == [2, 2]
+    # node 2's token is rejected there (0.5 * 700 >= 1): of 699 weights the 350th is the first past 349.5
+    assert token.tolist() == ([0, 0] if temp == 0 else [349, 0])
+
+
 def test_verification_of_bad_tokens_and_unused_roots():
     c = _verify_case(3, 4, 100, 2, "star")
     c["tokens"][0, 1:] = torch.tensor([-1, 100, 2 ** 31 - 1], dtype=torch.int32)
