@@ -5,8 +5,8 @@
 // left of them), R their sum, x the node's token and q the distribution that x was drawn from
 // (1 at x where there is none), the node is accepted when u * q(x) * R < r(x); otherwise
 //   r <- max(r / R - q, 0)        (r(x) <- 0 where q is 1 at x).
-// Each test keeps the target's law: P(accept x) + the residual's mass add up to r / R.  The
-// last accepted node's r gives one more token: the first x whose running sum exceeds u * R.
+// Each test keeps the target's law, x being an independent draw from q: P(accept x) + the residual's mass
+// add up to r / R.  The last accepted node's r gives one more token: the first x whose running sum exceeds u * R.
 //
 // A token is chosen where a running sum of a hundred thousand terms passes a border; it has to be the
 // token that the definition gives, so sums in 32 bits are trusted only as far as their error goes:
