@@ -530,7 +530,7 @@ int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_t Hq, int32
  * not random), 1 at x.  next_token[b] is the first x whose running sum of the last r exceeds
  * sample_u[b] * sum(r).  The tokens then follow the target's distribution if the random numbers are uniform
  * and independent of the draft, and siblings were drawn independently, with replacement, from q (draft_probs
- * given) or chosen without looking at the target (NULL).  Draws without replacement (a sampled top-k, beams)
+ * given) or chosen in any way (NULL).  Draws without replacement (a sampled top-k, beams)
  * need another residual: with q given as above they do not keep the law.  Where no weight is
  * left the token is drawn from the node's whole distribution.  temperature <= 0: a token is accepted when
  * it is the row's first maximum, and that is next_token (draft_probs is not read).  NaN logits count as

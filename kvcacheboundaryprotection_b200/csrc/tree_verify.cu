@@ -92,7 +92,9 @@ struct alignas(16) Message {
   double sum;
 };
 
-// e^y, y <= 0, to about 1e-14: y = n ln2 / 32 + r, e^r by its series, 2^(n / 32) from a table.
+// e^y, y <= 0, by Tang's table-driven method (ACM TOMS 15, 1989): y = n ln2 / 32 + r, e^r by its series,
+// 2^(n / 32) from a table.  |r| <= ln2 / 64, so that the series' rest r^6 / 720 is below 3e-15; the reduction by
+// one rounded constant adds 2^-53 |y|.
 __device__ __forceinline__ double exp_of(double y, const double* table) {
   if (!(y > -700.0)) return 0.0;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the nearest integer is left in the low bits

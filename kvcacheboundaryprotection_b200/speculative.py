@@ -125,9 +125,9 @@ def verify_tree(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
 
     Returns path [B, T] int32 (accepted nodes, the root first, then -1), n_path [B] (their number)
     and next_token [B] (drawn from what the target has left at the last accepted node).  The tokens
-    follow the target's distribution if siblings were drawn independently, with replacement, from
-    ``draft_probs`` (draws without replacement, as of a sampled top-k, do not keep it) or, without
-    ``draft_probs``, were chosen in any way that does not look at the target or the random numbers."""
+    follow the target's distribution if the random numbers are uniform and independent of the draft, and
+    siblings were drawn independently, with replacement, from ``draft_probs`` (draws without replacement,
+    as of a sampled top-k, do not keep it) or, without ``draft_probs``, were chosen in any way."""
     dev = target.device
     if target.dim() != 3 or target.dtype not in (_BF16, _F32):
         raise ValueError("target must be [B, T, vocab] of bfloat16 or float32")

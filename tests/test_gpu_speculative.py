@@ -3,6 +3,7 @@ statements of the same formulas (tests/spec_ref.py), at the sizes and masks wher
 wrong.  Tolerances count roundings and are derived beside each check."""
 
 import math
+from decimal import Decimal, getcontext
 
 import numpy as np
 import pytest
@@ -489,6 +490,37 @@ def test_verification_at_the_ends_of_the_random_numbers():
     c["s"][:] = 2.0  # outside the range: still a token of the vocabulary
     _, n, token = _run_verify(c)
     assert (n == 1).all() and ((token >= 0) & (token < 999)).all()
+
+
+def test_the_double_weights_bits():
+    """e^-d of the double path to 6e-14.  Token 0 has the logit -d, token 1 the logit 0; a draft that is the target's
+    distribution but for its last fp32 digits leaves p - q of about 2^-24 p after a rejection, and the
+    draw between the two tokens changes where u passes r0 / (r0 + r1), which an error of w in p moves by at most
+    2^24 of it (q is at least a step below p, and r1 moves less): 1e-6 on either side holds 6e-14."""
+    getcontext().prec = 60
+    n = 512
+    d = (torch.rand(n, generator=_gen(3)).double() * 80).float()
+    d[:8] = torch.tensor([2.0 ** -20, 1e-3, 0.0108, 0.0109, 0.3465, 0.3466, 0.6931, 0.6932])
+    q = torch.zeros(n, 2, 3)
+    u = torch.zeros(2, n)
+    below = lambda p, steps: np.float32(p) * np.float32(1 - steps * 2.0 ** -23)  # noqa: E731
+    for i in range(n):
+        w = (-Decimal(d[i].item())).exp()
+        p0, p1 = w / (1 + w), 1 / (1 + w)
+        q[i, 0] = torch.tensor([below(p0, 2), below(p1, 2), 0.25])
+        r0, r1 = p0 - Decimal(q[i, 0, 0].item()), p1 - Decimal(q[i, 0, 1].item())
+        assert r0 > p0 * Decimal(2) ** -24 and r1 > p1 * Decimal(2) ** -24
+        border = r0 / (r0 + r1)
+        u[0, i], u[1, i] = float(border * (1 - Decimal("1e-6"))), float(border * (1 + Decimal("1e-6")))
+    target = torch.zeros(n, 2, 3)
+    target[:, :, 0] = -d[:, None]
+    target[:, :, 2] = -1000.0
+    par = torch.tensor([[-1, 0]] * n, dtype=torch.int32).cuda()
+    tokens = torch.full((n, 2), 2, dtype=torch.int32).cuda()  # no weight left: rejected
+    for side in range(2):
+        _, count, token = sp.verify_tree(target.cuda(), tokens, par, torch.full((n, 2), 0.5).cuda(), u[side].cuda(),
+                                         draft_probs=q.cuda())
+        assert (count == 1).all() and (token == side).all(), (token != side).nonzero().flatten().tolist()
 
 
 @pytest.mark.parametrize("draft", [False, True])
