@@ -146,6 +146,13 @@ __device__ __forceinline__ bool any_of_pair(int id, bool v) {
   return r != 0;
 }
 
+// log2 of a row's sum of weights; NaN where all its logits are -inf, as its outputs are (0 / 0); infinite, so that
+// every weight is 0, where the node is unused.
+__device__ __forceinline__ float lse_of(float M, float L, float c, bool used) {
+  if (!used) return __int_as_float(0x7f800000);
+  return L == 0.f ? __int_as_float(0x7fffffff) : fmaf(M, c, log2f(L));
+}
+
 // Key tiles of sequence b: its cache's, and the drafted one.
 __device__ __forceinline__ int len_of(const Args& a, int b) {
   if (!a.lens) return a.S;
@@ -859,10 +866,10 @@ __global__ void __launch_bounds__(threads_of(F), 1)
       const bool ok = !*bad;
       if (in && ok && (FormB || x == 0) && copy == 0 && hc == 0) {
         if (!whole) {
-          pstat[prow] = used ? make_float2(M, L) : make_float2(NEG_INF, 0.f);
+          pstat[prow] = used ? make_float2(M, L) : make_float2(NEG_INF, -1.f);  // (-1: an unused node's)
           if (Score) pexact[prow] = Lx;
         } else if (Score) {
-          a.lse[orow] = used ? fmaf(M, c, log2f(Lx)) : __int_as_float(0x7f800000);
+          a.lse[orow] = lse_of(M, Lx, c, used);
         }
       }
       const float inv = whole ? 1.f / L : 1.f;
@@ -1021,14 +1028,14 @@ __global__ void __launch_bounds__(threads_of(F), 1)
             for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
           }
         }
-        const bool used = L != 0.f;
+        const bool used = !(st[0].y < 0.f);
         const float inv = 1.f / L;
         const size_t orow = (static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G;
         uint32_t pk[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) pk[e] = used ? pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv) : 0u;
         *reinterpret_cast<uint4*>(a.out + orow * kD + d0) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        if (Score && d0 == 0) a.lse[orow] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
+        if (Score && d0 == 0) a.lse[orow] = lse_of(M, Lx, a.c, used);
       }
     __syncwarp();
     cluster_sync_all();  // its parts are read before a CTA leaves
@@ -1078,12 +1085,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const Args a) {
     if (Score && warp == 0) Lx = fmaf(e, exact[s * rows + prow], Lx);
     if (e != 0.f) o[0] = fmaf(e, v0, o[0]), o[1] = fmaf(e, v1, o[1]), o[2] = fmaf(e, v2, o[2]), o[3] = fmaf(e, v3, o[3]);
   }
-  const bool used = L != 0.f;  // (a node in use sees itself; the parts of another say nothing)
+  const bool used = !(a.pstat[slot(c0) * rows + prow].y < 0.f);
   const float inv = 1.f / L;
   const size_t orow = (static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + r % a.G;
   *reinterpret_cast<uint2*>(a.out + orow * kD + warp * 4) =
       used ? make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)) : make_uint2(0, 0);
-  if (Score && warp == 0) a.lse[orow] = used ? fmaf(M, a.c, log2f(Lx)) : __int_as_float(0x7f800000);
+  if (Score && warp == 0) a.lse[orow] = lse_of(M, Lx, a.c, used);
 }
 
 // ------------------------------------------------------------------------------------

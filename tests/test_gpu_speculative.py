@@ -149,6 +149,22 @@ def test_what_a_row_does_not_see_never_reaches_it(shape, bad):
                 assert (score[b, t].double().cpu() - clean_top[b, t]).abs().max() < 1e-4, (b, t)
 
 
+@pytest.mark.parametrize("T", [4, 20, 40, 100])
+@pytest.mark.parametrize("B,S,lens", [(1, 900, None), (2, 1200, [1200, 3]), (64, 130, None), (300, 300, None)])
+def test_rows_whose_logits_are_all_minus_infinity(T, B, S, lens):
+    """softmax gives 0 / 0 there: NaN in such rows and only there, however the units are cut and joined; unused nodes
+    stay 0."""
+    c = _attn_case(B, T, 8, 2, S, 4, mask="slots" if S < 1000 else None, lens=lens)
+    c["k"][:, 1], c["kd"][:, 1] = -float("inf"), -float("inf")
+    c["q"][:, 1:, 4:] = c["q"][:, 1:, 4:].abs() + 0.01  # kv head 1's rows but for the root's
+    c["q"][:, 0, 4:] = -0.5
+    c["parents"][:, T - 1] = -2
+    out = _run(c).float().cpu()
+    used = torch.tensor([[s is not None for s in ref.sees(p)] for p in c["parents"].tolist()])
+    assert (out[~used] == 0).all() and torch.isfinite(out[:, :, :4]).all()
+    assert torch.isnan(out[:, :, 4:][used]).all()  # (the root's: +inf logits)
+
+
 def test_a_value_that_is_seen_counts():
     """Infinities and NaN of a seen node's V reach the rows that see it, in their dims only."""
     c = _attn_case(1, 6, 8, 2, 200, 4, mask=None, kind="star")
