@@ -510,6 +510,7 @@ int kvbp_int8_linear(kvbp_stream_t stream, int32_t fp32_out, int32_t M, int32_t 
  * node_score [B][T][S + T] float (may be NULL, non-negative on entry) is max-accumulated with each
  * (node, key)'s largest probability over the heads: column s is slot s, S + j is node j.  (Pass the
  * same buffer for every layer; zero it before a step's first.)  Unused nodes: out is 0, scores stay.
+ * A node with a NaN among its weights gets NaN for all that it sees, which sets KVBP_DEV_NAN_SCORE.
  * K and V of slots and nodes that a row does not see never reach it.  lens outside [0, S] is cut
  * there and sets KVBP_DEV_INDEX.  Softmax statistics and sums are fp32.
  * workspace: kvbp_tree_attn_workspace bytes, 16-byte aligned (NULL where that is 0); free to reuse by

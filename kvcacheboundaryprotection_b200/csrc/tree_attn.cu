@@ -1104,7 +1104,8 @@ constexpr int kScOffQ = kTile;                      // K, then Q of one item
 constexpr int kScOffLse = 2 * kTile;                // float [128]
 constexpr int kScOffSee = kScOffLse + 128 * 4;      // uint4 [128]
 constexpr int kScOffBars = kScOffSee + kMaxNodes * 16;
-constexpr int kScOffMax = kScOffBars + 64;          // float [nodes, a multiple of 8][128 slots]
+constexpr int kScOffNan = kScOffBars + 64;          // uint32 [4] nodes with a NaN among their sums of weights
+constexpr int kScOffMax = kScOffNan + 16;           // float [nodes, a multiple of 8][128 slots]
 constexpr int score_smem(int T) { return kScOffMax + (T + 7) / 8 * 8 * 128 * 4; }
 
 struct ScoreArgs {
@@ -1124,6 +1125,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3)
   float* best = reinterpret_cast<float*>(base + kScOffMax);
   float* slse = reinterpret_cast<float*>(base + kScOffLse);
   uint4* see = reinterpret_cast<uint4*>(base + kScOffSee);
+  uint32_t* nans = reinterpret_cast<uint32_t*>(base + kScOffNan);
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + kScOffBars);
   uint64_t* full = bars;       // K and Q landed
   uint64_t* sfull = bars + 1;  // S^T written
@@ -1149,6 +1151,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   const int T8 = (a.T + 7) / 8 * 8;
+  if (tid < 4) nans[tid] = 0;
   for (int i = tid; i < T8 * 128; i += kScoreThreads) best[i] = 0.f;
   pdl_launch_dependents();
   pdl_wait();
@@ -1239,8 +1242,10 @@ __global__ void __launch_bounds__(kScoreThreads, 3)
       named_bar(1, 256);  // the previous item's statistics have been read
       for (int r = tid; r < gn * p.chunk; r += 256) {
         const int t = n0 + r % p.chunk;
-        slse[r] = t < a.T ? a.lse[(static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + g0 + r / p.chunk]
-                          : __int_as_float(0x7f800000);
+        const float l = t < a.T ? a.lse[(static_cast<size_t>(b) * a.T + t) * a.Hq + static_cast<size_t>(h) * a.G + g0 + r / p.chunk]
+                                : __int_as_float(0x7f800000);
+        slse[r] = l;
+        if (l != l) atomicOr(&nans[t >> 5], 1u << (t & 31));
       }
       wait(sfull, i & 1);
       named_bar(2, 256);
@@ -1287,8 +1292,11 @@ __global__ void __launch_bounds__(kScoreThreads, 3)
           const uint32_t w = sl < 32 ? m.x : sl < 64 ? m.y : sl < 96 ? m.z : m.w;
           if (!((w >> (sl & 31)) & 1u)) continue;
         }
-        const float v = best[t * 128 + sl];
-        if (v > 0.f)
+        // (a NaN logit makes all of the node's weights NaN; the maxima above leave NaN out)
+        const bool nan = (nans[t >> 5] >> (t & 31)) & 1u;
+        const float v = nan ? __int_as_float(0x7fffffff) : best[t * 128 + sl];
+        if (nan) set_err(a.err, kErrNanScore);
+        if (nan || v > 0.f)
           atomicMax(reinterpret_cast<int*>(p.score + (static_cast<size_t>(b) * a.T + t) * (static_cast<size_t>(a.S) + a.T) +
                                            (drafted ? a.S : tile * kKeys) + sl),
                     __float_as_int(v));

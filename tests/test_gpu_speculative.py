@@ -165,6 +165,30 @@ def test_rows_whose_logits_are_all_minus_infinity(T, B, S, lens):
     assert torch.isnan(out[:, :, 4:][used]).all()  # (the root's: +inf logits)
 
 
+@pytest.mark.parametrize("T,hq,hkv,S", [(6, 8, 2, 200), (40, 16, 2, 300), (128, 4, 4, 70), (3, 60, 1, 500)])
+def test_nan_weights_reach_the_scores(T, hq, hkv, S):
+    """A NaN in a node's query (one head of it): its scores are NaN for all that it sees, and only there; the error
+    word says so, and so does the commit that reads them."""
+    c = _attn_case(2, T, hq, hkv, S, 4, mask="slots", kind="star")
+    c["parents"][1, T - 1] = -2
+    c["q"][0, 2, hq // 2, 7] = float("nan")
+    c["q"][1, T - 1] = float("nan")  # an unused node's
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    score = torch.zeros(2, T, S + T, device="cuda")
+    _run(c, score, dev_err=err)
+    assert err.item() == 2
+    live = c["slot_pos"][0] >= 0
+    want = torch.zeros(2, T, S + T, dtype=torch.bool)
+    want[0, 2, :S] = live
+    want[0, 2, S], want[0, 2, S + 2] = True, True
+    assert torch.equal(torch.isnan(score).cpu(), want)
+    c["q"] = torch.nan_to_num(c["q"])
+    clean = torch.zeros_like(score)
+    err.zero_()
+    _run(c, clean, dev_err=err)
+    assert err.item() == 0 and torch.equal(torch.where(want.cuda(), 0, clean), torch.where(want.cuda(), 0, score))
+
+
 def test_a_value_that_is_seen_counts():
     """Infinities and NaN of a seen node's V reach the rows that see it, in their dims only."""
     c = _attn_case(1, 6, 8, 2, 200, 4, mask=None, kind="star")
