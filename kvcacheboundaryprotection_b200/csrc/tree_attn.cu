@@ -31,17 +31,21 @@
 //     and added by the rows that see them.
 // Rounding: S, sums and O are fp32; a weight is rounded once to bf16 (half a step, 2^-8 of it), in form A
 // the sum that divides is that of the rounded weights (an error common to all cancels), in form B, where
-// the issue slots count, that of the unrounded ones; out is rounded once.
-// Measured on B200 (graph replay): 64 sequences x 5 nodes x 4104 slots, 8 kv heads: 187 us, 5.5 TB/s of the
-// 6.46 of a copy (without the loads the same hand-overs between the warps take 122 us, without the softmax
-// 180: the two overlap but for the start of each unit); 1 x 64 nodes x 131071 slots, 8 kv heads: 143 us, the
-// tensor pipe 45 % busy, bound by the chain S -> weights -> P . V of each row tile (without the weights'
-// arithmetic 128 us); exponentials on the FMA pipe instead of the MUFU for 1/8 to 5/8 of the columns were
-// slower (161 -> 166-180 us at the time).
+// the issue slots count, that of the unrounded ones; out is rounded once.  The other attention kernels over
+// bf16 caches hold the weights as a sum of two bf16.  Here that costs a second P . V product and a second conversion: 218 -> 241 us
+// (64 sequences x 5 nodes x 4104 slots), 176 -> 225 (1 x 64 x 131071), 119-123 -> 126-130 (12 ragged x 33), 40.1 -> 41.8
+// (16 x 16 x 1032), 19.0 -> 19.4 (1 x 8 x 256), and takes the error of out (2-norm, against 64 bits) from 0.0018-0.0022
+// to the 0.0017 of its own rounding: a quarter of the time of large trees for less than a rounding of out.
+// Measured on B200, calls on changing inputs: 64 sequences x 5 nodes x 4104 slots, 8 kv heads: 218 us, 4.7 TB/s of the
+// 6.46 of a copy; 1 x 64 nodes x 131071 slots, 8 kv heads: 176 us, bound by the chain S -> weights -> P . V of each
+// row tile.  Replayed from a graph on the same inputs, a part of which is then in L2, 187 and 143 us; in that
+// state the first takes 122 us without the loads and 180 without the softmax (the two overlap but for the start of
+// each unit), the second 128 without the weights' arithmetic, its tensor pipe 45 % busy.  Exponentials
+// on the FMA pipe instead of the MUFU for 1/8 to 5/8 of the columns were slower (161 -> 166-180 us at the time).
 //
 // combine_kernel joins the parts of units that a border cut.  score_kernel forms p again from the final row
 // statistics: S^T = K . Q^T with a slot per thread, so that the maximum over heads stays in the thread and
-// the score rows are written along the slots (16 x 16 nodes x 1032 slots, 4 kv heads: 16 us of 37).
+// the score rows are written along the slots (16 x 16 nodes x 1032 slots, 4 kv heads: 16 us of 37, replayed).
 #include <type_traits>
 
 #include "common.cuh"
@@ -1466,7 +1470,7 @@ extern "C" int kvbp_tree_attn(kvbp_stream_t stream, int32_t B, int32_t T, int32_
     //  * n CTAs for each unit: borders between units;
     //  * the n a cluster, which joins its parts in shared memory (about one and a half), or n = 1.
     // Each wave of CTAs begins anew (about three).  clusters[n]: how many clusters of n CTAs with this much
-    // shared memory a B200 holds.  On B200: 64 units of 10 tiles 25 us by ranges over 148 CTAs, 20 us in
+    // shared memory a B200 holds.  On B200 (replayed): 64 units of 10 tiles 25 us by ranges over 148 CTAs, 20 us in
     // clusters of 2; 48 units of 65 (form B) 75 us by ranges, 70 us on 3 CTAs a unit; 512 units of 34
     // 189 us by ranges, 222 us in clusters of 2.
     static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};

@@ -20,7 +20,7 @@
 // next one's.  The CTAs exchange their sums through shared memory and take every decision alike.
 //
 // What bounds it is the chain of a path: a row is 2.3 us of loads and 2 of joins (warps, CTAs), and the next
-// row is known only then.  On B200 (graph replay): greedy 16 x 16 nodes x 152064 tokens, five levels: 25 us; one
+// row is known only then.  On B200 (graph replay on the same inputs, the smaller ones in L2): greedy 16 x 16 nodes x 152064 tokens, five levels: 25 us; one
 // sequence with a draft's distributions, two levels, a rejection and the draw: 28 us; 64 x 32 nodes with them:
 // 160 to 500 us with the inputs, the time of the sequence with the most rejections.
 #include <math.h>
