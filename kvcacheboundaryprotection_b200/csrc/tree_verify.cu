@@ -141,7 +141,6 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   const int T = a.T, V = a.V;
   for (int i = tid; i < T; i += kThreads) {
     s_par[i] = a.parents[static_cast<size_t>(b) * T + i];
-    if (rank == 0 && s_par[i] >= i) set_err(a.err, kErrIndex);  // names a later node: matches no accepted one
     s_tok[i] = a.tokens[static_cast<size_t>(b) * T + i];
     s_u[i] = a.accept_u[static_cast<size_t>(b) * T + i];
   }
@@ -154,7 +153,10 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   const float c = static_cast<float>(1.4426950408889634 * inv);
   if (s_par[0] != -1) {  // no tree
     if (rank == 0) {
-      for (int i = tid; i < T; i += kThreads) path[i] = -1;
+      for (int i = tid; i < T; i += kThreads) {
+        path[i] = -1;
+        if (s_par[i] >= i) set_err(a.err, kErrIndex);
+      }
       if (tid == 0) {
         a.n_path[b] = 0;
         a.next_token[b] = -1;
@@ -459,16 +461,19 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
     exact = false;
     share();
     read_row(false);
-    odd_row = !(S >= 0.0) || top == NEG_INF || top == -NEG_INF;
-    if (odd_row) read_row(true);
-    if (tid == 0 && rank == 0 && top == NEG_INF) set_err(a.err, kErrNanScore);  // (all the same weight then)
+    // A bound that is no small number bounds nothing (its terms are first order): at very low temperatures, c times
+    // a logit is rounded by more than the differences that count.  (It is infinite where the maximum is.)
+    odd_row = !(S >= 0.0) || !(eps < 0x1p-4f);
+    if (odd_row) {
+      read_row(true);
+      if (tid == 0 && rank == 0 && top == NEG_INF) set_err(a.err, kErrNanScore);  // (all the same weight then)
+      // a bound that decides nothing sends tests and draws to the double sums (a sum that is none: as at an
+      // infinite temperature)
+      if (!(eps < 0x1p-4f && S > 0.5 && S < 4.0 * V)) eps = 1e30f, S = 1.0;
+    }
     if (tid == 0) s_R[0] = greedy ? 1.0 : S, s_inv[0] = 1.0 / S, s_finv[0] = static_cast<float>(1.0 / S);
     E = 0.0;
     __syncthreads();
-    // A bound that is no small number bounds nothing (its terms are first order): at very low temperatures, c times
-    // a logit is rounded by more than the differences that count.  Nor does a sum that is none, as at an infinite
-    // temperature.
-    if (!greedy && !(eps < 0x1p-4f && S > 0.5 && S < 4.0 * V)) make_exact();
   };
 
   enter(0);
@@ -526,6 +531,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) verify_kernel(Args a
   }
   if (rank == 0) {
     for (int i = n + tid; i < T; i += kThreads) path[i] = -1;
+    for (int i = tid; i < T; i += kThreads)
+      if (s_par[i] >= i) set_err(a.err, kErrIndex);  // names no earlier node: matched no accepted one
     if (tid == 0) a.n_path[b] = n;
   }
   // ---- the next token
